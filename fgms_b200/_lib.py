@@ -14,7 +14,7 @@ LIB_PATH = os.path.join(_HERE, "libfgms_b200.so")
 
 OK = 0
 ERR_INVALID_ARG, ERR_CHANNEL_MISMATCH, ERR_UNSUPPORTED, ERR_CUDA, ERR_WORKSPACE, ERR_DEVICE = -1, -2, -3, -4, -5, -6
-DTYPE_F32, DTYPE_F16 = 0, 1
+DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
 MATH_FP32, MATH_TF32, MATH_F16 = 0, 1, 2
 
 # name -> (restype, argtypes); mirrors include/fgms_b200.h declaration by declaration
@@ -45,6 +45,9 @@ SIGNATURES = {
     "fgms_b200_neighbor_table_bytes": (c_size_t, [c_int, c_int]),
     "fgms_b200_build_neighbor_table": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int, c_int, c_void_p, c_size_t, c_void_p]),
     "fgms_b200_fwd_output_stationary": (c_int, [c_void_p] * 4 + [c_int] * 7 + [c_void_p, c_int, c_int, c_void_p]),
+    "fgms_b200_grouped_fwd": (c_int, [c_void_p] * 4 + [c_int] * 6 + [c_void_p]),
+    "fgms_b200_grouped_dgrad": (c_int, [c_void_p] * 4 + [c_int] * 6 + [c_void_p]),
+    "fgms_b200_grouped_wgrad": (c_int, [c_void_p] * 4 + [c_int] * 5 + [c_void_p]),
     "fgms_b200_peer_exchange_flag_bytes": (c_size_t, [c_int]),
     "fgms_b200_peer_exchange": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int64, ctypes.c_uint32, c_int64, c_int, c_void_p]),
     "fgms_b200_kernel_family": (c_int, [c_int] * 6),

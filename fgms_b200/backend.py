@@ -31,7 +31,8 @@ from . import _lib, _native
 
 __all__ = ["fgms_fusion_fwd_cuda", "fgms_fwd_cuda", "fgms_bwd_cuda", "fgms_dgrad_cuda", "fgms_wgrad_cuda",
            "wgrad_workspace", "wgrad_finalize", "fgms_wgrad_noalloc_cuda", "kernel_family", "fallback_count",
-           "device_status", "launch_count", "build_neighbor_table", "fgms_fwd_os_cuda"]
+           "device_status", "launch_count", "build_neighbor_table", "fgms_fwd_os_cuda", "fgms_grouped_fwd_cuda",
+           "fgms_grouped_dgrad_cuda", "fgms_grouped_wgrad_cuda"]
 
 _L = _lib.lib
 
@@ -259,6 +260,28 @@ def wgrad_finalize(kernel_grad: torch.Tensor, partial_f32: torch.Tensor) -> None
         raise ValueError("partial sums are shorter than kernel_grad")
     with torch.cuda.device(kernel_grad.device):
         _lib.check(_L.fgms_b200_wgrad_finalize(_ptr(kernel_grad), _ptr(partial_f32), kernel_grad.numel(), _stream()))
+
+
+def fgms_grouped_fwd_cuda(in_feats, kernel, out_feats, kpos, zero_rest=False):
+    """``out_feats[r] = in_feats[r] @ kernel[g]`` for the rows ``kpos[g] <= r < kpos[g + 1]`` of every group
+    (``fgms_b200_grouped_fwd``): the product of a layer of experts whose rows are in the order of their experts.
+
+    ``kernel`` is ``[groups, c_in, c_out]`` with any channel counts, float16, bfloat16 (tensor cores, fp32 sums) or float32 (exact fp32);
+    ``kpos`` an int32 tensor of ``groups + 1`` entries on the device, so that nothing waits for the sizes of the groups.  ``out_feats`` is
+    overwritten; rows of no group are left as they were, or with ``zero_rest`` become zeros.  Entries of ``kpos`` that are out of order or
+    out of range are counted by :func:`device_status`."""
+    _native.grouped_fwd(in_feats, kernel, out_feats, kpos, zero_rest)
+
+
+def fgms_grouped_dgrad_cuda(out_feats_grad, kernel, in_feats_grad, kpos, zero_rest=False):
+    """Input gradient of :func:`fgms_grouped_fwd_cuda`: ``in_feats_grad[r] = out_feats_grad[r] @ kernel[g].T``."""
+    _native.grouped_dgrad(out_feats_grad, kernel, in_feats_grad, kpos, zero_rest)
+
+
+def fgms_grouped_wgrad_cuda(in_feats, out_feats_grad, kernel_grad, kpos):
+    """Weight gradient of :func:`fgms_grouped_fwd_cuda`: ``kernel_grad[g] = in_feats[rows of g].T @ out_feats_grad[rows of g]``,
+    zeros for a group without rows.  ``kernel_grad`` is overwritten."""
+    _native.grouped_wgrad(in_feats, out_feats_grad, kernel_grad, kpos)
 
 
 def kernel_family(pass_: str, c_in: int, c_out: int, dtype: torch.dtype, arch80: bool = True, k_vol: int = 27) -> str:

@@ -25,6 +25,7 @@
 #include "backward_share.cuh"
 #include "peer_exchange.cuh"
 #include "umma_osfwd.cuh"
+#include "grouped_ffma.cuh"
 
 namespace {
 
@@ -317,6 +318,35 @@ int run_wgrad(const void* in_feats, const void* out_grad, void* kernel_grad, con
   return FGMS_OK;
 }
 
+// products of ragged groups of rows (csrc/grouped.cuh)
+template <int PASS>
+int run_grouped(const void* a, const void* b, void* d, const int32_t* kpos, int n_rows, int c_in, int c_out, int groups, int dtype, int zero_rest,
+                void* stream) {
+  if (n_rows < 0) return fail(FGMS_ERR_INVALID_ARG, "negative row count");
+  if (c_in < 1 || c_out < 1) return fail(FGMS_ERR_INVALID_ARG, "channel counts must be >= 1");
+  if (groups < 1 || groups > FGMS_GROUPED_MAX_GROUPS)
+    return fail(FGMS_ERR_INVALID_ARG, "groups %d outside [1, %d]", groups, FGMS_GROUPED_MAX_GROUPS);
+  if ((long long)groups * c_in > 0x7fffffffll || (long long)groups * c_out > 0x7fffffffll)
+    return fail(FGMS_ERR_INVALID_ARG, "groups times channels exceeds the int32 range");
+  if (dtype != FGMS_DTYPE_F32 && dtype != FGMS_DTYPE_F16 && dtype != FGMS_DTYPE_BF16) return fail(FGMS_ERR_INVALID_ARG, "unknown dtype %d", dtype);
+  const size_t es = dtype == FGMS_DTYPE_F32 ? 4 : 2, weights = (size_t)groups * c_in * c_out * es;
+  const size_t in = (size_t)n_rows * c_in * es, out = (size_t)n_rows * c_out * es;
+  const size_t a_bytes = PASS == fgms::GROUPED_DGRAD ? out : in, b_bytes = PASS == fgms::GROUPED_WGRAD ? out : weights;
+  const size_t d_bytes = PASS == fgms::GROUPED_FWD ? out : PASS == fgms::GROUPED_DGRAD ? in : weights;
+  if (!kpos || (a_bytes > 0 && !a) || (b_bytes > 0 && !b) || (d_bytes > 0 && !d)) return fail(FGMS_ERR_INVALID_ARG, "null pointer");
+  const Range ra{a, a_bytes}, rb{b, b_bytes}, rd{d, d_bytes}, rk{kpos, (size_t)(groups + 1) * sizeof(int32_t)};
+  if (rd.overlaps(ra) || rd.overlaps(rb) || rd.overlaps(rk)) return fail(FGMS_ERR_INVALID_ARG, "the output overlaps an input");
+  if (d_bytes == 0) return FGMS_OK;
+  DeviceInfo di;
+  if (int rc = device_info(&di)) return rc;
+  const fgms::GroupedParams p{a, b, d, kpos, n_rows, c_in, c_out, groups, zero_rest, di.reserved > 0};
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int rc = dtype == FGMS_DTYPE_F32   ? fgms::launch_grouped_ffma<float, PASS>(p, st, di.sms)
+                 : dtype == FGMS_DTYPE_F16 ? fgms::launch_grouped_ffma<__half, PASS>(p, st, di.sms)
+                                           : fgms::launch_grouped_ffma<__nv_bfloat16, PASS>(p, st, di.sms);
+  if (rc != 0) return fail(FGMS_ERR_CUDA, "grouped_ffma_kernel: %s", cudaGetErrorString(cudaGetLastError()));
+  return check_launch("grouped_ffma_kernel");
+}
 }  // namespace
 
 extern "C" {
@@ -914,6 +944,27 @@ int fgms_b200_fwd_output_stationary(const void* in_feats, const void* kernel, vo
   if (rc == 0) return check_launch("umma_osfwd_kernel");
   if (rc < 0) return fail(FGMS_ERR_CUDA, "umma_osfwd_kernel setup failed (%d)", rc);
   return fail(FGMS_ERR_INVALID_ARG, "tensors must be 16-byte aligned");
+}
+
+// ---------------------------------------------------------------------------------------------
+// Products of ragged groups of rows (csrc/grouped.cuh)
+// ---------------------------------------------------------------------------------------------
+int fgms_b200_grouped_fwd(const void* in_feats, const void* kernel, void* out_feats, const int32_t* kpos, int n_rows, int c_in, int c_out, int groups,
+                          int dtype, int zero_rest, void* stream) {
+  TraceRange trace_range("fgms_b200_grouped_fwd");
+  return run_grouped<fgms::GROUPED_FWD>(in_feats, kernel, out_feats, kpos, n_rows, c_in, c_out, groups, dtype, zero_rest, stream);
+}
+
+int fgms_b200_grouped_dgrad(const void* out_grad, const void* kernel, void* in_grad, const int32_t* kpos, int n_rows, int c_in, int c_out, int groups,
+                            int dtype, int zero_rest, void* stream) {
+  TraceRange trace_range("fgms_b200_grouped_dgrad");
+  return run_grouped<fgms::GROUPED_DGRAD>(out_grad, kernel, in_grad, kpos, n_rows, c_in, c_out, groups, dtype, zero_rest, stream);
+}
+
+int fgms_b200_grouped_wgrad(const void* in_feats, const void* out_grad, void* kernel_grad, const int32_t* kpos, int n_rows, int c_in, int c_out,
+                            int groups, int dtype, void* stream) {
+  TraceRange trace_range("fgms_b200_grouped_wgrad");
+  return run_grouped<fgms::GROUPED_WGRAD>(in_feats, out_grad, kernel_grad, kpos, n_rows, c_in, c_out, groups, dtype, 0, stream);
 }
 
 int64_t fgms_b200_device_status(int reset) {

@@ -639,6 +639,94 @@ Pyramid build_pyramid(const Tensor& coords, int levels, int what) {
 }
 
 // ---------------------------------------------------------------------------------------------
+// products of ragged groups of rows
+// ---------------------------------------------------------------------------------------------
+int grouped_dtype(const Tensor& t) {
+  if (t.scalar_type() == at::kHalf) return FGMS_DTYPE_F16;
+  if (t.scalar_type() == at::kBFloat16) return FGMS_DTYPE_BF16;
+  TORCH_CHECK_VALUE(t.scalar_type() == at::kFloat, "unsupported feature dtype ", t.scalar_type(),
+                    ": the grouped products take float16, bfloat16 or float32");
+  return FGMS_DTYPE_F32;
+}
+
+// rows [n, width] of the weights' type and device, where a row's width is the weights' dimension `side`
+void check_rows(const char* name, const Tensor& t, const Tensor& weights, int side) {
+  check_feat(name, t, 2, weights);
+  TORCH_CHECK_VALUE(t.device() == weights.device(), name, " must live on ", weights.device());
+  TORCH_CHECK_VALUE(t.size(1) == weights.size(side), name, " has ", t.size(1), " channels, the weights say ", weights.size(side));
+  TORCH_CHECK_VALUE(t.size(0) <= 0x7fffffff, name, " has more than 2^31 - 1 rows");
+}
+void check_groups(const char* name, const Tensor& weights, const Tensor& kpos) {
+  check_feat(name, weights, 3);
+  check_index("kpos", kpos, weights, 0);
+  TORCH_CHECK_VALUE(kpos.dim() == 1 && kpos.size(0) == weights.size(0) + 1, "kpos must have one entry more than there are groups: ",
+                    weights.size(0) + 1, ", got ", kpos.numel());
+  for (int d = 1; d < 3; ++d) TORCH_CHECK_VALUE(weights.size(d) <= 0x7fffffff, "more than 2^31 - 1 channels");
+}
+
+void grouped_fwd(const Tensor& in_feats, const Tensor& kernel, const Tensor& out, const Tensor& kpos, bool zero_rest) {
+  check_groups("kernel", kernel, kpos);
+  check_rows("in_feats", in_feats, kernel, 1);
+  check_rows("out_feats", out, kernel, 2);
+  TORCH_CHECK_VALUE(in_feats.size(0) == out.size(0), "in_feats and out_feats differ in rows");
+  const int dtype = grouped_dtype(kernel);
+  c10::cuda::CUDAGuard guard(kernel.device());
+  check_status(fgms_b200_grouped_fwd(ptr(in_feats), ptr(kernel), ptr(out), iptr(kpos), (int)out.size(0), (int)kernel.size(1), (int)kernel.size(2),
+                                     (int)kernel.size(0), dtype, zero_rest, stream_of(kernel)));
+}
+
+void grouped_dgrad(const Tensor& grad_out, const Tensor& kernel, const Tensor& in_grad, const Tensor& kpos, bool zero_rest) {
+  check_groups("kernel", kernel, kpos);
+  check_rows("out_feats_grad", grad_out, kernel, 2);
+  check_rows("in_feats_grad", in_grad, kernel, 1);
+  TORCH_CHECK_VALUE(in_grad.size(0) == grad_out.size(0), "out_feats_grad and in_feats_grad differ in rows");
+  const int dtype = grouped_dtype(kernel);
+  c10::cuda::CUDAGuard guard(kernel.device());
+  check_status(fgms_b200_grouped_dgrad(ptr(grad_out), ptr(kernel), ptr(in_grad), iptr(kpos), (int)in_grad.size(0), (int)kernel.size(1),
+                                       (int)kernel.size(2), (int)kernel.size(0), dtype, zero_rest, stream_of(kernel)));
+}
+
+void grouped_wgrad(const Tensor& in_feats, const Tensor& grad_out, const Tensor& kernel_grad, const Tensor& kpos) {
+  check_groups("kernel_grad", kernel_grad, kpos);
+  check_rows("in_feats", in_feats, kernel_grad, 1);
+  check_rows("out_feats_grad", grad_out, kernel_grad, 2);
+  TORCH_CHECK_VALUE(in_feats.size(0) == grad_out.size(0), "in_feats and out_feats_grad differ in rows");
+  const int dtype = grouped_dtype(kernel_grad);
+  c10::cuda::CUDAGuard guard(kernel_grad.device());
+  check_status(fgms_b200_grouped_wgrad(ptr(in_feats), ptr(grad_out), ptr(kernel_grad), iptr(kpos), (int)in_feats.size(0), (int)kernel_grad.size(1),
+                                       (int)kernel_grad.size(2), (int)kernel_grad.size(0), dtype, stream_of(kernel_grad)));
+}
+
+struct GroupedLinear : torch::autograd::Function<GroupedLinear> {
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& feats_, const Tensor& weight_, const Tensor& kpos) {
+    const Tensor feats = feats_.contiguous(), weight = weight_.contiguous();
+    check_groups("weight", weight, kpos);
+    check_rows("feats", feats, weight, 1);
+    Tensor out = at::empty({feats.size(0), weight.size(2)}, feats.options().requires_grad(false));
+    grouped_fwd(feats, weight, out, kpos, true);
+    ctx->save_for_backward({feats, weight, kpos});
+    return out;
+  }
+
+  // only the gradients that something needs; rows of no group have a gradient of zero
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &feats = saved[0], &weight = saved[1], &kpos = saved[2];
+    const Tensor grad_out = grads[0].contiguous();
+    Tensor in_grad, w_grad;
+    if (ctx->needs_input_grad(0)) {
+      in_grad = at::empty_like(feats);
+      grouped_dgrad(grad_out, weight, in_grad, kpos, true);
+    }
+    if (ctx->needs_input_grad(1)) {
+      w_grad = at::empty_like(weight);
+      grouped_wgrad(feats, grad_out, w_grad, kpos);
+    }
+    return {in_grad, w_grad, Tensor()};
+  }
+};
+
+// ---------------------------------------------------------------------------------------------
 // Python entry points (positional arguments only; the functions of backend.py / nn.py give them their names)
 // ---------------------------------------------------------------------------------------------
 const Tensor& feat_arg(PyObject* o, const char* name) {
@@ -744,6 +832,34 @@ PyObject* py_fwd_os(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+PyObject* py_grouped_fwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  expect(n, 5);
+  grouped_fwd(feat_arg(a[0], "in_feats"), feat_arg(a[1], "kernel"), feat_arg(a[2], "out_feats"), index_arg(a[3], "kpos"), bool_arg(a[4]));
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+PyObject* py_grouped_dgrad(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  expect(n, 5);
+  grouped_dgrad(feat_arg(a[0], "out_feats_grad"), feat_arg(a[1], "kernel"), feat_arg(a[2], "in_feats_grad"), index_arg(a[3], "kpos"), bool_arg(a[4]));
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+PyObject* py_grouped_wgrad(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  expect(n, 4);
+  grouped_wgrad(feat_arg(a[0], "in_feats"), feat_arg(a[1], "out_feats_grad"), feat_arg(a[2], "kernel_grad"), index_arg(a[3], "kpos"));
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+PyObject* py_grouped_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  expect(n, 3);
+  return THPVariable_Wrap(GroupedLinear::apply(feat_arg(a[0], "feats"), feat_arg(a[1], "weight"), index_arg(a[2], "kpos")));
+  END_HANDLE_TH_ERRORS
+}
+
 // (voxels per level, [(kpos, imap, omap) ...], [coords of level 1 ...]), or None for a cloud that does not suit
 PyObject* py_build_pyramid(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -768,6 +884,8 @@ PyMethodDef methods[] = {
     FGMS_METHOD("fwd_os", py_fwd_os),         FGMS_METHOD("sparse_conv", py_sparse_conv),
     FGMS_METHOD("sparse_stack", py_sparse_stack),
     FGMS_METHOD("wgrad_fp32_sums", py_wgrad_fp32_sums),
+    FGMS_METHOD("grouped_fwd", py_grouped_fwd), FGMS_METHOD("grouped_dgrad", py_grouped_dgrad),
+    FGMS_METHOD("grouped_wgrad", py_grouped_wgrad), FGMS_METHOD("grouped_linear", py_grouped_linear),
     FGMS_METHOD("build_pyramid", py_build_pyramid), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

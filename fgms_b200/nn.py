@@ -16,7 +16,7 @@ import torch
 
 from . import _native, backend
 
-__all__ = ["sparse_conv", "sparse_conv_inference", "SparseConv3d", "SparseUNet"]
+__all__ = ["sparse_conv", "sparse_conv_inference", "SparseConv3d", "SparseUNet", "grouped_linear", "GroupedLinear"]
 
 
 def sparse_conv(feats: torch.Tensor, weight: torch.Tensor, kmap, arch80: bool = True) -> torch.Tensor:
@@ -63,6 +63,29 @@ class SparseConv3d(torch.nn.Module):
 
     def forward(self, feats: torch.Tensor, kmap) -> torch.Tensor:
         return sparse_conv(feats, self.weight, kmap, self.arch80)
+
+
+def grouped_linear(feats: torch.Tensor, weight: torch.Tensor, kpos: torch.Tensor) -> torch.Tensor:
+    """``out[r] = feats[r] @ weight[g]`` for the rows ``kpos[g] <= r < kpos[g + 1]`` of every group; differentiable in ``feats`` and
+    ``weight``.  Rows of no group (a buffer with room to spare) are zero in the output and in the gradient of ``feats``, whatever they
+    hold.  Rows in the order of their groups come from a stable sort by group: ``order = ids.argsort(stable=True)``,
+    ``kpos = torch.searchsorted(ids[order], torch.arange(groups + 1, device=...), out_int32=True)``."""
+    return _native.grouped_linear(feats, weight, kpos)
+
+
+class GroupedLinear(torch.nn.Module):
+    """One ``c_in -> c_out`` matrix for each of ``groups`` groups of rows (experts), a ``[groups, c_in, c_out]`` weight initialised like
+    ``torch.nn.Linear``; ``forward(feats, kpos)`` is :func:`grouped_linear`."""
+
+    def __init__(self, c_in: int, c_out: int, groups: int, dtype=torch.float16, device="cuda"):
+        super().__init__()
+        self.c_in, self.c_out, self.groups = c_in, c_out, groups
+        bound = 1.0 / math.sqrt(c_in)
+        w = (torch.rand((groups, c_in, c_out), device=device, dtype=torch.float32) * 2 - 1) * bound
+        self.weight = torch.nn.Parameter(w.to(dtype))
+
+    def forward(self, feats: torch.Tensor, kpos: torch.Tensor) -> torch.Tensor:
+        return grouped_linear(feats, self.weight, kpos)
 
 
 _LAYER_FORWARD = SparseConv3d.forward

@@ -51,6 +51,7 @@ extern "C" {
  * backend/spconv.cu:47-48) */
 #define FGMS_DTYPE_F32 0
 #define FGMS_DTYPE_F16 1
+#define FGMS_DTYPE_BF16 2 /* fgms_b200_grouped_* and fgms_b200_adamw only */
 
 /* arithmetic of the per-offset contraction.  Accumulation is always fp32.
  *   FP32 : CUDA-core FFMA on the stored values (fp16 storage is widened exactly) — the
@@ -260,6 +261,29 @@ int fgms_b200_build_neighbor_table(const int32_t* kpos, const int32_t* in_map, c
 int fgms_b200_fwd_output_stationary(const void* in_feats, const void* kernel, void* out_feats, const int32_t* nbr,
                                     int n_in, int n_out, int c_in, int c_out, int k_vol, int dtype, int math,
                                     const void* bias, int relu, int accumulate, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Products of ragged groups of rows with a weight matrix each: a layer of experts.  What the operator above does for the pairs of a
+ * map, without a map and without its limit of 256 channels: the rows of group g are the ones from kpos[g] up to kpos[g + 1], and
+ *
+ *     fwd     out[r]     = in[r] * W[g]                               in_feats [n_rows, c_in], kernel [groups, c_in, c_out]
+ *     dgrad   in_grad[r] = out_grad[r] * W[g]^T
+ *     wgrad   dW[g]      = sum over the rows of g of in[r]^T * out_grad[r]   (zeros for a group without rows)
+ *
+ * Outputs are OVERWRITTEN, each value rounded once from one fp32 accumulator: the same bits on every run.  Rows of no group (before
+ * kpos[0], from kpos[groups] on) are not read; they are left as they were, or become zeros with `zero_rest`.  dtype: F32 (exact fp32 on
+ * the CUDA cores), F16 or BF16 (tensor cores with fp32 accumulation).  Any channel counts; fp16 / bf16 rows that do not start on
+ * 16-byte boundaries (channel counts that are no multiples of 8, unaligned tensors) run on the CUDA cores, many times slower.
+ * kpos is device memory and is not trusted: entries are clamped to [0, n_rows], an entry smaller than one before it counts as equal to that,
+ * and every entry so changed is counted (fgms_b200_device_status).  An output must not overlap an input.
+ * No counterpart in the reference, whose operator multiplies every row by up to k_vol matrices. */
+#define FGMS_GROUPED_MAX_GROUPS 1024
+int fgms_b200_grouped_fwd(const void* in_feats, const void* kernel, void* out_feats, const int32_t* kpos, int n_rows,
+                          int c_in, int c_out, int groups, int dtype, int zero_rest, void* stream);
+int fgms_b200_grouped_dgrad(const void* out_grad, const void* kernel, void* in_grad, const int32_t* kpos, int n_rows,
+                            int c_in, int c_out, int groups, int dtype, int zero_rest, void* stream);
+int fgms_b200_grouped_wgrad(const void* in_feats, const void* out_grad, void* kernel_grad, const int32_t* kpos,
+                            int n_rows, int c_in, int c_out, int groups, int dtype, void* stream);
 
 /* ---------------------------------------------------------------------------------------------
  * Multi-GPU: sum of the ranks' fp32 weight-gradient partial sums over peer memory.  No counterpart in the

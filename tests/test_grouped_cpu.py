@@ -1,0 +1,67 @@
+"""What the grouped products refuse, before they touch a device."""
+import pytest
+import torch
+
+from fgms_b200 import _lib, backend, nn
+
+P = 1 << 20  # never dereferenced: validation fails first
+
+
+def fwd(x=P, w=2 * P, out=3 * P, kpos=4 * P, rows=10, c_in=8, c_out=8, groups=4, dtype=_lib.DTYPE_BF16):
+    return _lib.lib.fgms_b200_grouped_fwd(x, w, out, kpos, rows, c_in, c_out, groups, dtype, 0, None)
+
+
+@pytest.mark.parametrize("args,text", [
+    (dict(rows=-1), "negative row count"),
+    (dict(c_in=0), "channel counts"),
+    (dict(c_out=-3), "channel counts"),
+    (dict(groups=0), "groups 0 outside"),
+    (dict(groups=1025), "groups 1025 outside"),
+    (dict(groups=1024, c_in=1 << 21), "int32 range"),
+    (dict(groups=1024, c_out=1 << 21), "int32 range"),
+    (dict(dtype=3), "unknown dtype"),
+    (dict(dtype=-1), "unknown dtype"),
+    (dict(kpos=None), "null pointer"),
+    (dict(x=None), "null pointer"),
+    (dict(w=None), "null pointer"),
+    (dict(out=None), "null pointer"),
+    (dict(out=P + 16), "overlaps"),
+    (dict(out=2 * P + 8), "overlaps"),
+    (dict(out=4 * P - 2), "overlaps"),
+])
+def test_forward_refuses(args, text):
+    assert fwd(**args) == _lib.ERR_INVALID_ARG and text in _lib.last_error()
+
+
+def test_gradients_refuse():
+    L = _lib.lib
+    assert L.fgms_b200_grouped_dgrad(P, 2 * P, 2 * P, 4 * P, 10, 8, 8, 4, 1, 0, None) == _lib.ERR_INVALID_ARG and "overlaps" in _lib.last_error()
+    assert L.fgms_b200_grouped_dgrad(P, 2 * P, 3 * P, None, 10, 8, 8, 4, 1, 0, None) == _lib.ERR_INVALID_ARG
+    assert L.fgms_b200_grouped_wgrad(P, 2 * P, None, 4 * P, 10, 8, 8, 4, 1, None) == _lib.ERR_INVALID_ARG
+    assert L.fgms_b200_grouped_wgrad(P, 2 * P, 2 * P, 4 * P, 10, 8, 8, 4, 1, None) == _lib.ERR_INVALID_ARG and "overlaps" in _lib.last_error()
+    assert L.fgms_b200_grouped_wgrad(None, None, 3 * P, 4 * P, 10, 8, 8, 4, 1, None) == _lib.ERR_INVALID_ARG
+
+
+def test_nothing_to_write_is_no_error():
+    assert fwd(x=None, out=None, rows=0) == _lib.OK
+    assert _lib.lib.fgms_b200_grouped_dgrad(None, P, None, 2 * P, 0, 8, 8, 4, 0, 0, None) == _lib.OK
+
+
+def test_the_operator_of_a_map_still_refuses_bf16():
+    assert _lib.lib.fgms_b200_fusion_fwd(None, None, None, None, None, None, None, 0, 4, 4, 8, 8, 8, 27, 0, _lib.DTYPE_BF16, 0, 0, None) == _lib.ERR_INVALID_ARG
+
+
+def test_tensors_on_the_host_are_refused():
+    x, w, out, kpos = torch.zeros(4, 8), torch.zeros(2, 8, 16), torch.zeros(4, 16), torch.zeros(3, dtype=torch.int32)
+    with pytest.raises(ValueError, match="CUDA"):
+        backend.fgms_grouped_fwd_cuda(x, w, out, kpos)
+    with pytest.raises(ValueError, match="CUDA"):
+        backend.fgms_grouped_dgrad_cuda(out, w, x, kpos)
+    with pytest.raises(ValueError, match="CUDA"):
+        backend.fgms_grouped_wgrad_cuda(x, out, w, kpos)
+    with pytest.raises(ValueError, match="CUDA"):
+        nn.grouped_linear(x, w, kpos)
+    with pytest.raises(TypeError):
+        backend.fgms_grouped_fwd_cuda(None, w, out, kpos)
+    with pytest.raises(ValueError, match="int32"):
+        nn.grouped_linear(x, w, None)
