@@ -7,7 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import c_char_p, c_int, c_int64, c_size_t, c_void_p
+from ctypes import c_char_p, c_double, c_int, c_int64, c_size_t, c_void_p
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libfgms_b200.so")
@@ -16,6 +16,17 @@ OK = 0
 ERR_INVALID_ARG, ERR_CHANNEL_MISMATCH, ERR_UNSUPPORTED, ERR_CUDA, ERR_WORKSPACE, ERR_DEVICE = -1, -2, -3, -4, -5, -6
 DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
 MATH_FP32, MATH_TF32, MATH_F16 = 0, 1, 2
+
+class AdamwTensor(ctypes.Structure):
+    _fields_ = [("param", c_void_p), ("grad", c_void_p), ("master", c_void_p), ("exp_avg", c_void_p), ("exp_avg_sq", c_void_p),
+                ("exp_avg_scale", c_void_p), ("exp_avg_sq_scale", c_void_p), ("count", c_int64), ("param_dtype", c_int), ("grad_dtype", c_int)]
+
+
+class AdamwOptions(ctypes.Structure):
+    _fields_ = [("lr", c_double), ("beta1", c_double), ("beta2", c_double), ("eps", c_double), ("weight_decay", c_double),
+                ("lr_device", c_void_p), ("grad_scale", c_void_p), ("found_inf", c_void_p), ("step", c_void_p),
+                ("seed", ctypes.c_uint32), ("state_bits", c_int)]
+
 
 # name -> (restype, argtypes); mirrors include/fgms_b200.h declaration by declaration
 SIGNATURES = {
@@ -48,6 +59,7 @@ SIGNATURES = {
     "fgms_b200_grouped_fwd": (c_int, [c_void_p] * 4 + [c_int] * 6 + [c_void_p]),
     "fgms_b200_grouped_dgrad": (c_int, [c_void_p] * 4 + [c_int] * 6 + [c_void_p]),
     "fgms_b200_grouped_wgrad": (c_int, [c_void_p] * 4 + [c_int] * 5 + [c_void_p]),
+    "fgms_b200_adamw": (c_int, [c_void_p, c_int, c_void_p, c_void_p]),
     "fgms_b200_peer_exchange_flag_bytes": (c_size_t, [c_int]),
     "fgms_b200_peer_exchange": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int64, ctypes.c_uint32, c_int64, c_int, c_void_p]),
     "fgms_b200_kernel_family": (c_int, [c_int] * 6),

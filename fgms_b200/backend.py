@@ -32,7 +32,7 @@ from . import _lib, _native
 __all__ = ["fgms_fusion_fwd_cuda", "fgms_fwd_cuda", "fgms_bwd_cuda", "fgms_dgrad_cuda", "fgms_wgrad_cuda",
            "wgrad_workspace", "wgrad_finalize", "fgms_wgrad_noalloc_cuda", "kernel_family", "fallback_count",
            "device_status", "launch_count", "build_neighbor_table", "fgms_fwd_os_cuda", "fgms_grouped_fwd_cuda",
-           "fgms_grouped_dgrad_cuda", "fgms_grouped_wgrad_cuda"]
+           "fgms_grouped_dgrad_cuda", "fgms_grouped_wgrad_cuda", "fgms_adamw_cuda"]
 
 _L = _lib.lib
 
@@ -282,6 +282,24 @@ def fgms_grouped_wgrad_cuda(in_feats, out_feats_grad, kernel_grad, kpos):
     """Weight gradient of :func:`fgms_grouped_fwd_cuda`: ``kernel_grad[g] = in_feats[rows of g].T @ out_feats_grad[rows of g]``,
     zeros for a group without rows.  ``kernel_grad`` is overwritten."""
     _native.grouped_wgrad(in_feats, out_feats_grad, kernel_grad, kpos)
+
+
+def fgms_adamw_cuda(params, grads, exp_avgs, exp_avg_sqs, step, lr, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.01, masters=None,
+                    exp_avg_scales=None, exp_avg_sq_scales=None, seed=0, grad_scale=None, found_inf=None):
+    """One AdamW step over lists of tensors, in one launch for each 400 of them (``fgms_b200_adamw``).
+
+    ``params`` and ``grads`` are float32, float16 or bfloat16, each by itself; with ``masters`` (float32 tensors, or None for a parameter without
+    one) the step is taken on the master and the parameter is its rounded copy.  ``exp_avgs`` and ``exp_avg_sqs`` are float32, or
+    ``torch.float8_e4m3fn`` with ``exp_avg_scales`` / ``exp_avg_sq_scales``, a float32 value for each 128 of a tensor's
+    (``codes.float() * scale`` is the moment; all zeros before the first step); codes are rounded up or down at random (``seed``, the
+    step and the index decide), so that the moving averages keep their mean.
+
+    ``step`` is an int32 tensor ``[steps done, 0]`` on the device, counted up by the call, so that a captured graph can be replayed;
+    ``lr`` a number, or a float32 tensor of one value on the device, which a replayed graph follows.  Gradients are divided by ``grad_scale``;
+    where ``found_inf`` is not zero the step is neither taken nor counted (both: float32 tensors of one value, as
+    ``torch.amp.GradScaler`` has them).  :class:`fgms_b200.optim.AdamW` keeps all of this for a network."""
+    _native.adamw(params, grads, exp_avgs, exp_avg_sqs, step, lr, beta1, beta2, eps, weight_decay, masters, exp_avg_scales, exp_avg_sq_scales,
+                  seed, grad_scale, found_inf)
 
 
 def kernel_family(pass_: str, c_in: int, c_out: int, dtype: torch.dtype, arch80: bool = True, k_vol: int = 27) -> str:

@@ -5,11 +5,14 @@
 // and checks the launch status.
 #include "../../include/fgms_b200.h"
 
+#include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
 #include <cstdlib>
+#include <vector>
 
 #include <nvtx3/nvToolsExt.h>
 
@@ -26,6 +29,7 @@
 #include "peer_exchange.cuh"
 #include "umma_osfwd.cuh"
 #include "grouped_ffma.cuh"
+#include "adamw.cuh"
 
 namespace {
 
@@ -346,6 +350,117 @@ int run_grouped(const void* a, const void* b, void* d, const int32_t* kpos, int 
                                            : fgms::launch_grouped_ffma<__nv_bfloat16, PASS>(p, st, di.sms);
   if (rc != 0) return fail(FGMS_ERR_CUDA, "grouped_ffma_kernel: %s", cudaGetErrorString(cudaGetLastError()));
   return check_launch("grouped_ffma_kernel");
+}
+
+// AdamW over many tensors (csrc/adamw.cuh)
+int check_adamw(const fgms_b200_adamw_tensor* tensors, int n, const fgms_b200_adamw_options* o) {
+  if (n < 0) return fail(FGMS_ERR_INVALID_ARG, "negative number of tensors");
+  if (!o || (n > 0 && !tensors) || !o->step) return fail(FGMS_ERR_INVALID_ARG, "null pointer");
+  if (o->state_bits != 32 && o->state_bits != 8) return fail(FGMS_ERR_INVALID_ARG, "state_bits must be 32 or 8, got %d", o->state_bits);
+  const auto in = [](double x, double lo, double hi) { return x >= lo && x < hi; };  // false for a NaN
+  if (!in(o->beta1, 0, 1) || !in(o->beta2, 0, 1)) return fail(FGMS_ERR_INVALID_ARG, "betas must be in [0, 1)");
+  if (!in(o->lr, 0, HUGE_VAL) || !in(o->weight_decay, 0, HUGE_VAL)) return fail(FGMS_ERR_INVALID_ARG, "lr and weight_decay must be finite and not negative");
+  if (!in(o->eps, 1e-37, HUGE_VAL)) return fail(FGMS_ERR_INVALID_ARG, "eps must be finite and at least 1e-37: a second moment of 0 is divided by it");
+  if ((reinterpret_cast<uintptr_t>(o->step) | reinterpret_cast<uintptr_t>(o->lr_device) | reinterpret_cast<uintptr_t>(o->grad_scale) |
+       reinterpret_cast<uintptr_t>(o->found_inf)) & 3)
+    return fail(FGMS_ERR_INVALID_ARG, "step, lr, grad_scale and found_inf must be 4-byte aligned");
+  struct Used { uintptr_t from, to; bool written; };
+  std::vector<Used> used;
+  used.reserve((size_t)n * 7 + 4);
+  const auto add = [&](const void* p, size_t bytes, bool written) {
+    if (p && bytes > 0) used.push_back({reinterpret_cast<uintptr_t>(p), reinterpret_cast<uintptr_t>(p) + bytes, written});
+  };
+  add(o->step, 8, true);
+  add(o->lr_device, 4, false);
+  add(o->grad_scale, 4, false);
+  add(o->found_inf, 4, false);
+  for (int i = 0; i < n; ++i) {
+    const fgms_b200_adamw_tensor& t = tensors[i];
+    if (t.count < 0 || t.count > (1ll << 40)) return fail(FGMS_ERR_INVALID_ARG, "tensor %d: count outside [0, 2^40]", i);
+    for (int dtype : {t.param_dtype, t.grad_dtype})
+      if (!dtype_ok(dtype) && dtype != FGMS_DTYPE_BF16) return fail(FGMS_ERR_INVALID_ARG, "tensor %d: unknown dtype %d", i, dtype);
+    if (t.count == 0) continue;
+    if (!t.param || !t.grad || !t.exp_avg || !t.exp_avg_sq || (o->state_bits == 8 && (!t.exp_avg_scale || !t.exp_avg_sq_scale)))
+      return fail(FGMS_ERR_INVALID_ARG, "tensor %d: null pointer", i);
+    const size_t count = (size_t)t.count, ps = t.param_dtype == FGMS_DTYPE_F32 ? 4 : 2, gs = t.grad_dtype == FGMS_DTYPE_F32 ? 4 : 2;
+    const size_t ms = o->state_bits == 8 ? 1 : 4, blocks = (count + fgms::ADAMW_BLOCK - 1) / fgms::ADAMW_BLOCK;
+    const uintptr_t words = reinterpret_cast<uintptr_t>(t.master) | (ps == 4 ? reinterpret_cast<uintptr_t>(t.param) : 0) |
+                            (gs == 4 ? reinterpret_cast<uintptr_t>(t.grad) : 0) |
+                            (ms == 4 ? reinterpret_cast<uintptr_t>(t.exp_avg) | reinterpret_cast<uintptr_t>(t.exp_avg_sq)
+                                     : reinterpret_cast<uintptr_t>(t.exp_avg_scale) | reinterpret_cast<uintptr_t>(t.exp_avg_sq_scale));
+    if ((words & 3) || ((reinterpret_cast<uintptr_t>(t.param) | reinterpret_cast<uintptr_t>(t.grad)) & 1))
+      return fail(FGMS_ERR_INVALID_ARG, "tensor %d: a pointer is not on a boundary of its type", i);
+    add(t.param, count * ps, true);
+    add(t.grad, count * gs, false);
+    add(t.master, count * 4, true);
+    add(t.exp_avg, count * ms, true);
+    add(t.exp_avg_sq, count * ms, true);
+    if (ms == 1) {
+      add(t.exp_avg_scale, blocks * 4, true);
+      add(t.exp_avg_sq_scale, blocks * 4, true);
+    }
+  }
+  std::sort(used.begin(), used.end(), [](const Used& a, const Used& b) { return a.from < b.from; });
+  uintptr_t any = 0, written = 0;  // where what lies before ends
+  for (const Used& u : used) {
+    if (u.from < (u.written ? any : written)) return fail(FGMS_ERR_INVALID_ARG, "a buffer that is written overlaps another one: is a tensor in the list twice?");
+    any = std::max(any, u.to);
+    if (u.written) written = std::max(written, u.to);
+  }
+  return FGMS_OK;
+}
+
+template <bool EIGHT, int N>
+int launch_adamw(const fgms_b200_adamw_tensor* tensors, int n, const fgms_b200_adamw_options& o, bool last, int sms, cudaStream_t st) {
+  static thread_local fgms::AdamwParams<N> p;  // 32 KB: not on the stack of a thread that may have little of it
+  p.lr = o.lr; p.beta1 = o.beta1; p.beta2 = o.beta2; p.decay = o.weight_decay;
+  p.b1 = (float)o.beta1; p.c1 = (float)(1.0 - o.beta1);
+  p.b2 = (float)o.beta2; p.c2 = (float)(1.0 - o.beta2);
+  p.eps = (float)o.eps;
+  p.seed = o.seed;
+  p.lr_device = o.lr_device; p.grad_scale = o.grad_scale; p.found_inf = o.found_inf;
+  p.step = o.step;
+  p.n = n; p.last = last;
+  long long chunks = 0;
+  for (int i = 0; i < n; ++i) {
+    const fgms_b200_adamw_tensor& t = tensors[i];
+    fgms::AdamwTensor& d = p.t[i];
+    d.param = t.param; d.grad = t.grad; d.master = t.master; d.m = t.exp_avg; d.v = t.exp_avg_sq;
+    d.m_scale = t.exp_avg_scale; d.v_scale = t.exp_avg_sq_scale;
+    d.count = t.count;
+    d.first_chunk = (int)chunks;
+    d.param_type = (uint8_t)t.param_dtype; d.grad_type = (uint8_t)t.grad_dtype;
+    const uintptr_t wide = reinterpret_cast<uintptr_t>(t.param) | reinterpret_cast<uintptr_t>(t.grad) | reinterpret_cast<uintptr_t>(t.master);
+    const uintptr_t moments = reinterpret_cast<uintptr_t>(t.exp_avg) | reinterpret_cast<uintptr_t>(t.exp_avg_sq);
+    d.aligned = (wide & 15) == 0 && (moments & (EIGHT ? 7 : 15)) == 0;
+    d.pad = 0;
+    chunks += (t.count + fgms::ADAMW_CHUNK - 1) / fgms::ADAMW_CHUNK;
+    if (chunks > 0x7fffffffll - 65536) return fail(FGMS_ERR_INVALID_ARG, "too many values in one call");
+  }
+  p.chunks = (int)chunks;
+  const long long most = 4ll * sms, grid = chunks < 1 ? 1 : chunks < most ? chunks : most;
+  if (fgms::launch_pdl(fgms::adamw_kernel<EIGHT, N>, dim3((unsigned)grid), fgms::ADAMW_THREADS, 0, st, p) != cudaSuccess)
+    return fail(FGMS_ERR_CUDA, "adamw_kernel: %s", cudaGetErrorString(cudaGetLastError()));
+  return check_launch("adamw_kernel");
+}
+
+int run_adamw(const fgms_b200_adamw_tensor* tensors, int n, const fgms_b200_adamw_options* o, cudaStream_t st) {
+  if (int rc = check_adamw(tensors, n, o)) return rc;
+  DeviceInfo di;
+  if (int rc = device_info(&di)) return rc;
+  for (int at = 0;;) {
+    const int left = n - at, now = left < fgms::ADAMW_MANY ? left : fgms::ADAMW_MANY;
+    const bool last = now == left;
+    int rc;
+    if (o->state_bits == 8)
+      rc = now <= fgms::ADAMW_FEW ? launch_adamw<true, fgms::ADAMW_FEW>(tensors + at, now, *o, last, di.sms, st)
+                                  : launch_adamw<true, fgms::ADAMW_MANY>(tensors + at, now, *o, last, di.sms, st);
+    else
+      rc = now <= fgms::ADAMW_FEW ? launch_adamw<false, fgms::ADAMW_FEW>(tensors + at, now, *o, last, di.sms, st)
+                                  : launch_adamw<false, fgms::ADAMW_MANY>(tensors + at, now, *o, last, di.sms, st);
+    if (rc != FGMS_OK || last) return rc;
+    at += now;
+  }
 }
 }  // namespace
 
@@ -965,6 +1080,15 @@ int fgms_b200_grouped_wgrad(const void* in_feats, const void* out_grad, void* ke
                             int groups, int dtype, void* stream) {
   TraceRange trace_range("fgms_b200_grouped_wgrad");
   return run_grouped<fgms::GROUPED_WGRAD>(in_feats, out_grad, kernel_grad, kpos, n_rows, c_in, c_out, groups, dtype, 0, stream);
+}
+
+int fgms_b200_adamw(const fgms_b200_adamw_tensor* tensors, int n, const fgms_b200_adamw_options* options, void* stream) {
+  TraceRange trace_range("fgms_b200_adamw");
+  try {
+    return run_adamw(tensors, n, options, static_cast<cudaStream_t>(stream));
+  } catch (const std::exception& e) {  // no memory for the list of buffers
+    return fail(FGMS_ERR_CUDA, "fgms_b200_adamw: %s", e.what());
+  }
 }
 
 int64_t fgms_b200_device_status(int reset) {

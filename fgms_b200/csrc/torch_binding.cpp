@@ -727,6 +727,92 @@ struct GroupedLinear : torch::autograd::Function<GroupedLinear> {
 };
 
 // ---------------------------------------------------------------------------------------------
+// AdamW over many tensors
+// ---------------------------------------------------------------------------------------------
+int adamw_dtype(const char* name, const Tensor& t) {
+  if (t.scalar_type() == at::kHalf) return FGMS_DTYPE_F16;
+  if (t.scalar_type() == at::kBFloat16) return FGMS_DTYPE_BF16;
+  TORCH_CHECK_VALUE(t.scalar_type() == at::kFloat, "unsupported ", name, " dtype ", t.scalar_type(), ": float16, bfloat16 or float32");
+  return FGMS_DTYPE_F32;
+}
+
+struct AdamwLists {
+  std::vector<Tensor> params, grads, exp_avgs, exp_avg_sqs, masters, exp_avg_scales, exp_avg_sq_scales;  // masters: undefined where there is none
+};
+
+// autograd notices that a tensor it has saved was written
+void written(const Tensor& t) {
+  if (t.defined() && !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
+void adamw(const AdamwLists& a, const Tensor& step, const Tensor& lr_tensor, const Tensor& grad_scale, const Tensor& found_inf, fgms_b200_adamw_options o) {
+  const size_t n = a.params.size();
+  TORCH_CHECK_VALUE(step.is_cuda() && step.scalar_type() == at::kInt && step.numel() == 2 && step.is_contiguous(),
+                    "step must be a contiguous int32 CUDA tensor of two entries: the steps done, and 0");
+  const auto device = step.device();
+  auto one = [&](const char* name, const Tensor& t) -> const float* {
+    if (!t.defined()) return nullptr;
+    TORCH_CHECK_VALUE(t.device() == device && t.scalar_type() == at::kFloat && t.numel() == 1, name, " must be one float32 value on ", device);
+    return t.data_ptr<float>();
+  };
+  o.lr_device = one("lr", lr_tensor);
+  o.grad_scale = one("grad_scale", grad_scale);
+  o.found_inf = one("found_inf", found_inf);
+  o.step = step.data_ptr<int32_t>();
+  const bool eight = !a.exp_avg_scales.empty() || !a.exp_avg_sq_scales.empty() || (n > 0 && a.exp_avgs.size() == n && a.exp_avgs[0].scalar_type() == at::kFloat8_e4m3fn);
+  o.state_bits = eight ? 8 : 32;
+  auto length = [&](const char* name, size_t got) { TORCH_CHECK_VALUE(got == n, name, " has ", got, " tensors, params ", n); };
+  length("grads", a.grads.size());
+  length("exp_avgs", a.exp_avgs.size());
+  length("exp_avg_sqs", a.exp_avg_sqs.size());
+  if (!a.masters.empty()) length("masters", a.masters.size());
+  if (eight) {
+    length("exp_avg_scales", a.exp_avg_scales.size());
+    length("exp_avg_sq_scales", a.exp_avg_sq_scales.size());
+  }
+  std::vector<fgms_b200_adamw_tensor> list(n);
+  for (size_t i = 0; i < n; ++i) {
+    const Tensor& p = a.params[i];
+    auto check = [&](const char* name, const Tensor& t, int64_t count, at::ScalarType type) {
+      TORCH_CHECK_VALUE(t.device() == device, name, " ", i, " must live on ", device, ", got ", t.device());
+      TORCH_CHECK_VALUE(t.is_contiguous(), name, " ", i, " must be contiguous");
+      TORCH_CHECK_VALUE(t.numel() == count, name, " ", i, " must have ", count, " values, got ", t.numel());
+      TORCH_CHECK_VALUE(t.scalar_type() == type, name, " ", i, " must have dtype ", type, ", got ", t.scalar_type());
+    };
+    const int64_t count = p.numel(), blocks = (count + 127) / 128;
+    const at::ScalarType moment = eight ? at::kFloat8_e4m3fn : at::kFloat;
+    check("param", p, count, p.scalar_type());
+    check("grad", a.grads[i], count, a.grads[i].scalar_type());
+    check("exp_avg", a.exp_avgs[i], count, moment);
+    check("exp_avg_sq", a.exp_avg_sqs[i], count, moment);
+    fgms_b200_adamw_tensor& t = list[i];
+    t = {};
+    t.count = count;
+    t.param = ptr(p);
+    t.grad = ptr(a.grads[i]);
+    t.exp_avg = ptr(a.exp_avgs[i]);
+    t.exp_avg_sq = ptr(a.exp_avg_sqs[i]);
+    t.param_dtype = adamw_dtype("parameter", p);
+    t.grad_dtype = adamw_dtype("gradient", a.grads[i]);
+    if (!a.masters.empty() && a.masters[i].defined()) {
+      check("master", a.masters[i], count, at::kFloat);
+      t.master = static_cast<float*>(ptr(a.masters[i]));
+    }
+    if (eight) {
+      check("exp_avg_scale", a.exp_avg_scales[i], blocks, at::kFloat);
+      check("exp_avg_sq_scale", a.exp_avg_sq_scales[i], blocks, at::kFloat);
+      t.exp_avg_scale = static_cast<float*>(ptr(a.exp_avg_scales[i]));
+      t.exp_avg_sq_scale = static_cast<float*>(ptr(a.exp_avg_sq_scales[i]));
+    }
+  }
+  c10::cuda::CUDAGuard guard(device);
+  check_status(fgms_b200_adamw(list.data(), (int)n, &o, stream_of(step)));
+  written(step);
+  for (const auto* tensors : {&a.params, &a.exp_avgs, &a.exp_avg_sqs, &a.masters, &a.exp_avg_scales, &a.exp_avg_sq_scales})
+    for (const Tensor& t : *tensors) written(t);
+}
+
+// ---------------------------------------------------------------------------------------------
 // Python entry points (positional arguments only; the functions of backend.py / nn.py give them their names)
 // ---------------------------------------------------------------------------------------------
 const Tensor& feat_arg(PyObject* o, const char* name) {
@@ -793,20 +879,66 @@ PyObject* py_sparse_conv(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return THPVariable_Wrap(SparseConv::apply(feats, weight, kpos, imap, omap, int_arg(a[5]), bool_arg(a[6])));
   END_HANDLE_TH_ERRORS
 }
+std::vector<Tensor> tensor_list(PyObject* list, const char* name, bool gaps = false) {
+  TORCH_CHECK_TYPE(PyList_Check(list) || PyTuple_Check(list), name, " must be a list of tensors");
+  const Py_ssize_t n = PySequence_Fast_GET_SIZE(list);
+  std::vector<Tensor> out;
+  out.reserve(n);
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    PyObject* o = PySequence_Fast_GET_ITEM(list, i);
+    if (gaps && o == Py_None) out.emplace_back();
+    else out.push_back(feat_arg(o, name));
+  }
+  return out;
+}
+double double_arg(PyObject* o) {
+  const double v = PyFloat_AsDouble(o);
+  if (v == -1.0 && PyErr_Occurred()) throw python_error();
+  return v;
+}
+
+// (params, grads, exp_avgs, exp_avg_sqs, step, lr, beta1, beta2, eps, weight_decay, masters, exp_avg_scales, exp_avg_sq_scales, seed, grad_scale, found_inf)
+PyObject* py_adamw(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  expect(n, 16);
+  AdamwLists lists;
+  lists.params = tensor_list(a[0], "params");
+  lists.grads = tensor_list(a[1], "grads");
+  lists.exp_avgs = tensor_list(a[2], "exp_avgs");
+  lists.exp_avg_sqs = tensor_list(a[3], "exp_avg_sqs");
+  if (a[10] != Py_None) lists.masters = tensor_list(a[10], "masters", true);
+  if (a[11] != Py_None) lists.exp_avg_scales = tensor_list(a[11], "exp_avg_scales");
+  if (a[12] != Py_None) lists.exp_avg_sq_scales = tensor_list(a[12], "exp_avg_sq_scales");
+  fgms_b200_adamw_options o = {};
+  Tensor lr_tensor;
+  if (THPVariable_Check(a[5])) lr_tensor = THPVariable_Unpack(a[5]);
+  if (lr_tensor.defined() && !lr_tensor.is_cuda()) {
+    TORCH_CHECK_VALUE(lr_tensor.numel() == 1, "lr must be one value");
+    o.lr = lr_tensor.item<double>();
+    lr_tensor = Tensor();
+  } else if (!lr_tensor.defined()) {
+    o.lr = double_arg(a[5]);
+  }
+  o.beta1 = double_arg(a[6]);
+  o.beta2 = double_arg(a[7]);
+  o.eps = double_arg(a[8]);
+  o.weight_decay = double_arg(a[9]);
+  const int64_t seed = int_arg(a[13]);
+  TORCH_CHECK_VALUE(seed >= 0 && seed <= 0xffffffffll, "seed must be in [0, 2^32)");
+  o.seed = (uint32_t)seed;
+  auto maybe = [](PyObject* t, const char* name) { return t == Py_None ? Tensor() : feat_arg(t, name); };
+  adamw(lists, feat_arg(a[4], "step"), lr_tensor, maybe(a[14], "grad_scale"), maybe(a[15], "found_inf"), o);
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
 // (in_feats, [kernels], [kpos, in_map, out_map of every map], [src, skip, map, n_in, n_out of every layer], arch80) -> the last layer's
 // output, or None where the layers are to be run one by one
 PyObject* py_sparse_stack(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   expect(n, 5);
   const Tensor& feats = feat_arg(a[0], "in_feats");
-  auto tensors = [](PyObject* list, const char* name) {
-    TORCH_CHECK_TYPE(PyList_Check(list), name, " must be a list");
-    std::vector<Tensor> out;
-    out.reserve(PyList_GET_SIZE(list));
-    for (Py_ssize_t i = 0; i < PyList_GET_SIZE(list); ++i) out.push_back(feat_arg(PyList_GET_ITEM(list, i), name));
-    return out;
-  };
-  const std::vector<Tensor> weights = tensors(a[1], "kernels"), maps = tensors(a[2], "maps");
+  const std::vector<Tensor> weights = tensor_list(a[1], "kernels"), maps = tensor_list(a[2], "maps");
   TORCH_CHECK_TYPE(PyList_Check(a[3]), "plan must be a list");
   StackPlan plan;
   for (Py_ssize_t i = 0; i < PyList_GET_SIZE(a[3]); ++i) plan.push_back(int_arg(PyList_GET_ITEM(a[3], i)));
@@ -886,6 +1018,7 @@ PyMethodDef methods[] = {
     FGMS_METHOD("wgrad_fp32_sums", py_wgrad_fp32_sums),
     FGMS_METHOD("grouped_fwd", py_grouped_fwd), FGMS_METHOD("grouped_dgrad", py_grouped_dgrad),
     FGMS_METHOD("grouped_wgrad", py_grouped_wgrad), FGMS_METHOD("grouped_linear", py_grouped_linear),
+    FGMS_METHOD("adamw", py_adamw),
     FGMS_METHOD("build_pyramid", py_build_pyramid), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -286,6 +286,45 @@ int fgms_b200_grouped_wgrad(const void* in_feats, const void* out_grad, void* ke
                             int n_rows, int c_in, int c_out, int groups, int dtype, void* stream);
 
 /* ---------------------------------------------------------------------------------------------
+ * One AdamW step over many tensors, in one launch for each 400 of them.  With t = step[0] + 1:
+ *
+ *     g = grad / grad_scale        m = beta1 m + (1 - beta1) g        v = beta2 v + (1 - beta2) g^2
+ *     w = w (1 - lr weight_decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ *
+ * in fp32, where w is the fp32 `master` of a tensor that has one, else the parameter; the parameter becomes w rounded once.
+ * state_bits 32: exp_avg and exp_avg_sq are fp32.  state_bits 8: both are e4m3 codes (one byte each) with an fp32 scale for each 128
+ * values, ceil(count / 128) of them, code * scale being the value; a value is rounded up with the probability of the part that is cut off (random bits: a
+ * hash of seed, t and the value's index), so that a moving average keeps its mean, and an exp_avg_sq above zero stays above zero.  A gradient
+ * that is not finite makes its block of 128 NaN from then on, as it makes its own moments NaN with 32 bits.
+ * All zeros are the state before the first step.  Parameters and gradients: F32, F16 or BF16, each by itself.  Any alignment.
+ * No buffer that is written may overlap another one (FGMS_ERR_INVALID_ARG): a tensor cannot be in the list twice. */
+typedef struct {
+  void* param;
+  const void* grad;
+  float* master; /* or NULL */
+  void* exp_avg;
+  void* exp_avg_sq;
+  float* exp_avg_scale;    /* state_bits 8 only */
+  float* exp_avg_sq_scale; /* state_bits 8 only */
+  int64_t count;
+  int param_dtype;
+  int grad_dtype;
+} fgms_b200_adamw_tensor;
+
+typedef struct {
+  double lr, beta1, beta2, eps, weight_decay;
+  const float* lr_device;  /* or NULL: one value in device memory that stands for lr (a replayed graph follows it) */
+  const float* grad_scale; /* or NULL: one value in device memory */
+  const float* found_inf;  /* or NULL: one value in device memory; where it is not 0 the step is neither taken nor counted */
+  int32_t* step;           /* device, two entries: the steps done so far, counted up by the call; and 0 */
+  uint32_t seed;
+  int state_bits;
+} fgms_b200_adamw_options;
+
+/* `tensors` (of `n`) and `options` are host memory, read before the call returns. */
+int fgms_b200_adamw(const fgms_b200_adamw_tensor* tensors, int n, const fgms_b200_adamw_options* options, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
  * Multi-GPU: sum of the ranks' fp32 weight-gradient partial sums over peer memory.  No counterpart in the
  * reference (it has no multi-GPU path); it stands where a data-parallel caller would otherwise issue an
  * all-reduce of the [k_vol, c_in, c_out] fp32 sums that fgms_b200_wgrad leaves in its workspace.
