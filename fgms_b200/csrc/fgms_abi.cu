@@ -29,6 +29,7 @@
 #include "peer_exchange.cuh"
 #include "umma_osfwd.cuh"
 #include "grouped_ffma.cuh"
+#include "grouped_umma.cuh"
 #include "adamw.cuh"
 
 namespace {
@@ -345,6 +346,15 @@ int run_grouped(const void* a, const void* b, void* d, const int32_t* kpos, int 
   if (int rc = device_info(&di)) return rc;
   const fgms::GroupedParams p{a, b, d, kpos, n_rows, c_in, c_out, groups, zero_rest, di.reserved > 0};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  bool tensor_cores = false;
+  if (dtype != FGMS_DTYPE_F32) {
+    if (fgms::grouped_umma_takes(p, &tensor_cores)) {
+      if (fgms::launch_grouped_umma<PASS>(p, dtype == FGMS_DTYPE_BF16, st, di.sms, di.max_smem_optin) != 0)
+        return fail(FGMS_ERR_CUDA, "grouped_umma_kernel: %s", cudaGetErrorString(cudaGetLastError()));
+      return check_launch("grouped_umma_kernel");
+    }
+    if (tensor_cores) g_fallbacks.fetch_add(1, std::memory_order_relaxed);  // pointers not 16-byte aligned: CUDA-core path, counted
+  }
   const int rc = dtype == FGMS_DTYPE_F32   ? fgms::launch_grouped_ffma<float, PASS>(p, st, di.sms)
                  : dtype == FGMS_DTYPE_F16 ? fgms::launch_grouped_ffma<__half, PASS>(p, st, di.sms)
                                            : fgms::launch_grouped_ffma<__nv_bfloat16, PASS>(p, st, di.sms);

@@ -292,6 +292,17 @@ __host__ __device__ constexpr uint32_t mnmajor32_offset(uint32_t k, uint32_t byt
 
 }  // namespace umma
 
+// The driver's encoder of tensor maps, or null; one that was not found is looked up again by the next call.
+inline void* tensor_map_encoder() {
+  static std::atomic<void*> known{nullptr};
+  void* fn = known.load(std::memory_order_acquire);
+  if (fn != nullptr) return fn;
+  cudaDriverEntryPointQueryResult found = cudaDriverEntryPointSymbolNotFound;
+  if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess) return nullptr;
+  known.store(fn, std::memory_order_release);
+  return fn;
+}
+
 // Tensor map over weights [k_vol, c_in, c_out] whose box is `box_rows` rows of one 128-byte column block (0: all c_in of a matrix): what tma_load_2d writes, block after block box_rows * 128 bytes apart, is the 128-byte-swizzled operand: MN-major (forward: rows = contraction index) or
 // K-major (input gradient: rows = output index), which differ only for 32-bit elements.  Columns beyond c_out come as zeros.
 // Made for every call (42 ns): nothing is kept by an address.  The encoder wants a context, which a host thread has after its first
@@ -300,16 +311,8 @@ __host__ __device__ constexpr uint32_t mnmajor32_offset(uint32_t k, uint32_t byt
 inline int weight_tensor_map(CUtensorMap* map, const void* weights, int k_vol, int c_in, int c_out, bool f16, bool mn_major, int box_rows = 0) {
   using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                               const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-  static std::atomic<Encode> known{nullptr};
-  Encode encode = known.load(std::memory_order_acquire);
-  if (encode == nullptr) {
-    void* fn = nullptr;
-    cudaDriverEntryPointQueryResult found = cudaDriverEntryPointSymbolNotFound;
-    const cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &found);
-    if (e != cudaSuccess || found != cudaDriverEntryPointSuccess || fn == nullptr) return -1000 - (int)CUDA_ERROR_NOT_FOUND;
-    encode = reinterpret_cast<Encode>(fn);
-    known.store(encode, std::memory_order_release);
-  }
+  const Encode encode = reinterpret_cast<Encode>(tensor_map_encoder());
+  if (encode == nullptr) return -1000 - (int)CUDA_ERROR_NOT_FOUND;
   const int es = f16 ? 2 : 4;
   const cuuint64_t dims[2] = {(cuuint64_t)c_out, (cuuint64_t)k_vol * c_in}, pitch[1] = {(cuuint64_t)c_out * es};
   const cuuint32_t box[2] = {(cuuint32_t)(128 / es), (cuuint32_t)(box_rows > 0 ? box_rows : c_in)}, steps[2] = {1, 1};
