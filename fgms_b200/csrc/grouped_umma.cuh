@@ -16,7 +16,7 @@
 //   warp 1      MMA issuer (of the pair's even CTA)
 //   warp 2      weight gradient: the rows behind a group's last one in its last stage are the next group's; they are cleared in
 //               shared memory between the copy and the MMA
-//   warps 4-7   epilogue: tcgen05.ld, neighbouring lanes exchange halves of two rows so that each stores two channels
+//   warps 4-11  epilogue: tcgen05.ld in the shape of MMA fragments, a transposition through shared memory (stmatrix), 16-byte stores along the rows
 //
 // Two accumulators in tensor memory: the epilogue of a tile runs beside the next one's MMAs.  All waits are bounded; a wait that runs out sets the
 // CTA's abort flag and is counted.
@@ -26,9 +26,11 @@
 namespace fgms {
 
 constexpr int GU_K = 64;  // contraction length of a stage: 128 bytes
-constexpr int GU_THREADS = 256;
+constexpr int GU_EPI_WARP0 = 4, GU_EPI_WARPS = 8;
+constexpr int GU_THREADS = (GU_EPI_WARP0 + GU_EPI_WARPS) * 32;
 constexpr int GU_MAX_STAGES = 12;
 constexpr int GU_A_BYTES = 128 * GU_K * 2;
+constexpr int GU_PATCH_BYTES = 32 * 128 * 2;  // of four epilogue warps
 
 struct GuShared {
   uint64_t full[GU_MAX_STAGES];    // of the even CTA: both CTAs' halves of the stage are there
@@ -43,6 +45,7 @@ struct GuShared {
 constexpr int GU_SHARED_BYTES = (sizeof(GuShared) + 15) & ~15;
 
 struct GuConfig {
+  int parts;        // CTAs that share a tile's contraction (SPLIT), 1 otherwise
   int tile_n;       // rows (weight gradient: input channels) of a tile at most: a multiple of 16 CG, at most 256
   int stages;
   int stage_bytes;  // of a CTA: a multiple of 1024
@@ -94,22 +97,23 @@ __device__ __forceinline__ uint32_t at_leader(uint32_t addr) {
   asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
   return r;
 }
-// arrivals at a barrier of either CTA of the pair
-__device__ __forceinline__ void pair_arrive(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
-}
+// Arrivals at a barrier of either CTA of the pair.  No write to memory that the other CTA's threads read goes with them: the accumulator has been
+// read, a copy will report its bytes, rows of this CTA's own memory have been cleared and fenced for the tensor cores.  So they do not
+// release at cluster scope, which waits until all earlier copies and stores of the thread have been performed: 1300 cycles a stage
+// in the producer, as much as the whole product takes without (2048 -> 4096 on 8192 rows 194 us, so 112).
+__device__ __forceinline__ void pair_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
 __device__ __forceinline__ void pair_expect(uint32_t bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.release.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+  asm volatile("mbarrier.arrive.expect_tx.shared::cluster.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ bool pair_test(uint32_t bar, uint32_t parity) {
   uint32_t ok;
-  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
                : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
   return ok != 0;
 }
 __device__ __forceinline__ bool pair_park(uint32_t bar, uint32_t parity) {
   uint32_t ok;
-  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
                : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
   return ok != 0;
 }
@@ -151,57 +155,108 @@ __device__ __forceinline__ void pair_load_3d(uint32_t dst, const CUtensorMap* ma
                  "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z)
                  : "memory");
 }
+// 16 lanes by 32 consecutive columns, as four fragments of 16 x 8: thread t has lanes t / 4 and t / 4 + 8, columns 2 (t % 4) and the next
+__device__ __forceinline__ void tmem_ld_16x8x4(uint32_t taddr, uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+        "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+      : "r"(taddr)
+      : "memory");
+}
+// Four warps of the epilogue meet.  Every one of them comes: the waits before are bounded, and whether they go on is decided together.
+__device__ __forceinline__ void four_sync(int half) { asm volatile("barrier.cta.sync %0, 128;" ::"r"(1 + half) : "memory"); }
+__device__ __forceinline__ bool four_agree(int half, bool ok) {
+  uint32_t all;
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.and.pred q, %2, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+               : "=r"(all) : "r"((uint32_t)ok), "r"(1 + half) : "memory");
+  return all != 0;
+}
+__device__ __forceinline__ void cluster_sync() { asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory"); }
+// a word to this CTA's address `addr` in CTA `to` of the cluster
+__device__ __forceinline__ void put_at(int to, uint32_t addr, uint32_t value) {
+  asm volatile("{\n\t.reg .b32 there;\n\tmapa.shared::cluster.u32 there, %0, %1;\n\tst.shared::cluster.b32 [there], %2;\n\t}" ::"r"(addr), "r"(to), "r"(value) : "memory");
+}
 template <int CG>
 __device__ __forceinline__ void pair_sync() {
   if (CG == 1) __syncthreads();
-  else asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+  else cluster_sync();
 }
 }  // namespace umma
 
-// What a tile is: the same for every role.
-struct GuTile {
+// The tiles of a pair, one after the other: the same walk in every role.  Steps are added up, without a division a tile: those of 64-bit numbers
+// and the search for the group took the epilogue of a short tile as long as its stores.
+template <int PASS, int CG, bool SPLIT>
+struct GuTiles {
   int g, m0, n0, n, n_mma;  // group; first channel (of the pair); first row or column; how many; the same as the MMA takes it
   int k0, k_len;            // weight gradient: the group's first row and how many; otherwise 0 and the channels of the contraction
-};
-template <int PASS, int CG>
-struct GuTiles {
+  int blocks, b0, b1;       // stages of the contraction; those of this CTA
   const int *first, *tiles;
-  int groups, tile_n, m_tiles, n_tiles, c_k, c_in;
-  long long total;
-  __device__ __forceinline__ GuTiles(const GroupedParams& p, int tile_n_, const int* first_, const int* tiles_)
-      : first(first_), tiles(tiles_), groups(p.groups), tile_n(tile_n_), c_in(p.c_in) {
+  int left, step_m, step_q, m, q, m_tiles;  // q: row tile, or of the weight gradient tile of input channels
+  int tile_n, c_in, step_g, n_tiles, share, parts;
+  __device__ __forceinline__ GuTiles(const GroupedParams& p, const GuConfig& cfg, const int* first_, const int* tiles_)
+      : first(first_), tiles(tiles_), tile_n(cfg.tile_n), c_in(p.c_in), parts(cfg.parts) {
     const int channels = PASS == GROUPED_DGRAD ? p.c_in : p.c_out;
-    c_k = PASS == GROUPED_DGRAD ? p.c_out : p.c_in;
+    const int ctas = SPLIT ? parts : CG, at = (int)blockIdx.x / ctas, step = (int)gridDim.x / ctas;
     m_tiles = (channels + 128 * CG - 1) / (128 * CG);
     n_tiles = (p.c_in + tile_n - 1) / tile_n;
-    total = PASS == GROUPED_WGRAD ? (long long)groups * n_tiles * m_tiles : (long long)tiles[groups] * m_tiles;
-  }
-  __device__ __forceinline__ GuTile at(long long t) const {
-    GuTile r;
-    const int q = (int)(t / m_tiles);
-    r.m0 = (int)(t - (long long)q * m_tiles) * (128 * CG);
+    const int total = (PASS == GROUPED_WGRAD ? p.groups * n_tiles : tiles[p.groups]) * m_tiles;  // the launch sees to it that this is an int
+    left = at < total ? (total - 1 - at) / step + 1 : 0;
+    q = at / m_tiles;
+    m = at - q * m_tiles;
+    step_q = step / m_tiles;
+    step_m = step - step_q * m_tiles;
+    g = share = 0;
     if (PASS == GROUPED_WGRAD) {
-      r.g = q / n_tiles;
-      r.n0 = (q - r.g * n_tiles) * tile_n;
-      r.n = min(tile_n, c_in - r.n0);
-      r.k0 = first[r.g];
-      r.k_len = first[r.g + 1] - r.k0;
+      g = q / n_tiles;
+      q -= g * n_tiles;
+      step_g = step_q / n_tiles;
+      step_q -= step_g * n_tiles;
+      k_len = -1;
     } else {
-      r.g = find_segment(tiles, groups, q);
-      // a group's rows are shared out evenly over its tiles: (tiles - 1) * share is less than its rows, as share <= tile_n
-      const int rows = first[r.g + 1] - first[r.g], count = tiles[r.g + 1] - tiles[r.g], i = q - tiles[r.g];
-      const int share = ((rows + count - 1) / count + 16 * CG - 1) / (16 * CG) * (16 * CG);
-      r.n0 = first[r.g] + i * share;
-      r.n = min(share, rows - i * share);
-      r.k0 = 0;
-      r.k_len = c_k;
+      k0 = 0;
+      k_len = PASS == GROUPED_DGRAD ? p.c_out : p.c_in;
     }
-    r.n_mma = (r.n + 16 * CG - 1) / (16 * CG) * (16 * CG);
-    return r;
+    n_mma = n = blocks = b0 = b1 = 0;
+    if (left > 0) fill();
+  }
+  __device__ __forceinline__ void fill() {
+    m0 = m * (128 * CG);
+    if (PASS == GROUPED_WGRAD) {
+      n0 = q * tile_n;
+      n = min(tile_n, c_in - n0);
+      k0 = first[g];
+      k_len = first[g + 1] - k0;
+    } else {
+      while (tiles[g + 1] <= q) { ++g; share = 0; }
+      const int rows = first[g + 1] - first[g], count = tiles[g + 1] - tiles[g], i = q - tiles[g];
+      // a group's rows are shared out evenly over its tiles: (count - 1) * share is less than its rows, as share <= tile_n
+      if (share == 0) share = ((rows + count - 1) / count + 16 * CG - 1) / (16 * CG) * (16 * CG);
+      n0 = first[g] + i * share;
+      n = min(share, rows - i * share);
+    }
+    n_mma = (n + 16 * CG - 1) / (16 * CG) * (16 * CG);
+    blocks = b1 = (k_len + GU_K - 1) / GU_K;
+    if (SPLIT) {
+      const int part = (int)blockIdx.x % parts;
+      b0 = (int)((long long)blocks * part / parts);
+      b1 = (int)((long long)blocks * (part + 1) / parts);
+    }
+  }
+  __device__ __forceinline__ void next() {
+    if (--left <= 0) return;
+    m += step_m;
+    q += step_q;
+    if (m >= m_tiles) { m -= m_tiles; ++q; }
+    if (PASS == GROUPED_WGRAD) {
+      g += step_g;
+      if (q >= n_tiles) { q -= n_tiles; ++g; }
+    }
+    fill();
   }
 };
 
-template <int PASS, int CG>
+template <int PASS, int CG, bool SPLIT>
 __global__ void __launch_bounds__(GU_THREADS, 1)
     grouped_umma_kernel(GroupedParams p, GuConfig cfg, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                         const __grid_constant__ CUtensorMap map_b16) {
@@ -209,7 +264,7 @@ __global__ void __launch_bounds__(GU_THREADS, 1)
   constexpr bool A_MN = PASS != GROUPED_DGRAD, B_MN = PASS == GROUPED_WGRAD;
   extern __shared__ uint8_t gu_smem[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(gu_smem) + 1023) & ~static_cast<uintptr_t>(1023));
-  GuShared* sh = reinterpret_cast<GuShared*>(smem + (size_t)cfg.stages * cfg.stage_bytes);
+  GuShared* sh = reinterpret_cast<GuShared*>(smem + (size_t)cfg.stages * cfg.stage_bytes + GU_EPI_WARPS / 4 * GU_PATCH_BYTES);
   int* first = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(sh) + GU_SHARED_BYTES);  // [groups + 1]
   int* tiles = first + p.groups + 1;                                                     // [groups + 1]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -224,7 +279,7 @@ __global__ void __launch_bounds__(GU_THREADS, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(smem_u32(&sh->tmem_full[b]), 1);
-      mbar_init(smem_u32(&sh->tmem_empty[b]), 4 * CG);
+      mbar_init(smem_u32(&sh->tmem_empty[b]), GU_EPI_WARPS * CG);
     }
     mbar_init(smem_u32(&sh->drained), 1);
     sh->abort_flag = 0;
@@ -240,8 +295,7 @@ __global__ void __launch_bounds__(GU_THREADS, 1)
   pair_sync<CG>();  // barriers and tensor memory of both CTAs are there
   tc_fence_after();
   const uint32_t tmem = sh->tmem_base;
-  const GuTiles<PASS, CG> all(p, cfg.tile_n, first, tiles);
-  const long long t0 = blockIdx.x / CG, step = gridDim.x / CG;
+  GuTiles<PASS, CG, SPLIT> tile(p, cfg, first, tiles);
   const uint32_t stage0 = smem_u32(smem);
   bool ok = true;
 
@@ -250,17 +304,15 @@ __global__ void __launch_bounds__(GU_THREADS, 1)
     if (elect_one()) {
       int s = 0;
       uint32_t ph = 1;
-      for (long long t = t0; t < all.total && ok; t += step) {
-        const GuTile tile = all.at(t);
+      for (; tile.left > 0 && ok; tile.next()) {
         const int m0 = tile.m0 + (int)rank * 128, half = tile.n_mma / CG, n0 = tile.n0 + (int)rank * half;
-        const int blocks = (tile.k_len + GU_K - 1) / GU_K;
         const uint32_t b_bytes = B_MN ? (uint32_t)((half + 63) / 64) * 8192u : (uint32_t)half * 128u;
-        for (int kb = 0; kb < blocks; ++kb) {
+        for (int kb = tile.b0; kb < tile.b1; ++kb) {
           ok = pair_wait<false>(smem_u32(&sh->empty[s]), ph, abort_flag);
           if (!ok) break;
           const uint32_t a = stage0 + (uint32_t)(s * cfg.stage_bytes), b = a + GU_A_BYTES;
           const int k = tile.k0 + kb * GU_K;
-          const bool clear = PASS == GROUPED_WGRAD && (tile.k_len - kb * GU_K) % 16 != 0 && kb + 1 == blocks;
+          const bool clear = PASS == GROUPED_WGRAD && (tile.k_len - kb * GU_K) % 16 != 0 && kb + 1 == tile.blocks;
           // a stage to be cleared is reported to this CTA's warp 2, which reports it on
           const uint32_t bar = clear ? smem_u32(&sh->landed[s]) : at_leader<CG>(smem_u32(&sh->full[s]));
           pair_expect(bar, GU_A_BYTES + b_bytes);
@@ -294,10 +346,9 @@ __global__ void __launch_bounds__(GU_THREADS, 1)
       constexpr uint32_t a_step = (A_MN ? 2048u : 32u) >> 4, b_step = (B_MN ? 2048u : 32u) >> 4;
       int s = 0, buf = 0;
       uint32_t ph = 0, buf_ph = 1;
-      for (long long t = t0; t < all.total && ok; t += step) {
-        const GuTile tile = all.at(t);
-        const int steps = (tile.k_len + 15) / 16;  // of the contraction: 16 each, four a stage
-        if (steps == 0) continue;
+      for (; tile.left > 0 && ok; tile.next()) {
+        const int steps = min((tile.k_len + 15) / 16, tile.b1 * 4) - tile.b0 * 4;  // of the contraction: 16 each, four a stage
+        if (steps <= 0) continue;
         ok = pair_wait<true>(smem_u32(&sh->tmem_empty[buf]), buf_ph, abort_flag);
         if (!ok) break;
         tc_fence_after();
@@ -331,75 +382,99 @@ __global__ void __launch_bounds__(GU_THREADS, 1)
     // ------------------------------------------------------------------ rows behind a group's last one
     int s = 0;
     uint32_t odd = 0;  // phases of the barriers, a bit a stage
-    for (long long t = t0; t < all.total && ok; t += step) {
-      const GuTile tile = all.at(t);
-      const int blocks = (tile.k_len + GU_K - 1) / GU_K, there = tile.k_len % GU_K;
-      if (blocks == 0) continue;
-      s = (s + blocks - 1) % cfg.stages;
-      if (there % 16 != 0) {
+    for (; tile.left > 0 && ok; tile.next()) {
+      const int there = tile.k_len % GU_K;
+      if (tile.b0 == tile.b1) continue;
+      s = (s + tile.b1 - tile.b0 - 1) % cfg.stages;
+      if (there % 16 != 0 && tile.b1 == tile.blocks) {
         ok = pair_wait<false>(smem_u32(&sh->landed[s]), (odd >> s) & 1u, abort_flag);
         if (!ok) break;
         odd ^= 1u << s;
         // to the next multiple of 16: the MMA goes no further.  A row is 128 bytes of each block of 64 channels.
         const uint32_t base = stage0 + (uint32_t)(s * cfg.stage_bytes);
-        const int rows = 16 - there % 16, chans = GU_A_BYTES / 8192 + (tile.n_mma / CG + 63) / 64;
-        for (int i = lane; i < rows * chans * 8; i += 32) {
-          const int chunk = i & 7, r = (i >> 3) % rows, c = (i >> 3) / rows;
-          asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(base + (uint32_t)(c * 8192 + (there + r) * 128 + chunk * 16)), "r"(0) : "memory");
-        }
-        fence_proxy_async();
+        const int blocks_there = GU_A_BYTES / 8192 + (tile.n_mma / CG + 63) / 64;
+        for (int c = lane >> 3; c < blocks_there; c += 4)
+          for (int r = there; r % 16 != 0; ++r)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(base + (uint32_t)(c * 8192 + r * 128 + (lane & 7) * 16)), "r"(0) : "memory");
+        fence_proxy_async();  // what the tensor cores read of this CTA's memory from here on
         __syncwarp();
         if (lane == 0) pair_arrive(at_leader<CG>(smem_u32(&sh->full[s])));
       }
       s = s + 1 == cfg.stages ? 0 : s + 1;
     }
-  } else if (warp >= 4) {
+  } else if (warp >= GU_EPI_WARP0) {
     // ------------------------------------------------------------------ epilogue
-    const int quarter = warp - 4;  // lanes of tensor memory that this warp may read
+    const int quarter = warp & 3;  // lanes of tensor memory that this warp may read
+    const int half = (warp - GU_EPI_WARP0) >> 2;  // of the tile's columns, in turns of 32
     const int channels = PASS == GROUPED_DGRAD ? p.c_in : p.c_out;
     uint16_t* out = static_cast<uint16_t*>(p.d);
-    if (PASS != GROUPED_WGRAD && p.zero_rest) zero_other_rows(p.d, (size_t)channels * 2, first, p.groups, p.n_rows, threadIdx.x - 128, 128);
+    if (PASS != GROUPED_WGRAD && p.zero_rest)
+      zero_other_rows(p.d, (size_t)channels * 2, first, p.groups, p.n_rows, threadIdx.x - GU_EPI_WARP0 * 32, GU_EPI_WARPS * 32);
+    const size_t pitch = 2 * (size_t)channels;
+    // The patch of four warps: 32 rows of 128 channels, 256 bytes each, whose 16-byte chunks are permuted so that neither the eight rows of a
+    // matrix nor eight consecutive chunks of a row meet in a bank.
+    const uint32_t patch = stage0 + (uint32_t)(cfg.stages * cfg.stage_bytes) + (uint32_t)half * GU_PATCH_BYTES;
+    const auto chunk_at = [&](int row, int chunk) { return patch + (uint32_t)(row * 256 + (chunk ^ (row & 7)) * 16); };
+    const uint32_t put = chunk_at(lane & 7, quarter * 4 + (lane >> 3));  // rows eight apart: 2048 bytes on
     int buf = 0;
     uint32_t ph = 0;
-    for (long long t = t0; t < all.total && ok; t += step) {
-      const GuTile tile = all.at(t);
+    for (; !SPLIT && tile.left > 0 && ok; tile.next()) {
       const bool some = tile.k_len > 0;  // a group without rows has a gradient of zeros
-      // Even lanes store row j, odd ones row j + 1, two channels each.
-      const int ch = tile.m0 + (int)rank * 128 + quarter * 32 + (lane & ~1);
+      const int ch = tile.m0 + (int)rank * 128 + (lane & 15) * 8;
+      uint16_t* to = out + (PASS == GROUPED_WGRAD ? (size_t)tile.g * p.c_in + tile.n0 : (size_t)tile.n0) * channels + ch;
       const bool mine = ch < channels;
-      uint16_t* to = out + (PASS == GROUPED_WGRAD ? ((size_t)tile.g * p.c_in + tile.n0) * channels : (size_t)tile.n0 * channels) + ch + (size_t)(lane & 1) * channels;
       if (some) {
-        ok = pair_wait<false>(smem_u32(&sh->tmem_full[buf]), ph, abort_flag);
-        ok = __all_sync(0xffffffffu, ok) != 0;
+        ok = four_agree(half, pair_wait<false>(smem_u32(&sh->tmem_full[buf]), ph, abort_flag));
         if (!ok) break;
         tc_fence_after();
       }
       const uint32_t from = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * cfg.tile_n);
-      for (int j0 = 0; j0 < tile.n_mma; j0 += 16) {
-        uint32_t v[16];
+      for (int j0 = half * 32; j0 < tile.n_mma; j0 += 64) {
+        // 32 rows (columns of the accumulator, of which the last 16 may not be used) of the warp's 32 channels
+        uint32_t v[32];
         if (some) {
-          tmem_ld16(from + (uint32_t)j0, v);
+          tmem_ld_16x8x4(from + (uint32_t)j0, reinterpret_cast<uint32_t(&)[16]>(v[0]));
+          tmem_ld_16x8x4(from + (uint32_t)j0 + (16u << 16), reinterpret_cast<uint32_t(&)[16]>(v[16]));
           tmem_ld_wait();
         } else {
 #pragma unroll
-          for (int j = 0; j < 16; ++j) v[j] = 0u;
+          for (int j = 0; j < 32; ++j) v[j] = 0u;
         }
-        if (some && j0 + 16 >= tile.n_mma) {  // the last of them: the accumulator is free
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) pair_arrive(at_leader<CG>(smem_u32(&sh->tmem_empty[buf])));
-        }
+        four_sync(half);  // the patch has been read
 #pragma unroll
-        for (int j = 0; j < 16; j += 2) {
-          const uint32_t give = (lane & 1) ? v[j] : v[j + 1], got = __shfl_xor_sync(0xffffffffu, give, 1);
-          const float lo = __uint_as_float((lane & 1) ? got : v[j]), hi = __uint_as_float((lane & 1) ? v[j + 1] : got);
-          uint32_t two;
-          if (cfg.bf16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(two) : "f"(hi), "f"(lo));
-          else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(two) : "f"(hi), "f"(lo));
-          if (mine && j0 + j + (lane & 1) < tile.n) *reinterpret_cast<uint32_t*>(to + (size_t)(j0 + j) * channels) = two;
+        for (int i = 0; i < 4; ++i) {  // eight rows
+          uint32_t h[4];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {  // of eight channels each
+            const float lo = __uint_as_float(v[(c >> 1) * 16 + i * 4 + (c & 1) * 2]), hi = __uint_as_float(v[(c >> 1) * 16 + i * 4 + (c & 1) * 2 + 1]);
+            if (cfg.bf16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(h[c]) : "f"(hi), "f"(lo));
+            else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(h[c]) : "f"(hi), "f"(lo));
+          }
+          asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(put + (uint32_t)i * 2048u), "r"(h[0]), "r"(h[1]), "r"(h[2]),
+                       "r"(h[3])
+                       : "memory");
         }
+        four_sync(half);
+        const int r0 = quarter * 8 + (lane >> 4);  // two rows a store, eight a warp
+        uint4 o[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(o[i].x), "=r"(o[i].y), "=r"(o[i].z), "=r"(o[i].w) : "r"(chunk_at(r0 + 2 * i, lane & 15)) : "memory");
+        uint16_t* row = to + (size_t)(j0 + r0) * channels;
+        const int rows = mine ? tile.n - j0 - r0 : 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i, row += pitch)
+          if (2 * i < rows) {
+            // a weight gradient is read once, when the step is over: 64 groups of a few rows, 2048 -> 1024, 57 us without the hint, 52 with
+            if (PASS == GROUPED_WGRAD) __stcs(reinterpret_cast<uint4*>(row), o[i]);
+            else *reinterpret_cast<uint4*>(row) = o[i];
+          }
       }
       if (some) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) pair_arrive(at_leader<CG>(smem_u32(&sh->tmem_empty[buf])));
         buf ^= 1;
         if (buf == 0) ph ^= 1u;
       }
@@ -408,6 +483,56 @@ __global__ void __launch_bounds__(GU_THREADS, 1)
   if (!ok) report_problem();
   __syncwarp();
   tc_fence_before();
+  if constexpr (SPLIT) {
+    // ------------------------------------------------------------------ sums of the parts
+    // Every CTA has the sums over its share of the contraction in tensor memory.  It hands the columns (rows of the output) to the CTA that finishes
+    // them, in shared memory over its ring, [part][column][128 channels]; that one adds them in the order of the parts: the same bits on every run.
+    cluster_sync();  // all copies and MMAs of all parts are done
+    tc_fence_after();
+    const int part = (int)blockIdx.x % cfg.parts, width = (tile.n_mma + cfg.parts - 1) / cfg.parts;
+    if (warp >= GU_EPI_WARP0 && tile.left > 0) {
+      const int quarter = warp & 3, half = (warp - GU_EPI_WARP0) >> 2;
+      for (int j0 = half * 16; j0 < tile.n_mma; j0 += 32) {
+        uint32_t v[16];
+        if (tile.b1 > tile.b0) {
+          tmem_ld16(tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)j0, v);
+          tmem_ld_wait();
+        } else {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) v[j] = 0u;
+        }
+        int to = j0 / width, c = j0 - to * width;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          put_at(to, stage0 + (uint32_t)(((part * width + c) * 128 + quarter * 32 + lane) * 4), v[j]);
+          if (++c == width) { c = 0; ++to; }
+        }
+      }
+    }
+    cluster_sync();
+    if (warp >= GU_EPI_WARP0 && tile.left > 0) {
+      const int channels = PASS == GROUPED_DGRAD ? p.c_in : p.c_out, thread = (int)threadIdx.x - GU_EPI_WARP0 * 32;
+      const int ch = 2 * (thread & 63);
+      const int n = min(width, tile.n - part * width);
+      uint16_t* out = static_cast<uint16_t*>(p.d) +
+                      ((PASS == GROUPED_WGRAD ? (size_t)tile.g * p.c_in + tile.n0 : (size_t)tile.n0) + part * width) * channels + tile.m0 + ch;
+      if (tile.m0 + ch < channels)
+        for (int c = thread >> 6; c < n; c += GU_EPI_WARPS / 2) {
+          float lo = 0.f, hi = 0.f;
+          for (int q = 0; q < cfg.parts; ++q) {
+            float a, b;
+            asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(a), "=f"(b) : "r"(stage0 + (uint32_t)(((q * width + c) * 128 + ch) * 4)) : "memory");
+            lo += a;
+            hi += b;
+          }
+          uint32_t two;
+          if (cfg.bf16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(two) : "f"(hi), "f"(lo));
+          else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(two) : "f"(hi), "f"(lo));
+          *reinterpret_cast<uint32_t*>(out + (size_t)c * channels) = two;
+        }
+    }
+    tc_fence_before();
+  }
   if (*abort_flag) {  // copies may still be on their way into this CTA's memory
     const long long start = clock64();
     while (clock64() - start < 2000000) __nanosleep(1000);
@@ -442,29 +567,103 @@ inline int grouped_tensor_map(CUtensorMap* map, const void* data, int cols, int 
   return rc == CUDA_SUCCESS ? 0 : -1000 - (int)rc;
 }
 
-// Whether the kernel takes a call: what the tensor maps and the stores ask for.
+// Whether the kernel takes a call: what the tensor maps and the stores ask for; tiles (of 64 x 128 values at least) are counted in an int.
 inline bool grouped_umma_takes(const GroupedParams& p, bool* shape) {
-  *shape = p.c_in % 8 == 0 && p.c_out % 8 == 0 && p.n_rows > 0;
+  const long long wide = p.c_in > p.c_out ? p.c_in : p.c_out, rows = (long long)p.n_rows > (long long)p.groups * p.c_in ? p.n_rows : (long long)p.groups * p.c_in;
+  *shape = p.c_in % 8 == 0 && p.c_out % 8 == 0 && p.n_rows > 0 && (rows / 64 + p.groups) * (wide / 128 + 1) < 0x7fffffffll;
   return *shape && ((reinterpret_cast<uintptr_t>(p.a) | reinterpret_cast<uintptr_t>(p.b) | reinterpret_cast<uintptr_t>(p.d)) & 15) == 0;
 }
 
-template <int PASS, int CG>
-int launch_grouped_umma_as(const GroupedParams& p, bool bf16, int tile_n, cudaStream_t st, int sms, int max_smem) {
+// A way to cut a product up.
+struct GuCut {
+  int cg, tile_n, parts;
+};
+
+// at most: no more groups have rows than there are rows
+template <int PASS>
+long long grouped_tiles(const GroupedParams& p, const GuCut& cut) {
+  const int channels = PASS == GROUPED_DGRAD ? p.c_in : p.c_out;
+  const long long m = (channels + 128 * cut.cg - 1) / (128 * cut.cg);
+  if (PASS == GROUPED_WGRAD) return m * p.groups * ((p.c_in + cut.tile_n - 1) / cut.tile_n);
+  return m * (p.n_rows / cut.tile_n + (p.n_rows < p.groups ? p.n_rows : p.groups));
+}
+
+// The cut that is expected to take the least time, from the sizes that the host knows: rows are taken to be spread evenly.
+//
+// Measured, microseconds (bf16, launches in a row; c, a stage of a tile: on an idle chip / on a full one):
+//   n columns             64            128           256
+//   one CTA          0.21 / 0.24   0.22 / 0.30   0.29 / 0.50
+//   a pair           0.21 / 0.23   0.21 / 0.28   0.29 / 0.42
+// and 4 for everything around it (a pair 0.8 more), 0.5 and 0.0055 a column for the epilogue, beside the next tile's stages.  So pairs of 256 columns
+// where there is work for all: 16 groups of 1024 rows 2048 -> 2048 98 us, single CTAs 112, 128 columns 125 and 134; narrower tiles and single CTAs
+// (of tiles that do as well the narrowest: they leave room for more stages, and 96 rows in 64 groups 2048 -> 1024 take 46.4 us instead of 50.4) where
+// there is not: 1000 rows 1024 -> 1024 11.1 us, so 8.1; 4096 rows in 8 groups 512 -> 512 9.1, so 7.3.
+// Parts: a cluster for every tile, whose CTAs share the contraction; 2 and 0.024 a column more for adding up.  One row 4096 -> 4096 17.4 us, with four
+// parts 9.2; the gradient of a 256 x 256 matrix over 30000 rows 94, with eight parts 19; but only while all clusters run at once, as every further round of
+// them starts from nothing (1000 rows 1024 -> 1024 with four parts 28).
+inline float grouped_stage_us(int cg, float n, float load) {
+  const float idle = n <= 128.f ? 0.2f + 0.02f * n / 128.f : 0.22f + 0.07f * (n - 128.f) / 128.f;
+  const float full = cg == 2 ? (n <= 128.f ? 0.2f + 0.08f * n / 128.f : 0.28f + 0.14f * (n - 128.f) / 128.f)
+                             : (n <= 128.f ? 0.2f + 0.1f * n / 128.f : 0.3f + 0.2f * (n - 128.f) / 128.f);
+  return idle + (full - idle) * (load < 1.f ? load : 1.f);
+}
+
+template <int PASS, typename Clusters>
+GuCut grouped_cut(const GroupedParams& p, int sms, Clusters clusters_at_once) {
+  static constexpr GuCut CUTS[] = {{1, 64, 1},  {1, 128, 1}, {1, 256, 1}, {2, 128, 1}, {2, 256, 1}, {1, 32, 2},  {1, 64, 2},
+                                   {1, 128, 2}, {1, 32, 4},  {1, 64, 4},  {1, 128, 4}, {1, 32, 8},  {1, 64, 8},  {1, 128, 8}};
+  const int channels = PASS == GROUPED_DGRAD ? p.c_in : p.c_out;
+  const float groups = (float)(PASS == GROUPED_WGRAD || p.groups < p.n_rows ? p.groups : p.n_rows), rows = (float)p.n_rows / groups;
+  const float blocks = PASS == GROUPED_WGRAD ? rows / 64.f + 0.5f : (float)(((PASS == GROUPED_DGRAD ? p.c_out : p.c_in) + 63) / 64);
+  GuCut best = CUTS[0];
+  float least = 0.f;
+  for (const GuCut& cut : CUTS) {
+    if (cut.cg > sms) continue;
+    const float m = (float)((channels + 128 * cut.cg - 1) / (128 * cut.cg)), width = (float)cut.tile_n;
+    float tiles, n;
+    if (PASS == GROUPED_WGRAD) {
+      tiles = groups * (float)((p.c_in + cut.tile_n - 1) / cut.tile_n);
+      n = p.c_in < cut.tile_n ? (float)p.c_in : width;
+    } else {
+      tiles = groups * (rows <= width ? 1.f : rows / width + 0.5f);
+      n = rows < width ? rows : width;
+    }
+    tiles *= m;
+    const float epilogue = 0.5f + 0.0055f * n, slots = (float)(sms / cut.cg);
+    float us;
+    if (cut.parts > 1) {
+      if (blocks < 2.f * (float)cut.parts || grouped_tiles<PASS>(p, cut) > clusters_at_once(cut.parts)) continue;
+      us = 4.f + blocks / (float)cut.parts * grouped_stage_us(1, n, tiles * (float)cut.parts / slots) + 2.f + 0.024f * n;
+    } else {
+      const float rounds = tiles <= slots ? 1.f : tiles / slots + 0.5f, tile = blocks * grouped_stage_us(cut.cg, n, tiles / slots);
+      us = (cut.cg == 2 ? 4.8f : 4.f) + tile + (rounds - 1.f) * (tile > epilogue ? tile : epilogue) + epilogue;
+    }
+    if (least == 0.f || us < least) {
+      least = us;
+      best = cut;
+    }
+  }
+  return best;
+}
+
+template <int PASS, int CG, bool SPLIT>
+int launch_grouped_umma_as(const GroupedParams& p, bool bf16, const GuCut& cut, cudaStream_t st, int sms, int max_smem) {
   GuConfig cfg;
-  cfg.tile_n = tile_n;
+  cfg.parts = SPLIT ? cut.parts : 1;
+  cfg.tile_n = cut.tile_n;
   cfg.bf16 = bf16;
-  const int b_bytes = PASS == GROUPED_WGRAD ? (tile_n / CG + 63) / 64 * 8192 : tile_n / CG * 128;
+  const int b_bytes = PASS == GROUPED_WGRAD ? (cfg.tile_n / CG + 63) / 64 * 8192 : cfg.tile_n / CG * 128;
   cfg.stage_bytes = GU_A_BYTES + b_bytes;
-  const int rest = 1024 + GU_SHARED_BYTES + (2 * p.groups + 2) * (int)sizeof(int);
+  const int rest = 1024 + GU_EPI_WARPS / 4 * GU_PATCH_BYTES + GU_SHARED_BYTES + (2 * p.groups + 2) * (int)sizeof(int);
   cfg.stages = (max_smem - rest) / cfg.stage_bytes;
   if (cfg.stages > GU_MAX_STAGES) cfg.stages = GU_MAX_STAGES;
-  if (cfg.stages < 2) return -1;
+  if (cfg.stages < 2 || (SPLIT && cfg.stages * cfg.stage_bytes < (cfg.tile_n + cut.parts) * 512)) return -1;
   cfg.smem = rest + cfg.stages * cfg.stage_bytes;
-  const int channels = PASS == GROUPED_DGRAD ? p.c_in : p.c_out, m_tiles = (channels + 128 * CG - 1) / (128 * CG);
-  const long long n_tiles = PASS == GROUPED_WGRAD ? (long long)p.groups * ((p.c_in + tile_n - 1) / tile_n) : (long long)p.n_rows / tile_n + p.groups;
-  long long pairs = n_tiles * m_tiles;
-  if (pairs > sms / CG) pairs = sms / CG;
-  if (pairs < 1) pairs = 1;
+  // SPLIT: a cluster for every tile there may be; otherwise pairs (or CTAs) go from tile to tile
+  long long clusters = grouped_tiles<PASS>(p, cut);
+  if (!SPLIT && clusters > sms / CG) clusters = sms / CG;
+  if (clusters < 1) clusters = 1;
+  const int ctas = SPLIT ? cut.parts : CG;
   CUtensorMap a, b, b16;
   int rc;
   if (PASS == GROUPED_WGRAD) {  // p.a: in, p.b: out_grad
@@ -474,14 +673,14 @@ int launch_grouped_umma_as(const GroupedParams& p, bool bf16, int tile_n, cudaSt
   } else {
     rc = grouped_tensor_map(&a, p.b, p.c_out, p.c_in, p.groups, PASS == GROUPED_FWD ? 64 : 128, bf16);
     const int width = PASS == GROUPED_FWD ? p.c_in : p.c_out;
-    if (rc == 0) rc = grouped_tensor_map(&b, p.a, width, p.n_rows, 0, tile_n / CG, bf16);
+    if (rc == 0) rc = grouped_tensor_map(&b, p.a, width, p.n_rows, 0, cfg.tile_n / CG, bf16);
     if (rc == 0) rc = grouped_tensor_map(&b16, p.a, width, p.n_rows, 0, 16, bf16);
   }
   if (rc != 0) return rc;
   static std::atomic<int> granted[64];
-  if (ensure_smem(grouped_umma_kernel<PASS, CG>, cfg.smem, granted) != 0) return -1;
+  if (ensure_smem(grouped_umma_kernel<PASS, CG, SPLIT>, cfg.smem, granted) != 0) return -1;
   cudaLaunchConfig_t lc = {};
-  lc.gridDim = dim3((unsigned)(pairs * CG));
+  lc.gridDim = dim3((unsigned)(clusters * ctas));
   lc.blockDim = dim3(GU_THREADS);
   lc.dynamicSmemBytes = (size_t)cfg.smem;
   lc.stream = st;
@@ -489,17 +688,56 @@ int launch_grouped_umma_as(const GroupedParams& p, bool bf16, int tile_n, cudaSt
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
   at[1].id = cudaLaunchAttributeClusterDimension;
-  at[1].val.clusterDim.x = CG;
+  at[1].val.clusterDim.x = (unsigned)ctas;
   at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
   lc.attrs = at;
-  lc.numAttrs = CG == 2 ? 2 : 1;
-  return cudaLaunchKernelEx(&lc, grouped_umma_kernel<PASS, CG>, p, cfg, a, b, b16) == cudaSuccess ? 0 : -1;
+  lc.numAttrs = ctas > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&lc, grouped_umma_kernel<PASS, CG, SPLIT>, p, cfg, a, b, b16) == cudaSuccess ? 0 : -1;
+}
+
+// Clusters of `parts` CTAs that the device runs at the same time, each with all of an SM's shared memory: clusters do not straddle its groups
+// of SMs, so 128 CTAs in clusters of eight do not fit on 148.  Asked once a device; fewer SMs than all of them: in proportion.
+template <int PASS>
+int grouped_clusters_at_once(int parts, int sms, int max_smem) {
+  static std::atomic<int> known[64][4];
+  static std::atomic<int> granted[64];
+  int dev = 0, all = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64 || parts < 2) return 0;
+  std::atomic<int>& at = known[dev][parts == 2 ? 0 : parts == 4 ? 1 : 2];
+  if (cudaDeviceGetAttribute(&all, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+  int n = at.load(std::memory_order_acquire);
+  if (n == 0) {
+    if (ensure_smem(grouped_umma_kernel<PASS, 1, true>, max_smem, granted) != 0) return 0;
+    cudaLaunchConfig_t lc = {};
+    lc.gridDim = dim3((unsigned)(parts * all));
+    lc.blockDim = dim3(GU_THREADS);
+    lc.dynamicSmemBytes = (size_t)max_smem;
+    cudaLaunchAttribute cluster[1];
+    cluster[0].id = cudaLaunchAttributeClusterDimension;
+    cluster[0].val.clusterDim.x = (unsigned)parts;
+    cluster[0].val.clusterDim.y = cluster[0].val.clusterDim.z = 1;
+    lc.attrs = cluster;
+    lc.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&n, grouped_umma_kernel<PASS, 1, true>, &lc) != cudaSuccess || n < 1) {
+      cudaGetLastError();
+      n = -1;
+    }
+    at.store(n, std::memory_order_release);
+  }
+  return n < 0 ? 0 : n * sms / all;
+}
+
+template <int PASS>
+int launch_grouped_umma_cut(const GroupedParams& p, bool bf16, const GuCut& cut, cudaStream_t st, int sms, int max_smem) {
+  if (cut.parts > 1) return launch_grouped_umma_as<PASS, 1, true>(p, bf16, cut, st, sms, max_smem);
+  return cut.cg == 2 ? launch_grouped_umma_as<PASS, 2, false>(p, bf16, cut, st, sms, max_smem)
+                     : launch_grouped_umma_as<PASS, 1, false>(p, bf16, cut, st, sms, max_smem);
 }
 
 template <int PASS>
 int launch_grouped_umma(const GroupedParams& p, bool bf16, cudaStream_t st, int sms, int max_smem) {
-  if (sms >= 2 && (PASS == GROUPED_DGRAD ? p.c_in : p.c_out) > 128) return launch_grouped_umma_as<PASS, 2>(p, bf16, 256, st, sms, max_smem);
-  return launch_grouped_umma_as<PASS, 1>(p, bf16, 128, st, sms, max_smem);
+  const auto at_once = [&](int parts) { return grouped_clusters_at_once<PASS>(parts, sms, max_smem); };
+  return launch_grouped_umma_cut<PASS>(p, bf16, grouped_cut<PASS>(p, sms, at_once), st, sms, max_smem);
 }
 
 }  // namespace fgms

@@ -113,6 +113,25 @@ def test_against_the_definition(sizes, c_in, c_out, dtype, which):
     assert backend.device_status() == 0
 
 
+# few tiles with a long contraction, which several CTAs share: channels for the products of rows, rows for the weight gradient
+LONG = [([1], 4096, 4096), ([20], 4000, 200), ([1, 0, 6], 2056, 136), ([33, 60], 2560, 72), ([1000], 4096, 128), ([5], 200, 4096), ([30, 9], 136, 3000),
+        ([3000], 256, 256), ([5000, 3, 0], 128, 264), ([8001], 504, 512), ([2047, 1], 24, 40), ([9000, 4000], 64, 64)]
+
+
+@pytest.mark.parametrize("which", PASSES)
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("sizes,c_in,c_out", LONG, ids=[f"{len(s)}g{sum(s)}r_{a}x{b}" for s, a, b in LONG])
+def test_long_contractions(sizes, c_in, c_out, dtype, which):
+    from fgms_b200 import backend
+    backend.device_status()
+    layer = Layer(dtype, sizes, c_in, c_out, start=3, rest=40, seed=len(sizes) + c_in)
+    first = layer.check(which)
+    assert torch.equal(first, layer.run(which))
+    if which != "wgrad":
+        layer.check(which, zero_rest=True)
+    assert backend.device_status() == 0
+
+
 @pytest.mark.parametrize("which", PASSES)
 @pytest.mark.parametrize("dtype", list(TYPES))
 @pytest.mark.parametrize("c_in,c_out", [(64, 128), (50, 33)])
