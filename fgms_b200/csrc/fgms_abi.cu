@@ -448,7 +448,7 @@ int launch_adamw(const fgms_b200_adamw_tensor* tensors, int n, const fgms_b200_a
     if (chunks > 0x7fffffffll - 65536) return fail(FGMS_ERR_INVALID_ARG, "too many values in one call");
   }
   p.chunks = (int)chunks;
-  const long long most = 4ll * sms, grid = chunks < 1 ? 1 : chunks < most ? chunks : most;
+  const long long most = 3ll * sms, grid = chunks < 1 ? 1 : chunks < most ? chunks : most;
   if (fgms::launch_pdl(fgms::adamw_kernel<EIGHT, N>, dim3((unsigned)grid), fgms::ADAMW_THREADS, 0, st, p) != cudaSuccess)
     return fail(FGMS_ERR_CUDA, "adamw_kernel: %s", cudaGetErrorString(cudaGetLastError()));
   return check_launch("adamw_kernel");
