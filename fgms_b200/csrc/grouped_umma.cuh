@@ -172,7 +172,6 @@ __device__ __forceinline__ bool four_agree(int half, bool ok) {
                : "=r"(all) : "r"((uint32_t)ok), "r"(1 + half) : "memory");
   return all != 0;
 }
-__device__ __forceinline__ void cluster_sync() { asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory"); }
 // a word to this CTA's address `addr` in CTA `to` of the cluster
 __device__ __forceinline__ void put_at(int to, uint32_t addr, uint32_t value) {
   asm volatile("{\n\t.reg .b32 there;\n\tmapa.shared::cluster.u32 there, %0, %1;\n\tst.shared::cluster.b32 [there], %2;\n\t}" ::"r"(addr), "r"(to), "r"(value) : "memory");

@@ -121,6 +121,9 @@ __device__ __forceinline__ void griddep_end(bool beside) {
 // what this thread may read of global memory, its TMA copies behind the fence may read too
 __device__ __forceinline__ void fence_proxy_async_global() { asm volatile("fence.proxy.async.global;" ::: "memory"); }
 
+// all threads of all CTAs of the cluster
+__device__ __forceinline__ void cluster_sync() { asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory"); }
+
 // ------------------------------------------------------------------ cp.async (16-byte, zero fill)
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
   const uint32_t n = valid ? 16u : 0u;

@@ -194,10 +194,14 @@ class UNetStep:
     gathered in 16-byte pieces and would run on the CUDA-core kernels, 32-byte rows run on the tensor cores.  The
     padded weight rows multiply zeros and their gradient is zero; ``weights[0]`` / ``w_grads[0]`` show the real
     ``c_in`` rows only.  ``set_input`` refreshes the padded copy when the caller's features change.
+
+    ``optimizer``: arguments of :class:`fgms_b200.optim.AdamW` (``{"lr": 1e-3, "state_bits": 8}``).  ``run()`` then ends with a step
+    over all weights, which lie in one flat tensor; ``update()`` takes it by itself.  The weights keep a float32 copy in ``optimizer.state``.
+    Several ranks take the same step, as their gradients are the same bits.
     """
 
     def __init__(self, spec, umaps: UNetMaps, weights, feats, grad_out, group=None, bucket_bytes: int = 6 << 20,
-                 arch80: bool = True, exchange: bool | None = None, transport: str = "nccl"):
+                 arch80: bool = True, exchange: bool | None = None, transport: str = "nccl", optimizer: dict | None = None):
         import torch
         from . import _lib, backend
         from .dist import world_size
@@ -326,6 +330,12 @@ class UNetStep:
                 wgrad[14], wgrad[15] = self._ws.data_ptr(), self._ws.numel() * 4
         self._bucket_end = {last: (lo, hi) for lo, hi, last in self.buckets}
         self.launches_per_step = len(self.spec) * 3 - 1
+        self.optimizer = None
+        if optimizer is not None:
+            from .optim import AdamW
+            self._w_flat.grad = self.w_grad
+            self.optimizer = AdamW([self._w_flat], **optimizer)
+            self.launches_per_step += 1
         # what the caller sees: the layer list as given, the stem's real input channels only
         self.run_spec, self.spec = self.spec, report_spec
         self._w_run = list(self.weights)
@@ -390,11 +400,19 @@ class UNetStep:
         if self.multi:
             check(L.fgms_b200_wgrad_finalize(self.w_grad.data_ptr(), self._total32.data_ptr(), self.w_grad.numel(), st))
 
+    def update(self):
+        """A step of the optimizer with the gradients of the last backward."""
+        if self.optimizer is None:
+            raise ValueError("update() needs UNetStep(..., optimizer={...})")
+        self.optimizer.step()
+
     def run(self):
         import torch
         with torch.cuda.device(self.device):
             self.forward()
             self.backward()
+            if self.optimizer is not None:
+                self.update()
 
     def profile(self, reps: int = 5, flush=None, apart: bool = False):
         """Per-call device times of the step (mean over ``reps`` steps, CUDA events around every operator call):
