@@ -42,7 +42,7 @@ template <int N>
 struct AdamwParams {
   double lr, beta1, beta2, decay;
   float b1, c1, b2, c2, eps;  // c = 1 - b
-  uint32_t seed;
+  uint32_t seed, minus_zero;
   const float *lr_device, *grad_scale, *found_inf;
   int* step;  // [2]: steps done, and blocks that have finished this one
   int n, chunks, last;  // last: the launch that counts the step
@@ -125,6 +125,11 @@ __device__ __forceinline__ uint64_t adamw_add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
+__device__ __forceinline__ uint64_t adamw_add2_down(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rz.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
 __device__ __forceinline__ uint64_t adamw_fma2(uint64_t a, uint64_t b, uint64_t c) {
   uint64_t d;
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
@@ -172,17 +177,24 @@ __device__ __forceinline__ void adamw_store_codes(void* to, float* scales, long 
   const float inverse = held ? __fdiv_rn(1.f, scale) : 0.f;
   uint32_t w[2] = {0u, 0u};
 #pragma unroll
-  for (int e = 0; e < 8; e += 2) adamw_part(adamw_mul2(adamw_two(x[e], x[e + 1]), adamw_two(inverse, inverse)), y[e], y[e + 1]);
+  for (int e = 6; e >= 0; e -= 2) {
+    float u[2], whole[2];
+    adamw_part(adamw_mul2(adamw_two(x[e], x[e + 1]), adamw_two(inverse, inverse)), u[0], u[1]);
+    u[0] = fminf(fabsf(u[0]), ADAMW_E4M3_MAX);
+    u[1] = fminf(fabsf(u[1]), ADAMW_E4M3_MAX);
+    // From 2^-6 on three bits of the mantissa stay: with the bias taken off the exponent they are the code.  Below, codes are 2^-9 apart: the whole
+    // part of 512 u + lot / 2^16.  Both come from the bits of floats, 1 + lot / 2^16 and 2^23 + the sum rounded down: conversions would
+    // go through a pipe of a quarter of the rate.
+    const uint64_t lots = adamw_add2(adamw_two(__uint_as_float(0x3f800000u | lot[e] << 7), __uint_as_float(0x3f800000u | lot[e + 1] << 7)), adamw_two(-1.f, -1.f));
+    adamw_part(adamw_add2_down(adamw_fma2(adamw_two(u[0], u[1]), adamw_two(512.f, 512.f), lots), adamw_two(8388608.f, 8388608.f)), whole[0], whole[1]);
 #pragma unroll
-  for (int e = 7; e >= 0; --e) {
-    const float u = fminf(fabsf(y[e]), ADAMW_E4M3_MAX);
-    // From 2^-6 on three bits of the mantissa stay: with the bias taken off the exponent they are the code.  Below, codes are 2^-9 apart, as they are
-    // between 2^-6 and 2^-5: half of u + 2^-6 has their exponent, one less.
-    const float from = u < 0.015625f ? __fmaf_rn(u, 0.5f, 0.0078125f) : u;
-    uint32_t code = (__float_as_uint(from) + (lot[e] << 4) - ((127u - 7u) << 23)) >> 20;
-    if (FLOOR) code = max(code, u > 0.f ? 1u : 0u);
-    else code |= (__float_as_uint(x[e]) >> 24) & 0x80u;
-    w[e / 4] = w[e / 4] * 256u + code;
+    for (int q = 1; q >= 0; --q) {
+      const uint32_t normal = (__float_as_uint(u[q]) + (lot[e + q] << 4) - ((127u - 7u) << 23)) >> 20;
+      uint32_t code = u[q] < 0.015625f ? __float_as_uint(whole[q]) & 15u : normal;
+      if (FLOOR) code = max(code, u[q] > 0.f ? 1u : 0u);
+      else code |= (__float_as_uint(x[e + q]) >> 24) & 0x80u;
+      w[e / 4] = w[e / 4] * 256u + code;
+    }
   }
   uint8_t* p = static_cast<uint8_t*>(to) + i;
   if (vec) {
@@ -197,7 +209,7 @@ __device__ __forceinline__ void adamw_store_codes(void* to, float* scales, long 
 
 // What a step needs of its numbers.
 struct AdamwStep {
-  float rate, root, keep, unscale;
+  float rate, root, keep, unscale, none;
   uint32_t key;
 };
 
@@ -244,12 +256,15 @@ __device__ __forceinline__ void adamw_values(const P& p, const AdamwTensor& t, c
     adamw_widen(0, in.v, v);
   }
   uint32_t lot_m[8], lot_v[8];
+  // Products that are to be rounded before they are added: with a -0 that is not known when the kernel is compiled.  A packed product and a sum of its own are made
+  // one operation with one rounding, their .rn notwithstanding (one moment in five was off by a step).
+  const uint64_t none = adamw_two(now.none, now.none);
   const uint64_t b1 = adamw_two(p.b1, p.b1), c1 = adamw_two(p.c1, p.c1), b2 = adamw_two(p.b2, p.b2), c2 = adamw_two(p.c2, p.c2);
 #pragma unroll
   for (int e = 0; e < 8; e += 2) {
     const uint64_t gg = adamw_mul2(adamw_two(g[e], g[e + 1]), adamw_two(now.unscale, now.unscale));
-    adamw_part(adamw_add2(adamw_mul2(adamw_two(m[e], m[e + 1]), b1), adamw_mul2(gg, c1)), m[e], m[e + 1]);
-    adamw_part(adamw_add2(adamw_mul2(adamw_two(v[e], v[e + 1]), b2), adamw_mul2(adamw_mul2(gg, gg), c2)), v[e], v[e + 1]);
+    adamw_part(adamw_add2(adamw_fma2(adamw_two(m[e], m[e + 1]), b1, none), adamw_fma2(gg, c1, none)), m[e], m[e + 1]);
+    adamw_part(adamw_add2(adamw_fma2(adamw_two(v[e], v[e + 1]), b2, none), adamw_fma2(adamw_mul2(gg, gg), c2, none)), v[e], v[e + 1]);
     float size[2];  // within 2^-23 of the root, also of a subnormal number
     asm("sqrt.approx.f32 %0, %1;" : "=f"(size[0]) : "f"(v[e]));
     asm("sqrt.approx.f32 %0, %1;" : "=f"(size[1]) : "f"(v[e + 1]));
@@ -322,6 +337,7 @@ __global__ void __launch_bounds__(ADAMW_THREADS, 3) adamw_kernel(const __grid_co
     s_now.root = (float)(1.0 / sqrt(1.0 - pow2));
     s_now.keep = (float)(1.0 - lr * p.decay);
     s_now.unscale = p.grad_scale ? __fdiv_rn(1.f, *p.grad_scale) : 1.f;
+    s_now.none = __uint_as_float(p.minus_zero);
     s_now.key = adamw_mix((t * 0x9E3779B9u) ^ p.seed);
   }
   __syncthreads();

@@ -428,6 +428,7 @@ int launch_adamw(const fgms_b200_adamw_tensor* tensors, int n, const fgms_b200_a
   p.b2 = (float)o.beta2; p.c2 = (float)(1.0 - o.beta2);
   p.eps = (float)o.eps;
   p.seed = o.seed;
+  p.minus_zero = 0x80000000u;
   p.lr_device = o.lr_device; p.grad_scale = o.grad_scale; p.found_inf = o.found_inf;
   p.step = o.step;
   p.n = n; p.last = last;

@@ -460,3 +460,45 @@ def test_layers_of_experts_learn_in_one_step_each():
         # the first step: lr * sign(gradient) where it is well above eps, the weight's rounding besides
         want = b * (1 - 1e-2 * 0.01) - 1e-2 * g.double() / (g.double().abs() + 1e-8)
         assert ((w.double() - want).abs() <= want.abs() * 2.0 ** -8 + 1e-2 * 2.0 ** -18).all()
+
+
+def one_operation_at_a_time(x, lot, floor):
+    """Codes and scales in fp32, every operation rounded by itself: what the kernel computes two at a time."""
+    n = x.numel()
+    x, lot = blocks(x), blocks(lot)
+    top = x.abs().amax(1, keepdim=True)
+    scale = top * (1.0 / 448.0)
+    u = (x.abs() * (torch.ones_like(scale) / scale)).clamp(max=448.0)
+    normal = ((u.view(torch.int32) + (lot.int() << 4)) & -(1 << 20)).view(torch.float32)
+    small = torch.floor(u * 512.0 + lot.float() * 2.0 ** -16)
+    if floor:
+        small = torch.where(u > 0, small.clamp(min=1.0), small)
+    code = torch.copysign(torch.where(u >= 2.0 ** -6, normal, small * 2.0 ** -9), x)
+    return code.view(-1)[:n].to(torch.float8_e4m3fn), scale.view(-1)
+
+
+def mixed(h):
+    h = ((h ^ (h >> 16)) * 0x85EBCA6B) & 0xFFFFFFFF
+    h = ((h ^ (h >> 13)) * 0xC2B2AE35) & 0xFFFFFFFF
+    return h ^ (h >> 16)
+
+
+@pytest.mark.parametrize("grad", ["fp32", "fp16", "bf16"])
+def test_codes_are_the_same_bits_as_the_formulas_in_fp32(grad):
+    """So that a step can be repeated, and checked, by anything that rounds as fp32 does."""
+    s = State(counts=[128 * 4096, 1000, 77], param="fp32", grad=grad, bits=8, seed=13)
+    s.g[0].view(-1, 128).mul_(torch.logspace(-3, 1, 4096, device="cuda").to(s.g[0].dtype)[:, None])
+    for seed in (1, 2):
+        want = []
+        t = int(s.step[0]) + 1
+        key = int(mixed(torch.tensor((t * 0x9E3779B9 & 0xFFFFFFFF) ^ seed)))
+        f32 = lambda c, sc: (blocks(c.float()) * sc[:, None]).view(-1)[:c.numel()]
+        for m, v, ms, vs, g in zip(s.m, s.v, s.ms, s.vs, s.g):
+            g = g.float()
+            m, v = f32(m, ms) * B1 + g * (1.0 - B1), f32(v, vs) * B2 + (g * g) * (1.0 - B2)
+            h = mixed((torch.arange(g.numel(), device="cuda") * 0x9E3779B1 + key) & 0xFFFFFFFF)
+            want.append((one_operation_at_a_time(m, h & 0xFFFF, False), one_operation_at_a_time(v, h >> 16, True)))
+        s.run(seed=seed)
+        for i, ((m, ms), (v, vs)) in enumerate(want):
+            assert torch.equal(s.ms[i], ms) and torch.equal(s.vs[i], vs)
+            assert torch.equal(s.m[i].float(), m.float()) and torch.equal(s.v[i].float(), v.float())
