@@ -376,6 +376,8 @@ __global__ void __launch_bounds__(GU_THREADS, 1)
       pair_commit<CG>(smem_u32(&sh->drained));
       mbar_wait(smem_u32(&sh->drained), 0u, nullptr);
     }
+    // the odd CTA: the commits' arrivals at its barriers are behind it before it may end
+    if (CG == 2 && rank != 0) mbar_parked_wait(smem_u32(&sh->drained), 0u, nullptr);
     __syncwarp();
   } else if (warp == 2 && PASS == GROUPED_WGRAD) {
     // ------------------------------------------------------------------ rows behind a group's last one

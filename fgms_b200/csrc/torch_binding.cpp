@@ -16,6 +16,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/graph_task.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <pybind11/pybind11.h>
@@ -641,6 +642,11 @@ Pyramid build_pyramid(const Tensor& coords, int levels, int what) {
 // ---------------------------------------------------------------------------------------------
 // products of ragged groups of rows
 // ---------------------------------------------------------------------------------------------
+// autograd notices that a tensor it has saved was written
+void written(const Tensor& t) {
+  if (t.defined() && !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 int grouped_dtype(const Tensor& t) {
   if (t.scalar_type() == at::kHalf) return FGMS_DTYPE_F16;
   if (t.scalar_type() == at::kBFloat16) return FGMS_DTYPE_BF16;
@@ -673,6 +679,7 @@ void grouped_fwd(const Tensor& in_feats, const Tensor& kernel, const Tensor& out
   c10::cuda::CUDAGuard guard(kernel.device());
   check_status(fgms_b200_grouped_fwd(ptr(in_feats), ptr(kernel), ptr(out), iptr(kpos), (int)out.size(0), (int)kernel.size(1), (int)kernel.size(2),
                                      (int)kernel.size(0), dtype, zero_rest, stream_of(kernel)));
+  written(out);
 }
 
 void grouped_dgrad(const Tensor& grad_out, const Tensor& kernel, const Tensor& in_grad, const Tensor& kpos, bool zero_rest) {
@@ -684,6 +691,7 @@ void grouped_dgrad(const Tensor& grad_out, const Tensor& kernel, const Tensor& i
   c10::cuda::CUDAGuard guard(kernel.device());
   check_status(fgms_b200_grouped_dgrad(ptr(grad_out), ptr(kernel), ptr(in_grad), iptr(kpos), (int)in_grad.size(0), (int)kernel.size(1),
                                        (int)kernel.size(2), (int)kernel.size(0), dtype, zero_rest, stream_of(kernel)));
+  written(in_grad);
 }
 
 void grouped_wgrad(const Tensor& in_feats, const Tensor& grad_out, const Tensor& kernel_grad, const Tensor& kpos) {
@@ -695,6 +703,7 @@ void grouped_wgrad(const Tensor& in_feats, const Tensor& grad_out, const Tensor&
   c10::cuda::CUDAGuard guard(kernel_grad.device());
   check_status(fgms_b200_grouped_wgrad(ptr(in_feats), ptr(grad_out), ptr(kernel_grad), iptr(kpos), (int)in_feats.size(0), (int)kernel_grad.size(1),
                                        (int)kernel_grad.size(2), (int)kernel_grad.size(0), dtype, stream_of(kernel_grad)));
+  written(kernel_grad);
 }
 
 struct GroupedLinear : torch::autograd::Function<GroupedLinear> {
@@ -722,6 +731,14 @@ struct GroupedLinear : torch::autograd::Function<GroupedLinear> {
       w_grad = at::empty_like(weight);
       grouped_wgrad(feats, grad_out, w_grad, kpos);
     }
+    if (!at::GradMode::is_enabled()) return {in_grad, w_grad, Tensor()};
+    // a graph of the backward was asked for: it ends here, and says so to whoever goes through it
+    for (Tensor* t : {&in_grad, &w_grad}) {
+      if (!t->defined()) continue;
+      t->set_requires_grad(true);
+      const auto ends = std::make_shared<torch::autograd::DelayedError>("grouped_linear is not differentiable twice", 1);
+      *t = (*ends)({*t})[0];
+    }
     return {in_grad, w_grad, Tensor()};
   }
 };
@@ -739,11 +756,6 @@ int adamw_dtype(const char* name, const Tensor& t) {
 struct AdamwLists {
   std::vector<Tensor> params, grads, exp_avgs, exp_avg_sqs, masters, exp_avg_scales, exp_avg_sq_scales;  // masters: undefined where there is none
 };
-
-// autograd notices that a tensor it has saved was written
-void written(const Tensor& t) {
-  if (t.defined() && !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
-}
 
 void adamw(const AdamwLists& a, const Tensor& step, const Tensor& lr_tensor, const Tensor& grad_scale, const Tensor& found_inf, fgms_b200_adamw_options o) {
   const size_t n = a.params.size();

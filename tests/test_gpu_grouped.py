@@ -387,3 +387,27 @@ def test_refusals():
         backend.fgms_grouped_wgrad_cuda(x[:9], out, w, kpos)
     with pytest.raises(ValueError, match="one entry more"):
         nn.grouped_linear(x, w, kpos[:2])
+
+
+def test_a_second_derivative_is_refused_when_it_is_taken():
+    from fgms_b200 import nn
+    layer = Layer("fp32", [20, 30], 16, 24, seed=18)
+    x, w = layer.x.clone().requires_grad_(), layer.w.clone().requires_grad_()
+    gx, gw = torch.autograd.grad((nn.grouped_linear(x, w, layer.kpos) ** 2).sum(), (x, w), create_graph=True)
+    plain = torch.autograd.grad((nn.grouped_linear(x, w, layer.kpos) ** 2).sum(), (x, w))
+    assert torch.equal(gx, plain[0]) and torch.equal(gw, plain[1])
+    with pytest.raises(RuntimeError, match="not differentiable twice"):
+        (gx.sum() + gw.sum()).backward()
+    (only,) = torch.autograd.grad((nn.grouped_linear(x, layer.w, layer.kpos) ** 2).sum(), (x,), create_graph=True)
+    assert torch.equal(only, plain[0])
+
+
+def test_autograd_notices_that_an_output_was_written():
+    from fgms_b200 import backend
+    layer = Layer("fp32", [20, 30], 16, 24, seed=19)
+    out = torch.ones_like(layer.g, requires_grad=True)
+    loss = (out * out).sum()
+    with torch.no_grad():
+        backend.fgms_grouped_fwd_cuda(layer.x, layer.w, out, layer.kpos)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
