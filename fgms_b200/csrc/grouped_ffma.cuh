@@ -94,6 +94,7 @@ __global__ void __launch_bounds__(gf_threads(TILE), TILE == 128 ? 2 : 4) grouped
   umma::griddep_wait();
   if (!p.alone) umma::griddep_launch_dependents();
   build_group_table(TILE, p.kpos, p.n_rows, p.groups, first, tiles);
+  if (PARTS) umma::cluster_sync();  // all parts have started: their shared memory may be written
 
   const T *a = static_cast<const T*>(p.a), *b = static_cast<const T*>(p.b);
   T* d = static_cast<T*>(p.d);

@@ -23,7 +23,7 @@ class AdamW(torch.optim.Optimizer):
     traffic; codes are rounded at random, reproducibly for a ``seed``.  float16 and bfloat16 parameters get a float32 ``master`` copy, without
     which updates of less than half a step of their type are lost, unless ``master=False``.  Works in a captured graph (the steps are
     counted on the device; ``lr`` may be a float32 tensor of one value there) and with ``torch.amp.GradScaler``, whose scale and verdict
-    the kernel reads.  Parameters must be contiguous CUDA tensors; a parameter without a gradient is passed over.  No sparse gradients,
+    the kernel reads.  Before a capture every parameter must have taken a step, as its state would be made anew by every replay.  Parameters must be contiguous CUDA tensors; a parameter without a gradient is passed over.  No sparse gradients,
     no ``amsgrad``, no ``maximize``."""
 
     _step_supports_amp_scaling = True  # GradScaler hands over its scale and what it found instead of waiting for the device
@@ -60,6 +60,12 @@ class AdamW(torch.optim.Optimizer):
         if group["master"] and p.dtype != torch.float32:
             s["master"] = p.detach().to(torch.float32, copy=True, memory_format=torch.contiguous_format)
 
+    @staticmethod
+    def _not_in_a_capture():
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a captured step needs parameters that have all taken the same steps before the capture: their state would be made "
+                               "anew by every replay")
+
     @torch.no_grad()
     def step(self, closure=None):
         loss = None
@@ -79,6 +85,7 @@ class AdamW(torch.optim.Optimizer):
                 if not p.is_cuda or not p.is_contiguous():
                     raise ValueError("parameters must be contiguous CUDA tensors")
                 if "step" not in self.state[p]:
+                    self._not_in_a_capture()
                     if p.device not in fresh:
                         fresh[p.device] = torch.zeros(2, dtype=torch.int32, device=p.device)
                     self._init_state(group, p, fresh[p.device])
@@ -88,6 +95,7 @@ class AdamW(torch.optim.Optimizer):
                 states = [self.state[p] for p in params]
                 step = states[0]["step"]
                 if sharing[key] != len(params):  # the others do not take this step
+                    self._not_in_a_capture()
                     step = step.clone()
                     for s in states:
                         s["step"] = step

@@ -502,3 +502,55 @@ def test_codes_are_the_same_bits_as_the_formulas_in_fp32(grad):
         for i, ((m, ms), (v, vs)) in enumerate(want):
             assert torch.equal(s.ms[i], ms) and torch.equal(s.vs[i], vs)
             assert torch.equal(s.m[i].float(), m.float()) and torch.equal(s.v[i].float(), v.float())
+
+
+def test_values_beyond_32_bits():
+    """A tensor of more than 2^31 values: the last ones take the step of the formula, those that an offset cut to 32 bits would meet keep to theirs."""
+    from fgms_b200 import backend
+    n = 2 ** 31 + 3000
+    p = torch.full((n,), 0.5, device="cuda", dtype=torch.bfloat16)
+    g = torch.zeros(n, device="cuda", dtype=torch.bfloat16)
+    g[-1000:] = 1.0
+    m, v = (torch.zeros(n, device="cuda", dtype=torch.uint8).view(torch.float8_e4m3fn) for _ in range(2))
+    ms, vs = (torch.zeros((n + 127) // 128, device="cuda") for _ in range(2))
+    step = torch.zeros(2, dtype=torch.int32, device="cuda")
+    backend.fgms_adamw_cuda([p], [g], [m], [v], step, 0.25, weight_decay=0.0, exp_avg_scales=[ms], exp_avg_sq_scales=[vs])
+    assert (p[-1000:] == 0.25).all() and (p[:5000] == 0.5).all() and (p[n // 2:n // 2 + 5000] == 0.5).all() and (p[-3000:-1000] == 0.5).all()
+    assert ms[-1] > 0 and not ms[:-9].any() and vs[-1] > 0 and not vs[:-9].any()
+    assert (m[-1000:].float() > 0).all() and (v[-1000:].float() > 0).all() and not m[-3000:-1000].float().any()
+
+
+def test_optimizer_in_a_capture():
+    """Refused where the state would be made anew by every replay: before the first step, and where a parameter parts from the others."""
+    from fgms_b200 import optim
+    a, b = small_net(), small_net()
+    mine, other = optim.AdamW(a.parameters(), lr=1e-2), optim.AdamW(b.parameters(), lr=1e-2)
+    give_gradients(a, 0)
+    give_gradients(b, 0)
+    side = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="before the capture"):
+        with torch.cuda.graph(graph, stream=side):
+            mine.step()
+    torch.cuda.synchronize()
+    assert not any("exp_avg" in s for s in mine.state.values())
+    mine.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        mine.step()
+    for _ in range(3):
+        graph.replay()
+    for _ in range(4):
+        other.step()
+    assert all(torch.equal(p, q) for p, q in zip(a.parameters(), b.parameters()))
+    kept = next(a.parameters()).grad
+    next(a.parameters()).grad = None
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="before the capture"):
+        with torch.cuda.graph(graph):
+            mine.step()
+    torch.cuda.synchronize()
+    next(a.parameters()).grad = kept
+    mine.step()
+    other.step()
+    assert all(torch.equal(p, q) for p, q in zip(a.parameters(), b.parameters()))

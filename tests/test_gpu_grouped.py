@@ -411,3 +411,49 @@ def test_autograd_notices_that_an_output_was_written():
         backend.fgms_grouped_fwd_cuda(layer.x, layer.w, out, layer.kpos)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         loss.backward()
+
+
+@pytest.mark.parametrize("which", PASSES)
+@pytest.mark.parametrize("keep", [8, 64])
+def test_with_sms_kept_free(which, keep):
+    from fgms_b200 import _lib
+    assert _lib.lib.fgms_b200_set_reserved_sms(keep) == _lib.OK
+    try:
+        for dtype, sizes, c_in, c_out in (("bf16", [300, 0, 700], 256, 520), ("bf16", [3], 4096, 136), ("fp32", [300, 0, 70], 100, 130)):
+            Layer(dtype, sizes, c_in, c_out, seed=20).check(which)
+    finally:
+        _lib.lib.fgms_b200_set_reserved_sms(0)
+
+
+@pytest.mark.parametrize("which", PASSES)
+@pytest.mark.parametrize("dtype", ["fp16", "fp32"])
+@pytest.mark.parametrize("c_in,c_out", [(8, 70000), (70000, 8), (1, 40001)])
+def test_very_wide(dtype, which, c_in, c_out):
+    Layer(dtype, [3, 0, 14], c_in, c_out, seed=21).check(which)
+
+
+def test_rows_beyond_32_bits():
+    """More than 2^31 values in the rows: the last ones are the ones that are multiplied."""
+    from fgms_b200 import backend
+    rows, c = (1 << 20) + 77, 2056
+    x = torch.zeros((rows, c), dtype=torch.float16, device="cuda")
+    x[-70:] = torch.randn((70, c), device="cuda").half()
+    w = (torch.randn((2, c, 64), device="cuda") * c ** -0.5).half()
+    kpos = kpos_of([rows - 50, 50])
+    out = torch.empty((rows, 64), dtype=torch.float16, device="cuda")
+    backend.fgms_grouped_fwd_cuda(x, w, out, kpos)
+    for s, i in ((slice(-70, -50), 0), (slice(-50, None), 1)):
+        near(out[s], x[s].double() @ w[i].double(), x[s].double().abs() @ w[i].double().abs(), c)
+    assert not out[:-70].any()
+    dw = torch.empty_like(w)
+    out.fill_(1)
+    backend.fgms_grouped_wgrad_cuda(x, out, dw, kpos)
+    for s, i in ((slice(-70, -50), 0), (slice(-50, None), 1)):
+        want = x[s].double().sum(0)[:, None].expand(-1, 64)
+        near(dw[i], want, x[s].double().abs().sum(0)[:, None].expand(-1, 64), 70)
+    back = torch.empty_like(x)
+    out.zero_()
+    out[-50:] = 1
+    backend.fgms_grouped_dgrad_cuda(out, w, back, kpos)
+    near(back[-50:], w[1].double().sum(1).expand(50, -1), w[1].double().abs().sum(1).expand(50, -1), 64)
+    assert not back[:-50].any()
