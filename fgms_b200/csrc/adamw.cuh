@@ -344,21 +344,25 @@ __global__ void __launch_bounds__(ADAMW_THREADS, 3) adamw_kernel(const __grid_co
     at.find(p, blockIdx.x);
     if (at.all) in.template read<true>(p.t[at.k], at.first + mine, 8);
   }
-  if (threadIdx.x == 0) {
+  // The powers in 64 bits, as 1 - beta^t has few of beta's; what is made of them in 32.  A warp each: they are the longest part of a small step.
+  if (threadIdx.x % 32 == 0 && threadIdx.x < 96) {
     const uint32_t t = (uint32_t)p.step[0] + 1u;
-    double pow1 = 1.0, pow2 = 1.0, s1 = p.beta1, s2 = p.beta2;
-    for (uint32_t e = t; e; e >>= 1) {
-      if (e & 1u) { pow1 *= s1; pow2 *= s2; }
-      s1 *= s1;
-      s2 *= s2;
-    }
     const double lr = p.lr_device ? (double)*p.lr_device : p.lr;
-    s_now.rate = (float)(lr / (1.0 - pow1));
-    s_now.root = (float)(1.0 / sqrt(1.0 - pow2));
-    s_now.keep = (float)(1.0 - lr * p.decay);
-    s_now.unscale = p.grad_scale ? __fdiv_rn(1.f, *p.grad_scale) : 1.f;
-    s_now.none = __uint_as_float(p.minus_zero);
-    s_now.key = adamw_mix((t * 0x9E3779B9u) ^ p.seed);
+    if (threadIdx.x == 64) {
+      s_now.keep = (float)(1.0 - lr * p.decay);
+      s_now.unscale = p.grad_scale ? __fdiv_rn(1.f, *p.grad_scale) : 1.f;
+      s_now.none = __uint_as_float(p.minus_zero);
+      s_now.key = adamw_mix((t * 0x9E3779B9u) ^ p.seed);
+    } else {
+      double power = 1.0, square = threadIdx.x == 0 ? p.beta1 : p.beta2;
+      for (uint32_t e = t; e; e >>= 1) {
+        if (e & 1u) power *= square;
+        square *= square;
+      }
+      const float rest = (float)(1.0 - power);
+      if (threadIdx.x == 0) s_now.rate = __fdiv_rn((float)lr, rest);
+      else s_now.root = __fdiv_rn(1.f, __fsqrt_rn(rest));
+    }
   }
   __syncthreads();
   const AdamwStep now = s_now;
@@ -384,7 +388,6 @@ __global__ void __launch_bounds__(ADAMW_THREADS, 3) adamw_kernel(const __grid_co
   if (p.last) {
     __syncthreads();
     if (threadIdx.x == 0) {
-      __threadfence();
       if (atomicAdd(p.step + 1, 1) == (int)gridDim.x - 1) {
         p.step[1] = 0;
         p.step[0] += 1;

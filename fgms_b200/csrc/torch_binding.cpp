@@ -753,8 +753,10 @@ int adamw_dtype(const char* name, const Tensor& t) {
   return FGMS_DTYPE_F32;
 }
 
+// The tensors of the caller's lists, which hold them for the length of the call: a hundred references counted up and down cost as much as the launch.
+using TensorList = std::vector<const Tensor*>;
 struct AdamwLists {
-  std::vector<Tensor> params, grads, exp_avgs, exp_avg_sqs, masters, exp_avg_scales, exp_avg_sq_scales;  // masters: undefined where there is none
+  TensorList params, grads, exp_avgs, exp_avg_sqs, masters, exp_avg_scales, exp_avg_sq_scales;  // masters: null where there is none
 };
 
 void adamw(const AdamwLists& a, const Tensor& step, const Tensor& lr_tensor, const Tensor& grad_scale, const Tensor& found_inf, fgms_b200_adamw_options o) {
@@ -771,7 +773,7 @@ void adamw(const AdamwLists& a, const Tensor& step, const Tensor& lr_tensor, con
   o.grad_scale = one("grad_scale", grad_scale);
   o.found_inf = one("found_inf", found_inf);
   o.step = step.data_ptr<int32_t>();
-  const bool eight = !a.exp_avg_scales.empty() || !a.exp_avg_sq_scales.empty() || (n > 0 && a.exp_avgs.size() == n && a.exp_avgs[0].scalar_type() == at::kFloat8_e4m3fn);
+  const bool eight = !a.exp_avg_scales.empty() || !a.exp_avg_sq_scales.empty() || (n > 0 && a.exp_avgs.size() == n && a.exp_avgs[0]->scalar_type() == at::kFloat8_e4m3fn);
   o.state_bits = eight ? 8 : 32;
   auto length = [&](const char* name, size_t got) { TORCH_CHECK_VALUE(got == n, name, " has ", got, " tensors, params ", n); };
   length("grads", a.grads.size());
@@ -784,7 +786,7 @@ void adamw(const AdamwLists& a, const Tensor& step, const Tensor& lr_tensor, con
   }
   std::vector<fgms_b200_adamw_tensor> list(n);
   for (size_t i = 0; i < n; ++i) {
-    const Tensor& p = a.params[i];
+    const Tensor &p = *a.params[i], &g = *a.grads[i], &m = *a.exp_avgs[i], &v = *a.exp_avg_sqs[i];
     auto check = [&](const char* name, const Tensor& t, int64_t count, at::ScalarType type) {
       TORCH_CHECK_VALUE(t.device() == device, name, " ", i, " must live on ", device, ", got ", t.device());
       TORCH_CHECK_VALUE(t.is_contiguous(), name, " ", i, " must be contiguous");
@@ -794,34 +796,35 @@ void adamw(const AdamwLists& a, const Tensor& step, const Tensor& lr_tensor, con
     const int64_t count = p.numel(), blocks = (count + 127) / 128;
     const at::ScalarType moment = eight ? at::kFloat8_e4m3fn : at::kFloat;
     check("param", p, count, p.scalar_type());
-    check("grad", a.grads[i], count, a.grads[i].scalar_type());
-    check("exp_avg", a.exp_avgs[i], count, moment);
-    check("exp_avg_sq", a.exp_avg_sqs[i], count, moment);
+    check("grad", g, count, g.scalar_type());
+    check("exp_avg", m, count, moment);
+    check("exp_avg_sq", v, count, moment);
     fgms_b200_adamw_tensor& t = list[i];
     t = {};
     t.count = count;
     t.param = ptr(p);
-    t.grad = ptr(a.grads[i]);
-    t.exp_avg = ptr(a.exp_avgs[i]);
-    t.exp_avg_sq = ptr(a.exp_avg_sqs[i]);
+    t.grad = ptr(g);
+    t.exp_avg = ptr(m);
+    t.exp_avg_sq = ptr(v);
     t.param_dtype = adamw_dtype("parameter", p);
-    t.grad_dtype = adamw_dtype("gradient", a.grads[i]);
-    if (!a.masters.empty() && a.masters[i].defined()) {
-      check("master", a.masters[i], count, at::kFloat);
-      t.master = static_cast<float*>(ptr(a.masters[i]));
+    t.grad_dtype = adamw_dtype("gradient", g);
+    if (!a.masters.empty() && a.masters[i]) {
+      check("master", *a.masters[i], count, at::kFloat);
+      t.master = static_cast<float*>(ptr(*a.masters[i]));
     }
     if (eight) {
-      check("exp_avg_scale", a.exp_avg_scales[i], blocks, at::kFloat);
-      check("exp_avg_sq_scale", a.exp_avg_sq_scales[i], blocks, at::kFloat);
-      t.exp_avg_scale = static_cast<float*>(ptr(a.exp_avg_scales[i]));
-      t.exp_avg_sq_scale = static_cast<float*>(ptr(a.exp_avg_sq_scales[i]));
+      check("exp_avg_scale", *a.exp_avg_scales[i], blocks, at::kFloat);
+      check("exp_avg_sq_scale", *a.exp_avg_sq_scales[i], blocks, at::kFloat);
+      t.exp_avg_scale = static_cast<float*>(ptr(*a.exp_avg_scales[i]));
+      t.exp_avg_sq_scale = static_cast<float*>(ptr(*a.exp_avg_sq_scales[i]));
     }
   }
   c10::cuda::CUDAGuard guard(device);
   check_status(fgms_b200_adamw(list.data(), (int)n, &o, stream_of(step)));
   written(step);
   for (const auto* tensors : {&a.params, &a.exp_avgs, &a.exp_avg_sqs, &a.masters, &a.exp_avg_scales, &a.exp_avg_sq_scales})
-    for (const Tensor& t : *tensors) written(t);
+    for (const Tensor* t : *tensors)
+      if (t) written(*t);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -891,15 +894,14 @@ PyObject* py_sparse_conv(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return THPVariable_Wrap(SparseConv::apply(feats, weight, kpos, imap, omap, int_arg(a[5]), bool_arg(a[6])));
   END_HANDLE_TH_ERRORS
 }
-std::vector<Tensor> tensor_list(PyObject* list, const char* name, bool gaps = false) {
+std::vector<const Tensor*> tensor_list(PyObject* list, const char* name, bool gaps = false) {
   TORCH_CHECK_TYPE(PyList_Check(list) || PyTuple_Check(list), name, " must be a list of tensors");
   const Py_ssize_t n = PySequence_Fast_GET_SIZE(list);
-  std::vector<Tensor> out;
+  std::vector<const Tensor*> out;
   out.reserve(n);
   for (Py_ssize_t i = 0; i < n; ++i) {
     PyObject* o = PySequence_Fast_GET_ITEM(list, i);
-    if (gaps && o == Py_None) out.emplace_back();
-    else out.push_back(feat_arg(o, name));
+    out.push_back(gaps && o == Py_None ? nullptr : &feat_arg(o, name));
   }
   return out;
 }
@@ -950,7 +952,14 @@ PyObject* py_sparse_stack(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   expect(n, 5);
   const Tensor& feats = feat_arg(a[0], "in_feats");
-  const std::vector<Tensor> weights = tensor_list(a[1], "kernels"), maps = tensor_list(a[2], "maps");
+  auto tensors = [](PyObject* list, const char* name) {
+    TORCH_CHECK_TYPE(PyList_Check(list), name, " must be a list");
+    std::vector<Tensor> out;
+    out.reserve(PyList_GET_SIZE(list));
+    for (Py_ssize_t i = 0; i < PyList_GET_SIZE(list); ++i) out.push_back(feat_arg(PyList_GET_ITEM(list, i), name));
+    return out;
+  };
+  const std::vector<Tensor> weights = tensors(a[1], "kernels"), maps = tensors(a[2], "maps");
   TORCH_CHECK_TYPE(PyList_Check(a[3]), "plan must be a list");
   StackPlan plan;
   for (Py_ssize_t i = 0; i < PyList_GET_SIZE(a[3]); ++i) plan.push_back(int_arg(PyList_GET_ITEM(a[3], i)));
