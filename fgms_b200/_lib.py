@@ -56,9 +56,10 @@ SIGNATURES = {
     "fgms_b200_neighbor_table_bytes": (c_size_t, [c_int, c_int]),
     "fgms_b200_build_neighbor_table": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int, c_int, c_void_p, c_size_t, c_void_p]),
     "fgms_b200_fwd_output_stationary": (c_int, [c_void_p] * 4 + [c_int] * 7 + [c_void_p, c_int, c_int, c_void_p]),
-    "fgms_b200_grouped_fwd": (c_int, [c_void_p] * 4 + [c_int] * 6 + [c_void_p]),
-    "fgms_b200_grouped_dgrad": (c_int, [c_void_p] * 4 + [c_int] * 6 + [c_void_p]),
-    "fgms_b200_grouped_wgrad": (c_int, [c_void_p] * 4 + [c_int] * 5 + [c_void_p]),
+    "fgms_b200_grouped_fwd": (c_int, [c_void_p] * 4 + [c_int] * 6 + [c_void_p, c_size_t, c_void_p]),
+    "fgms_b200_grouped_dgrad": (c_int, [c_void_p] * 4 + [c_int] * 6 + [c_void_p, c_size_t, c_void_p]),
+    "fgms_b200_grouped_wgrad": (c_int, [c_void_p] * 4 + [c_int] * 5 + [c_void_p, c_size_t, c_void_p]),
+    "fgms_b200_grouped_workspace_bytes": (c_size_t, [c_int] + [c_void_p] * 3 + [c_int] * 5),
     "fgms_b200_adamw": (c_int, [c_void_p, c_int, c_void_p, c_void_p]),
     "fgms_b200_peer_exchange_flag_bytes": (c_size_t, [c_int]),
     "fgms_b200_peer_exchange": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int64, ctypes.c_uint32, c_int64, c_int, c_void_p]),

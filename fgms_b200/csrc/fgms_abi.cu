@@ -30,6 +30,7 @@
 #include "umma_osfwd.cuh"
 #include "grouped_ffma.cuh"
 #include "grouped_umma.cuh"
+#include "grouped_pitch.cuh"
 #include "adamw.cuh"
 
 namespace {
@@ -324,9 +325,43 @@ int run_wgrad(const void* in_feats, const void* out_grad, void* kernel_grad, con
 }
 
 // products of ragged groups of rows (csrc/grouped.cuh)
+// The call on copies whose rows a tensor map can describe (csrc/grouped_pitch.cuh).
+template <int PASS>
+int run_grouped_copied(fgms::GroupedParams p, const fgms::GroupedCopies& c, uint8_t* workspace, bool bf16, cudaStream_t st, const DeviceInfo& di) {
+  const auto rows_of = [](const fgms::GroupedCopies::One& o, const void* src, void* dst, int src_pitch, int dst_pitch) {
+    return fgms::GroupedRows{static_cast<const uint16_t*>(src), static_cast<uint16_t*>(dst), o.needed ? o.rows : 0, src_pitch, dst_pitch, o.len};
+  };
+  const auto grid_for = [&](long long rows, int len) {
+    const long long warps = rows * ((len + fgms::GP_SEGMENT - 1) / fgms::GP_SEGMENT), blocks = (warps + 7) / 8, most = 8ll * di.sms;
+    return dim3((unsigned)(blocks < 1 ? 1 : blocks < most ? blocks : most));
+  };
+  void* d = p.d;
+  const int zero_rest = p.zero_rest;
+  if (c.a.needed || c.b.needed) {
+    const fgms::GroupedRows x = rows_of(c.a, p.a, workspace + c.a.at, c.a.len, c.a.pitch), y = rows_of(c.b, p.b, workspace + c.b.at, c.b.len, c.b.pitch);
+    if (fgms::launch_pdl(fgms::grouped_copy_kernel, grid_for(x.rows + y.rows, x.len > y.len ? x.len : y.len), fgms::GP_THREADS, 0, st, x, y) != cudaSuccess)
+      return fail(FGMS_ERR_CUDA, "grouped_copy_kernel: %s", cudaGetErrorString(cudaGetLastError()));
+    if (int rc = check_launch("grouped_copy_kernel")) return rc;
+  }
+  if (c.a.needed) { p.a = workspace + c.a.at; p.a_pitch = c.a.pitch; }
+  if (c.b.needed) { p.b = workspace + c.b.at; p.b_pitch = c.b.pitch; }
+  if (c.d.needed) { p.d = workspace + c.d.at; p.d_pitch = c.d.pitch; p.zero_rest = 0; }
+  bool shape = false;
+  if (!fgms::grouped_umma_takes(p, &shape) || fgms::launch_grouped_umma<PASS>(p, bf16, st, di.sms, di.max_smem_optin) != 0)
+    return fail(FGMS_ERR_CUDA, "grouped_umma_kernel: %s", cudaGetErrorString(cudaGetLastError()));
+  if (int rc = check_launch("grouped_umma_kernel")) return rc;
+  if (!c.d.needed) return FGMS_OK;
+  const fgms::GroupedRows out = rows_of(c.d, workspace + c.d.at, d, c.d.pitch, c.d.len);
+  const cudaError_t e = PASS == fgms::GROUPED_WGRAD
+                            ? fgms::launch_pdl(fgms::grouped_copy_kernel, grid_for(out.rows, out.len), fgms::GP_THREADS, 0, st, out, fgms::GroupedRows{})
+                            : fgms::launch_pdl(fgms::grouped_copy_back_kernel, grid_for(out.rows, out.len), fgms::GP_THREADS, 0, st, out, p.kpos, p.groups, zero_rest);
+  if (e != cudaSuccess) return fail(FGMS_ERR_CUDA, "grouped_copy_back_kernel: %s", cudaGetErrorString(cudaGetLastError()));
+  return check_launch("grouped_copy_back_kernel");
+}
+
 template <int PASS>
 int run_grouped(const void* a, const void* b, void* d, const int32_t* kpos, int n_rows, int c_in, int c_out, int groups, int dtype, int zero_rest,
-                void* stream) {
+                void* workspace, size_t workspace_bytes, void* stream) {
   if (n_rows < 0) return fail(FGMS_ERR_INVALID_ARG, "negative row count");
   if (c_in < 1 || c_out < 1) return fail(FGMS_ERR_INVALID_ARG, "channel counts must be >= 1");
   if (groups < 1 || groups > FGMS_GROUPED_MAX_GROUPS)
@@ -344,7 +379,14 @@ int run_grouped(const void* a, const void* b, void* d, const int32_t* kpos, int 
   if (d_bytes == 0) return FGMS_OK;
   DeviceInfo di;
   if (int rc = device_info(&di)) return rc;
-  const fgms::GroupedParams p{a, b, d, kpos, n_rows, c_in, c_out, groups, zero_rest, di.reserved > 0};
+  fgms::GroupedParams p{};
+  p.a = a; p.b = b; p.d = d; p.kpos = kpos;
+  p.n_rows = n_rows; p.c_in = c_in; p.c_out = c_out; p.groups = groups;
+  p.zero_rest = zero_rest;
+  p.a_pitch = PASS == fgms::GROUPED_DGRAD ? c_out : c_in;
+  p.b_pitch = c_out;
+  p.d_pitch = PASS == fgms::GROUPED_DGRAD ? c_in : c_out;
+  p.alone = di.reserved > 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   bool tensor_cores = false;
   if (dtype != FGMS_DTYPE_F32) {
@@ -352,6 +394,14 @@ int run_grouped(const void* a, const void* b, void* d, const int32_t* kpos, int 
       if (fgms::launch_grouped_umma<PASS>(p, dtype == FGMS_DTYPE_BF16, st, di.sms, di.max_smem_optin) != 0)
         return fail(FGMS_ERR_CUDA, "grouped_umma_kernel: %s", cudaGetErrorString(cudaGetLastError()));
       return check_launch("grouped_umma_kernel");
+    }
+    if (workspace && workspace_bytes > 0) {
+      const fgms::GroupedCopies c = fgms::grouped_copies<PASS>(a, b, d, n_rows, c_in, c_out, groups);
+      if (c.total > workspace_bytes || (reinterpret_cast<uintptr_t>(workspace) & 255))
+        return fail(FGMS_ERR_WORKSPACE, "a workspace of %zu bytes on a 256-byte boundary is needed", c.total);
+      const Range rw{workspace, c.total};
+      if (rw.overlaps(ra) || rw.overlaps(rb) || rw.overlaps(rd) || rw.overlaps(rk)) return fail(FGMS_ERR_WORKSPACE, "the workspace overlaps a tensor");
+      if (c.total > 0) return run_grouped_copied<PASS>(p, c, static_cast<uint8_t*>(workspace), dtype == FGMS_DTYPE_BF16, st, di);
     }
     if (tensor_cores) g_fallbacks.fetch_add(1, std::memory_order_relaxed);  // pointers not 16-byte aligned: CUDA-core path, counted
   }
@@ -1076,21 +1126,29 @@ int fgms_b200_fwd_output_stationary(const void* in_feats, const void* kernel, vo
 // Products of ragged groups of rows (csrc/grouped.cuh)
 // ---------------------------------------------------------------------------------------------
 int fgms_b200_grouped_fwd(const void* in_feats, const void* kernel, void* out_feats, const int32_t* kpos, int n_rows, int c_in, int c_out, int groups,
-                          int dtype, int zero_rest, void* stream) {
+                          int dtype, int zero_rest, void* workspace, size_t workspace_bytes, void* stream) {
   TraceRange trace_range("fgms_b200_grouped_fwd");
-  return run_grouped<fgms::GROUPED_FWD>(in_feats, kernel, out_feats, kpos, n_rows, c_in, c_out, groups, dtype, zero_rest, stream);
+  return run_grouped<fgms::GROUPED_FWD>(in_feats, kernel, out_feats, kpos, n_rows, c_in, c_out, groups, dtype, zero_rest, workspace, workspace_bytes, stream);
 }
 
 int fgms_b200_grouped_dgrad(const void* out_grad, const void* kernel, void* in_grad, const int32_t* kpos, int n_rows, int c_in, int c_out, int groups,
-                            int dtype, int zero_rest, void* stream) {
+                            int dtype, int zero_rest, void* workspace, size_t workspace_bytes, void* stream) {
   TraceRange trace_range("fgms_b200_grouped_dgrad");
-  return run_grouped<fgms::GROUPED_DGRAD>(out_grad, kernel, in_grad, kpos, n_rows, c_in, c_out, groups, dtype, zero_rest, stream);
+  return run_grouped<fgms::GROUPED_DGRAD>(out_grad, kernel, in_grad, kpos, n_rows, c_in, c_out, groups, dtype, zero_rest, workspace, workspace_bytes, stream);
 }
 
 int fgms_b200_grouped_wgrad(const void* in_feats, const void* out_grad, void* kernel_grad, const int32_t* kpos, int n_rows, int c_in, int c_out,
-                            int groups, int dtype, void* stream) {
+                            int groups, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
   TraceRange trace_range("fgms_b200_grouped_wgrad");
-  return run_grouped<fgms::GROUPED_WGRAD>(in_feats, out_grad, kernel_grad, kpos, n_rows, c_in, c_out, groups, dtype, 0, stream);
+  return run_grouped<fgms::GROUPED_WGRAD>(in_feats, out_grad, kernel_grad, kpos, n_rows, c_in, c_out, groups, dtype, 0, workspace, workspace_bytes, stream);
+}
+
+size_t fgms_b200_grouped_workspace_bytes(int pass, const void* a, const void* b, const void* d, int n_rows, int c_in, int c_out, int groups, int dtype) {
+  if (dtype != FGMS_DTYPE_F16 && dtype != FGMS_DTYPE_BF16) return 0;
+  if (n_rows < 1 || c_in < 1 || c_out < 1 || groups < 1 || groups > FGMS_GROUPED_MAX_GROUPS) return 0;
+  if (pass == 0) return fgms::grouped_copies<fgms::GROUPED_FWD>(a, b, d, n_rows, c_in, c_out, groups).total;
+  if (pass == 1) return fgms::grouped_copies<fgms::GROUPED_DGRAD>(a, b, d, n_rows, c_in, c_out, groups).total;
+  return pass == 2 ? fgms::grouped_copies<fgms::GROUPED_WGRAD>(a, b, d, n_rows, c_in, c_out, groups).total : 0;
 }
 
 int fgms_b200_adamw(const fgms_b200_adamw_tensor* tensors, int n, const fgms_b200_adamw_options* options, void* stream) {

@@ -24,6 +24,7 @@ struct GroupedParams {
   const int32_t* kpos;  // [groups + 1]
   int n_rows, c_in, c_out, groups;
   int zero_rest;  // forward, input gradient: rows of no group become zeros
+  int a_pitch, b_pitch, d_pitch;  // values from a row to the next: the widths, except on the tensor cores with copied rows
   int alone;      // see GmsParams
 };
 

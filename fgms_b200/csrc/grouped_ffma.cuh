@@ -1,5 +1,5 @@
 // Grouped products on the CUDA cores: fp32 storage in exact fp32, and fp16 / bf16 whose rows do not start on 16-byte boundaries (widths
-// that are no multiples of 8, views), which a tensor map cannot describe.  Any size, any alignment.
+// that are no multiples of 8, views), which a tensor map cannot describe, where copying them does not pay (grouped_pitch.cuh).  Any size, any alignment.
 //
 // A CTA computes tiles of TILE x TILE values of D, the contraction in steps of 16: both operands are widened to fp32 on their way
 // into shared memory, laid out with the contraction index outermost, and every thread keeps 8 rows by TILE / 16 columns of sums in registers as packed

@@ -20,6 +20,12 @@
 //
 // Two accumulators in tensor memory: the epilogue of a tile runs beside the next one's MMAs.  All waits are bounded; a wait that runs out sets the
 // CTA's abort flag and is counted.
+//
+// 32768 rows of 32 even groups 2048 -> 4096, bf16, kept busy for half a second: forward 445-452 us (1225 TFLOP/s), input gradient 451-457, weight gradient 464,
+// where the library's batched product takes 441-444 and one product of that many operations 403-416; all run into the power limit.  A short burst 385
+// (1430 TFLOP/s), 97 us a quarter of it.  What bounds that: without loads behind the first ring 78 us instead of 97, without the epilogue 91, without its stores
+// 91; the tensor pipe alone would be 60.  So it is the 64 KB a stage that a pair reads from L2 (42 bytes a cycle and SM), then the stores that share
+// the way.  96 rows in 64 groups 2048 -> 1024 46 us, 5.8 TB/s of weights.
 #pragma once
 #include "grouped.cuh"
 
@@ -443,8 +449,8 @@ __global__ void __launch_bounds__(GU_THREADS, 1)
     const int channels = PASS == GROUPED_DGRAD ? p.c_in : p.c_out;
     uint16_t* out = static_cast<uint16_t*>(p.d);
     if (PASS != GROUPED_WGRAD && p.zero_rest)
-      zero_other_rows(p.d, (size_t)channels * 2, first, p.groups, p.n_rows, threadIdx.x - GU_EPI_WARP0 * 32, GU_EPI_WARPS * 32);
-    const size_t pitch = 2 * (size_t)channels;
+      zero_other_rows(p.d, (size_t)p.d_pitch * 2, first, p.groups, p.n_rows, threadIdx.x - GU_EPI_WARP0 * 32, GU_EPI_WARPS * 32);
+    const size_t pitch = 2 * (size_t)p.d_pitch;
     // The patch of four warps: 32 rows of 128 channels, 256 bytes each, whose 16-byte chunks are permuted so that neither the eight rows of a
     // matrix nor eight consecutive chunks of a row meet in a bank.
     const uint32_t patch = stage0 + (uint32_t)(cfg.stages * cfg.stage_bytes) + (uint32_t)half * GU_PATCH_BYTES;
@@ -455,7 +461,7 @@ __global__ void __launch_bounds__(GU_THREADS, 1)
     for (; !SPLIT && tile.left > 0 && ok; tile.next()) {
       const bool some = tile.k_len > 0;  // a group without rows has a gradient of zeros
       const int ch = tile.m0 + (int)rank * 128 + (lane & 15) * 8;
-      uint16_t* to = out + (PASS == GROUPED_WGRAD ? (size_t)tile.g * p.c_in + tile.n0 : (size_t)tile.n0) * channels + ch;
+      uint16_t* to = out + (PASS == GROUPED_WGRAD ? (size_t)tile.g * p.c_in + tile.n0 : (size_t)tile.n0) * p.d_pitch + ch;
       const bool mine = ch < channels;
       if (some) {
         ok = four_agree(half, pair_wait<false>(smem_u32(&sh->tmem_full[buf]), ph, abort_flag));
@@ -495,7 +501,7 @@ __global__ void __launch_bounds__(GU_THREADS, 1)
         for (int i = 0; i < 4; ++i)
           asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
                        : "=r"(o[i].x), "=r"(o[i].y), "=r"(o[i].z), "=r"(o[i].w) : "r"(chunk_at(r0 + 2 * i, lane & 15)) : "memory");
-        uint16_t* row = to + (size_t)(j0 + r0) * channels;
+        uint16_t* row = to + (size_t)(j0 + r0) * p.d_pitch;
         const int rows = mine ? tile.n - j0 - r0 : 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i, row += pitch)
@@ -549,7 +555,7 @@ __global__ void __launch_bounds__(GU_THREADS, 1)
       const int ch = 2 * (thread & 63);
       const int n = min(width, tile.n - part * width);
       uint16_t* out = static_cast<uint16_t*>(p.d) +
-                      ((PASS == GROUPED_WGRAD ? (size_t)tile.g * p.c_in + tile.n0 : (size_t)tile.n0) + part * width) * channels + tile.m0 + ch;
+                      ((PASS == GROUPED_WGRAD ? (size_t)tile.g * p.c_in + tile.n0 : (size_t)tile.n0) + part * width) * p.d_pitch + tile.m0 + ch;
       if (tile.m0 + ch < channels)
         for (int c = thread >> 6; c < n; c += GU_EPI_WARPS / 2) {
           float lo = 0.f, hi = 0.f;
@@ -562,7 +568,7 @@ __global__ void __launch_bounds__(GU_THREADS, 1)
           uint32_t two;
           if (cfg.bf16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(two) : "f"(hi), "f"(lo));
           else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(two) : "f"(hi), "f"(lo));
-          *reinterpret_cast<uint32_t*>(out + (size_t)c * channels) = two;
+          *reinterpret_cast<uint32_t*>(out + (size_t)c * p.d_pitch) = two;
         }
     }
     tc_fence_before();
@@ -579,15 +585,15 @@ __global__ void __launch_bounds__(GU_THREADS, 1)
   }
 }
 
-// A tensor map of 16-bit values, boxes of 64 values (128 bytes, swizzled) by `box` rows: of a matrix [rows][cols], or with `mats` > 0 of that
-// many of them.
-inline int grouped_tensor_map(CUtensorMap* map, const void* data, int cols, int rows, int mats, int box, bool bf16) {
+// A tensor map of 16-bit values, boxes of 64 values (128 bytes, swizzled) by `box` rows: of a matrix [rows][cols] of rows `row` values apart, or with
+// `mats` > 0 of that many of them.
+inline int grouped_tensor_map(CUtensorMap* map, const void* data, int cols, int row, int rows, int mats, int box, bool bf16) {
   using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                               const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
   const Encode encode = reinterpret_cast<Encode>(tensor_map_encoder());
   if (encode == nullptr) return -1000 - (int)CUDA_ERROR_NOT_FOUND;
   const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)(mats > 0 ? mats : 1)};
-  const cuuint64_t pitch[2] = {(cuuint64_t)cols * 2, (cuuint64_t)cols * 2 * (cuuint64_t)rows};
+  const cuuint64_t pitch[2] = {(cuuint64_t)row * 2, (cuuint64_t)row * 2 * (cuuint64_t)rows};
   const cuuint32_t boxes[3] = {64, (cuuint32_t)box, 1}, steps[3] = {1, 1, 1};
   const auto made = [&] {
     return encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, mats > 0 ? 3 : 2, const_cast<void*>(data), dims, pitch, boxes,
@@ -604,7 +610,7 @@ inline int grouped_tensor_map(CUtensorMap* map, const void* data, int cols, int 
 // Whether the kernel takes a call: what the tensor maps and the stores ask for; tiles (of 64 x 128 values at least) are counted in an int.
 inline bool grouped_umma_takes(const GroupedParams& p, bool* shape) {
   const long long wide = p.c_in > p.c_out ? p.c_in : p.c_out, rows = (long long)p.n_rows > (long long)p.groups * p.c_in ? p.n_rows : (long long)p.groups * p.c_in;
-  *shape = p.c_in % 8 == 0 && p.c_out % 8 == 0 && p.n_rows > 0 && (rows / 64 + p.groups) * (wide / 128 + 1) < 0x7fffffffll;
+  *shape = p.a_pitch % 8 == 0 && p.b_pitch % 8 == 0 && p.d_pitch % 8 == 0 && p.n_rows > 0 && (rows / 64 + p.groups) * (wide / 128 + 1) < 0x7fffffffll;
   return *shape && ((reinterpret_cast<uintptr_t>(p.a) | reinterpret_cast<uintptr_t>(p.b) | reinterpret_cast<uintptr_t>(p.d)) & 15) == 0;
 }
 
@@ -704,14 +710,14 @@ int launch_grouped_umma_as(const GroupedParams& p, bool bf16, const GuCut& cut, 
   CUtensorMap a, b, b16;
   int rc;
   if (PASS == GROUPED_WGRAD) {  // p.a: in, p.b: out_grad
-    rc = grouped_tensor_map(&a, p.b, p.c_out, p.n_rows, 0, 64, bf16);
-    if (rc == 0) rc = grouped_tensor_map(&b, p.a, p.c_in, p.n_rows, 0, 64, bf16);
+    rc = grouped_tensor_map(&a, p.b, p.c_out, p.b_pitch, p.n_rows, 0, 64, bf16);
+    if (rc == 0) rc = grouped_tensor_map(&b, p.a, p.c_in, p.a_pitch, p.n_rows, 0, 64, bf16);
     b16 = b;
   } else {
-    rc = grouped_tensor_map(&a, p.b, p.c_out, p.c_in, p.groups, PASS == GROUPED_FWD ? 64 : 128, bf16);
+    rc = grouped_tensor_map(&a, p.b, p.c_out, p.b_pitch, p.c_in, p.groups, PASS == GROUPED_FWD ? 64 : 128, bf16);
     const int width = PASS == GROUPED_FWD ? p.c_in : p.c_out;
-    if (rc == 0) rc = grouped_tensor_map(&b, p.a, width, p.n_rows, 0, cfg.tile_n / CG, bf16);
-    if (rc == 0) rc = grouped_tensor_map(&b16, p.a, width, p.n_rows, 0, 16, bf16);
+    if (rc == 0) rc = grouped_tensor_map(&b, p.a, width, p.a_pitch, p.n_rows, 0, cfg.tile_n / CG, bf16);
+    if (rc == 0) rc = grouped_tensor_map(&b16, p.a, width, p.a_pitch, p.n_rows, 0, 16, bf16);
   }
   if (rc != 0) return rc;
   static std::atomic<int> granted[64];

@@ -670,6 +670,21 @@ void check_groups(const char* name, const Tensor& weights, const Tensor& kpos) {
   for (int d = 1; d < 3; ++d) TORCH_CHECK_VALUE(weights.size(d) <= 0x7fffffff, "more than 2^31 - 1 channels");
 }
 
+// Rows that no tensor map can describe are copied: into PyTorch's caching allocator's memory, so that calls on different streams or threads never share
+// it.  Where there is none, the call has another way.
+Tensor grouped_workspace(int pass, const Tensor& a, const Tensor& b, const Tensor& d, int64_t rows, const Tensor& kernel, int dtype) {
+  const size_t bytes = fgms_b200_grouped_workspace_bytes(pass, ptr(a), ptr(b), ptr(d), (int)rows, (int)kernel.size(1), (int)kernel.size(2),
+                                                         (int)kernel.size(0), dtype);
+  if (bytes == 0) return {};
+  try {
+    return at::empty({(int64_t)bytes}, kernel.options().dtype(at::kByte).requires_grad(false));
+  } catch (const c10::OutOfMemoryError&) {
+    return {};
+  }
+}
+void* space(const Tensor& ws) { return ws.defined() ? ws.data_ptr() : nullptr; }
+size_t space_bytes(const Tensor& ws) { return ws.defined() ? (size_t)ws.numel() : 0; }
+
 void grouped_fwd(const Tensor& in_feats, const Tensor& kernel, const Tensor& out, const Tensor& kpos, bool zero_rest) {
   check_groups("kernel", kernel, kpos);
   check_rows("in_feats", in_feats, kernel, 1);
@@ -677,8 +692,9 @@ void grouped_fwd(const Tensor& in_feats, const Tensor& kernel, const Tensor& out
   TORCH_CHECK_VALUE(in_feats.size(0) == out.size(0), "in_feats and out_feats differ in rows");
   const int dtype = grouped_dtype(kernel);
   c10::cuda::CUDAGuard guard(kernel.device());
+  const Tensor ws = grouped_workspace(0, in_feats, kernel, out, out.size(0), kernel, dtype);
   check_status(fgms_b200_grouped_fwd(ptr(in_feats), ptr(kernel), ptr(out), iptr(kpos), (int)out.size(0), (int)kernel.size(1), (int)kernel.size(2),
-                                     (int)kernel.size(0), dtype, zero_rest, stream_of(kernel)));
+                                     (int)kernel.size(0), dtype, zero_rest, space(ws), space_bytes(ws), stream_of(kernel)));
   written(out);
 }
 
@@ -689,8 +705,9 @@ void grouped_dgrad(const Tensor& grad_out, const Tensor& kernel, const Tensor& i
   TORCH_CHECK_VALUE(in_grad.size(0) == grad_out.size(0), "out_feats_grad and in_feats_grad differ in rows");
   const int dtype = grouped_dtype(kernel);
   c10::cuda::CUDAGuard guard(kernel.device());
+  const Tensor ws = grouped_workspace(1, grad_out, kernel, in_grad, in_grad.size(0), kernel, dtype);
   check_status(fgms_b200_grouped_dgrad(ptr(grad_out), ptr(kernel), ptr(in_grad), iptr(kpos), (int)in_grad.size(0), (int)kernel.size(1),
-                                       (int)kernel.size(2), (int)kernel.size(0), dtype, zero_rest, stream_of(kernel)));
+                                       (int)kernel.size(2), (int)kernel.size(0), dtype, zero_rest, space(ws), space_bytes(ws), stream_of(kernel)));
   written(in_grad);
 }
 
@@ -701,8 +718,9 @@ void grouped_wgrad(const Tensor& in_feats, const Tensor& grad_out, const Tensor&
   TORCH_CHECK_VALUE(in_feats.size(0) == grad_out.size(0), "in_feats and out_feats_grad differ in rows");
   const int dtype = grouped_dtype(kernel_grad);
   c10::cuda::CUDAGuard guard(kernel_grad.device());
+  const Tensor ws = grouped_workspace(2, in_feats, grad_out, kernel_grad, in_feats.size(0), kernel_grad, dtype);
   check_status(fgms_b200_grouped_wgrad(ptr(in_feats), ptr(grad_out), ptr(kernel_grad), iptr(kpos), (int)in_feats.size(0), (int)kernel_grad.size(1),
-                                       (int)kernel_grad.size(2), (int)kernel_grad.size(0), dtype, stream_of(kernel_grad)));
+                                       (int)kernel_grad.size(2), (int)kernel_grad.size(0), dtype, space(ws), space_bytes(ws), stream_of(kernel_grad)));
   written(kernel_grad);
 }
 

@@ -272,18 +272,26 @@ int fgms_b200_fwd_output_stationary(const void* in_feats, const void* kernel, vo
  *
  * Outputs are OVERWRITTEN, each value rounded once from one fp32 accumulator: the same bits on every run.  Rows of no group (before
  * kpos[0], from kpos[groups] on) are not read; they are left as they were, or become zeros with `zero_rest`.  dtype: F32 (exact fp32 on
- * the CUDA cores), F16 or BF16 (tensor cores with fp32 accumulation).  Any channel counts; fp16 / bf16 rows that do not start on
- * 16-byte boundaries (channel counts that are no multiples of 8, unaligned tensors) run on the CUDA cores, many times slower.
+ * the CUDA cores), F16 or BF16 (tensor cores with fp32 accumulation).  Any channel counts.  fp16 / bf16 rows that do not start on
+ * 16-byte boundaries (channel counts that are no multiples of 8, unaligned tensors) are copied to rows that do, and outputs back, in a
+ * `workspace` of fgms_b200_grouped_workspace_bytes() bytes, 256-byte aligned (0: none is needed, or the call is too small for that to
+ * pay); with workspace = NULL they run on the CUDA cores, many times slower.
  * kpos is device memory and is not trusted: entries are clamped to [0, n_rows], an entry smaller than one before it counts as equal to that,
  * and every entry so changed is counted (fgms_b200_device_status).  An output must not overlap an input.
  * No counterpart in the reference, whose operator multiplies every row by up to k_vol matrices. */
 #define FGMS_GROUPED_MAX_GROUPS 1024
 int fgms_b200_grouped_fwd(const void* in_feats, const void* kernel, void* out_feats, const int32_t* kpos, int n_rows,
-                          int c_in, int c_out, int groups, int dtype, int zero_rest, void* stream);
+                          int c_in, int c_out, int groups, int dtype, int zero_rest, void* workspace,
+                          size_t workspace_bytes, void* stream);
 int fgms_b200_grouped_dgrad(const void* out_grad, const void* kernel, void* in_grad, const int32_t* kpos, int n_rows,
-                            int c_in, int c_out, int groups, int dtype, int zero_rest, void* stream);
+                            int c_in, int c_out, int groups, int dtype, int zero_rest, void* workspace,
+                            size_t workspace_bytes, void* stream);
 int fgms_b200_grouped_wgrad(const void* in_feats, const void* out_grad, void* kernel_grad, const int32_t* kpos,
-                            int n_rows, int c_in, int c_out, int groups, int dtype, void* stream);
+                            int n_rows, int c_in, int c_out, int groups, int dtype, void* workspace,
+                            size_t workspace_bytes, void* stream);
+/* For pass 0 fwd, 1 dgrad, 2 wgrad and the three tensors of that call, in its order; only their alignment is looked at. */
+size_t fgms_b200_grouped_workspace_bytes(int pass, const void* first, const void* second, const void* output, int n_rows,
+                                         int c_in, int c_out, int groups, int dtype);
 
 /* ---------------------------------------------------------------------------------------------
  * One AdamW step over many tensors, in one launch for each 400 of them.  With t = step[0] + 1:

@@ -457,3 +457,70 @@ def test_rows_beyond_32_bits():
     backend.fgms_grouped_dgrad_cuda(out, w, back, kpos)
     near(back[-50:], w[1].double().sum(1).expand(50, -1), w[1].double().abs().sum(1).expand(50, -1), 64)
     assert not back[:-50].any()
+
+
+@pytest.mark.parametrize("which", PASSES)
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("sizes,c_in,c_out,shift", [([300, 0, 700], 1001, 1003, 0), ([900, 40, 1500], 512, 517, 0), ([2100, 300], 257, 1024, 0),
+                                                    ([400, 600, 128], 1024, 768, 1), ([400, 600, 128], 1024, 768, 4), ([30000], 65, 131, 0)])
+def test_rows_that_are_copied_to_boundaries(sizes, c_in, c_out, shift, dtype, which):
+    """Widths that are no multiples of 8 and views off a boundary, in calls that are large enough for copies to pay."""
+    from fgms_b200 import _lib, backend
+    layer = Layer(dtype, sizes, c_in, c_out, start=5, rest=30, seed=22)
+    if shift:
+        def moved(v):
+            flat = torch.empty(v.numel() + shift, dtype=v.dtype, device="cuda")
+            flat[shift:].view(v.shape).copy_(v)
+            return flat[shift:].view(v.shape)
+        layer.x, layer.g, layer.w = moved(layer.x), moved(layer.g), moved(layer.w)
+    a, b, d = {"fwd": (layer.x, layer.w, layer.g), "dgrad": (layer.g, layer.w, layer.x), "wgrad": (layer.x, layer.g, layer.w)}[which]
+    copied = _lib.lib.fgms_b200_grouped_workspace_bytes(PASSES.index(which), a.data_ptr(), b.data_ptr(), d.data_ptr(), layer.rows, c_in, c_out,
+                                                        len(sizes), {"fp16": _lib.DTYPE_F16, "bf16": _lib.DTYPE_BF16}[dtype])
+    assert copied > 0
+    fallbacks, launches = backend.fallback_count(), backend.launch_count()
+    first = layer.check(which)
+    assert backend.fallback_count() == fallbacks and backend.launch_count() - launches >= 2
+    assert torch.equal(first, layer.run(which))
+    if which != "wgrad":
+        layer.check(which, zero_rest=True)
+    backend.device_status()
+    layer.kpos[1] = layer.rows + 7        # one entry out of range, and the ones behind it out of order
+    out = layer.run(which)
+    assert backend.device_status() == len(sizes)
+    if which != "wgrad":  # all rows from the first on are the first group's
+        rows = slice(5, 5 + sum(sizes))
+        x, w = (layer.x, layer.w[0]) if which == "fwd" else (layer.g, layer.w[0].T)
+        near(out[rows], x[rows].double() @ w.double(), x[rows].double().abs() @ w.double().abs(), w.size(0))
+        assert (out[:5] == 7).all()
+
+
+def test_copied_rows_in_a_graph():
+    """The workspace is the graph's own."""
+    layers = [Layer("bf16", [500, 700], 513, 771, seed=s, fill=0.0) for s in (23, 24)]
+    want = [[l.run(w) for w in PASSES] for l in layers]
+    graphs, got = [], []
+    for l in layers:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            got.append([l.run(w) for w in PASSES])
+    for _ in range(2):
+        for g in graphs:
+            g.replay()
+    assert all(torch.equal(a, b) for g, w in zip(got, want) for a, b in zip(g, w))
+
+
+def test_workspace_is_checked():
+    from fgms_b200 import _lib
+    layer = Layer("bf16", [500, 700], 513, 771, seed=25)
+    out = torch.empty_like(layer.g)
+    need = _lib.lib.fgms_b200_grouped_workspace_bytes(0, layer.x.data_ptr(), layer.w.data_ptr(), out.data_ptr(), layer.rows, 513, 771, 2, _lib.DTYPE_BF16)
+    ws = torch.empty(need + 512, dtype=torch.uint8, device="cuda")
+    call = lambda at, size: _lib.lib.fgms_b200_grouped_fwd(layer.x.data_ptr(), layer.w.data_ptr(), out.data_ptr(), layer.kpos.data_ptr(), layer.rows, 513, 771, 2,
+                                                           _lib.DTYPE_BF16, 0, at, size, torch.cuda.current_stream().cuda_stream)
+    assert call(ws.data_ptr(), need - 1) == _lib.ERR_WORKSPACE and call(ws.data_ptr() + 16, need) == _lib.ERR_WORKSPACE
+    assert call(layer.w.data_ptr() // 256 * 256, need) == _lib.ERR_WORKSPACE
+    exact, magnitude, n = layer.exact("fwd")
+    for at, size in ((ws.data_ptr(), need), (None, 0)):  # without one: the CUDA cores
+        out.zero_()
+        assert call(at, size) == _lib.OK
+        near(out, exact, magnitude, n)

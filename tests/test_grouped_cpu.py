@@ -8,7 +8,7 @@ P = 1 << 20  # never dereferenced: validation fails first
 
 
 def fwd(x=P, w=2 * P, out=3 * P, kpos=4 * P, rows=10, c_in=8, c_out=8, groups=4, dtype=_lib.DTYPE_BF16):
-    return _lib.lib.fgms_b200_grouped_fwd(x, w, out, kpos, rows, c_in, c_out, groups, dtype, 0, None)
+    return _lib.lib.fgms_b200_grouped_fwd(x, w, out, kpos, rows, c_in, c_out, groups, dtype, 0, None, 0, None)
 
 
 @pytest.mark.parametrize("args,text", [
@@ -35,16 +35,16 @@ def test_forward_refuses(args, text):
 
 def test_gradients_refuse():
     L = _lib.lib
-    assert L.fgms_b200_grouped_dgrad(P, 2 * P, 2 * P, 4 * P, 10, 8, 8, 4, 1, 0, None) == _lib.ERR_INVALID_ARG and "overlaps" in _lib.last_error()
-    assert L.fgms_b200_grouped_dgrad(P, 2 * P, 3 * P, None, 10, 8, 8, 4, 1, 0, None) == _lib.ERR_INVALID_ARG
-    assert L.fgms_b200_grouped_wgrad(P, 2 * P, None, 4 * P, 10, 8, 8, 4, 1, None) == _lib.ERR_INVALID_ARG
-    assert L.fgms_b200_grouped_wgrad(P, 2 * P, 2 * P, 4 * P, 10, 8, 8, 4, 1, None) == _lib.ERR_INVALID_ARG and "overlaps" in _lib.last_error()
-    assert L.fgms_b200_grouped_wgrad(None, None, 3 * P, 4 * P, 10, 8, 8, 4, 1, None) == _lib.ERR_INVALID_ARG
+    assert L.fgms_b200_grouped_dgrad(P, 2 * P, 2 * P, 4 * P, 10, 8, 8, 4, 1, 0, None, 0, None) == _lib.ERR_INVALID_ARG and "overlaps" in _lib.last_error()
+    assert L.fgms_b200_grouped_dgrad(P, 2 * P, 3 * P, None, 10, 8, 8, 4, 1, 0, None, 0, None) == _lib.ERR_INVALID_ARG
+    assert L.fgms_b200_grouped_wgrad(P, 2 * P, None, 4 * P, 10, 8, 8, 4, 1, None, 0, None) == _lib.ERR_INVALID_ARG
+    assert L.fgms_b200_grouped_wgrad(P, 2 * P, 2 * P, 4 * P, 10, 8, 8, 4, 1, None, 0, None) == _lib.ERR_INVALID_ARG and "overlaps" in _lib.last_error()
+    assert L.fgms_b200_grouped_wgrad(None, None, 3 * P, 4 * P, 10, 8, 8, 4, 1, None, 0, None) == _lib.ERR_INVALID_ARG
 
 
 def test_nothing_to_write_is_no_error():
     assert fwd(x=None, out=None, rows=0) == _lib.OK
-    assert _lib.lib.fgms_b200_grouped_dgrad(None, P, None, 2 * P, 0, 8, 8, 4, 0, 0, None) == _lib.OK
+    assert _lib.lib.fgms_b200_grouped_dgrad(None, P, None, 2 * P, 0, 8, 8, 4, 0, 0, None, 0, None) == _lib.OK
 
 
 def test_the_operator_of_a_map_still_refuses_bf16():
@@ -65,3 +65,19 @@ def test_tensors_on_the_host_are_refused():
         backend.fgms_grouped_fwd_cuda(None, w, out, kpos)
     with pytest.raises(ValueError, match="int32"):
         nn.grouped_linear(x, w, None)
+
+
+def test_workspace_for_rows_off_a_boundary():
+    """None where none is needed (whole rows of 16 bytes, fp32), where the call is too small for copies to pay, or where nothing is right."""
+    q = _lib.lib.fgms_b200_grouped_workspace_bytes
+    F16, BF16, F32 = _lib.DTYPE_F16, _lib.DTYPE_BF16, _lib.DTYPE_F32
+    assert q(0, P, P, P, 5000, 1024, 1024, 8, F16) == 0
+    assert q(0, P, P, P, 5000, 1001, 1003, 8, F32) == 0
+    assert q(0, P, P, P, 5, 1001, 1003, 8, F16) == 0
+    up = lambda rows, width: (rows * width * 2 + 255) // 256 * 256
+    assert q(0, P, P, P, 5000, 1001, 1003, 8, BF16) == up(5000, 1008) + up(8 * 1001, 1008) + up(5000, 1008)
+    assert q(1, P, P, P, 5000, 1024, 1003, 8, F16) == up(5000, 1008) + up(8 * 1024, 1008)   # in_grad has whole rows
+    assert q(2, P, P, P, 5000, 1003, 1024, 8, F16) == up(5000, 1008)
+    assert q(0, P + 2, P, P, 5000, 1024, 1024, 8, F16) == up(5000, 1024)                    # a view
+    assert q(0, P, P, P + 8, 5000, 1024, 1024, 8, F16) == up(5000, 1024)
+    assert q(3, P, P, P, 5000, 1001, 1003, 8, F16) == 0 and q(0, P, P, P, 0, 1001, 1003, 8, F16) == 0 and q(0, P, P, P, 5, 0, 3, 8, F16) == 0
