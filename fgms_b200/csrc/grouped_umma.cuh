@@ -23,9 +23,8 @@
 //
 // 32768 rows of 32 even groups 2048 -> 4096, bf16, kept busy for half a second: forward 445-452 us (1225 TFLOP/s), input gradient 451-457, weight gradient 464,
 // where the library's batched product takes 441-444 and one product of that many operations 403-416; all run into the power limit.  A short burst 385
-// (1430 TFLOP/s), 97 us a quarter of it.  What bounds that: without loads behind the first ring 78 us instead of 97, without the epilogue 91, without its stores
-// 91; the tensor pipe alone would be 60.  So it is the 64 KB a stage that a pair reads from L2 (42 bytes a cycle and SM), then the stores that share
-// the way.  96 rows in 64 groups 2048 -> 1024 46 us, 5.8 TB/s of weights.
+// (1430 TFLOP/s), 97 us a quarter of it.  What bounds that is the tensor pipe, busy for 87 % of it: 78 us without loads
+// behind the first ring, 91 without the epilogue or its stores, which share the way to L2 with the 64 KB a stage that a pair reads.  96 rows in 64 groups 2048 -> 1024 46 us, 5.8 TB/s of weights.
 #pragma once
 #include "grouped.cuh"
 
