@@ -609,7 +609,7 @@ inline int grouped_tensor_map(CUtensorMap* map, const void* data, int cols, int 
 // Whether the kernel takes a call: what the tensor maps and the stores ask for; tiles (of 64 x 128 values at least) are counted in an int.
 inline bool grouped_umma_takes(const GroupedParams& p, bool* shape) {
   const long long wide = p.c_in > p.c_out ? p.c_in : p.c_out, rows = (long long)p.n_rows > (long long)p.groups * p.c_in ? p.n_rows : (long long)p.groups * p.c_in;
-  *shape = p.a_pitch % 8 == 0 && p.b_pitch % 8 == 0 && p.d_pitch % 8 == 0 && p.n_rows > 0 && (rows / 64 + p.groups) * (wide / 128 + 1) < 0x7fffffffll;
+  *shape = p.a_pitch % 8 == 0 && p.b_pitch % 8 == 0 && p.d_pitch % 8 == 0 && p.n_rows > 0 && (rows / 64 + p.groups) * (wide / 128 + 1) < 0x7fff0000ll;
   return *shape && ((reinterpret_cast<uintptr_t>(p.a) | reinterpret_cast<uintptr_t>(p.b) | reinterpret_cast<uintptr_t>(p.d)) & 15) == 0;
 }
 
