@@ -554,3 +554,60 @@ def test_optimizer_in_a_capture():
     mine.step()
     other.step()
     assert all(torch.equal(p, q) for p, q in zip(a.parameters(), b.parameters()))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_parameters_of_different_types_in_a_group(bits):
+    """float32 parameters have no master beside those that do; each takes the step that it takes alone."""
+    from fgms_b200 import backend, optim
+    make = lambda: [torch.nn.Parameter(torch.full((300,), 0.5, device="cuda", dtype=t)) for t in (torch.float32, torch.bfloat16, torch.float16)]
+    together, alone = make(), make()
+    opts = [optim.AdamW(together, lr=1e-2, state_bits=bits)], [optim.AdamW([p], lr=1e-2, state_bits=bits) for p in alone]
+    for step in range(2):
+        for params in (together, alone):
+            for i, p in enumerate(params):
+                p.grad = torch.linspace(-1, 1, 300, device="cuda").mul_(i + step + 1).to(p.dtype)
+        launches = backend.launch_count()
+        opts[0][0].step()
+        assert backend.launch_count() - launches == 1
+        for o in opts[1]:
+            o.step()
+    assert all(torch.equal(p, q) for p, q in zip(together, alone))
+    assert ["master" in opts[0][0].state[p] for p in together] == [False, True, True]
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_whole_training_step_in_a_graph(bits):
+    """Products, gradients and update captured together: replays take the steps that eager ones take, to the bit."""
+    from fgms_b200 import nn, optim
+    kpos = torch.tensor([0, 70, 70, 150, 200], dtype=torch.int32, device="cuda")
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    x = torch.randn((210, 96), generator=gen, device="cuda").bfloat16()
+    nets, opts = [], []
+    for _ in range(2):
+        torch.manual_seed(2)
+        nets.append(torch.nn.ModuleList([nn.GroupedLinear(96, 256, 4, dtype=torch.bfloat16), nn.GroupedLinear(256, 96, 4, dtype=torch.bfloat16)]))
+        opts.append(optim.AdamW(nets[-1].parameters(), lr=1e-2, state_bits=bits))
+
+    def step(i):
+        out = nets[i][1](torch.relu(nets[i][0](x, kpos)), kpos)
+        ((out - x).float() ** 2).mean().backward()
+        opts[i].step()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(1)
+        opts[1].zero_grad(set_to_none=True)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        opts[1].zero_grad(set_to_none=True)
+        step(1)
+    for _ in range(3):
+        graph.replay()
+    for _ in range(4):
+        opts[0].zero_grad(set_to_none=True)
+        step(0)
+    assert opts[1].state[nets[1][0].weight]["step"].tolist() == [4, 0]
+    assert all(torch.equal(p, q) for p, q in zip(nets[0].parameters(), nets[1].parameters()))
