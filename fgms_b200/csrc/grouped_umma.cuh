@@ -125,19 +125,21 @@ __device__ __forceinline__ bool pair_park(uint32_t bar, uint32_t parity) {
 }
 // the bounded waits of mbar_wait (SPIN) and mbar_parked_wait, for barriers that the other CTA of a pair arrives at
 template <bool SPIN>
-__device__ __forceinline__ bool pair_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+__device__ __forceinline__ bool pair_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, long long limit = WAIT_LIMIT_CYCLES) {
   if (pair_test(bar, parity)) return true;
   const long long start = clock64();
   for (uint32_t it = 1;; ++it) {
     if (SPIN ? pair_test(bar, parity) : pair_park(bar, parity)) return true;
     if (!SPIN || (it & 255u) == 0) {
       if (*abort_flag) return false;
-      if (clock64() - start > WAIT_LIMIT_CYCLES) break;
+      if (clock64() - start > limit) break;
     }
   }
   *abort_flag = 1;
   return false;
 }
+// a wait for a whole tile: what a wait has, and a microsecond for each of its stages (a group may have millions)
+__device__ __forceinline__ long long tile_wait_limit(int stages) { return WAIT_LIMIT_CYCLES + 2000ll * stages; }
 // box of a tensor map, into this CTA's shared memory; its bytes are reported to `bar`, with CG = 2 of either CTA
 template <int CG>
 __device__ __forceinline__ void pair_load_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
@@ -414,8 +416,6 @@ __global__ void __launch_bounds__(GU_THREADS, 1)
       pair_commit<CG>(smem_u32(&sh->drained));
       mbar_wait(smem_u32(&sh->drained), 0u, nullptr);
     }
-    // the odd CTA: the commits' arrivals at its barriers are behind it before it may end
-    if (CG == 2 && rank != 0) mbar_parked_wait(smem_u32(&sh->drained), 0u, nullptr);
     __syncwarp();
   } else if (warp == 2 && PASS == GROUPED_WGRAD) {
     // ------------------------------------------------------------------ rows behind a group's last one
@@ -426,7 +426,7 @@ __global__ void __launch_bounds__(GU_THREADS, 1)
       if (tile.b0 == tile.b1) continue;
       s = (s + tile.b1 - tile.b0 - 1) % cfg.stages;
       if (there % 16 != 0 && tile.b1 == tile.blocks) {
-        ok = pair_wait<false>(smem_u32(&sh->landed[s]), (odd >> s) & 1u, abort_flag);
+        ok = pair_wait<false>(smem_u32(&sh->landed[s]), (odd >> s) & 1u, abort_flag, tile_wait_limit(tile.blocks));
         if (!ok) break;
         odd ^= 1u << s;
         // to the next multiple of 16: the MMA goes no further.  A row is 128 bytes of each block of 64 channels.
@@ -463,7 +463,7 @@ __global__ void __launch_bounds__(GU_THREADS, 1)
       uint16_t* to = out + (PASS == GROUPED_WGRAD ? (size_t)tile.g * p.c_in + tile.n0 : (size_t)tile.n0) * p.d_pitch + ch;
       const bool mine = ch < channels;
       if (some) {
-        ok = four_agree(half, pair_wait<false>(smem_u32(&sh->tmem_full[buf]), ph, abort_flag));
+        ok = four_agree(half, pair_wait<false>(smem_u32(&sh->tmem_full[buf]), ph, abort_flag, tile_wait_limit(tile.blocks)));
         if (!ok) break;
         tc_fence_after();
       }
@@ -520,6 +520,8 @@ __global__ void __launch_bounds__(GU_THREADS, 1)
     }
   }
   if (!ok) report_problem();
+  // The odd CTA: the commits' arrivals at its barriers are behind it before it may end.  (Its epilogue has seen all of them but the last.)
+  if (CG == 2 && rank != 0 && warp == GU_EPI_WARP0) mbar_parked_wait(smem_u32(&sh->drained), 0u, nullptr);
   __syncwarp();
   tc_fence_before();
   if constexpr (SPLIT) {

@@ -524,3 +524,20 @@ def test_workspace_is_checked():
         out.zero_()
         assert call(at, size) == _lib.OK
         near(out, exact, magnitude, n)
+
+
+def test_a_group_of_many_million_rows():
+    """A tile whose stages take longer than any single wait is no wait that ran out (the other groups keep it from being shared by several CTAs)."""
+    from fgms_b200 import backend
+    rows, groups = 500_000_000, 200
+    x = torch.zeros((rows, 8), dtype=torch.bfloat16, device="cuda")
+    g = torch.ones((rows, 8), dtype=torch.bfloat16, device="cuda")
+    x[::250_000_000] = 1
+    x[-1] = 2
+    dw = torch.empty((groups, 8, 8), dtype=torch.bfloat16, device="cuda")
+    kpos = torch.full((groups + 1,), rows, dtype=torch.int32, device="cuda")
+    kpos[0] = 0
+    backend.device_status()
+    backend.fgms_grouped_wgrad_cuda(x, g, dw, kpos)
+    assert backend.device_status() == 0
+    assert (dw[0] == 4).all() and not dw[1:].any()
