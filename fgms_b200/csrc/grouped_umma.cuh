@@ -138,8 +138,8 @@ __device__ __forceinline__ bool pair_wait(uint32_t bar, uint32_t parity, volatil
   *abort_flag = 1;
   return false;
 }
-// a wait for a whole tile: what a wait has, and a microsecond for each of its stages (a group may have millions)
-__device__ __forceinline__ long long tile_wait_limit(int stages) { return WAIT_LIMIT_CYCLES + 2000ll * stages; }
+// a wait for whole tiles: what a wait has, and a microsecond for each of their stages (a group may have millions)
+__device__ __forceinline__ long long tile_wait_limit(long long stages) { return WAIT_LIMIT_CYCLES + 2000ll * stages; }
 // box of a tensor map, into this CTA's shared memory; its bytes are reported to `bar`, with CG = 2 of either CTA
 template <int CG>
 __device__ __forceinline__ void pair_load_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
@@ -421,13 +421,16 @@ __global__ void __launch_bounds__(GU_THREADS, 1)
     // ------------------------------------------------------------------ rows behind a group's last one
     int s = 0;
     uint32_t odd = 0;  // phases of the barriers, a bit a stage
+    long long passed = 0;  // stages since the last wait: tiles without such rows are not waited for
     for (; tile.left > 0 && ok; tile.next()) {
       const int there = tile.k_len % GU_K;
       if (tile.b0 == tile.b1) continue;
+      passed += tile.b1 - tile.b0;
       s = (s + tile.b1 - tile.b0 - 1) % cfg.stages;
       if (there % 16 != 0 && tile.b1 == tile.blocks) {
-        ok = pair_wait<false>(smem_u32(&sh->landed[s]), (odd >> s) & 1u, abort_flag, tile_wait_limit(tile.blocks));
+        ok = pair_wait<false>(smem_u32(&sh->landed[s]), (odd >> s) & 1u, abort_flag, tile_wait_limit(passed));
         if (!ok) break;
+        passed = 0;
         odd ^= 1u << s;
         // to the next multiple of 16: the MMA goes no further.  A row is 128 bytes of each block of 64 channels.
         const uint32_t base = stage0 + (uint32_t)(s * cfg.stage_bytes);

@@ -541,3 +541,23 @@ def test_a_group_of_many_million_rows():
     backend.fgms_grouped_wgrad_cuda(x, g, dw, kpos)
     assert backend.device_status() == 0
     assert (dw[0] == 4).all() and not dw[1:].any()
+
+
+def test_ragged_groups_behind_many_million_rows():
+    """The rows behind a group's last one are cleared by a warp that passes over tiles without such rows: its wait lasts as long as all of those
+    may take.  Whichever tiles the first group's CTA gets next, their groups end inside a stage."""
+    from fgms_b200 import backend
+    first, groups = 499_999_984, 200  # a multiple of 16: nothing to clear
+    rows = first + 5 * (groups - 1)
+    x = torch.zeros((rows, 8), dtype=torch.bfloat16, device="cuda")
+    g = torch.ones((rows, 8), dtype=torch.bfloat16, device="cuda")
+    x[::250_000_000] = 1
+    x[first:] = torch.arange(1, groups, device="cuda").bfloat16().repeat_interleave(5)[:, None] * 2.0 ** -8
+    dw = torch.empty((groups, 8, 8), dtype=torch.bfloat16, device="cuda")
+    kpos = kpos_of([first] + [5] * (groups - 1))
+    backend.device_status()
+    backend.fgms_grouped_wgrad_cuda(x, g, dw, kpos)
+    assert backend.device_status() == 0
+    assert (dw[0] == 2).all()
+    want = 5 * torch.arange(1, groups, device="cuda").double() * 2.0 ** -8  # exact in fp32, rounded once
+    assert torch.equal(dw[1:], want.bfloat16()[:, None, None].expand(-1, 8, 8))
