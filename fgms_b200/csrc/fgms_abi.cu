@@ -364,6 +364,9 @@ int run_grouped(const void* a, const void* b, void* d, const int32_t* kpos, int 
                 void* workspace, size_t workspace_bytes, void* stream) {
   if (n_rows < 0) return fail(FGMS_ERR_INVALID_ARG, "negative row count");
   if (c_in < 1 || c_out < 1) return fail(FGMS_ERR_INVALID_ARG, "channel counts must be >= 1");
+  // the kernels count in steps of up to 256 from the first row or channel to behind the last
+  if (n_rows > FGMS_GROUPED_MAX_EXTENT || c_in > FGMS_GROUPED_MAX_EXTENT || c_out > FGMS_GROUPED_MAX_EXTENT)
+    return fail(FGMS_ERR_INVALID_ARG, "more than %d rows or channels", FGMS_GROUPED_MAX_EXTENT);
   if (groups < 1 || groups > FGMS_GROUPED_MAX_GROUPS)
     return fail(FGMS_ERR_INVALID_ARG, "groups %d outside [1, %d]", groups, FGMS_GROUPED_MAX_GROUPS);
   if ((long long)groups * c_in > 0x7fffffffll || (long long)groups * c_out > 0x7fffffffll)
@@ -1146,6 +1149,7 @@ int fgms_b200_grouped_wgrad(const void* in_feats, const void* out_grad, void* ke
 size_t fgms_b200_grouped_workspace_bytes(int pass, const void* a, const void* b, const void* d, int n_rows, int c_in, int c_out, int groups, int dtype) {
   if (dtype != FGMS_DTYPE_F16 && dtype != FGMS_DTYPE_BF16) return 0;
   if (n_rows < 1 || c_in < 1 || c_out < 1 || groups < 1 || groups > FGMS_GROUPED_MAX_GROUPS) return 0;
+  if (n_rows > FGMS_GROUPED_MAX_EXTENT || c_in > FGMS_GROUPED_MAX_EXTENT || c_out > FGMS_GROUPED_MAX_EXTENT) return 0;
   if (pass == 0) return fgms::grouped_copies<fgms::GROUPED_FWD>(a, b, d, n_rows, c_in, c_out, groups).total;
   if (pass == 1) return fgms::grouped_copies<fgms::GROUPED_DGRAD>(a, b, d, n_rows, c_in, c_out, groups).total;
   return pass == 2 ? fgms::grouped_copies<fgms::GROUPED_WGRAD>(a, b, d, n_rows, c_in, c_out, groups).total : 0;

@@ -191,6 +191,12 @@ __device__ __forceinline__ void pair_sync() {
 }
 }  // namespace umma
 
+// How many of a group's rows its tiles take, `count` of at most `tile` rows, as evenly as multiples of `unit` (which divides `tile`) allow: (count - 1)
+// shares are less than its rows, as none is more than `tile`.  Rows and tiles together may be more than an int holds.
+__host__ __device__ __forceinline__ int grouped_share(int rows, int count, int unit) {
+  return (int)(((unsigned)rows + (unsigned)count - 1u) / (unsigned)count + (unsigned)unit - 1u) / unit * unit;
+}
+
 // The tiles of a pair, one after the other: the same walk in every role.  Steps are added up, without a division a tile: those of 64-bit numbers
 // and the search for the group took the epilogue of a short tile as long as its stores.
 template <int PASS, int CG, bool SPLIT>
@@ -252,8 +258,7 @@ struct GuTiles {
     } else {
       while (tiles[g + 1] <= q) { ++g; share = 0; }
       const int rows = first[g + 1] - first[g], count = tiles[g + 1] - tiles[g], i = q - tiles[g];
-      // a group's rows are shared out evenly over its tiles: (count - 1) * share is less than its rows, as share <= tile_n
-      if (share == 0) share = ((rows + count - 1) / count + 16 * CG - 1) / (16 * CG) * (16 * CG);
+      if (share == 0) share = grouped_share(rows, count, 16 * CG);
       n0 = first[g] + i * share;
       n = min(share, rows - i * share);
     }

@@ -280,6 +280,7 @@ int fgms_b200_fwd_output_stationary(const void* in_feats, const void* kernel, vo
  * and every entry so changed is counted (fgms_b200_device_status).  An output must not overlap an input.
  * No counterpart in the reference, whose operator multiplies every row by up to k_vol matrices. */
 #define FGMS_GROUPED_MAX_GROUPS 1024
+#define FGMS_GROUPED_MAX_EXTENT (0x7fffffff - 1024) /* rows; channels */
 int fgms_b200_grouped_fwd(const void* in_feats, const void* kernel, void* out_feats, const int32_t* kpos, int n_rows,
                           int c_in, int c_out, int groups, int dtype, int zero_rest, void* workspace,
                           size_t workspace_bytes, void* stream);

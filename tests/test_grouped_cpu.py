@@ -1,4 +1,8 @@
 """What the grouped products refuse, before they touch a device."""
+import os
+import shutil
+import subprocess
+
 import pytest
 import torch
 
@@ -81,3 +85,32 @@ def test_workspace_for_rows_off_a_boundary():
     assert q(0, P + 2, P, P, 5000, 1024, 1024, 8, F16) == up(5000, 1024)                    # a view
     assert q(0, P, P, P + 8, 5000, 1024, 1024, 8, F16) == up(5000, 1024)
     assert q(3, P, P, P, 5000, 1001, 1003, 8, F16) == 0 and q(0, P, P, P, 0, 1001, 1003, 8, F16) == 0 and q(0, P, P, P, 5, 0, 3, 8, F16) == 0
+
+
+MOST = 0x7fffffff - 1024
+
+
+@pytest.mark.parametrize("size", ["rows", "c_in", "c_out"])
+def test_rows_and_channels_whose_steps_an_int_does_not_hold_are_refused(size):
+    """The kernels go from the first to behind the last in steps of up to 256."""
+    for n in (MOST + 1, 0x7fffffff):
+        sizes = {"rows": 10, "c_in": 8, "c_out": 8, "groups": 1, **{size: n}}
+        assert fwd(**sizes) == _lib.ERR_INVALID_ARG and "more than" in _lib.last_error()
+        dims = (sizes["rows"], sizes["c_in"], sizes["c_out"], 1, _lib.DTYPE_BF16)
+        assert _lib.lib.fgms_b200_grouped_dgrad(P, 2 * P, 3 * P, 4 * P, *dims, 0, None, 0, None) == _lib.ERR_INVALID_ARG and "more than" in _lib.last_error()
+        assert _lib.lib.fgms_b200_grouped_wgrad(P, 2 * P, 3 * P, 4 * P, *dims, None, 0, None) == _lib.ERR_INVALID_ARG and "more than" in _lib.last_error()
+        assert _lib.lib.fgms_b200_grouped_workspace_bytes(0, P + 2, 2 * P, 3 * P, *dims) == 0
+    assert fwd(**{"groups": 1, size: MOST}) == _lib.ERR_INVALID_ARG and "overlaps" in _lib.last_error()  # taken, were it not for these addresses
+
+
+def test_shares_of_a_group(tmp_path):
+    """How a group's rows are shared out over its tiles, up to the most rows there may be (``tests/plans/grouped_share.cu``)."""
+    nvcc = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
+    if not (os.path.exists(nvcc) or shutil.which(nvcc)):
+        pytest.skip("nvcc not available")
+    exe = str(tmp_path / "grouped_share")
+    src = os.path.join(os.path.dirname(os.path.abspath(__file__)), "plans", "grouped_share.cu")
+    build = subprocess.run([nvcc, "-std=c++17", "-gencode", "arch=compute_100a,code=sm_100a", "-o", exe, src], capture_output=True, text=True)
+    assert build.returncode == 0, build.stdout + build.stderr
+    run = subprocess.run([exe], capture_output=True, text=True, timeout=60)
+    assert run.returncode == 0, run.stdout + run.stderr
