@@ -377,6 +377,8 @@ int run_grouped(const void* a, const void* b, void* d, const int32_t* kpos, int 
   const size_t a_bytes = PASS == fgms::GROUPED_DGRAD ? out : in, b_bytes = PASS == fgms::GROUPED_WGRAD ? out : weights;
   const size_t d_bytes = PASS == fgms::GROUPED_FWD ? out : PASS == fgms::GROUPED_DGRAD ? in : weights;
   if (!kpos || (a_bytes > 0 && !a) || (b_bytes > 0 && !b) || (d_bytes > 0 && !d)) return fail(FGMS_ERR_INVALID_ARG, "null pointer");
+  if (((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b) | reinterpret_cast<uintptr_t>(d)) & (es - 1)) || (reinterpret_cast<uintptr_t>(kpos) & 3))
+    return fail(FGMS_ERR_INVALID_ARG, "a pointer is not on a boundary of its type");
   const Range ra{a, a_bytes}, rb{b, b_bytes}, rd{d, d_bytes}, rk{kpos, (size_t)(groups + 1) * sizeof(int32_t)};
   if (rd.overlaps(ra) || rd.overlaps(rb) || rd.overlaps(rk)) return fail(FGMS_ERR_INVALID_ARG, "the output overlaps an input");
   if (d_bytes == 0) return FGMS_OK;

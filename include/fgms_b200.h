@@ -272,7 +272,7 @@ int fgms_b200_fwd_output_stationary(const void* in_feats, const void* kernel, vo
  *
  * Outputs are OVERWRITTEN, each value rounded once from one fp32 accumulator: the same bits on every run.  Rows of no group (before
  * kpos[0], from kpos[groups] on) are not read; they are left as they were, or become zeros with `zero_rest`.  dtype: F32 (exact fp32 on
- * the CUDA cores), F16 or BF16 (tensor cores with fp32 accumulation).  Any channel counts.  fp16 / bf16 rows that do not start on
+ * the CUDA cores), F16 or BF16 (tensor cores with fp32 accumulation).  Any channel counts, any address on a boundary of its type.  fp16 / bf16 rows that do not start on
  * 16-byte boundaries (channel counts that are no multiples of 8, unaligned tensors) are copied to rows that do, and outputs back, in a
  * `workspace` of fgms_b200_grouped_workspace_bytes() bytes, 256-byte aligned (0: none is needed, or the call is too small for that to
  * pay); with workspace = NULL they run on the CUDA cores, many times slower.

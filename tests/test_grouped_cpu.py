@@ -114,3 +114,12 @@ def test_shares_of_a_group(tmp_path):
     assert build.returncode == 0, build.stdout + build.stderr
     run = subprocess.run([exe], capture_output=True, text=True, timeout=60)
     assert run.returncode == 0, run.stdout + run.stderr
+
+
+@pytest.mark.parametrize("dtype,off", [(_lib.DTYPE_BF16, 1), (_lib.DTYPE_F16, 3), (_lib.DTYPE_F32, 2)])
+def test_pointers_off_a_boundary_of_their_type_are_refused(dtype, off):
+    for name, at in (("x", P), ("w", 2 * P), ("out", 3 * P)):
+        assert fwd(**{name: at + off}, dtype=dtype) == _lib.ERR_INVALID_ARG and "boundary" in _lib.last_error()
+    assert fwd(kpos=4 * P + 2, dtype=dtype) == _lib.ERR_INVALID_ARG and "boundary" in _lib.last_error()
+    for call, tail in ((_lib.lib.fgms_b200_grouped_dgrad, (0, None, 0, None)), (_lib.lib.fgms_b200_grouped_wgrad, (None, 0, None))):
+        assert call(P + off, 2 * P, 3 * P, 4 * P, 10, 8, 8, 4, dtype, *tail) == _lib.ERR_INVALID_ARG and "boundary" in _lib.last_error()
