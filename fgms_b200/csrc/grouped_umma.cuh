@@ -695,6 +695,14 @@ GuCut grouped_cut(const GroupedParams& p, int sms, Clusters clusters_at_once) {
   return best;
 }
 
+// The shared memory that the kernel may be launched with, always the most there is: a launch of a smaller size would set the limit down for a question
+// about the largest (grouped_clusters_at_once), whose answer would then depend on which call came first.
+template <int PASS, int CG, bool SPLIT>
+int grant_grouped_umma(int max_smem) {
+  static std::atomic<int> granted[64];
+  return ensure_smem(grouped_umma_kernel<PASS, CG, SPLIT>, max_smem, granted);
+}
+
 template <int PASS, int CG, bool SPLIT>
 int launch_grouped_umma_as(const GroupedParams& p, bool bf16, const GuCut& cut, cudaStream_t st, int sms, int max_smem) {
   GuConfig cfg;
@@ -729,8 +737,7 @@ int launch_grouped_umma_as(const GroupedParams& p, bool bf16, const GuCut& cut, 
     if (rc == 0) rc = grouped_tensor_map(&b16, p.a, width, p.a_pitch, p.n_rows, 0, 16, bf16);
   }
   if (rc != 0) return rc;
-  static std::atomic<int> granted[64];
-  if (ensure_smem(grouped_umma_kernel<PASS, CG, SPLIT>, cfg.smem, granted) != 0) return -1;
+  if (grant_grouped_umma<PASS, CG, SPLIT>(max_smem) != 0) return -1;
   cudaLaunchConfig_t lc = {};
   lc.gridDim = dim3((unsigned)(clusters * ctas));
   lc.blockDim = dim3(GU_THREADS);
@@ -748,18 +755,18 @@ int launch_grouped_umma_as(const GroupedParams& p, bool bf16, const GuCut& cut, 
 }
 
 // Clusters of `parts` CTAs that the device runs at the same time, each with all of an SM's shared memory: clusters do not straddle its groups
-// of SMs, so 128 CTAs in clusters of eight do not fit on 148.  Asked once a device; fewer SMs than all of them: in proportion.
+// of SMs, so 128 CTAs in clusters of eight do not fit on 148.  Answered once a device (a question that failed is asked again); fewer SMs than
+// all of them: in proportion.
 template <int PASS>
 int grouped_clusters_at_once(int parts, int sms, int max_smem) {
-  static std::atomic<int> known[64][4];
-  static std::atomic<int> granted[64];
+  static std::atomic<int> known[64][4];  // and one, 0: not known
   int dev = 0, all = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64 || parts < 2) return 0;
   std::atomic<int>& at = known[dev][parts == 2 ? 0 : parts == 4 ? 1 : 2];
   if (cudaDeviceGetAttribute(&all, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
-  int n = at.load(std::memory_order_acquire);
-  if (n == 0) {
-    if (ensure_smem(grouped_umma_kernel<PASS, 1, true>, max_smem, granted) != 0) return 0;
+  int n = at.load(std::memory_order_acquire) - 1;
+  if (n < 0) {
+    if (grant_grouped_umma<PASS, 1, true>(max_smem) != 0) return 0;
     cudaLaunchConfig_t lc = {};
     lc.gridDim = dim3((unsigned)(parts * all));
     lc.blockDim = dim3(GU_THREADS);
@@ -770,13 +777,13 @@ int grouped_clusters_at_once(int parts, int sms, int max_smem) {
     cluster[0].val.clusterDim.y = cluster[0].val.clusterDim.z = 1;
     lc.attrs = cluster;
     lc.numAttrs = 1;
-    if (cudaOccupancyMaxActiveClusters(&n, grouped_umma_kernel<PASS, 1, true>, &lc) != cudaSuccess || n < 1) {
+    if (cudaOccupancyMaxActiveClusters(&n, grouped_umma_kernel<PASS, 1, true>, &lc) != cudaSuccess || n < 0) {
       cudaGetLastError();
-      n = -1;
+      return 0;
     }
-    at.store(n, std::memory_order_release);
+    at.store(n + 1, std::memory_order_release);
   }
-  return n < 0 ? 0 : n * sms / all;
+  return n * sms / all;
 }
 
 template <int PASS>

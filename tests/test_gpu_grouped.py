@@ -561,3 +561,36 @@ def test_ragged_groups_behind_many_million_rows():
     assert (dw[0] == 2).all()
     want = 5 * torch.arange(1, groups, device="cuda").double() * 2.0 ** -8  # exact in fp32, rounded once
     assert torch.equal(dw[1:], want.bfloat16()[:, None, None].expand(-1, 8, 8))
+
+
+_ORDER = """
+import sys, hashlib, torch
+from fgms_b200 import backend
+gen = torch.Generator(device="cuda").manual_seed(1)
+def call(c_in, c_out):
+    w = torch.randn((1, c_in, c_out), generator=gen, device="cuda").bfloat16()
+    x = torch.randn((1, c_in), generator=gen, device="cuda").bfloat16()
+    x[0, 0], x[0, -1] = 2.0 ** 20, -2.0 ** 20  # so large that the order of the sums shows in every value
+    w[0, -1] = w[0, 0]
+    out = torch.empty((1, c_out), device="cuda", dtype=torch.bfloat16)
+    backend.fgms_grouped_fwd_cuda(x, w, out, torch.tensor([0, 1], device="cuda", dtype=torch.int32))
+    return hashlib.sha256(out.view(torch.int16).cpu().numpy().tobytes()).hexdigest()
+if sys.argv[1] == "behind":
+    call(768, 768)
+    gen.manual_seed(1)
+print(call(4096, 1024))
+"""
+
+
+def test_same_bits_whichever_call_came_first():
+    """How a contraction is shared out, and so the order of its sums, does not depend on the calls before: each in a process of its own."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    bits = []
+    for order in ("alone", "behind"):
+        run = subprocess.run([sys.executable, "-c", _ORDER, order], capture_output=True, text=True, cwd=root, timeout=300)
+        assert run.returncode == 0, run.stderr
+        bits.append(run.stdout.strip())
+    assert bits[0] == bits[1] and len(bits[0]) == 64

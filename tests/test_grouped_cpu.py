@@ -103,17 +103,35 @@ def test_rows_and_channels_whose_steps_an_int_does_not_hold_are_refused(size):
     assert fwd(**{"groups": 1, size: MOST}) == _lib.ERR_INVALID_ARG and "overlaps" in _lib.last_error()  # taken, were it not for these addresses
 
 
-def test_shares_of_a_group(tmp_path):
-    """How a group's rows are shared out over its tiles, up to the most rows there may be (``tests/plans/grouped_share.cu``)."""
+def program(name, tmp_path):
+    """The program ``tests/plans/<name>.cu``: a function that runs it and returns what it prints."""
     nvcc = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
     if not (os.path.exists(nvcc) or shutil.which(nvcc)):
         pytest.skip("nvcc not available")
-    exe = str(tmp_path / "grouped_share")
-    src = os.path.join(os.path.dirname(os.path.abspath(__file__)), "plans", "grouped_share.cu")
+    exe = str(tmp_path / name)
+    src = os.path.join(os.path.dirname(os.path.abspath(__file__)), "plans", name + ".cu")
     build = subprocess.run([nvcc, "-std=c++17", "-gencode", "arch=compute_100a,code=sm_100a", "-o", exe, src], capture_output=True, text=True)
     assert build.returncode == 0, build.stdout + build.stderr
-    run = subprocess.run([exe], capture_output=True, text=True, timeout=60)
-    assert run.returncode == 0, run.stdout + run.stderr
+
+    def run(*args):
+        done = subprocess.run([exe, *map(str, args)], capture_output=True, text=True, timeout=60)
+        assert done.returncode == 0, done.stdout + done.stderr
+        return done.stdout
+    return run
+
+
+def test_shares_of_a_group(tmp_path):
+    """How a group's rows are shared out over its tiles, up to the most rows there may be."""
+    program("grouped_share", tmp_path)()
+
+
+def test_the_cut_does_not_depend_on_the_calls_before(tmp_path):
+    """Clusters of eight for one row 4096 -> 1024: in a fresh process, behind a call with fewer parts, and once a question that failed is answered."""
+    run = program("grouped_limit", tmp_path)
+    alone = run(0, 0)
+    assert "clusters of 8" in alone
+    assert run(1, 0) == alone
+    assert run(2, 3) == alone
 
 
 @pytest.mark.parametrize("dtype,off", [(_lib.DTYPE_BF16, 1), (_lib.DTYPE_F16, 3), (_lib.DTYPE_F32, 2)])
