@@ -25,7 +25,8 @@ constexpr int ADAMW_PER_THREAD = 8;  // consecutive values
 constexpr int ADAMW_CHUNK = ADAMW_THREADS * ADAMW_PER_THREAD;
 constexpr int ADAMW_BLOCK = 128;  // values that share a scale: 16 lanes
 constexpr float ADAMW_E4M3_MAX = 448.0f;
-constexpr float ADAMW_SMALLEST = 7.88860905e-31f;  // 2^-100: a block whose largest value is smaller is held as zeros
+constexpr float ADAMW_SMALLEST = 7.88860905e-31f;      // 2^-100: a block of first moments whose largest value is smaller is held as zeros
+constexpr float ADAMW_SCALE_SMALLEST = 1.17549435e-38f;  // 2^-126: of second moments, so that codes stand for multiples of 2^-135, the smallest of them for that
 
 struct AdamwTensor {
   void* param;
@@ -186,9 +187,10 @@ __device__ __forceinline__ void adamw_store_codes(void* to, float* scales, long 
   float top = adamw_max3(adamw_max3(y[0], y[1], y[2]), adamw_max3(y[3], y[4], y[5]), adamw_max3(y[6], y[7], 0.f));
 #pragma unroll
   for (int o = 8; o > 0; o >>= 1) top = adamw_max3(top, __shfl_xor_sync(0xffffffffu, top, o), 0.f);
-  const bool finite = top < __uint_as_float(0x7f800000u), held = finite && top >= ADAMW_SMALLEST;
+  const bool finite = top < __uint_as_float(0x7f800000u), held = finite && (FLOOR ? top > 0.f : top >= ADAMW_SMALLEST);
   // a block with a value that is not finite is not held: its scale says so, and its values are NaN from then on
-  const float scale = held ? __fmul_rn(top, (float)(1.0 / 448.0)) : finite ? 0.f : __uint_as_float(0x7fc00000u);
+  float scale = held ? __fmul_rn(top, (float)(1.0 / 448.0)) : finite ? 0.f : __uint_as_float(0x7fc00000u);
+  if (FLOOR && held) scale = fmaxf(scale, ADAMW_SCALE_SMALLEST);  // (its inverse is finite; a product of a code and it may be subnormal, and is not 0)
   const float inverse = held ? __fdiv_rn(1.f, scale) : 0.f;
   uint32_t w[2] = {0u, 0u};
 #pragma unroll

@@ -611,3 +611,41 @@ def test_a_whole_training_step_in_a_graph(bits):
         step(0)
     assert opts[1].state[nets[1][0].weight]["step"].tolist() == [4, 0]
     assert all(torch.equal(p, q) for p, q in zip(nets[0].parameters(), nets[1].parameters()))
+
+
+@pytest.mark.parametrize("size", [1e-13, 1e-15, 1e-17, 1e-19, 1e-20])
+def test_a_tiny_second_moment_stays_above_zero_in_8_bits(size):
+    """A block of gradients so small that their squares are near fp32's smallest numbers, then none: the update is that of the moments, not m divided
+    by eps.  A value of v is off by a code at most, an eighth of it or 2^-135, and by fp32's subnormal steps before that.
+
+    The second step is exactly 0.9 * 0.1 / 0.19 / sqrt(0.999 * 0.001 / 0.001999) = 0.670 of the rate; with m off by an eighth upwards and v downwards (where it is
+    off by more it is larger) at most 0.670 * 1.125 / sqrt(0.875) = 0.81 of it."""
+    from fgms_b200 import backend
+    lr, n = 0.5, 300
+    p = torch.ones(n, device="cuda")
+    g = torch.full((n,), size, device="cuda")
+    g[::3] *= -0.5
+    m, v = (torch.zeros(n, device="cuda", dtype=torch.uint8).view(torch.float8_e4m3fn) for _ in range(2))
+    ms, vs = (torch.zeros(3, device="cuda") for _ in range(2))
+    step = torch.zeros(2, dtype=torch.int32, device="cuda")
+    call = lambda: backend.fgms_adamw_cuda([p], [g], [m], [v], step, lr, B1, B2, 1e-30, 0.0, exp_avg_scales=[ms], exp_avg_sq_scales=[vs])
+    want = (1 - B2) * g.double() ** 2
+    call()
+    got = held(v, vs)
+    assert (got > 0).all()
+    assert ((got - want).abs() <= (want / 8).clamp(min=2.0 ** -135) * (1 + 2.0 ** -20) + 2.0 ** -147).all()
+    before = p.clone()
+    g.zero_()
+    call()
+    assert (held(v, vs) > 0).all()
+    assert ((p - before).abs() <= 0.82 * lr).all()
+
+
+def test_a_block_of_zeros_is_held_as_zeros():
+    s = State(counts=[300], param="fp32", bits=8, seed=14, steps=0)
+    for t in (s.m[0].view(torch.uint8), s.v[0].view(torch.uint8), s.ms[0], s.vs[0]):
+        t.zero_()
+    s.g[0][:128] = 0
+    s.run()
+    assert not s.m[0].float()[:128].any() and not s.v[0].float()[:128].any() and s.ms[0][0] == 0 and s.vs[0][0] == 0
+    assert s.vs[0][1] > 0
