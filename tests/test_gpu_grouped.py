@@ -594,3 +594,15 @@ def test_same_bits_whichever_call_came_first():
         assert run.returncode == 0, run.stderr
         bits.append(run.stdout.strip())
     assert bits[0] == bits[1] and len(bits[0]) == 64
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_rows_cleared_for_the_other_cta_of_a_pair(dtype):
+    """Weight gradient of groups that all end inside a stage, tile after tile by pairs of CTAs: each clears its part of what the even one's MMAs read.
+    What lies behind a group's last row is the next group's, a thousand times as large; behind the last group NaN."""
+    layer = Layer(dtype, [301 + 38 * i for i in range(16)], 1024, 1024, rest=40, seed=26)
+    for i, s in layer.each():
+        layer.x[s] *= 2.0 ** (10 * (i % 2) - 5)
+    first = layer.check("wgrad")
+    for _ in range(10):
+        assert torch.equal(first, layer.run("wgrad"))
