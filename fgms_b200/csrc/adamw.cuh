@@ -47,6 +47,7 @@ struct AdamwParams {
   const float *lr_device, *grad_scale, *found_inf;
   int* step;  // [2]: steps done, and blocks that have finished this one
   int n, chunks, last;  // last: the launch that counts the step
+  int alone;            // see GmsParams
   AdamwTensor t[N];
 };
 
@@ -336,7 +337,7 @@ template <bool EIGHT, int N>
 __global__ void __launch_bounds__(ADAMW_THREADS, 3) adamw_kernel(const __grid_constant__ AdamwParams<N> p) {
   __shared__ AdamwStep s_now;
   umma::griddep_wait();
-  umma::griddep_launch_dependents();
+  if (!p.alone) umma::griddep_launch_dependents();
   if (p.found_inf && *p.found_inf != 0.f) return;  // the step is not taken, nor counted
   // a whole chunk's values are read while the one before is worked on
   AdamwAt<AdamwParams<N>> at;

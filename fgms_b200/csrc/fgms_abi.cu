@@ -339,7 +339,7 @@ int run_grouped_copied(fgms::GroupedParams p, const fgms::GroupedCopies& c, uint
   const int zero_rest = p.zero_rest;
   if (c.a.needed || c.b.needed) {
     const fgms::GroupedRows x = rows_of(c.a, p.a, workspace + c.a.at, c.a.len, c.a.pitch), y = rows_of(c.b, p.b, workspace + c.b.at, c.b.len, c.b.pitch);
-    if (fgms::launch_pdl(fgms::grouped_copy_kernel, grid_for(x.rows + y.rows, x.len > y.len ? x.len : y.len), fgms::GP_THREADS, 0, st, x, y) != cudaSuccess)
+    if (fgms::launch_pdl(fgms::grouped_copy_kernel, grid_for(x.rows + y.rows, x.len > y.len ? x.len : y.len), fgms::GP_THREADS, 0, st, x, y, p.alone) != cudaSuccess)
       return fail(FGMS_ERR_CUDA, "grouped_copy_kernel: %s", cudaGetErrorString(cudaGetLastError()));
     if (int rc = check_launch("grouped_copy_kernel")) return rc;
   }
@@ -353,8 +353,9 @@ int run_grouped_copied(fgms::GroupedParams p, const fgms::GroupedCopies& c, uint
   if (!c.d.needed) return FGMS_OK;
   const fgms::GroupedRows out = rows_of(c.d, workspace + c.d.at, d, c.d.pitch, c.d.len);
   const cudaError_t e = PASS == fgms::GROUPED_WGRAD
-                            ? fgms::launch_pdl(fgms::grouped_copy_kernel, grid_for(out.rows, out.len), fgms::GP_THREADS, 0, st, out, fgms::GroupedRows{})
-                            : fgms::launch_pdl(fgms::grouped_copy_back_kernel, grid_for(out.rows, out.len), fgms::GP_THREADS, 0, st, out, p.kpos, p.groups, zero_rest);
+                            ? fgms::launch_pdl(fgms::grouped_copy_kernel, grid_for(out.rows, out.len), fgms::GP_THREADS, 0, st, out, fgms::GroupedRows{}, p.alone)
+                            : fgms::launch_pdl(fgms::grouped_copy_back_kernel, grid_for(out.rows, out.len), fgms::GP_THREADS, 0, st, out, p.kpos, p.groups, zero_rest,
+                                              p.alone);
   if (e != cudaSuccess) return fail(FGMS_ERR_CUDA, "grouped_copy_back_kernel: %s", cudaGetErrorString(cudaGetLastError()));
   return check_launch("grouped_copy_back_kernel");
 }
@@ -476,7 +477,7 @@ int check_adamw(const fgms_b200_adamw_tensor* tensors, int n, const fgms_b200_ad
 }
 
 template <bool EIGHT, int N>
-int launch_adamw(const fgms_b200_adamw_tensor* tensors, int n, const fgms_b200_adamw_options& o, bool last, int sms, cudaStream_t st) {
+int launch_adamw(const fgms_b200_adamw_tensor* tensors, int n, const fgms_b200_adamw_options& o, bool last, const DeviceInfo& di, cudaStream_t st) {
   static thread_local fgms::AdamwParams<N> p;  // 32 KB: not on the stack of a thread that may have little of it
   p.lr = o.lr; p.beta1 = o.beta1; p.beta2 = o.beta2; p.decay = o.weight_decay;
   p.b1 = (float)o.beta1; p.c1 = (float)(1.0 - o.beta1);
@@ -487,6 +488,7 @@ int launch_adamw(const fgms_b200_adamw_tensor* tensors, int n, const fgms_b200_a
   p.lr_device = o.lr_device; p.grad_scale = o.grad_scale; p.found_inf = o.found_inf;
   p.step = o.step;
   p.n = n; p.last = last;
+  p.alone = di.reserved > 0;
   long long chunks = 0;
   for (int i = 0; i < n; ++i) {
     const fgms_b200_adamw_tensor& t = tensors[i];
@@ -504,7 +506,7 @@ int launch_adamw(const fgms_b200_adamw_tensor* tensors, int n, const fgms_b200_a
     if (chunks > 0x7fffffffll - 65536) return fail(FGMS_ERR_INVALID_ARG, "too many values in one call");
   }
   p.chunks = (int)chunks;
-  const long long most = 3ll * sms, grid = chunks < 1 ? 1 : chunks < most ? chunks : most;
+  const long long most = 3ll * di.sms, grid = chunks < 1 ? 1 : chunks < most ? chunks : most;
   if (fgms::launch_pdl(fgms::adamw_kernel<EIGHT, N>, dim3((unsigned)grid), fgms::ADAMW_THREADS, 0, st, p) != cudaSuccess)
     return fail(FGMS_ERR_CUDA, "adamw_kernel: %s", cudaGetErrorString(cudaGetLastError()));
   return check_launch("adamw_kernel");
@@ -519,11 +521,11 @@ int run_adamw(const fgms_b200_adamw_tensor* tensors, int n, const fgms_b200_adam
     const bool last = now == left;
     int rc;
     if (o->state_bits == 8)
-      rc = now <= fgms::ADAMW_FEW ? launch_adamw<true, fgms::ADAMW_FEW>(tensors + at, now, *o, last, di.sms, st)
-                                  : launch_adamw<true, fgms::ADAMW_MANY>(tensors + at, now, *o, last, di.sms, st);
+      rc = now <= fgms::ADAMW_FEW ? launch_adamw<true, fgms::ADAMW_FEW>(tensors + at, now, *o, last, di, st)
+                                  : launch_adamw<true, fgms::ADAMW_MANY>(tensors + at, now, *o, last, di, st);
     else
-      rc = now <= fgms::ADAMW_FEW ? launch_adamw<false, fgms::ADAMW_FEW>(tensors + at, now, *o, last, di.sms, st)
-                                  : launch_adamw<false, fgms::ADAMW_MANY>(tensors + at, now, *o, last, di.sms, st);
+      rc = now <= fgms::ADAMW_FEW ? launch_adamw<false, fgms::ADAMW_FEW>(tensors + at, now, *o, last, di, st)
+                                  : launch_adamw<false, fgms::ADAMW_MANY>(tensors + at, now, *o, last, di, st);
     if (rc != FGMS_OK || last) return rc;
     at += now;
   }

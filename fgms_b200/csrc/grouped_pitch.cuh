@@ -36,19 +36,20 @@ __device__ __forceinline__ void grouped_copy_rows(const GroupedRows& r, long lon
   }
 }
 
-// two matrices (either may have no rows)
-__global__ void __launch_bounds__(GP_THREADS) grouped_copy_kernel(GroupedRows x, GroupedRows y) {
+// two matrices (either may have no rows); alone: see GmsParams
+__global__ void __launch_bounds__(GP_THREADS) grouped_copy_kernel(GroupedRows x, GroupedRows y, int alone) {
   umma::griddep_wait();
-  umma::griddep_launch_dependents();
+  if (!alone) umma::griddep_launch_dependents();
   grouped_copy_rows(x, 0, x.rows, false);
   grouped_copy_rows(y, 0, y.rows, false);
 }
 
 // the rows of the groups; the others are left as they were, or become zeros
-__global__ void __launch_bounds__(GP_THREADS) grouped_copy_back_kernel(GroupedRows r, const int32_t* __restrict__ kpos, int groups, int zero_rest) {
+__global__ void __launch_bounds__(GP_THREADS) grouped_copy_back_kernel(GroupedRows r, const int32_t* __restrict__ kpos, int groups, int zero_rest,
+                                                                      int alone) {
   __shared__ int ends[2];
   umma::griddep_wait();
-  umma::griddep_launch_dependents();
+  if (!alone) umma::griddep_launch_dependents();
   if (threadIdx.x < 32) {  // as build_group_table has them (which has counted the entries that were changed)
     int last = 0;
     for (int s = threadIdx.x; s <= groups; s += 32) last = max(last, (int)min((long long)max(__ldg(kpos + s), 0), r.rows));

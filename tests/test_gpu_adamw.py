@@ -649,3 +649,21 @@ def test_a_block_of_zeros_is_held_as_zeros():
     s.run()
     assert not s.m[0].float()[:128].any() and not s.v[0].float()[:128].any() and s.ms[0][0] == 0 and s.vs[0][0] == 0
     assert s.vs[0][1] > 0
+
+
+@pytest.mark.parametrize("keep", [8, 64])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_with_sms_kept_free(bits, keep):
+    """Steps behind one another, of several launches each: the same as with all SMs, to the bit."""
+    from fgms_b200 import _lib
+    kept, free = (State(counts=[(i * 37) % 300 for i in range(450)] + [100003], param="fp16", master=True, bits=bits, seed=15) for _ in range(2))
+    for _ in range(3):
+        free.run()
+    assert _lib.lib.fgms_b200_set_reserved_sms(keep) == _lib.OK
+    try:
+        for _ in range(3):
+            kept.run()
+    finally:
+        _lib.lib.fgms_b200_set_reserved_sms(0)
+    view = lambda t: t.view(torch.uint8) if t.dtype == torch.float8_e4m3fn else t
+    assert all(torch.equal(view(a), view(b)) for a, b in zip(kept.all(), free.all()))

@@ -606,3 +606,19 @@ def test_rows_cleared_for_the_other_cta_of_a_pair(dtype):
     first = layer.check("wgrad")
     for _ in range(10):
         assert torch.equal(first, layer.run("wgrad"))
+
+
+@pytest.mark.parametrize("keep", [8, 64])
+def test_copied_rows_with_sms_kept_free(keep):
+    from fgms_b200 import _lib, backend
+    layer = Layer("bf16", [300, 0, 700], 1001, 1003, start=5, rest=30, seed=27)
+    assert _lib.lib.fgms_b200_set_reserved_sms(keep) == _lib.OK
+    try:
+        for which in PASSES:
+            launches = backend.launch_count()
+            layer.check(which)
+            assert backend.launch_count() - launches >= 2
+            if which != "wgrad":
+                layer.check(which, zero_rest=True)
+    finally:
+        _lib.lib.fgms_b200_set_reserved_sms(0)

@@ -141,3 +141,13 @@ def test_pointers_off_a_boundary_of_their_type_are_refused(dtype, off):
     assert fwd(kpos=4 * P + 2, dtype=dtype) == _lib.ERR_INVALID_ARG and "boundary" in _lib.last_error()
     for call, tail in ((_lib.lib.fgms_b200_grouped_dgrad, (0, None, 0, None)), (_lib.lib.fgms_b200_grouped_wgrad, (None, 0, None))):
         assert call(P + off, 2 * P, 3 * P, 4 * P, 10, 8, 8, 4, dtype, *tail) == _lib.ERR_INVALID_ARG and "boundary" in _lib.last_error()
+
+
+@pytest.mark.parametrize("source", ["grouped.cuh", "grouped_umma.cuh", "grouped_ffma.cuh", "grouped_pitch.cuh", "adamw.cuh"])
+def test_nothing_behind_is_let_go_early_with_sms_kept_free(source):
+    """``fgms_b200_set_reserved_sms``: what is enqueued behind a launch starts when it has ended, so no kernel lets it go before."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    with open(os.path.join(root, "fgms_b200", "csrc", source)) as f:
+        for line in f:
+            if "griddep_launch_dependents()" in line:
+                assert "if (!p.alone)" in line or "if (!alone)" in line, line
