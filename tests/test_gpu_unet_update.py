@@ -82,3 +82,40 @@ def test_module_with_the_optimizer():
     for p, b in zip(net.parameters(), before):
         want = b.double() * (1 - 1e-5) - 1e-3 * p.grad.double() / (p.grad.double().abs() + 1e-8)
         assert ((p.double() - want).abs() <= want.abs() * 2.0 ** -11 + 1e-3 * 2.0 ** -19 + 2.0 ** -25).all()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_replays_take_the_steps_of_the_formula(bits):
+    """Each replay's step in 64 bits from the master and the moments before it and from the gradient that the replay itself left, which holds although the
+    gradients' last bits differ from run to run.  Differences: a moment is off by 2^-22 of its terms, the update by 2^-20 of its size with the
+    terms of m in m's place, the value by 2^-22 of itself."""
+    lr, b1, b2, eps, decay = 1e-4, 0.9, 0.999, 1e-8, 0.1
+    step = stack(optimizer={"lr": lr, "betas": (b1, b2), "eps": eps, "weight_decay": decay, "state_bits": bits})
+    step.run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step.run()
+    state = step.optimizer.state[step._w_flat]
+
+    def moment(name):
+        held = state[name].float().double().view(-1)
+        if bits == 32:
+            return held
+        return held * state[name + "_scale"].double().repeat_interleave(128)[:held.numel()]
+    for t in (2, 3, 4):
+        w, m, v = state["master"].double().view(-1), moment("exp_avg"), moment("exp_avg_sq")
+        feats_in = step.val[step.out_name].clone()
+        step.w_grad.zero_()
+        graph.replay()
+        g = step.w_grad.double().view(-1)
+        assert g.any() and not torch.equal(feats_in, step.val[step.out_name])  # this replay's own forward and gradient
+        terms = b1 * m.abs() + (1 - b1) * g.abs()
+        m, v = b1 * m + (1 - b1) * g, b2 * v + (1 - b2) * g * g
+        rate, denominator = lr / (1 - b1 ** t), (v / (1 - b2 ** t)).sqrt() + eps
+        want = w * (1 - lr * decay) - rate * m / denominator
+        now = state["master"].double().view(-1)
+        assert ((now - want).abs() <= w.abs() * 2.0 ** -22 + rate * terms / denominator * 2.0 ** -20 + 2.0 ** -149).all()
+        moved = (now - w).abs()
+        assert (moved[g != 0] > 0).double().mean() > 0.99 and torch.equal(step._w_flat, state["master"].half())
+        assert state["step"].tolist() == [t, 0]
