@@ -333,7 +333,6 @@ class UNetStep:
         self.optimizer = None
         if optimizer is not None:
             from .optim import AdamW
-            self._w_flat.grad = self.w_grad
             self.optimizer = AdamW([self._w_flat], **optimizer)
             self.launches_per_step += 1
         # what the caller sees: the layer list as given, the stem's real input channels only
@@ -404,6 +403,7 @@ class UNetStep:
         """A step of the optimizer with the gradients of the last backward."""
         if self.optimizer is None:
             raise ValueError("update() needs UNetStep(..., optimizer={...})")
+        self._w_flat.grad = self.w_grad  # also behind an optimizer.zero_grad(), which drops it
         self.optimizer.step()
 
     def run(self):

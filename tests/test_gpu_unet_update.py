@@ -119,3 +119,15 @@ def test_replays_take_the_steps_of_the_formula(bits):
         moved = (now - w).abs()
         assert (moved[g != 0] > 0).double().mean() > 0.99 and torch.equal(step._w_flat, state["master"].half())
         assert state["step"].tolist() == [t, 0]
+
+
+@pytest.mark.parametrize("set_to_none", [True, False])
+def test_the_update_is_taken_behind_zero_grad(set_to_none):
+    """The optimizer is a PyTorch one, and loops over those clear gradients: the step's own, which every backward overwrites, are used all the same."""
+    step = stack(optimizer={"lr": 1e-4})
+    for t in (1, 2):
+        before = step._w_flat.clone()
+        step.optimizer.zero_grad(set_to_none=set_to_none)
+        step.run()
+        assert step.w_grad.any() and not torch.equal(step._w_flat, before)
+        assert step.optimizer.state[step._w_flat]["step"].tolist() == [t, 0]
