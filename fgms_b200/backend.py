@@ -292,7 +292,7 @@ def fgms_adamw_cuda(params, grads, exp_avgs, exp_avg_sqs, step, lr, beta1=0.9, b
     one) the step is taken on the master and the parameter is its rounded copy.  ``exp_avgs`` and ``exp_avg_sqs`` are float32, or
     ``torch.float8_e4m3fn`` with ``exp_avg_scales`` / ``exp_avg_sq_scales``, a float32 value for each 128 of a tensor's
     (``codes.float() * scale`` is the moment; all zeros before the first step); codes are rounded up or down at random (``seed``, the
-    step and the index decide), so that the moving averages keep their mean.
+    step and the index decide), so that the moving averages keep their mean; a second moment below 1/229376 of the largest of its 128 is held at that.
 
     ``step`` is an int32 tensor ``[steps done, 0]`` on the device, counted up by the call, so that a captured graph can be replayed;
     ``lr`` a number, or a float32 tensor of one value on the device, which a replayed graph follows.  Gradients are divided by ``grad_scale``;

@@ -1,4 +1,4 @@
-"""AdamW for the networks of this package: one launch for all parameters, moments in 32 or in 8 bits.
+"""AdamW for the networks of this package: one launch for parameters that take their steps together, moments in 32 or in 8 bits.
 
 The layers leave gradients (``nn``, ``unet.UNetStep``); this is what takes a step with them.  The kernel is
 ``backend.fgms_adamw_cuda`` (``csrc/adamw.cuh``).
@@ -21,10 +21,15 @@ class AdamW(torch.optim.Optimizer):
 
     ``state_bits=8`` keeps both moments as e4m3 codes with a float32 scale for each 128 values, a quarter of the memory and of the
     traffic; codes are rounded at random, reproducibly for a ``seed``.  float16 and bfloat16 parameters get a float32 ``master`` copy, without
-    which updates of less than half a step of their type are lost, unless ``master=False``.  Works in a captured graph (the steps are
+    which updates of less than half a step of their type are lost, unless ``master=False``; whoever else writes such a parameter writes
+    ``state[p]["master"]`` too, as the next step starts from that.  Works in a captured graph (the steps are
     counted on the device; ``lr`` may be a float32 tensor of one value there) and with ``torch.amp.GradScaler``, whose scale and verdict
-    the kernel reads.  Before a capture every parameter must have taken a step, as its state would be made anew by every replay.  Parameters must be contiguous CUDA tensors; a parameter without a gradient is passed over.  No sparse gradients,
-    no ``amsgrad``, no ``maximize``."""
+    the kernel reads.  Before a capture every parameter must have taken a step, as its state would be made anew by every replay; after it the graph works on
+    the state there is: ``load_state_dict`` makes another, and a step outside the graph has to be taken by the same parameters.  Parameters must
+    be contiguous CUDA tensors; a parameter without a gradient is passed over.  No sparse gradients, no ``amsgrad``, no ``maximize``.
+
+    The parameters of a group that have all taken the same steps share the count of them, and a launch for each 400.  Those that miss a step have a
+    count and a launch of their own from then on, also if the others miss one later; only ``load_state_dict`` brings equal counts together."""
 
     _step_supports_amp_scaling = True  # GradScaler hands over its scale and what it found instead of waiting for the device
 

@@ -303,8 +303,10 @@ size_t fgms_b200_grouped_workspace_bytes(int pass, const void* first, const void
  * in fp32, where w is the fp32 `master` of a tensor that has one, else the parameter; the parameter becomes w rounded once.
  * state_bits 32: exp_avg and exp_avg_sq are fp32.  state_bits 8: both are e4m3 codes (one byte each) with an fp32 scale for each 128
  * values, ceil(count / 128) of them, code * scale being the value; a value is rounded up with the probability of the part that is cut off (random bits: a
- * hash of seed, t and the value's index), so that a moving average keeps its mean, and an exp_avg_sq above zero stays above zero.  A gradient
- * that is not finite makes its block of 128 NaN from then on, as it makes its own moments NaN with 32 bits.
+ * hash of seed, t and the value's index), so that a moving average keeps its mean.  An exp_avg_sq above zero stays above zero: below the smallest code
+ * of its block (1/229376 of the largest value) it is held at that code, and its value moves by less than with 32 bits.  A gradient that is not
+ * finite, or whose square is not in fp32, makes its block of 128 NaN from then on (the square that of exp_avg_sq), where with 32 bits it makes
+ * its own moments NaN or infinite.
  * All zeros are the state before the first step.  Parameters and gradients: F32, F16 or BF16, each by itself.  Any alignment.
  * No buffer that is written may overlap another one (FGMS_ERR_INVALID_ARG): a tensor cannot be in the list twice. */
 typedef struct {

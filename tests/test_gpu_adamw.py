@@ -667,3 +667,26 @@ def test_with_sms_kept_free(bits, keep):
         _lib.lib.fgms_b200_set_reserved_sms(0)
     view = lambda t: t.view(torch.uint8) if t.dtype == torch.float8_e4m3fn else t
     assert all(torch.equal(view(a), view(b)) for a, b in zip(kept.all(), free.all()))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_gradient_whose_square_is_not_finite(bits):
+    """The step itself is that of the formula (an infinite denominator for the value, everything else as without it).  Its second moment is infinite from then on,
+    with 8 bits that of its block NaN; first moments stay finite."""
+    a, b = (State(counts=[1000], param="fp32", bits=bits, seed=16) for _ in range(2))
+    a.g[0][300] = 1e20
+    before = a.p[0][300].item()
+    for s in (a, b):
+        s.run()
+    at = torch.zeros(1000, dtype=torch.bool, device="cuda")
+    at[300] = True
+    assert torch.equal(a.p[0][~at], b.p[0][~at])
+    assert abs(a.p[0][300].item() - before * (1 - LR * DECAY)) <= abs(before) * 2.0 ** -22
+    (m,), (v,) = a.moments()
+    assert torch.isfinite(m).all()
+    if bits == 8:
+        at[256:384] = True
+        assert torch.isnan(v[at]).all()
+    else:
+        assert torch.isinf(v[at]).all()
+    assert torch.equal(v[~at], b.moments()[1][0][~at])
