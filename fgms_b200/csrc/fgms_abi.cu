@@ -478,7 +478,7 @@ int check_adamw(const fgms_b200_adamw_tensor* tensors, int n, const fgms_b200_ad
 
 template <bool EIGHT, int N>
 int launch_adamw(const fgms_b200_adamw_tensor* tensors, int n, const fgms_b200_adamw_options& o, bool last, const DeviceInfo& di, cudaStream_t st) {
-  static thread_local fgms::AdamwParams<N> p;  // up to 32 KB: kept, as a new one would be cleared by every call
+  static thread_local fgms::AdamwParams<N> p;  // up to 32 KB, kept by the thread: only the copies that the launch makes are on its stack
   p.lr = o.lr; p.beta1 = o.beta1; p.beta2 = o.beta2; p.decay = o.weight_decay;
   p.b1 = (float)o.beta1; p.c1 = (float)(1.0 - o.beta1);
   p.b2 = (float)o.beta2; p.c2 = (float)(1.0 - o.beta2);
