@@ -28,6 +28,23 @@ class AdamwOptions(ctypes.Structure):
                 ("seed", ctypes.c_uint32), ("state_bits", c_int)]
 
 
+class DropoutArgs(ctypes.Structure):
+    _fields_ = ([(n, c_void_p) for n in ("x", "residual", "out")] + [(n, c_int64) for n in ("x_pitch", "residual_pitch", "out_pitch", "rows", "width")] +
+                [("rng", c_void_p), ("rng_used", c_void_p), ("p", c_double), ("dtype", c_int)])
+
+
+class RmsNormArgs(ctypes.Structure):
+    _fields_ = ([(n, c_void_p) for n in ("x", "residual", "weight", "out", "sum", "scale", "rstd")] +
+                [(n, c_int64) for n in ("x_pitch", "residual_pitch", "out_pitch", "sum_pitch", "rows", "width")] +
+                [("rng", c_void_p), ("rng_used", c_void_p), ("eps", c_double), ("p", c_double), ("dtype", c_int), ("weight_dtype", c_int)])
+
+
+class RmsNormBwdArgs(ctypes.Structure):
+    _fields_ = ([(n, c_void_p) for n in ("out_grad", "sum", "sum_grad", "weight", "rstd", "x_grad", "residual_grad", "weight_grad")] +
+                [(n, c_int64) for n in ("out_grad_pitch", "sum_pitch", "sum_grad_pitch", "x_grad_pitch", "residual_grad_pitch", "rows", "width")] +
+                [("rng_used", c_void_p), ("workspace", c_void_p), ("workspace_bytes", c_size_t), ("p", c_double), ("dtype", c_int), ("weight_dtype", c_int)])
+
+
 # name -> (restype, argtypes); mirrors include/fgms_b200.h declaration by declaration
 SIGNATURES = {
     "fgms_b200_fusion_fwd": (c_int, [c_void_p] * 7 + [c_int64] + [c_int] * 6 + [c_int64] + [c_int] * 3 + [c_void_p]),
@@ -61,6 +78,12 @@ SIGNATURES = {
     "fgms_b200_grouped_wgrad": (c_int, [c_void_p] * 4 + [c_int] * 5 + [c_void_p, c_size_t, c_void_p]),
     "fgms_b200_grouped_workspace_bytes": (c_size_t, [c_int] + [c_void_p] * 3 + [c_int] * 5),
     "fgms_b200_adamw": (c_int, [c_void_p, c_int, c_void_p, c_void_p]),
+    "fgms_b200_dropout": (c_int, [c_void_p, c_void_p]),
+    "fgms_b200_dropout_bwd": (c_int, [c_void_p, c_void_p]),
+    "fgms_b200_rms_norm": (c_int, [c_void_p, c_void_p]),
+    "fgms_b200_rms_norm_bwd_workspace_bytes": (c_size_t, [c_int64, c_int64]),
+    "fgms_b200_rms_norm_bwd": (c_int, [c_void_p, c_void_p]),
+    "fgms_b200_quantize_rows": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int, c_void_p]),
     "fgms_b200_peer_exchange_flag_bytes": (c_size_t, [c_int]),
     "fgms_b200_peer_exchange": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int64, ctypes.c_uint32, c_int64, c_int, c_void_p]),
     "fgms_b200_kernel_family": (c_int, [c_int] * 6),

@@ -32,7 +32,8 @@ from . import _lib, _native
 __all__ = ["fgms_fusion_fwd_cuda", "fgms_fwd_cuda", "fgms_bwd_cuda", "fgms_dgrad_cuda", "fgms_wgrad_cuda",
            "wgrad_workspace", "wgrad_finalize", "fgms_wgrad_noalloc_cuda", "kernel_family", "fallback_count",
            "device_status", "launch_count", "build_neighbor_table", "fgms_fwd_os_cuda", "fgms_grouped_fwd_cuda",
-           "fgms_grouped_dgrad_cuda", "fgms_grouped_wgrad_cuda", "fgms_adamw_cuda"]
+           "fgms_grouped_dgrad_cuda", "fgms_grouped_wgrad_cuda", "fgms_adamw_cuda", "fgms_rms_norm_cuda", "fgms_rms_norm_bwd_cuda",
+           "fgms_quantize_rows_cuda", "fgms_dropout_cuda", "fgms_dropout_bwd_cuda"]
 
 _L = _lib.lib
 
@@ -300,6 +301,45 @@ def fgms_adamw_cuda(params, grads, exp_avgs, exp_avg_sqs, step, lr, beta1=0.9, b
     ``torch.amp.GradScaler`` has them).  :class:`fgms_b200.optim.AdamW` keeps all of this for a network."""
     _native.adamw(params, grads, exp_avgs, exp_avg_sqs, step, lr, beta1, beta2, eps, weight_decay, masters, exp_avg_scales, exp_avg_sq_scales,
                   seed, grad_scale, found_inf)
+
+
+def fgms_rms_norm_cuda(x, weight, out, eps=1e-6, residual=None, residual_out=None, scale=None, rstd=None, dropout=0.0, rng=None, rng_used=None):
+    """``out = h * weight / sqrt(mean(h ** 2) + eps)`` for the rows of ``h = residual + dropped x`` (``fgms_b200_rms_norm``).
+
+    Rows are ``[rows, width]`` of float32, float16 or bfloat16, any distance apart, up to 32768 wide; ``weight`` is of their type or float32.
+    ``residual_out`` gets ``h``, rounded once (the norm takes it before that), ``rstd`` (float32, one a row) what
+    :func:`fgms_rms_norm_bwd_cuda` needs.  With ``scale`` (float32, one a row) ``out`` is int8 codes, ``codes * scale`` being the values: what
+    :func:`fgms_grouped_i8_fwd_cuda` multiplies; a row that is not finite has a scale of NaN.  ``dropout``, ``rng`` and ``rng_used``: see
+    :func:`fgms_dropout_cuda`.  ``out`` and ``residual_out`` may be ``x`` or ``residual`` themselves."""
+    _native.rms_norm_into(x, weight, out, eps, residual, residual_out, scale, rstd, dropout, rng, rng_used)
+
+
+def fgms_rms_norm_bwd_cuda(out_grad, h, weight, rstd, x_grad=None, weight_grad=None, h_grad=None, residual_grad=None, dropout=0.0, rng_used=None):
+    """Gradient of :func:`fgms_rms_norm_cuda` from ``h`` (``residual_out``, or ``x`` where there was neither residual nor dropout) and ``rstd``:
+    ``residual_grad = dh``, ``x_grad`` the same where x was kept, ``weight_grad`` (the weight's type, summed in float32 in a fixed order).
+    ``h_grad`` is what else flows back into ``h``.  Outputs that are None are left out."""
+    _native.rms_norm_bwd(out_grad, h, weight, rstd, x_grad, weight_grad, h_grad, residual_grad, dropout, rng_used)
+
+
+def fgms_quantize_rows_cuda(x, codes, scale):
+    """Rows in 8 bits with a scale each, ``codes * scale`` being the values, the largest magnitude of a row its code 127
+    (``fgms_b200_quantize_rows``): weights whose rows are output channels get their codes this way."""
+    _native.quantize_rows_into(x, codes, scale)
+
+
+def fgms_dropout_cuda(x, out, p, rng, residual=None, rng_used=None):
+    """``out = residual + dropped x`` (``fgms_b200_dropout``): a value is dropped with probability ``p``, rounded to a multiple of 2^-16, the others are
+    divided by the probability of that.  No mask is stored: the lots are Philox 4x32-10 of the seed, the number of the call, row and column.
+
+    ``rng`` is an int64 tensor ``[seed, calls made, 0]`` on the device (:func:`fgms_b200.nn.rng_state`), counted up by the call, so that a
+    captured graph drops other values in every replay; calls that share it must not run at the same time.  ``rng_used`` (int64, two entries) gets
+    what the backward needs."""
+    _native.dropout_into(x, out, p, rng, residual, rng_used)
+
+
+def fgms_dropout_bwd_cuda(out_grad, x_grad, p, rng_used):
+    """Gradient of :func:`fgms_dropout_cuda`: what dropped x drops, with the same lots (the residual's gradient is ``out_grad`` itself)."""
+    _native.dropout_bwd(out_grad, x_grad, p, rng_used)
 
 
 def kernel_family(pass_: str, c_in: int, c_out: int, dtype: torch.dtype, arch80: bool = True, k_vol: int = 27) -> str:

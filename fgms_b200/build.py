@@ -18,9 +18,9 @@ from importlib import metadata
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libfgms_b200.so")
-SOURCES = [os.path.join(CSRC, "fgms_abi.cu")]
+SOURCES = [os.path.join(CSRC, "fgms_abi.cu"), os.path.join(CSRC, "layers_abi.cu")]
 NVCC_FLAGS = [
-    "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
+    "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "--threads", "2",
     # no GNU-unique symbols: two builds of the library in one process keep their launch state apart
     "-Xcompiler", "-fPIC,-fno-gnu-unique", "-shared", "-cudart", "shared", "-ldl",
 ]

@@ -14,8 +14,7 @@
 #include <cstdlib>
 #include <vector>
 
-#include <nvtx3/nvToolsExt.h>
-
+#include "host.cuh"
 #include "common.cuh"
 #include "simt_kernels.cuh"
 #include "ffma_rows.cuh"
@@ -35,55 +34,7 @@
 
 namespace {
 
-thread_local char g_err[512] = "";
-std::atomic<long long> g_launches{0};
-// launches that the shape alone would have sent to the tensor-core kernels but that ran on the CUDA-core
-// kernels (base pointers not 16-byte aligned): fgms_b200_fallback_count()
-std::atomic<long long> g_fallbacks{0};
-// SMs the persistent kernels leave free (fgms_b200_set_reserved_sms): room for a kernel of another stream
-std::atomic<int> g_reserved_sms{0};
-
-int fail(int code, const char* fmt, ...) {
-  va_list ap;
-  va_start(ap, fmt);
-  vsnprintf(g_err, sizeof(g_err), fmt, ap);
-  va_end(ap);
-  return code;
-}
-
-int check_launch(const char* what) {
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return fail(FGMS_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
-  g_launches.fetch_add(1, std::memory_order_relaxed);
-  return FGMS_OK;
-}
-
-struct DeviceInfo {
-  int sms = 0;       // to launch on
-  int reserved = 0;  // to leave free
-  int max_smem_optin = 0;
-};
-
-int device_info(DeviceInfo* out) {
-  static thread_local int cached_dev = -1;
-  static thread_local DeviceInfo cached;
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return fail(FGMS_ERR_CUDA, "cudaGetDevice: %s", cudaGetErrorString(e));
-  if (dev != cached_dev) {
-    cudaDeviceProp prop;
-    e = cudaGetDeviceProperties(&prop, dev);
-    if (e != cudaSuccess) return fail(FGMS_ERR_CUDA, "cudaGetDeviceProperties: %s", cudaGetErrorString(e));
-    cached.sms = prop.multiProcessorCount;
-    cached.max_smem_optin = (int)prop.sharedMemPerBlockOptin;
-    cached_dev = dev;
-  }
-  *out = cached;
-  const int keep = g_reserved_sms.load(std::memory_order_relaxed);
-  out->reserved = keep;
-  if (keep > 0) out->sms = cached.sms - keep > 1 ? cached.sms - keep : 1;
-  return FGMS_OK;
-}
+using namespace fgms_host;
 
 bool dtype_ok(int dtype) { return dtype == FGMS_DTYPE_F32 || dtype == FGMS_DTYPE_F16; }
 
@@ -208,24 +159,6 @@ int check_fwd_args(const void* in_feats, const void* kernel, void* out_feats, co
 }
 
 size_t elem_size(int dtype) { return dtype == FGMS_DTYPE_F16 ? 2 : 4; }
-
-// NVTX range named after the entry point, open for the duration of the host call (the enqueue); a timeline tool
-// shows the kernels launched inside it under that name.  Without a tool attached the calls return at once.
-struct TraceRange {
-  explicit TraceRange(const char* name) { nvtxRangePushA(name); }
-  ~TraceRange() { nvtxRangePop(); }
-  TraceRange(const TraceRange&) = delete;
-  TraceRange& operator=(const TraceRange&) = delete;
-};
-
-struct Range {
-  const void* p;
-  size_t bytes;
-  bool overlaps(const Range& o) const {
-    const uintptr_t a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(o.p);
-    return a < b + o.bytes && b < a + bytes;
-  }
-};
 
 int check_dgrad_args(const void* out_grad, const void* kernel, const void* in_grad, const int32_t* kpos, const int32_t* in_map,
                      const int32_t* out_map, int64_t map_len, int n_in, int n_out, int c_in, int c_out, int k_vol, int dtype, int math) {
@@ -1172,13 +1105,8 @@ int64_t fgms_b200_device_status(int reset) {
   cudaError_t e = cudaDeviceSynchronize();
   if (e != cudaSuccess) return fail(FGMS_ERR_CUDA, "cudaDeviceSynchronize: %s", cudaGetErrorString(e));
   unsigned long long v = 0;
-  e = cudaMemcpyFromSymbol(&v, fgms::g_device_problems, sizeof(v));
-  if (e != cudaSuccess) return fail(FGMS_ERR_CUDA, "cudaMemcpyFromSymbol: %s", cudaGetErrorString(e));
-  if (reset) {
-    unsigned long long z = 0;
-    e = cudaMemcpyToSymbol(fgms::g_device_problems, &z, sizeof(z));
-    if (e != cudaSuccess) return fail(FGMS_ERR_CUDA, "cudaMemcpyToSymbol: %s", cudaGetErrorString(e));
-  }
+  if (int rc = fgms_host::take_problems(fgms::g_device_problems, reset, &v)) return rc;
+  if (int rc = fgms_host::take_layer_problems(reset, &v)) return rc;
   return (int64_t)v;
 }
 

@@ -1,0 +1,339 @@
+// Entry points of what stands between and around layers of groups: norm, dropout, rows and products in 8 bits, a layer of experts for a few tokens
+// (see include/fgms_b200.h for the contract of each).  They have no counterpart in the reference.
+#include "../../include/fgms_b200.h"
+
+#include <cmath>
+
+#include "host.cuh"
+#include "dropout.cuh"
+#include "row_norm.cuh"
+
+namespace fgms_host {
+int take_layer_problems(int reset, unsigned long long* sum) { return take_problems(fgms::g_device_problems, reset, sum); }
+}  // namespace fgms_host
+
+namespace {
+
+using namespace fgms_host;
+
+bool layer_dtype_ok(int dtype) { return dtype == FGMS_DTYPE_F32 || dtype == FGMS_DTYPE_F16 || dtype == FGMS_DTYPE_BF16; }
+size_t layer_elem(int dtype) { return dtype == FGMS_DTYPE_F32 ? 4 : 2; }
+
+// Rows of `width` values in memory, `pitch` values apart (of a single row: whatever the caller says).
+struct RowSpan {
+  const void* p;
+  int64_t rows, pitch, width;
+  size_t es;
+  RowSpan(const void* p_, int64_t rows_, int64_t pitch_, int64_t width_, size_t es_) : p(p_), rows(rows_), pitch(rows_ > 1 ? pitch_ : width_), width(width_), es(es_) {}
+  bool any() const { return p != nullptr && rows > 0; }
+  size_t bytes() const { return rows > 0 ? ((size_t)(rows - 1) * (size_t)pitch + (size_t)width) * es : 0; }
+  // whether any value of one is a value of the other, except where both are the very same rows
+  bool collides(const RowSpan& o) const {
+    if (!any() || !o.any()) return false;
+    const uintptr_t a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(o.p);
+    const size_t row = (size_t)pitch * es, mine = (size_t)width * es, its = (size_t)o.width * o.es;
+    if (row == (size_t)o.pitch * o.es) {
+      if (a == b && es == o.es && width == o.width) return false;
+      const size_t apart = b > a ? (size_t)(b - a) % row : (row - (size_t)(a - b) % row) % row;  // columns side by side in the same rows
+      if (apart >= mine && row - apart >= its) return false;
+    }
+    return Range{p, bytes()}.overlaps(Range{o.p, o.bytes()});
+  }
+  bool same(const RowSpan& o) const { return any() && o.any() && p == o.p; }
+  bool on_boundary() const { return (reinterpret_cast<uintptr_t>(p) & (es - 1)) == 0; }
+  bool vec(size_t boundary) const { return (reinterpret_cast<uintptr_t>(p) & (boundary - 1)) == 0 && (rows <= 1 || (size_t)pitch * es % boundary == 0); }
+};
+
+int check_span(const char* name, const RowSpan& s, bool needed) {
+  if (!s.p) return needed && s.rows > 0 ? fail(FGMS_ERR_INVALID_ARG, "%s: null pointer", name) : FGMS_OK;
+  if (s.rows > 1 && s.pitch < s.width) return fail(FGMS_ERR_INVALID_ARG, "%s: rows are %lld values apart, %lld wide", name, (long long)s.pitch, (long long)s.width);
+  if (s.pitch > 0x7fffffffll * 16) return fail(FGMS_ERR_INVALID_ARG, "%s: rows too far apart", name);
+  if (!s.on_boundary()) return fail(FGMS_ERR_INVALID_ARG, "%s is not on a boundary of its type", name);
+  return FGMS_OK;
+}
+
+int check_rows(int64_t rows, int64_t width, int64_t most) {
+  if (rows < 0 || rows > 0x7fffffffll) return fail(FGMS_ERR_INVALID_ARG, "rows %lld outside [0, 2^31 - 1]", (long long)rows);
+  if (width < 1 || width > most) return fail(FGMS_ERR_INVALID_ARG, "width %lld outside [1, %lld]", (long long)width, (long long)most);
+  return FGMS_OK;
+}
+
+// the lots below which a value is dropped
+int drop_threshold(double p, uint32_t* threshold, float* factor) {
+  if (!(p >= 0.0 && p <= 1.0)) return fail(FGMS_ERR_INVALID_ARG, "the probability of dropping must be in [0, 1], got %g", p);
+  *threshold = (uint32_t)std::lrint(p * 65536.0);
+  *factor = *threshold < 65536u ? (float)(65536.0 / (65536.0 - (double)*threshold)) : 0.f;
+  return FGMS_OK;
+}
+
+int check_state(const char* name, const void* at, bool needed) {
+  if (needed && !at) return fail(FGMS_ERR_INVALID_ARG, "%s: null pointer", name);
+  if (reinterpret_cast<uintptr_t>(at) & 7) return fail(FGMS_ERR_INVALID_ARG, "%s is not on a boundary of its type", name);
+  return FGMS_OK;
+}
+
+int run_dropout(const fgms_b200_dropout_args& a, bool backward, cudaStream_t st) {
+  if (int rc = check_rows(a.rows, a.width, 0x7ffffff0ll)) return rc;
+  if (!layer_dtype_ok(a.dtype)) return fail(FGMS_ERR_INVALID_ARG, "unknown dtype %d", a.dtype);
+  fgms::DropoutParams p{};
+  if (int rc = drop_threshold(a.p, &p.drop.threshold, &p.drop.factor)) return rc;
+  const size_t es = layer_elem(a.dtype);
+  const RowSpan x{a.x, a.rows, a.x_pitch, a.width, es}, residual{backward ? nullptr : a.residual, a.rows, a.residual_pitch, a.width, es},
+      out{a.out, a.rows, a.out_pitch, a.width, es};
+  if (int rc = check_span("x", x, true)) return rc;
+  if (int rc = check_span("residual", residual, false)) return rc;
+  if (int rc = check_span("out", out, true)) return rc;
+  if (int rc = check_state("rng", a.rng, !backward)) return rc;
+  if (int rc = check_state("rng_used", a.rng_used, backward)) return rc;
+  if (out.collides(x) || out.collides(residual)) return fail(FGMS_ERR_INVALID_ARG, "the output overlaps an input");
+  const Range written{a.out, out.bytes()}, state{a.rng, backward ? 0u : 24u}, used{a.rng_used, a.rng_used ? 16u : 0u};
+  for (const Range& r : {state, used})
+    if (r.p && r.bytes && (r.overlaps(written) || r.overlaps(Range{a.x, x.bytes()}) || (residual.any() && r.overlaps(Range{a.residual, residual.bytes()}))))
+      return fail(FGMS_ERR_INVALID_ARG, "the generator's state overlaps a tensor");
+  if (!backward && a.rng_used && state.overlaps(used)) return fail(FGMS_ERR_INVALID_ARG, "rng_used overlaps rng");
+  if (a.rows == 0) return FGMS_OK;
+  DeviceInfo di;
+  if (int rc = device_info(&di)) return rc;
+  p.x = a.x;
+  p.residual = residual.p;
+  p.out = a.out;
+  p.rows = a.rows;
+  p.width = (int)a.width;
+  p.x_pitch = a.x_pitch;
+  p.residual_pitch = a.residual_pitch;
+  p.out_pitch = a.out_pitch;
+  p.x_vec = x.vec(16);
+  p.residual_vec = residual.vec(16);
+  p.out_vec = out.vec(16);
+  p.drop.state = reinterpret_cast<long long*>(a.rng);
+  p.drop.used = reinterpret_cast<long long*>(a.rng_used);
+  p.alone = di.reserved > 0;
+  const long long chunks = a.rows * ((a.width + fgms::ROW_CHUNK - 1) / fgms::ROW_CHUNK);
+  const long long blocks = (chunks + fgms::DROP_THREADS - 1) / fgms::DROP_THREADS, most = 8ll * di.sms;
+  const dim3 grid((unsigned)(blocks < most ? blocks : most));
+  const auto launch = [&](auto type) {
+    using T = decltype(type);
+    return backward ? fgms::launch_pdl(fgms::dropout_kernel<T, true>, grid, fgms::DROP_THREADS, 0, st, p)
+                    : fgms::launch_pdl(fgms::dropout_kernel<T, false>, grid, fgms::DROP_THREADS, 0, st, p);
+  };
+  const cudaError_t e = a.dtype == FGMS_DTYPE_F32 ? launch(float()) : a.dtype == FGMS_DTYPE_F16 ? launch(__half()) : launch(__nv_bfloat16());
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return fail(FGMS_ERR_CUDA, "dropout_kernel: %s", cudaGetErrorString(e));
+  }
+  return check_launch("dropout_kernel");
+}
+
+// the types of rows and weight that a norm is built for: the weight's is the rows' or fp32
+template <typename F>
+cudaError_t with_types(int dtype, int weight_dtype, F&& f) {
+  if (dtype == FGMS_DTYPE_F32) return f(float(), float());
+  if (dtype == FGMS_DTYPE_F16) return weight_dtype == FGMS_DTYPE_F32 ? f(__half(), float()) : f(__half(), __half());
+  return weight_dtype == FGMS_DTYPE_F32 ? f(__nv_bfloat16(), float()) : f(__nv_bfloat16(), __nv_bfloat16());
+}
+int check_norm_types(int dtype, int weight_dtype) {
+  if (!layer_dtype_ok(dtype)) return fail(FGMS_ERR_INVALID_ARG, "unknown dtype %d", dtype);
+  if (weight_dtype != dtype && weight_dtype != FGMS_DTYPE_F32) return fail(FGMS_ERR_UNSUPPORTED, "the weight's type must be that of the rows, or fp32");
+  return FGMS_OK;
+}
+
+int run_rms_norm(const fgms_b200_rms_norm_args& a, bool norm, cudaStream_t st) {
+  if (int rc = check_rows(a.rows, a.width, fgms::NORM_MAX_WIDTH)) return rc;
+  if (int rc = check_norm_types(a.dtype, norm ? a.weight_dtype : a.dtype)) return rc;
+  if (norm && !(a.eps >= 0.0 && a.eps < 1e30)) return fail(FGMS_ERR_INVALID_ARG, "eps must be finite and not negative, got %g", a.eps);
+  fgms::NormParams p{};
+  if (int rc = drop_threshold(a.p, &p.drop.threshold, &p.drop.factor)) return rc;
+  const bool eight = a.scale != nullptr, drop = p.drop.threshold > 0;
+  if (eight && drop) return fail(FGMS_ERR_UNSUPPORTED, "no dropout with an output in 8 bits");
+  const size_t es = layer_elem(a.dtype);
+  const RowSpan x{a.x, a.rows, a.x_pitch, a.width, es}, residual{a.residual, a.rows, a.residual_pitch, a.width, es},
+      out{a.out, a.rows, a.out_pitch, a.width, eight ? 1u : es}, sum{a.sum, a.rows, a.sum_pitch, a.width, es};
+  const RowSpan weight{a.weight, 1, a.width, a.width, layer_elem(a.weight_dtype)}, scale{a.scale, 1, a.rows, a.rows, 4}, rstd{a.rstd, 1, a.rows, a.rows, 4};
+  if (int rc = check_span("x", x, true)) return rc;
+  if (int rc = check_span("residual", residual, false)) return rc;
+  if (int rc = check_span("out", out, true)) return rc;
+  if (int rc = check_span("sum", sum, false)) return rc;
+  if (norm)
+    if (int rc = check_span("weight", weight, true)) return rc;
+  if (int rc = check_span("scale", scale, false)) return rc;
+  if (int rc = check_span("rstd", rstd, false)) return rc;
+  if (int rc = check_state("rng", a.rng, drop)) return rc;
+  if (int rc = check_state("rng_used", a.rng_used, false)) return rc;
+  if (a.rows == 0) return FGMS_OK;
+  const RowSpan state{drop ? a.rng : nullptr, 1, 3, 3, 8}, used{drop ? a.rng_used : nullptr, 1, 2, 2, 8};
+  const RowSpan outputs[] = {out, sum, scale, rstd, state, used}, inputs[] = {x, residual, weight};
+  for (int i = 0; i < 6; ++i) {
+    for (const RowSpan& in : inputs)
+      if (outputs[i].collides(in) || (outputs[i].same(in) && (i >= 2 || &in == &inputs[2]))) return fail(FGMS_ERR_INVALID_ARG, "an output overlaps an input");
+    for (int j = 0; j < i; ++j)
+      if (outputs[i].collides(outputs[j]) || outputs[i].same(outputs[j])) return fail(FGMS_ERR_INVALID_ARG, "two outputs overlap");
+  }
+  DeviceInfo di;
+  if (int rc = device_info(&di)) return rc;
+  p.x = a.x;
+  p.residual = a.residual;
+  p.weight = a.weight;
+  p.out = a.out;
+  p.sum = a.sum;
+  p.scale = a.scale;
+  p.rstd = a.rstd;
+  p.rows = a.rows;
+  p.x_pitch = a.x_pitch;
+  p.residual_pitch = a.residual_pitch;
+  p.out_pitch = a.out_pitch;
+  p.sum_pitch = a.sum_pitch;
+  p.width = (int)a.width;
+  p.norm = norm;
+  p.x_vec = x.vec(16);
+  p.residual_vec = residual.vec(16);
+  p.out_vec = out.vec(eight ? 8 : 16);
+  p.sum_vec = sum.vec(16);
+  p.weight_vec = weight.vec(16);
+  p.eps = (float)a.eps;
+  p.inverse_width = 1.f / (float)a.width;
+  p.drop.state = reinterpret_cast<long long*>(a.rng);
+  p.drop.used = reinterpret_cast<long long*>(a.rng_used);
+  p.alone = di.reserved > 0;
+  const cudaError_t e = with_types(a.dtype, norm ? a.weight_dtype : a.dtype, [&](auto t, auto w) {
+    using T = decltype(t);
+    using W = decltype(w);
+    return eight ? fgms::launch_rms_norm<T, W, true>(p, st, di.sms) : fgms::launch_rms_norm<T, W, false>(p, st, di.sms);
+  });
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return fail(FGMS_ERR_CUDA, "rms_norm_kernel: %s", cudaGetErrorString(e));
+  }
+  return check_launch("rms_norm_kernel");
+}
+
+int run_rms_norm_bwd(const fgms_b200_rms_norm_bwd_args& a, cudaStream_t st) {
+  if (int rc = check_rows(a.rows, a.width, fgms::NORM_MAX_WIDTH)) return rc;
+  if (int rc = check_norm_types(a.dtype, a.weight_dtype)) return rc;
+  fgms::NormGradParams p{};
+  if (int rc = drop_threshold(a.p, &p.drop.threshold, &p.drop.factor)) return rc;
+  const bool drop = p.drop.threshold > 0;
+  const size_t es = layer_elem(a.dtype);
+  const auto span = [&](const void* at, int64_t pitch) { return RowSpan{at, a.rows, pitch, a.width, es}; };
+  const RowSpan dy = span(a.out_grad, a.out_grad_pitch), h = span(a.sum, a.sum_pitch), dsum = span(a.sum_grad, a.sum_grad_pitch), dx = span(a.x_grad, a.x_grad_pitch),
+                dresidual = span(a.residual_grad, a.residual_grad_pitch);
+  const RowSpan weight{a.weight, 1, a.width, a.width, layer_elem(a.weight_dtype)}, dw{a.weight_grad, 1, a.width, a.width, layer_elem(a.weight_dtype)},
+      rstd{a.rstd, 1, a.rows, a.rows, 4};
+  if (int rc = check_span("out_grad", dy, true)) return rc;
+  if (int rc = check_span("sum", h, true)) return rc;
+  if (int rc = check_span("sum_grad", dsum, false)) return rc;
+  if (int rc = check_span("x_grad", dx, false)) return rc;
+  if (int rc = check_span("residual_grad", dresidual, false)) return rc;
+  if (int rc = check_span("weight", weight, true)) return rc;
+  if (int rc = check_span("weight_grad", dw, false)) return rc;
+  if (int rc = check_span("rstd", rstd, a.rows > 0)) return rc;
+  if (int rc = check_state("rng_used", a.rng_used, drop)) return rc;
+  DeviceInfo di;
+  if (int rc = device_info(&di)) return rc;
+  const fgms::NormGradCut cut = fgms::norm_grad_cut(a.rows, (int)a.width, di.sms);
+  const size_t needed = a.weight_grad ? (size_t)cut.blocks * (size_t)a.width * 4 : 0;
+  if (needed > 0 && (!a.workspace || a.workspace_bytes < needed || (reinterpret_cast<uintptr_t>(a.workspace) & 15)))
+    return fail(FGMS_ERR_WORKSPACE, "a workspace of %zu bytes on a 16-byte boundary is needed", needed);
+  const RowSpan space{needed ? a.workspace : nullptr, 1, (int64_t)needed, (int64_t)needed, 1}, used{drop ? a.rng_used : nullptr, 1, 2, 2, 8};
+  const RowSpan outputs[] = {dx, dresidual, dw, space}, inputs[] = {dy, h, dsum, weight, rstd, used};
+  for (int i = 0; i < 4; ++i) {
+    for (int j = 0; j < 6; ++j)
+      if (outputs[i].collides(inputs[j]) || (outputs[i].same(inputs[j]) && (i >= 2 || j >= 3))) return fail(FGMS_ERR_INVALID_ARG, "an output overlaps an input");
+    for (int j = 0; j < i; ++j)
+      if (outputs[i].collides(outputs[j]) || outputs[i].same(outputs[j])) return fail(FGMS_ERR_INVALID_ARG, "two outputs overlap");
+  }
+  if (a.rows == 0) {  // no row adds anything to the weight's gradient
+    if (a.weight_grad && cudaMemsetAsync(a.weight_grad, 0, dw.bytes(), st) != cudaSuccess)
+      return fail(FGMS_ERR_CUDA, "cudaMemsetAsync: %s", cudaGetErrorString(cudaGetLastError()));
+    return FGMS_OK;
+  }
+  p.dy = a.out_grad;
+  p.sum = a.sum;
+  p.dsum = a.sum_grad;
+  p.weight = a.weight;
+  p.rstd = a.rstd;
+  p.dx = a.x_grad;
+  p.dresidual = a.residual_grad;
+  p.parts = a.weight_grad ? static_cast<float*>(a.workspace) : nullptr;
+  p.rows = a.rows;
+  p.dy_pitch = a.out_grad_pitch;
+  p.sum_pitch = a.sum_pitch;
+  p.dsum_pitch = a.sum_grad_pitch;
+  p.dx_pitch = a.x_grad_pitch;
+  p.dresidual_pitch = a.residual_grad_pitch;
+  p.width = (int)a.width;
+  p.dy_vec = dy.vec(16);
+  p.sum_vec = h.vec(16);
+  p.dsum_vec = dsum.vec(16);
+  p.dx_vec = dx.vec(16);
+  p.dresidual_vec = dresidual.vec(16);
+  p.weight_vec = weight.vec(16);
+  p.inverse_width = 1.f / (float)a.width;
+  p.drop.used = const_cast<long long*>(reinterpret_cast<const long long*>(a.rng_used));
+  p.alone = di.reserved > 0;
+  cudaError_t e = with_types(a.dtype, a.weight_dtype, [&](auto t, auto w) { return fgms::launch_rms_norm_grad<decltype(t), decltype(w)>(p, cut, st); });
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return fail(FGMS_ERR_CUDA, "rms_norm_grad_kernel: %s", cudaGetErrorString(e));
+  }
+  if (int rc = check_launch("rms_norm_grad_kernel")) return rc;
+  if (!a.weight_grad) return FGMS_OK;
+  const float* parts = p.parts;
+  e = a.weight_dtype == FGMS_DTYPE_F32   ? fgms::launch_rms_norm_weight_grad<float>(parts, cut.blocks, p.width, a.weight_grad, p.alone, st)
+      : a.weight_dtype == FGMS_DTYPE_F16 ? fgms::launch_rms_norm_weight_grad<__half>(parts, cut.blocks, p.width, a.weight_grad, p.alone, st)
+                                         : fgms::launch_rms_norm_weight_grad<__nv_bfloat16>(parts, cut.blocks, p.width, a.weight_grad, p.alone, st);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return fail(FGMS_ERR_CUDA, "rms_norm_weight_grad_kernel: %s", cudaGetErrorString(e));
+  }
+  return check_launch("rms_norm_weight_grad_kernel");
+}
+}  // namespace
+
+extern "C" {
+
+int fgms_b200_dropout(const fgms_b200_dropout_args* args, void* stream) {
+  TraceRange trace_range("fgms_b200_dropout");
+  if (!args) return fail(FGMS_ERR_INVALID_ARG, "null pointer");
+  return run_dropout(*args, false, static_cast<cudaStream_t>(stream));
+}
+
+int fgms_b200_dropout_bwd(const fgms_b200_dropout_args* args, void* stream) {
+  TraceRange trace_range("fgms_b200_dropout_bwd");
+  if (!args) return fail(FGMS_ERR_INVALID_ARG, "null pointer");
+  return run_dropout(*args, true, static_cast<cudaStream_t>(stream));
+}
+
+int fgms_b200_rms_norm(const fgms_b200_rms_norm_args* args, void* stream) {
+  TraceRange trace_range("fgms_b200_rms_norm");
+  if (!args) return fail(FGMS_ERR_INVALID_ARG, "null pointer");
+  return run_rms_norm(*args, true, static_cast<cudaStream_t>(stream));
+}
+
+size_t fgms_b200_rms_norm_bwd_workspace_bytes(int64_t rows, int64_t width) {
+  DeviceInfo di;
+  if (rows < 1 || width < 1 || width > fgms::NORM_MAX_WIDTH || device_info(&di) != FGMS_OK) return 0;
+  return (size_t)fgms::norm_grad_cut(rows, (int)width, di.sms).blocks * (size_t)width * 4;
+}
+
+int fgms_b200_rms_norm_bwd(const fgms_b200_rms_norm_bwd_args* args, void* stream) {
+  TraceRange trace_range("fgms_b200_rms_norm_bwd");
+  if (!args) return fail(FGMS_ERR_INVALID_ARG, "null pointer");
+  return run_rms_norm_bwd(*args, static_cast<cudaStream_t>(stream));
+}
+
+int fgms_b200_quantize_rows(const void* x, int64_t x_pitch, int8_t* codes, int64_t codes_pitch, float* scale, int64_t rows, int64_t width, int dtype, void* stream) {
+  TraceRange trace_range("fgms_b200_quantize_rows");
+  if (rows > 0 && !scale) return fail(FGMS_ERR_INVALID_ARG, "scale: null pointer");
+  fgms_b200_rms_norm_args a = {};
+  a.x = x;
+  a.x_pitch = x_pitch;
+  a.out = codes;
+  a.out_pitch = codes_pitch;
+  a.scale = scale;
+  a.rows = rows;
+  a.width = width;
+  a.dtype = a.weight_dtype = dtype;
+  return run_rms_norm(a, false, static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

@@ -1,0 +1,353 @@
+// Root-mean-square norm of rows with the residual's addition, and its gradient.
+//
+//   h = residual + drop(x)        r = 1 / sqrt(mean(h^2) + eps)        y = h r w
+//   gradient, with n = h r and g = dy w:
+//   dh = r (g - n mean(g n)) + dsum        dx = drop'(dh)        dresidual = dh        dw = sum over the rows of dy n
+//
+// Sums, statistics and everything in between are fp32; h is rounded once where it is stored, and y comes from the h before that.  An output in 8 bits is
+// round(y 127 / a) with the scale a / 127, a = max |y| of the row: symmetric, so that a product needs no offsets.  A row whose largest value is
+// below 2^-100 is zeros with a scale of zero; a row that holds a value which is not finite has a scale of NaN and codes of zero, so that a product with
+// it is NaN.
+//
+// One pass: a row's values stay in registers from their load to their store, CH chunks of eight a thread, `threads_per_row` threads a row.  Rows of up
+// to 256 CH values are a warp's each, wider ones a block's, with one exchange through shared memory for each reduction.
+#pragma once
+#include "row_values.cuh"
+
+namespace fgms {
+
+constexpr int NORM_MAX_THREADS = 1024;
+constexpr int NORM_WARP_ROWS = 4;  // rows (warps) of a block where a row is a warp's
+
+struct NormParams {
+  const void *x, *residual, *weight;  // residual: or null; weight: null without a norm (norm = 0)
+  void *out, *sum;                    // sum: or null
+  float *scale, *rstd;                // scale: of an output in 8 bits; rstd: or null
+  long long rows, x_pitch, residual_pitch, out_pitch, sum_pitch;
+  int width, norm;
+  bool x_vec, residual_vec, out_vec, sum_vec, weight_vec;
+  float eps, inverse_width;
+  DropParams drop;
+  int alone;  // see GmsParams
+};
+
+// |x| as an unsigned number: larger values are larger numbers, and NaN is above them all
+__device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+// Sum over the threads of a row; `part`: 32 words of shared memory that no reduction shortly before has used.
+template <bool WARP>
+__device__ __forceinline__ float row_sum(float v, float* part) {
+  v = warp_sum(v);
+  if (WARP) return v;
+  const int lane = threadIdx.x & 31, warps = (int)blockDim.x >> 5;
+  if (lane == 0) part[threadIdx.x >> 5] = v;
+  __syncthreads();
+  return warp_sum(lane < warps ? part[lane] : 0.f);
+}
+template <bool WARP>
+__device__ __forceinline__ uint32_t row_max(uint32_t v, uint32_t* part) {
+  v = __reduce_max_sync(0xffffffffu, v);
+  if (WARP) return v;
+  const int lane = threadIdx.x & 31, warps = (int)blockDim.x >> 5;
+  if (lane == 0) part[threadIdx.x >> 5] = v;
+  __syncthreads();
+  return __reduce_max_sync(0xffffffffu, lane < warps ? part[lane] : 0u);
+}
+
+// T: rows; W: the weight; CH: chunks a thread; WARP: a row is a warp's; EIGHT: the output is codes of 8 bits
+template <typename T, typename W, int CH, bool WARP, bool EIGHT, bool DROP>
+__global__ void __launch_bounds__(WARP ? 32 * NORM_WARP_ROWS : NORM_MAX_THREADS) rms_norm_kernel(const __grid_constant__ NormParams p) {
+  __shared__ float parts[4][32];
+  umma::griddep_wait();
+  if (!p.alone) umma::griddep_launch_dependents();
+  DropKey key;
+  if (DROP) key = drop_key(p.drop.state);
+  const int per_row = WARP ? 32 : (int)blockDim.x, thread = WARP ? (int)threadIdx.x & 31 : (int)threadIdx.x;
+  const long long rows_at_once = WARP ? (long long)gridDim.x * NORM_WARP_ROWS : (long long)gridDim.x;
+  int turn = 0;  // a row's reductions use other words than the last one's, which a slower warp may still read
+  for (long long row = WARP ? (long long)blockIdx.x * NORM_WARP_ROWS + (threadIdx.x >> 5) : (long long)blockIdx.x; row < p.rows; row += rows_at_once) {
+    RowRaw<T> raw[CH], add[CH];
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int col = (c * per_row + thread) * ROW_CHUNK, there = p.width - col;
+      raw[c] = row_load(static_cast<const T*>(p.x) + row * p.x_pitch + col, there, p.x_vec);
+      if (p.residual) add[c] = row_load(static_cast<const T*>(p.residual) + row * p.residual_pitch + col, there, p.residual_vec);
+    }
+    float h[CH][ROW_CHUNK], sum = 0.f;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int chunk = c * per_row + thread, col = chunk * ROW_CHUNK;
+      const uint32_t keep = DROP ? drop_keep(key, (uint32_t)chunk, (uint32_t)row, p.drop.threshold) : 0u;
+#pragma unroll
+      for (int e = 0; e < ROW_CHUNK; ++e) {
+        h[c][e] = row_value(raw[c], e);
+        if (DROP) h[c][e] = keep >> e & 1u ? h[c][e] * p.drop.factor : 0.f;
+        if (p.residual) h[c][e] += row_value(add[c], e);
+        sum += h[c][e] * h[c][e];
+      }
+      if (p.sum) row_store(static_cast<T*>(p.sum) + row * p.sum_pitch + col, h[c], p.width - col, p.sum_vec);
+    }
+    float r = 1.f;
+    if (p.norm) {
+      r = 1.f / sqrtf(row_sum<WARP>(sum, parts[turn]) * p.inverse_width + p.eps);
+      if (p.rstd && thread == 0) p.rstd[row] = r;
+    }
+    uint32_t largest = 0;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int col = (c * per_row + thread) * ROW_CHUNK, there = p.width - col;
+      if (there <= 0) {
+        if (EIGHT) {
+#pragma unroll
+          for (int e = 0; e < ROW_CHUNK; ++e) h[c][e] = 0.f;
+        }
+        continue;
+      }
+      if (p.norm) {
+        float w[ROW_CHUNK];
+        const W* from = static_cast<const W*>(p.weight) + col;
+        if (p.weight_vec && there >= ROW_CHUNK) {  // every row reads it again: from L1
+          RowRaw<W> v;
+#pragma unroll
+          for (int q = 0; q < (int)sizeof(W) / 2; ++q) *reinterpret_cast<uint4*>(v.w + 4 * q) = __ldg(reinterpret_cast<const uint4*>(from) + q);
+#pragma unroll
+          for (int e = 0; e < ROW_CHUNK; ++e) w[e] = row_value(v, e);
+        } else {
+#pragma unroll
+          for (int e = 0; e < ROW_CHUNK; ++e) w[e] = e < there ? to_f32(from[e]) : 0.f;
+        }
+#pragma unroll
+        for (int e = 0; e < ROW_CHUNK; ++e) h[c][e] = h[c][e] * r * w[e];
+      }
+      if (EIGHT) {
+#pragma unroll
+        for (int e = 0; e < ROW_CHUNK; ++e) largest = max(largest, e < there ? magnitude(h[c][e]) : 0u);
+      } else {
+        row_store(static_cast<T*>(p.out) + row * p.out_pitch + col, h[c], there, p.out_vec);
+      }
+    }
+    if (EIGHT) {
+      const float a = __uint_as_float(row_max<WARP>(largest, reinterpret_cast<uint32_t*>(parts[turn + 1])));
+      const bool finite = a < __uint_as_float(0x7f800000u), some = finite && a >= 7.88860905e-31f;  // 2^-100
+      const float to_code = some ? 127.f / a : 0.f;
+      if (thread == 0) p.scale[row] = finite ? (some ? a / 127.f : 0.f) : __uint_as_float(0x7fc00000u);
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        const int col = (c * per_row + thread) * ROW_CHUNK, there = p.width - col;
+        int8_t* to = static_cast<int8_t*>(p.out) + row * p.out_pitch + col;
+        uint32_t code[ROW_CHUNK];
+#pragma unroll
+        for (int e = 0; e < ROW_CHUNK; ++e) code[e] = some ? (uint32_t)__float2int_rn(h[c][e] * to_code) & 0xffu : 0u;
+        if (p.out_vec && there >= ROW_CHUNK) {
+          *reinterpret_cast<uint2*>(to) = make_uint2(code[0] | code[1] << 8 | code[2] << 16 | code[3] << 24, code[4] | code[5] << 8 | code[6] << 16 | code[7] << 24);
+        } else {
+#pragma unroll
+          for (int e = 0; e < ROW_CHUNK; ++e)
+            if (e < there) to[e] = (int8_t)code[e];
+        }
+      }
+    }
+    if (!WARP) turn ^= 2;
+  }
+  if (DROP) drop_count(p.drop);
+}
+
+struct NormGradParams {
+  const void *dy, *sum, *dsum, *weight;  // dsum: or null
+  const float* rstd;
+  void *dx, *dresidual;  // either may be null
+  float* parts;          // [blocks][width]: what each block's rows add to the weight's gradient, or null
+  long long rows, dy_pitch, sum_pitch, dsum_pitch, dx_pitch, dresidual_pitch;
+  int width;
+  bool dy_vec, sum_vec, dsum_vec, dx_vec, dresidual_vec, weight_vec;
+  float inverse_width;
+  DropParams drop;
+  int alone;
+};
+
+// The block's rows one after the other, their share of the weight's gradient in registers until the last one.
+template <typename T, typename W, int CH, bool WARP, bool DROP, int THREADS>
+__global__ void __launch_bounds__(THREADS) rms_norm_grad_kernel(const __grid_constant__ NormGradParams p) {
+  __shared__ float parts[2][32];
+  __shared__ float share[WARP ? NORM_WARP_ROWS : 1][WARP ? 32 * CH * ROW_CHUNK : 1];
+  umma::griddep_wait();
+  if (!p.alone) umma::griddep_launch_dependents();
+  DropKey key;
+  if (DROP) key = drop_key(p.drop.used);
+  const int per_row = WARP ? 32 : (int)blockDim.x, thread = WARP ? (int)threadIdx.x & 31 : (int)threadIdx.x;
+  const long long rows_at_once = WARP ? (long long)gridDim.x * NORM_WARP_ROWS : (long long)gridDim.x;
+  float dw[CH][ROW_CHUNK];
+#pragma unroll
+  for (int c = 0; c < CH; ++c)
+#pragma unroll
+    for (int e = 0; e < ROW_CHUNK; ++e) dw[c][e] = 0.f;
+  int turn = 0;
+  for (long long row = WARP ? (long long)blockIdx.x * NORM_WARP_ROWS + (threadIdx.x >> 5) : (long long)blockIdx.x; row < p.rows; row += rows_at_once) {
+    RowRaw<T> dy[CH], h[CH], extra[CH];
+    RowRaw<W> w[CH];
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int col = (c * per_row + thread) * ROW_CHUNK, there = p.width - col;
+      dy[c] = row_load(static_cast<const T*>(p.dy) + row * p.dy_pitch + col, there, p.dy_vec);
+      h[c] = row_load(static_cast<const T*>(p.sum) + row * p.sum_pitch + col, there, p.sum_vec);
+      if (p.dsum) extra[c] = row_load(static_cast<const T*>(p.dsum) + row * p.dsum_pitch + col, there, p.dsum_vec);
+    }
+    const float r = __ldg(p.rstd + row);
+    const auto weights = [&](int c) {
+      const int col = (c * per_row + thread) * ROW_CHUNK, there = p.width - col;
+      const W* from = static_cast<const W*>(p.weight) + col;
+      if (p.weight_vec && there >= ROW_CHUNK) {
+#pragma unroll
+        for (int q = 0; q < (int)sizeof(W) / 2; ++q) *reinterpret_cast<uint4*>(w[c].w + 4 * q) = __ldg(reinterpret_cast<const uint4*>(from) + q);
+      } else {
+        w[c] = row_load(from, there, false);
+      }
+    };
+    float dot = 0.f;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      weights(c);
+#pragma unroll
+      for (int e = 0; e < ROW_CHUNK; ++e) {
+        const float n = row_value(h[c], e) * r, d = row_value(dy[c], e);
+        dot += d * row_value(w[c], e) * n;
+        dw[c][e] += d * n;
+      }
+    }
+    const float mean = row_sum<WARP>(dot, parts[turn]) * p.inverse_width;
+    if (!WARP) turn ^= 1;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int chunk = c * per_row + thread, col = chunk * ROW_CHUNK, there = p.width - col;
+      if (there <= 0) continue;
+      if (CH > 1) weights(c);  // again from L1, instead of registers meanwhile
+      float dh[ROW_CHUNK];
+#pragma unroll
+      for (int e = 0; e < ROW_CHUNK; ++e) {
+        dh[e] = r * (row_value(dy[c], e) * row_value(w[c], e) - row_value(h[c], e) * r * mean);
+        if (p.dsum) dh[e] += row_value(extra[c], e);
+      }
+      if (p.dresidual) row_store(static_cast<T*>(p.dresidual) + row * p.dresidual_pitch + col, dh, there, p.dresidual_vec);
+      if (p.dx) {
+        if (DROP) {
+          const uint32_t keep = drop_keep(key, (uint32_t)chunk, (uint32_t)row, p.drop.threshold);
+#pragma unroll
+          for (int e = 0; e < ROW_CHUNK; ++e) dh[e] = keep >> e & 1u ? dh[e] * p.drop.factor : 0.f;
+        }
+        row_store(static_cast<T*>(p.dx) + row * p.dx_pitch + col, dh, there, p.dx_vec);
+      }
+    }
+  }
+  if (!p.parts) return;
+  float* to = p.parts + (size_t)blockIdx.x * p.width;
+  if (WARP) {  // the block's warps in their order
+    const int warp = (int)threadIdx.x >> 5;
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int e = 0; e < ROW_CHUNK; ++e) share[warp][(c * 32 + thread) * ROW_CHUNK + e] = dw[c][e];
+    __syncthreads();
+    for (int col = (int)threadIdx.x; col < p.width; col += 32 * NORM_WARP_ROWS) {
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < NORM_WARP_ROWS; ++i) sum += share[i][col];
+      to[col] = sum;
+    }
+  } else {
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int col = (c * per_row + thread) * ROW_CHUNK;
+#pragma unroll
+      for (int e = 0; e < ROW_CHUNK; ++e)
+        if (col + e < p.width) to[col + e] = dw[c][e];
+    }
+  }
+}
+
+// The blocks' shares in their order, 32 columns a block: eight rows of threads take every eighth share each and are added up in their order.
+constexpr int NORM_SHARES_Y = 8;
+template <typename W>
+__global__ void __launch_bounds__(32 * NORM_SHARES_Y) rms_norm_weight_grad_kernel(const float* __restrict__ parts, int n, int width, W* dw, int alone) {
+  __shared__ float sums[NORM_SHARES_Y][32];
+  umma::griddep_wait();
+  if (!alone) umma::griddep_launch_dependents();
+  const int col = (int)blockIdx.x * 32 + (threadIdx.x & 31), y = (int)threadIdx.x >> 5;
+  float sum = 0.f;
+  if (col < width) {
+#pragma unroll 8
+    for (int i = y; i < n; i += NORM_SHARES_Y) sum += __ldcg(parts + (size_t)i * width + col);
+  }
+  sums[y][threadIdx.x & 31] = sum;
+  __syncthreads();
+  if (y == 0 && col < width) {
+    sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < NORM_SHARES_Y; ++i) sum += sums[i][threadIdx.x & 31];
+    dw[col] = from_f32<W>(sum);
+  }
+}
+
+// Threads that a row of a block gets with CH chunks each.
+inline int norm_threads(int width, int ch) {
+  const int chunks = (width + ROW_CHUNK - 1) / ROW_CHUNK;
+  return ((chunks + ch - 1) / ch + 31) / 32 * 32;
+}
+
+template <typename T, typename W, int CH, bool WARP, bool EIGHT>
+cudaError_t launch_rms_norm_as(const NormParams& p, cudaStream_t st, int sms) {
+  const int threads = WARP ? 32 * NORM_WARP_ROWS : norm_threads(p.width, CH);
+  const long long blocks = WARP ? (p.rows + NORM_WARP_ROWS - 1) / NORM_WARP_ROWS : p.rows;
+  const long long at_once = (long long)sms * (2048 / threads);
+  const dim3 grid((unsigned)(blocks < at_once ? blocks : at_once));
+  if (!EIGHT && p.drop.threshold > 0) return launch_pdl(rms_norm_kernel<T, W, CH, WARP, false, true>, grid, threads, 0, st, p);
+  return launch_pdl(rms_norm_kernel<T, W, CH, WARP, EIGHT, false>, grid, threads, 0, st, p);
+}
+template <typename T, typename W, bool EIGHT>
+cudaError_t launch_rms_norm(const NormParams& p, cudaStream_t st, int sms) {
+  if (p.width <= 256) return launch_rms_norm_as<T, W, 1, true, EIGHT>(p, st, sms);
+  if (p.width <= 512) return launch_rms_norm_as<T, W, 2, true, EIGHT>(p, st, sms);
+  if (p.rows < sms || p.width <= 2048) {
+    if (p.width <= 8192) return launch_rms_norm_as<T, W, 1, false, EIGHT>(p, st, sms);
+  }
+  if (p.width <= 16384) return launch_rms_norm_as<T, W, 2, false, EIGHT>(p, st, sms);
+  return launch_rms_norm_as<T, W, 4, false, EIGHT>(p, st, sms);
+}
+constexpr int NORM_MAX_WIDTH = NORM_MAX_THREADS * 4 * ROW_CHUNK;
+
+// What a gradient is cut into: the blocks each leave a share of the weight's gradient.
+struct NormGradCut {
+  int ch, threads, blocks;
+  bool warp;
+};
+inline NormGradCut norm_grad_cut(long long rows, int width, int sms) {
+  NormGradCut c;
+  c.warp = width <= 512;
+  c.ch = width <= 256 ? 1 : width <= 512 ? 2 : width <= 4096 ? 1 : width <= 8192 ? 2 : 4;
+  c.threads = c.warp ? 32 * NORM_WARP_ROWS : norm_threads(width, c.ch);
+  const long long blocks = c.warp ? (rows + NORM_WARP_ROWS - 1) / NORM_WARP_ROWS : rows, at_once = (long long)sms * (c.threads <= 1024 ? 1024 / c.threads : 1);
+  c.blocks = (int)(blocks < at_once ? blocks : at_once);
+  return c;
+}
+template <typename T, typename W, int CH, bool WARP, int THREADS>
+cudaError_t launch_rms_norm_grad_as(const NormGradParams& p, const NormGradCut& cut, cudaStream_t st) {
+  const dim3 grid((unsigned)cut.blocks);
+  if (p.drop.threshold > 0) return launch_pdl(rms_norm_grad_kernel<T, W, CH, WARP, true, THREADS>, grid, cut.threads, 0, st, p);
+  return launch_pdl(rms_norm_grad_kernel<T, W, CH, WARP, false, THREADS>, grid, cut.threads, 0, st, p);
+}
+template <typename T, typename W>
+cudaError_t launch_rms_norm_grad(const NormGradParams& p, const NormGradCut& cut, cudaStream_t st) {
+  if (cut.warp) return cut.ch == 1 ? launch_rms_norm_grad_as<T, W, 1, true, 32 * NORM_WARP_ROWS>(p, cut, st) : launch_rms_norm_grad_as<T, W, 2, true, 32 * NORM_WARP_ROWS>(p, cut, st);
+  if (cut.ch == 1) return launch_rms_norm_grad_as<T, W, 1, false, 512>(p, cut, st);
+  return cut.ch == 2 ? launch_rms_norm_grad_as<T, W, 2, false, 512>(p, cut, st) : launch_rms_norm_grad_as<T, W, 4, false, 1024>(p, cut, st);
+}
+template <typename W>
+cudaError_t launch_rms_norm_weight_grad(const float* parts, int n, int width, void* dw, int alone, cudaStream_t st) {
+  return launch_pdl(rms_norm_weight_grad_kernel<W>, dim3((unsigned)((width + 31) / 32)), 32 * NORM_SHARES_Y, 0, st, parts, n, width, static_cast<W*>(dw), alone);
+}
+
+}  // namespace fgms

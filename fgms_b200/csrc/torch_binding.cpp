@@ -762,6 +762,296 @@ struct GroupedLinear : torch::autograd::Function<GroupedLinear> {
 };
 
 // ---------------------------------------------------------------------------------------------
+// between two layers: norm, dropout, rows in 8 bits
+// ---------------------------------------------------------------------------------------------
+int layer_dtype(const Tensor& t) {
+  if (t.scalar_type() == at::kHalf) return FGMS_DTYPE_F16;
+  if (t.scalar_type() == at::kBFloat16) return FGMS_DTYPE_BF16;
+  TORCH_CHECK_VALUE(t.scalar_type() == at::kFloat, "unsupported feature dtype ", t.scalar_type(), ": rows are float16, bfloat16 or float32");
+  return FGMS_DTYPE_F32;
+}
+
+// rows [n, width] whose values lie side by side; the rows themselves may be apart
+void check_row_values(const char* name, const Tensor& t, at::ScalarType type, const Tensor& like) {
+  TORCH_CHECK_VALUE(t.is_cuda(), name, " must be a CUDA tensor");
+  TORCH_CHECK_VALUE(t.device() == like.device(), name, " must live on ", like.device());
+  TORCH_CHECK_VALUE(t.scalar_type() == type, name, " must have dtype ", type, ", got ", t.scalar_type());
+  TORCH_CHECK_VALUE(t.dim() == 2, name, " must have 2 dimensions, got ", t.dim());
+  TORCH_CHECK_VALUE(t.size(0) == like.size(0) && t.size(1) == like.size(1), name, " is ", t.size(0), " x ", t.size(1), ", the rows are ", like.size(0), " x ",
+                    like.size(1));
+  TORCH_CHECK_VALUE(t.numel() == 0 || t.size(1) <= 1 || t.stride(1) == 1, name, " must have the values of a row side by side");
+  TORCH_CHECK_VALUE(t.numel() == 0 || t.size(0) <= 1 || t.stride(0) >= t.size(1), name, " has rows that overlap");
+}
+int64_t pitch(const Tensor& t) { return t.numel() > 0 && t.size(0) > 1 ? t.stride(0) : t.size(1); }
+// one value of a type for each of `n` rows or columns
+void* check_line(const char* name, const Tensor& t, at::ScalarType type, int64_t n, const Tensor& like) {
+  TORCH_CHECK_VALUE(t.device() == like.device(), name, " must live on ", like.device());
+  TORCH_CHECK_VALUE(t.scalar_type() == type, name, " must have dtype ", type, ", got ", t.scalar_type());
+  TORCH_CHECK_VALUE(t.is_contiguous() && t.dim() == 1 && t.numel() == n, name, " must be ", n, " values side by side");
+  return ptr(t);
+}
+int64_t* check_rng(const char* name, const Tensor* t, int64_t n, const Tensor& like) {
+  TORCH_CHECK_VALUE(t != nullptr, name, " is needed where values are dropped");
+  return static_cast<int64_t*>(check_line(name, *t, at::kLong, n, like));
+}
+// whether a probability, rounded to 16 bits, drops anything (the library refuses what is no probability)
+bool drops(double p) { return !(p >= 0.0 && p * 65536.0 <= 0.5); }
+
+struct NormCall {
+  const Tensor &x, *weight, &out;
+  const Tensor *residual, *sum, *scale, *rstd, *rng, *used;
+  double eps, p;
+};
+void rms_norm(const NormCall& c) {
+  const Tensor& x = c.x;
+  const int dtype = layer_dtype(x);
+  check_row_values("x", x, x.scalar_type(), x);
+  check_row_values("out", c.out, c.scale ? at::kChar : x.scalar_type(), x);
+  if (c.residual) check_row_values("residual", *c.residual, x.scalar_type(), x);
+  if (c.sum) check_row_values("residual_out", *c.sum, x.scalar_type(), x);
+  if (x.size(1) == 0) return;
+  fgms_b200_rms_norm_args a = {};
+  if (c.weight) {
+    TORCH_CHECK_VALUE(c.weight->scalar_type() == x.scalar_type() || c.weight->scalar_type() == at::kFloat, "weight must have dtype ", x.scalar_type(),
+                      " or float32, got ", c.weight->scalar_type());
+    a.weight = check_line("weight", *c.weight, c.weight->scalar_type(), x.size(1), x);
+    a.weight_dtype = layer_dtype(*c.weight);
+  }
+  if (c.scale) a.scale = static_cast<float*>(check_line("scale", *c.scale, at::kFloat, x.size(0), x));
+  if (c.rstd) a.rstd = static_cast<float*>(check_line("rstd", *c.rstd, at::kFloat, x.size(0), x));
+  const bool drop = drops(c.p);
+  if (drop) {
+    a.rng = check_rng("rng", c.rng, 3, x);
+    if (c.used) a.rng_used = check_rng("rng_used", c.used, 2, x);
+  }
+  a.x = ptr(x);
+  a.out = ptr(c.out);
+  a.x_pitch = pitch(x);
+  a.out_pitch = pitch(c.out);
+  if (c.residual) a.residual = ptr(*c.residual), a.residual_pitch = pitch(*c.residual);
+  if (c.sum) a.sum = ptr(*c.sum), a.sum_pitch = pitch(*c.sum);
+  a.rows = x.size(0);
+  a.width = x.size(1);
+  a.eps = c.eps;
+  a.p = c.p;
+  a.dtype = dtype;
+  c10::cuda::CUDAGuard guard(x.device());
+  if (c.weight) check_status(fgms_b200_rms_norm(&a, stream_of(x)));
+  else check_status(fgms_b200_quantize_rows(a.x, a.x_pitch, static_cast<int8_t*>(a.out), a.out_pitch, a.scale, a.rows, a.width, dtype, stream_of(x)));
+  written(c.out);
+  for (const Tensor* t : {c.sum, c.scale, c.rstd, drop ? c.rng : nullptr, drop ? c.used : nullptr})
+    if (t) written(*t);
+}
+
+struct NormGradCall {
+  const Tensor &out_grad, &sum, &weight, &rstd;
+  const Tensor *sum_grad, *x_grad, *residual_grad, *weight_grad, *used;
+  double p;
+};
+void rms_norm_bwd(const NormGradCall& c) {
+  const Tensor& h = c.sum;
+  fgms_b200_rms_norm_bwd_args a = {};
+  a.dtype = layer_dtype(h);
+  check_row_values("h", h, h.scalar_type(), h);
+  check_row_values("out_grad", c.out_grad, h.scalar_type(), h);
+  if (c.sum_grad) check_row_values("h_grad", *c.sum_grad, h.scalar_type(), h);
+  if (c.x_grad) check_row_values("x_grad", *c.x_grad, h.scalar_type(), h);
+  if (c.residual_grad) check_row_values("residual_grad", *c.residual_grad, h.scalar_type(), h);
+  TORCH_CHECK_VALUE(c.weight.scalar_type() == h.scalar_type() || c.weight.scalar_type() == at::kFloat, "weight must have dtype ", h.scalar_type(),
+                    " or float32, got ", c.weight.scalar_type());
+  a.weight = check_line("weight", c.weight, c.weight.scalar_type(), h.size(1), h);
+  a.weight_dtype = layer_dtype(c.weight);
+  a.rstd = static_cast<const float*>(check_line("rstd", c.rstd, at::kFloat, h.size(0), h));
+  if (c.weight_grad) a.weight_grad = check_line("weight_grad", *c.weight_grad, c.weight.scalar_type(), h.size(1), h);
+  if (drops(c.p)) a.rng_used = check_rng("rng_used", c.used, 2, h);
+  if (h.size(1) == 0) return;
+  a.out_grad = ptr(c.out_grad);
+  a.out_grad_pitch = pitch(c.out_grad);
+  a.sum = ptr(h);
+  a.sum_pitch = pitch(h);
+  if (c.sum_grad) a.sum_grad = ptr(*c.sum_grad), a.sum_grad_pitch = pitch(*c.sum_grad);
+  if (c.x_grad) a.x_grad = ptr(*c.x_grad), a.x_grad_pitch = pitch(*c.x_grad);
+  if (c.residual_grad) a.residual_grad = ptr(*c.residual_grad), a.residual_grad_pitch = pitch(*c.residual_grad);
+  a.rows = h.size(0);
+  a.width = h.size(1);
+  a.p = c.p;
+  c10::cuda::CUDAGuard guard(h.device());
+  Tensor ws;
+  if (c.weight_grad) {
+    a.workspace_bytes = fgms_b200_rms_norm_bwd_workspace_bytes(a.rows, a.width);
+    if (a.workspace_bytes > 0) {
+      ws = at::empty({(int64_t)a.workspace_bytes}, h.options().dtype(at::kByte).requires_grad(false));
+      a.workspace = ws.data_ptr();
+    }
+  }
+  check_status(fgms_b200_rms_norm_bwd(&a, stream_of(h)));
+  for (const Tensor* t : {c.x_grad, c.residual_grad, c.weight_grad})
+    if (t) written(*t);
+}
+
+void dropout(const Tensor& x, const Tensor& out, double p, const Tensor* rng, const Tensor* residual, const Tensor* used, bool backward) {
+  fgms_b200_dropout_args a = {};
+  a.dtype = layer_dtype(x);
+  check_row_values(backward ? "out_grad" : "x", x, x.scalar_type(), x);
+  check_row_values(backward ? "x_grad" : "out", out, x.scalar_type(), x);
+  if (residual) check_row_values("residual", *residual, x.scalar_type(), x);
+  if (!backward) a.rng = check_rng("rng", rng, 3, x);
+  if (used || backward) a.rng_used = check_rng("rng_used", used, 2, x);
+  if (x.size(1) == 0) return;
+  a.x = ptr(x);
+  a.x_pitch = pitch(x);
+  a.out = ptr(out);
+  a.out_pitch = pitch(out);
+  if (residual) a.residual = ptr(*residual), a.residual_pitch = pitch(*residual);
+  a.rows = x.size(0);
+  a.width = x.size(1);
+  a.p = p;
+  c10::cuda::CUDAGuard guard(x.device());
+  check_status(backward ? fgms_b200_dropout_bwd(&a, stream_of(x)) : fgms_b200_dropout(&a, stream_of(x)));
+  written(out);
+  if (!backward) written(*rng);
+  if (!backward && used) written(*used);
+}
+
+// any shape as rows of its last dimension
+Tensor as_rows(const Tensor& t) {
+  if (t.dim() == 2 && t.is_contiguous()) return t;
+  return (t.dim() == 0 ? t.reshape({1, 1}) : t.size(-1) == 0 ? t.reshape({0, 0}) : t.reshape({-1, t.size(-1)})).contiguous();
+}
+Tensor new_like(const Tensor& t) { return at::empty(t.sizes(), t.options().requires_grad(false)); }
+// a graph of the backward was asked for: it ends here, and says so to whoever goes through it
+void end_graph(std::initializer_list<Tensor*> grads, const char* what) {
+  if (!at::GradMode::is_enabled()) return;
+  for (Tensor* t : grads) {
+    if (!t->defined()) continue;
+    t->set_requires_grad(true);
+    const auto ends = std::make_shared<torch::autograd::DelayedError>(what, 1);
+    *t = (*ends)({*t})[0];
+  }
+}
+const Tensor* maybe_tensor(const Tensor& t) { return t.defined() ? &t : nullptr; }
+
+void check_norm_shapes(const Tensor& x, const Tensor& weight, const Tensor* residual) {
+  TORCH_CHECK_VALUE(x.is_cuda(), "x must be a CUDA tensor");
+  TORCH_CHECK_VALUE(x.dim() >= 1, "x must have at least one dimension");
+  TORCH_CHECK_VALUE(weight.dim() == 1 && weight.size(0) == x.size(-1), "weight must have ", x.size(-1), " values, as many as a row");
+  TORCH_CHECK_VALUE(!residual || residual->sizes() == x.sizes(), "residual must have the shape of x");
+}
+
+// The norm of one call: out, and with a residual or dropout the sum that it is the norm of.
+struct Normed {
+  Tensor out, sum, rstd, used;  // 2-D, but out and sum
+};
+Normed norm_forward(const Tensor& x_, const Tensor& weight_, const Tensor* residual_, double eps, double p, const Tensor* rng, bool for_backward) {
+  const Tensor x = as_rows(x_), weight = weight_.contiguous(), residual = residual_ ? as_rows(*residual_) : Tensor();
+  Normed n;
+  n.out = new_like(x_.is_contiguous() ? x_ : x);
+  if (n.out.dim() != x_.dim()) n.out = n.out.view(x_.sizes());
+  const bool drop = drops(p);
+  const Tensor out = as_rows(n.out);
+  Tensor sum;
+  if (residual_ || (drop && for_backward)) {
+    n.sum = at::empty_like(n.out);
+    sum = as_rows(n.sum);
+  }
+  if (for_backward) {
+    n.rstd = at::empty({x.size(0)}, x.options().dtype(at::kFloat).requires_grad(false));
+    if (drop) n.used = at::empty({2}, x.options().dtype(at::kLong).requires_grad(false));
+  }
+  rms_norm({x, &weight, out, maybe_tensor(residual), maybe_tensor(sum), nullptr, maybe_tensor(n.rstd), rng, maybe_tensor(n.used), eps, p});
+  return n;
+}
+
+struct RmsNorm : torch::autograd::Function<RmsNorm> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& weight,
+                                                const std::optional<Tensor>& residual, const std::optional<Tensor>& rng, double eps, double p) {
+    Normed n = norm_forward(x, weight, residual ? &*residual : nullptr, eps, p, rng ? &*rng : nullptr, true);
+    ctx->saved_data["p"] = p;
+    ctx->saved_data["residual"] = residual.has_value();
+    ctx->save_for_backward({n.sum.defined() ? n.sum : x, weight, n.rstd, n.used});
+    ctx->set_materialize_grads(false);
+    if (residual) return {n.out, n.sum};
+    return {n.out};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const double p = ctx->saved_data["p"].toDouble();
+    const bool residual = ctx->saved_data["residual"].toBool(), drop = drops(p);
+    const Tensor h = as_rows(saved[0]), weight = saved[1].contiguous();
+    const Tensor dy = grads[0].defined() ? as_rows(grads[0]) : at::zeros_like(h);
+    const Tensor dsum = residual && grads[1].defined() ? as_rows(grads[1]) : Tensor();
+    const bool want_x = ctx->needs_input_grad(0), want_residual = residual && ctx->needs_input_grad(2);
+    Tensor x_grad, residual_grad, weight_grad;
+    if (want_x) x_grad = new_like(h);
+    if (want_residual && (drop || !want_x)) residual_grad = new_like(h);
+    if (ctx->needs_input_grad(1)) weight_grad = new_like(weight);
+    rms_norm_bwd({dy, h, weight, saved[2], maybe_tensor(dsum), maybe_tensor(x_grad), maybe_tensor(residual_grad), maybe_tensor(weight_grad),
+                  maybe_tensor(saved[3]), p});
+    if (x_grad.defined()) x_grad = x_grad.view(saved[0].sizes());
+    if (residual_grad.defined()) residual_grad = residual_grad.view(saved[0].sizes());
+    if (want_residual && !residual_grad.defined()) residual_grad = x_grad;  // the same values
+    if (at::GradMode::is_enabled() && residual_grad.defined() && residual_grad.is_same(x_grad)) residual_grad = x_grad.clone();
+    end_graph({&x_grad, &weight_grad, &residual_grad}, "rms_norm is not differentiable twice");
+    return {x_grad, weight_grad, residual_grad, Tensor(), Tensor(), Tensor()};
+  }
+};
+
+struct Dropout : torch::autograd::Function<Dropout> {
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x_, double p, const Tensor& rng, const std::optional<Tensor>& residual_) {
+    const Tensor x = as_rows(x_), residual = residual_ ? as_rows(*residual_) : Tensor();
+    const Tensor used = at::empty({2}, x.options().dtype(at::kLong).requires_grad(false)), out = new_like(x);
+    dropout(x, out, p, &rng, maybe_tensor(residual), &used, false);
+    ctx->saved_data["p"] = p;
+    ctx->saved_data["residual"] = residual.defined();
+    ctx->save_for_backward({used});
+    return out.view(x_.sizes());
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    Tensor x_grad;
+    if (ctx->needs_input_grad(0)) {
+      const Tensor g = as_rows(grads[0]);
+      x_grad = new_like(g);
+      dropout(g, x_grad, ctx->saved_data["p"].toDouble(), nullptr, nullptr, &saved[0], true);
+      x_grad = x_grad.view(grads[0].sizes());
+      end_graph({&x_grad}, "dropout is not differentiable twice");
+    }
+    return {x_grad, Tensor(), Tensor(), ctx->saved_data["residual"].toBool() ? grads[0] : Tensor()};
+  }
+};
+
+Tensor nn_dropout(const Tensor& x, double p, const Tensor& rng, const Tensor* residual) {
+  TORCH_CHECK_VALUE(x.is_cuda(), "x must be a CUDA tensor");
+  TORCH_CHECK_VALUE(!residual || residual->sizes() == x.sizes(), "residual must have the shape of x");
+  if (at::GradMode::is_enabled() && (x.requires_grad() || (residual && residual->requires_grad())))
+    return Dropout::apply(x, p, rng, residual ? std::optional<Tensor>(*residual) : std::nullopt);
+  const Tensor rows = as_rows(x), other = residual ? as_rows(*residual) : Tensor(), out = new_like(rows);
+  dropout(rows, out, p, &rng, maybe_tensor(other), nullptr, false);
+  return out.view(x.sizes());
+}
+
+// Codes in rows that are multiples of 16 bytes apart, as the products in 8 bits like them.
+Tensor new_codes(int64_t rows, int64_t width, const Tensor& like) {
+  const auto options = like.options().dtype(at::kChar).requires_grad(false);
+  const int64_t room = (width + 15) / 16 * 16;
+  Tensor codes = at::empty({rows, room}, options);
+  return room == width ? codes : codes.narrow(1, 0, width);
+}
+// (codes, scale, sum): without a weight there is no norm; the sum is undefined without a residual
+std::array<Tensor, 3> rms_norm_int8(const Tensor& x_, const Tensor* weight_, const Tensor* residual_, double eps) {
+  if (weight_) check_norm_shapes(x_, *weight_, residual_);
+  TORCH_CHECK_VALUE(x_.dim() == 2, "x must have 2 dimensions, got ", x_.dim());
+  TORCH_CHECK_VALUE(!(at::GradMode::is_enabled() && (x_.requires_grad() || (weight_ && weight_->requires_grad()) || (residual_ && residual_->requires_grad()))),
+                    "codes of 8 bits have no gradient: call it under torch.no_grad()");
+  const Tensor x = x_.stride(1) == 1 || x_.size(1) <= 1 ? x_ : x_.contiguous(), weight = weight_ ? weight_->contiguous() : Tensor();
+  const Tensor residual = residual_ ? as_rows(*residual_) : Tensor();
+  std::array<Tensor, 3> r = {new_codes(x.size(0), x.size(1), x), at::empty({x.size(0)}, x.options().dtype(at::kFloat).requires_grad(false)),
+                             residual_ ? at::empty({x.size(0), x.size(1)}, x.options().requires_grad(false)) : Tensor()};
+  rms_norm({x, maybe_tensor(weight), r[0], maybe_tensor(residual), maybe_tensor(r[2]), &r[1], nullptr, nullptr, nullptr, eps, 0.0});
+  return r;
+}
+
+// ---------------------------------------------------------------------------------------------
 // AdamW over many tensors
 // ---------------------------------------------------------------------------------------------
 int adamw_dtype(const char* name, const Tensor& t) {
@@ -1049,6 +1339,90 @@ PyObject* py_build_pyramid(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+const Tensor* maybe_arg(PyObject* o, const char* name) { return o == Py_None ? nullptr : &feat_arg(o, name); }
+
+// (x, weight, out, eps, residual, residual_out, scale, rstd, p, rng, rng_used)
+PyObject* py_rms_norm_into(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  expect(n, 11);
+  rms_norm({feat_arg(a[0], "x"), &feat_arg(a[1], "weight"), feat_arg(a[2], "out"), maybe_arg(a[4], "residual"), maybe_arg(a[5], "residual_out"),
+            maybe_arg(a[6], "scale"), maybe_arg(a[7], "rstd"), maybe_arg(a[9], "rng"), maybe_arg(a[10], "rng_used"), double_arg(a[3]), double_arg(a[8])});
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+// (out_grad, h, weight, rstd, x_grad, weight_grad, h_grad, residual_grad, p, rng_used)
+PyObject* py_rms_norm_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  expect(n, 10);
+  rms_norm_bwd({feat_arg(a[0], "out_grad"), feat_arg(a[1], "h"), feat_arg(a[2], "weight"), feat_arg(a[3], "rstd"), maybe_arg(a[6], "h_grad"),
+                maybe_arg(a[4], "x_grad"), maybe_arg(a[7], "residual_grad"), maybe_arg(a[5], "weight_grad"), maybe_arg(a[9], "rng_used"), double_arg(a[8])});
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+// (x, out, p, rng, residual, rng_used)
+PyObject* py_dropout_into(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  expect(n, 6);
+  dropout(feat_arg(a[0], "x"), feat_arg(a[1], "out"), double_arg(a[2]), &feat_arg(a[3], "rng"), maybe_arg(a[4], "residual"), maybe_arg(a[5], "rng_used"), false);
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+// (out_grad, x_grad, p, rng_used)
+PyObject* py_dropout_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  expect(n, 4);
+  dropout(feat_arg(a[0], "out_grad"), feat_arg(a[1], "x_grad"), double_arg(a[2]), nullptr, nullptr, &feat_arg(a[3], "rng_used"), true);
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+// (x, codes, scale)
+PyObject* py_quantize_rows_into(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  expect(n, 3);
+  const Tensor& scale = feat_arg(a[2], "scale");
+  rms_norm({feat_arg(a[0], "x"), nullptr, feat_arg(a[1], "codes"), nullptr, nullptr, &scale, nullptr, nullptr, nullptr, 0.0, 0.0});
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+// (x, weight, eps, residual, p, rng): out, or with a residual (out, sum)
+PyObject* py_rms_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  expect(n, 6);
+  const Tensor &x = feat_arg(a[0], "x"), &weight = feat_arg(a[1], "weight"), *residual = maybe_arg(a[3], "residual"), *rng = maybe_arg(a[5], "rng");
+  const double eps = double_arg(a[2]), p = double_arg(a[4]);
+  check_norm_shapes(x, weight, residual);
+  Tensor out, sum;
+  if (at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad() || (residual && residual->requires_grad()))) {
+    auto r = RmsNorm::apply(x, weight, residual ? std::optional<Tensor>(*residual) : std::nullopt, rng ? std::optional<Tensor>(*rng) : std::nullopt, eps, p);
+    out = r[0];
+    if (residual) sum = r[1];
+  } else {
+    const Normed r = norm_forward(x, weight, residual, eps, p, rng, false);
+    out = r.out;
+    sum = r.sum;
+  }
+  if (!residual) return THPVariable_Wrap(out);
+  return Py_BuildValue("(NN)", THPVariable_Wrap(out), THPVariable_Wrap(sum));
+  END_HANDLE_TH_ERRORS
+}
+// (x, weight or None, eps, residual): (codes, scale), or with a residual (codes, scale, sum)
+PyObject* py_rms_norm_int8(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  expect(n, 4);
+  const Tensor* residual = maybe_arg(a[3], "residual");
+  const auto r = rms_norm_int8(feat_arg(a[0], "x"), maybe_arg(a[1], "weight"), residual, double_arg(a[2]));
+  if (!residual) return Py_BuildValue("(NN)", THPVariable_Wrap(r[0]), THPVariable_Wrap(r[1]));
+  return Py_BuildValue("(NNN)", THPVariable_Wrap(r[0]), THPVariable_Wrap(r[1]), THPVariable_Wrap(r[2]));
+  END_HANDLE_TH_ERRORS
+}
+// (x, p, rng, residual)
+PyObject* py_dropout(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  expect(n, 4);
+  return THPVariable_Wrap(nn_dropout(feat_arg(a[0], "x"), double_arg(a[1]), feat_arg(a[2], "rng"), maybe_arg(a[3], "residual")));
+  END_HANDLE_TH_ERRORS
+}
+
 #define FGMS_METHOD(name, fn) {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(fn)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {
     FGMS_METHOD("fusion_fwd", py_fusion_fwd), FGMS_METHOD("seq_fwd", py_seq_fwd),         FGMS_METHOD("bwd", py_bwd),
@@ -1058,6 +1432,9 @@ PyMethodDef methods[] = {
     FGMS_METHOD("grouped_fwd", py_grouped_fwd), FGMS_METHOD("grouped_dgrad", py_grouped_dgrad),
     FGMS_METHOD("grouped_wgrad", py_grouped_wgrad), FGMS_METHOD("grouped_linear", py_grouped_linear),
     FGMS_METHOD("adamw", py_adamw),
+    FGMS_METHOD("rms_norm_into", py_rms_norm_into), FGMS_METHOD("rms_norm_bwd", py_rms_norm_bwd), FGMS_METHOD("rms_norm", py_rms_norm),
+    FGMS_METHOD("rms_norm_int8", py_rms_norm_int8), FGMS_METHOD("quantize_rows_into", py_quantize_rows_into),
+    FGMS_METHOD("dropout_into", py_dropout_into), FGMS_METHOD("dropout_bwd", py_dropout_bwd), FGMS_METHOD("dropout", py_dropout),
     FGMS_METHOD("build_pyramid", py_build_pyramid), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

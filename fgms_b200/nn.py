@@ -16,7 +16,8 @@ import torch
 
 from . import _native, backend
 
-__all__ = ["sparse_conv", "sparse_conv_inference", "SparseConv3d", "SparseUNet", "grouped_linear", "GroupedLinear"]
+__all__ = ["sparse_conv", "sparse_conv_inference", "SparseConv3d", "SparseUNet", "grouped_linear", "GroupedLinear", "rms_norm", "RMSNorm",
+           "rms_norm_int8", "quantize_rows", "rng_state", "dropout", "Dropout"]
 
 
 def sparse_conv(feats: torch.Tensor, weight: torch.Tensor, kmap, arch80: bool = True) -> torch.Tensor:
@@ -86,6 +87,72 @@ class GroupedLinear(torch.nn.Module):
 
     def forward(self, feats: torch.Tensor, kpos: torch.Tensor) -> torch.Tensor:
         return grouped_linear(feats, self.weight, kpos)
+
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: torch.Tensor | None = None, dropout: float = 0.0,
+             rng: torch.Tensor | None = None):
+    """``h * weight / sqrt(mean(h ** 2) + eps)`` over the last dimension of ``h = residual + dropout(x)``; differentiable in ``x``, ``weight`` and
+    ``residual``.  With a ``residual`` the result is ``(out, h)``, ``h`` being what the next layer adds to; without one it is ``out``.  One pass over
+    the rows for all of it.  ``weight`` is of the type of ``x`` or float32.  ``rng``: see :func:`dropout`."""
+    return _native.rms_norm(x, weight, eps, residual, dropout, rng)
+
+
+def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: torch.Tensor | None = None):
+    """:func:`rms_norm` with the output in 8 bits, for the products behind it: ``(codes, scale)`` or ``(codes, scale, h)``, where
+    ``codes * scale[:, None]`` is the normed row.  Codes are int8 rows that start 16 bytes apart.  No autograd."""
+    return _native.rms_norm_int8(x, weight, eps, residual)
+
+
+def quantize_rows(x: torch.Tensor):
+    """``(codes, scale)``: the rows of ``x`` in 8 bits with a float32 scale each.  No autograd."""
+    return _native.rms_norm_int8(x, None, 0.0, None)
+
+
+def rng_state(seed: int = 0, device="cuda") -> torch.Tensor:
+    """The state of :func:`dropout`'s generator on a device: ``[seed, calls made, 0]``."""
+    if not 0 <= seed < 2 ** 63:
+        raise ValueError("seed must be in [0, 2^63)")
+    return torch.tensor([seed, 0, 0], dtype=torch.int64, device=device)
+
+
+def dropout(x: torch.Tensor, p: float, rng: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:
+    """``residual + x * kept / (1 - p)``, with a mask that is never stored: the backward draws the same lots again.  ``rng`` comes from
+    :func:`rng_state` and counts the calls, on the device: a replayed graph drops other values every time.  Differentiable in ``x`` and
+    ``residual``.  The lots of a value hang on its row and column, the last dimension being the columns."""
+    return _native.dropout(x, p, rng, residual)
+
+
+class RMSNorm(torch.nn.Module):
+    """:func:`rms_norm` with its weight; ``forward(x)`` is the normed rows, ``forward(x, residual)`` those and the sum.  ``dropout`` is applied to ``x`` in
+    training, with a state of its own (``seed``)."""
+
+    def __init__(self, width: int, eps: float = 1e-6, dropout: float = 0.0, dtype=torch.float32, device="cuda", seed: int = 0):
+        super().__init__()
+        if not 0.0 <= dropout <= 1.0:
+            raise ValueError(f"dropout must be in [0, 1], got {dropout}")
+        self.width, self.eps, self.dropout = width, eps, dropout
+        self.weight = torch.nn.Parameter(torch.ones(width, dtype=dtype, device=device))
+        self.register_buffer("rng", rng_state(seed, device) if dropout > 0 else None)
+
+    def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None):
+        p = self.dropout if self.training else 0.0
+        return rms_norm(x, self.weight, self.eps, residual, p, self.rng)
+
+
+class Dropout(torch.nn.Module):
+    """:func:`dropout` with a state of its own; outside training ``x``, or ``residual + x``."""
+
+    def __init__(self, p: float = 0.5, device="cuda", seed: int = 0):
+        super().__init__()
+        if not 0.0 <= p <= 1.0:
+            raise ValueError(f"p must be in [0, 1], got {p}")
+        self.p = p
+        self.register_buffer("rng", rng_state(seed, device))
+
+    def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:
+        if self.training and self.p > 0:
+            return dropout(x, self.p, self.rng, residual)
+        return x if residual is None else residual + x
 
 
 _LAYER_FORWARD = SparseConv3d.forward

@@ -336,6 +336,88 @@ typedef struct {
 int fgms_b200_adamw(const fgms_b200_adamw_tensor* tensors, int n, const fgms_b200_adamw_options* options, void* stream);
 
 /* ---------------------------------------------------------------------------------------------
+ * What stands between two layers of groups.  Rows are `pitch` values apart, a row's values side by side; any alignment (16-byte aligned
+ * rows are faster).  dtype of rows: F32, F16 or BF16; sums and statistics are fp32.  An output may be the very rows of an input (in place) and may
+ * share no memory with anything else (FGMS_ERR_INVALID_ARG).  The structures are host memory, read before the call returns.
+ *
+ * Dropout: x is dropped where its lot is below round(p 65536), else multiplied by 65536 / (65536 - round(p 65536)).  Lots are 16 bits of Philox
+ * 4x32-10: key the seed, counter (column / 8, row, number of the call), eight lots a counter, the lower half of a word before the upper one.  No mask is
+ * stored: the backward evaluates the same lots from rng_used.
+ *   rng       device, three int64: the seed, the number of calls made, and 0.  A call counts itself there, so that a replayed graph drops other
+ *             values every time; two calls on the same state must not run at the same time.  A call without rows is not counted.
+ *   rng_used  device, two int64: where the call leaves seed and number for its backward (NULL: nowhere); read by the backward.
+ * fgms_b200_dropout: out = residual + dropped x (residual may be NULL).  fgms_b200_dropout_bwd: out = dropped x with the lots of rng_used, where x
+ * is the gradient of the output; the residual's gradient is that itself. */
+typedef struct {
+  const void* x;
+  const void* residual; /* or NULL */
+  void* out;
+  int64_t x_pitch, residual_pitch, out_pitch;
+  int64_t rows, width;
+  int64_t* rng;
+  int64_t* rng_used;
+  double p;
+  int dtype;
+} fgms_b200_dropout_args;
+
+int fgms_b200_dropout(const fgms_b200_dropout_args* args, void* stream);
+int fgms_b200_dropout_bwd(const fgms_b200_dropout_args* args, void* stream);
+
+/* Root-mean-square norm with the residual's addition:
+ *   h = residual + dropped x (residual NULL: dropped x; p = 0: nothing is dropped)      out = h / sqrt(mean(h^2) + eps) * weight
+ * `sum` (or NULL) gets h, rounded once; the norm takes the h before that.  `rstd` (or NULL) gets 1 / sqrt(mean(h^2) + eps), fp32, for the backward.
+ * With `scale` the output is in 8 bits: int8 codes round(y 127 / a) and the scale a / 127 for each row, where a is the row's largest magnitude;
+ * below 2^-100 the row is zeros and its scale 0; a row that is not finite has the scale NaN and codes 0.  No dropout then (FGMS_ERR_UNSUPPORTED).
+ * weight_dtype: that of the rows, or F32.  width: at most 32768. */
+typedef struct {
+  const void* x;
+  const void* residual; /* or NULL */
+  const void* weight;   /* [width] */
+  void* out;            /* rows of the type, or with `scale` of int8 */
+  void* sum;            /* or NULL */
+  float* scale;         /* [rows], or NULL */
+  float* rstd;          /* [rows], or NULL */
+  int64_t x_pitch, residual_pitch, out_pitch, sum_pitch;
+  int64_t rows, width;
+  int64_t* rng; /* p > 0 */
+  int64_t* rng_used;
+  double eps, p;
+  int dtype, weight_dtype;
+} fgms_b200_rms_norm_args;
+
+int fgms_b200_rms_norm(const fgms_b200_rms_norm_args* args, void* stream);
+
+/* Its gradient, from `sum` (x itself where there was neither residual nor dropout) and `rstd`:
+ *   residual_grad = dh = rstd (g - n mean(g n)) + sum_grad     with g = out_grad weight, n = sum rstd
+ *   x_grad = dh where x was kept, times the factor             weight_grad = sum over the rows of out_grad n, added up in fp32 in a fixed order
+ * sum_grad (what else flows back into `sum`), x_grad, residual_grad and weight_grad (weight_dtype) may each be NULL; weight_grad needs a
+ * workspace of fgms_b200_rms_norm_bwd_workspace_bytes on the current device, 16-byte aligned, whose contents do not matter. */
+typedef struct {
+  const void* out_grad;
+  const void* sum;
+  const void* sum_grad; /* or NULL */
+  const void* weight;
+  const float* rstd;
+  void* x_grad;        /* or NULL */
+  void* residual_grad; /* or NULL */
+  void* weight_grad;   /* or NULL */
+  int64_t out_grad_pitch, sum_pitch, sum_grad_pitch, x_grad_pitch, residual_grad_pitch;
+  int64_t rows, width;
+  const int64_t* rng_used; /* p > 0 */
+  void* workspace;
+  size_t workspace_bytes;
+  double p;
+  int dtype, weight_dtype;
+} fgms_b200_rms_norm_bwd_args;
+
+size_t fgms_b200_rms_norm_bwd_workspace_bytes(int64_t rows, int64_t width);
+int fgms_b200_rms_norm_bwd(const fgms_b200_rms_norm_bwd_args* args, void* stream);
+
+/* Rows in 8 bits with a scale each, as fgms_b200_rms_norm leaves them, without a norm: weights get their codes this way (rows: output channels). */
+int fgms_b200_quantize_rows(const void* x, int64_t x_pitch, int8_t* codes, int64_t codes_pitch, float* scale, int64_t rows, int64_t width, int dtype,
+                            void* stream);
+
+/* ---------------------------------------------------------------------------------------------
  * Multi-GPU: sum of the ranks' fp32 weight-gradient partial sums over peer memory.  No counterpart in the
  * reference (it has no multi-GPU path); it stands where a data-parallel caller would otherwise issue an
  * all-reduce of the [k_vol, c_in, c_out] fp32 sums that fgms_b200_wgrad leaves in its workspace.
