@@ -84,6 +84,8 @@ SIGNATURES = {
     "fgms_b200_rms_norm_bwd_workspace_bytes": (c_size_t, [c_int64, c_int64]),
     "fgms_b200_rms_norm_bwd": (c_int, [c_void_p, c_void_p]),
     "fgms_b200_quantize_rows": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int, c_void_p]),
+    "fgms_b200_grouped_i8_fwd": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int64] + [c_void_p] * 3 + [c_int] * 6 + [c_void_p, c_size_t, c_void_p]),
+    "fgms_b200_grouped_i8_workspace_bytes": (c_size_t, [c_void_p, c_int64, c_void_p, c_int64] + [c_int] * 4),
     "fgms_b200_peer_exchange_flag_bytes": (c_size_t, [c_int]),
     "fgms_b200_peer_exchange": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int64, ctypes.c_uint32, c_int64, c_int, c_void_p]),
     "fgms_b200_kernel_family": (c_int, [c_int] * 6),

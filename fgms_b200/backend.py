@@ -33,7 +33,7 @@ __all__ = ["fgms_fusion_fwd_cuda", "fgms_fwd_cuda", "fgms_bwd_cuda", "fgms_dgrad
            "wgrad_workspace", "wgrad_finalize", "fgms_wgrad_noalloc_cuda", "kernel_family", "fallback_count",
            "device_status", "launch_count", "build_neighbor_table", "fgms_fwd_os_cuda", "fgms_grouped_fwd_cuda",
            "fgms_grouped_dgrad_cuda", "fgms_grouped_wgrad_cuda", "fgms_adamw_cuda", "fgms_rms_norm_cuda", "fgms_rms_norm_bwd_cuda",
-           "fgms_quantize_rows_cuda", "fgms_dropout_cuda", "fgms_dropout_bwd_cuda"]
+           "fgms_quantize_rows_cuda", "fgms_dropout_cuda", "fgms_dropout_bwd_cuda", "fgms_grouped_i8_fwd_cuda"]
 
 _L = _lib.lib
 
@@ -340,6 +340,16 @@ def fgms_dropout_cuda(x, out, p, rng, residual=None, rng_used=None):
 def fgms_dropout_bwd_cuda(out_grad, x_grad, p, rng_used):
     """Gradient of :func:`fgms_dropout_cuda`: what dropped x drops, with the same lots (the residual's gradient is ``out_grad`` itself)."""
     _native.dropout_bwd(out_grad, x_grad, p, rng_used)
+
+
+def fgms_grouped_i8_fwd_cuda(codes, scale, kernel, kernel_scale, out, kpos=None, zero_rest=False):
+    """:func:`fgms_grouped_fwd_cuda` in 8 bits (``fgms_b200_grouped_i8_fwd``): ``out[r] = (codes[r] @ kernel[g].T) * scale[r] * kernel_scale[g]``
+    for the rows ``kpos[g] <= r < kpos[g + 1]`` of every group; without ``kpos`` all rows are one group's.
+
+    ``codes`` is int8 ``[rows, c_in]`` with a float32 ``scale`` a row, ``kernel`` int8 ``[groups, c_out, c_in]`` with a ``kernel_scale`` a channel,
+    as :func:`fgms_quantize_rows_cuda` and :func:`fgms_rms_norm_cuda` leave them; the sums are exact (``c_in`` up to 131071).  ``out`` is float16, bfloat16 or
+    float32, overwritten; rows of no group are left as they were, or with ``zero_rest`` become zeros.  Rows that do not start 16 bytes apart cost a copy."""
+    _native.grouped_i8(codes, scale, kernel, kernel_scale, out, kpos, zero_rest)
 
 
 def kernel_family(pass_: str, c_in: int, c_out: int, dtype: torch.dtype, arch80: bool = True, k_vol: int = 27) -> str:

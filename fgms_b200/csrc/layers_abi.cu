@@ -6,6 +6,7 @@
 
 #include "host.cuh"
 #include "dropout.cuh"
+#include "grouped_i8.cuh"
 #include "row_norm.cuh"
 
 namespace fgms_host {
@@ -287,9 +288,117 @@ int run_rms_norm_bwd(const fgms_b200_rms_norm_bwd_args& a, cudaStream_t st) {
   }
   return check_launch("rms_norm_weight_grad_kernel");
 }
+// What of a product in 8 bits has to be copied to rows that a tensor map describes, and where to.
+struct I8Copies {
+  long long a_pitch, b_pitch;  // of the copies; 0: none is needed
+  size_t a_at, b_at, total;
+};
+I8Copies i8_copies(const RowSpan& a, const RowSpan& b) {
+  I8Copies c = {};
+  const auto one = [&](const RowSpan& s, long long* pitch, size_t* at) {
+    if (s.vec(16)) return;
+    *pitch = (s.width + 15) / 16 * 16;
+    *at = c.total;
+    c.total += ((size_t)s.rows * (size_t)*pitch + 255) / 256 * 256;
+  };
+  one(a, &c.a_pitch, &c.a_at);
+  one(b, &c.b_pitch, &c.b_at);
+  return c;
+}
+
+int run_grouped_i8(const int8_t* codes, int64_t codes_pitch, const float* code_scale, const int8_t* kernel, int64_t kernel_pitch, const float* kernel_scale,
+                   void* out, const int32_t* kpos, int n_rows, int c_in, int c_out, int groups, int dtype, int zero_rest, void* workspace,
+                   size_t workspace_bytes, cudaStream_t st) {
+  if (n_rows < 0) return fail(FGMS_ERR_INVALID_ARG, "negative row count");
+  if (c_in < 1 || c_out < 1) return fail(FGMS_ERR_INVALID_ARG, "channel counts must be >= 1");
+  if (c_in > fgms::GI_MAX_CONTRACTION) return fail(FGMS_ERR_INVALID_ARG, "more than %d channels to add up: their sum may leave an int32", fgms::GI_MAX_CONTRACTION);
+  if (n_rows > FGMS_GROUPED_MAX_EXTENT || c_out > FGMS_GROUPED_MAX_EXTENT) return fail(FGMS_ERR_INVALID_ARG, "more than %d rows or channels", FGMS_GROUPED_MAX_EXTENT);
+  if (groups < 1 || groups > FGMS_GROUPED_MAX_GROUPS) return fail(FGMS_ERR_INVALID_ARG, "groups %d outside [1, %d]", groups, FGMS_GROUPED_MAX_GROUPS);
+  if ((long long)groups * c_out > 0x7fffffffll) return fail(FGMS_ERR_INVALID_ARG, "groups times channels exceeds the int32 range");
+  if (((long long)n_rows / 64 + groups) * ((long long)c_out / 128 + 1) >= 0x7fff0000ll) return fail(FGMS_ERR_INVALID_ARG, "more tiles than an int32 counts");
+  if (!layer_dtype_ok(dtype)) return fail(FGMS_ERR_INVALID_ARG, "unknown dtype %d", dtype);
+  if (!kpos && groups != 1) return fail(FGMS_ERR_INVALID_ARG, "kpos may be null for a single group only");
+  const size_t es = layer_elem(dtype);
+  const RowSpan a{codes, n_rows, codes_pitch, c_in, 1}, b{kernel, (int64_t)groups * c_out, kernel_pitch, c_in, 1}, d{out, n_rows, c_out, c_out, es};
+  const RowSpan sa{code_scale, 1, n_rows, n_rows, 4}, sb{kernel_scale, 1, (int64_t)groups * c_out, (int64_t)groups * c_out, 4}, k{kpos, 1, groups + 1, groups + 1, 4};
+  if (int rc = check_span("codes", a, true)) return rc;
+  if (int rc = check_span("kernel", b, true)) return rc;
+  if (int rc = check_span("out", d, true)) return rc;
+  if (int rc = check_span("code_scale", sa, n_rows > 0)) return rc;
+  if (int rc = check_span("kernel_scale", sb, true)) return rc;
+  if (int rc = check_span("kpos", k, false)) return rc;
+  for (const RowSpan* in : {&a, &b, &sa, &sb, &k})
+    if (d.collides(*in) || d.same(*in)) return fail(FGMS_ERR_INVALID_ARG, "the output overlaps an input");
+  if (n_rows == 0) return FGMS_OK;
+  const I8Copies copies = i8_copies(a, b);
+  if (copies.total > 0) {
+    if (!workspace || workspace_bytes < copies.total || (reinterpret_cast<uintptr_t>(workspace) & 255))
+      return fail(FGMS_ERR_WORKSPACE, "rows that do not start on 16-byte boundaries need a workspace of %zu bytes on a 256-byte boundary", copies.total);
+    const Range w{workspace, copies.total};
+    for (const RowSpan* s : {&a, &b, &d, &sa, &sb, &k})
+      if (s->any() && w.overlaps(Range{s->p, s->bytes()})) return fail(FGMS_ERR_WORKSPACE, "the workspace overlaps a tensor");
+  }
+  DeviceInfo di;
+  if (int rc = device_info(&di)) return rc;
+  fgms::GroupedI8Params q{};
+  q.g.a = codes;
+  q.g.b = kernel;
+  q.g.d = out;
+  q.g.kpos = kpos;
+  q.g.n_rows = n_rows;
+  q.g.c_in = c_out;
+  q.g.c_out = (c_in + 1) / 2;
+  q.g.groups = groups;
+  q.g.zero_rest = zero_rest;
+  q.g.d_pitch = c_out;
+  q.g.alone = di.reserved > 0;
+  q.row_scale = code_scale;
+  q.channel_scale = kernel_scale;
+  q.dtype = dtype == FGMS_DTYPE_F32 ? 0 : dtype == FGMS_DTYPE_F16 ? 1 : 2;
+  q.direct = dtype == FGMS_DTYPE_F32 || !d.vec(16) || c_out % 8 != 0;
+  long long a_pitch = a.rows > 1 ? a.pitch : (c_in + 15) / 16 * 16, b_pitch = b.rows > 1 ? b.pitch : (c_in + 15) / 16 * 16;
+  if (copies.total > 0) {
+    uint8_t* to = static_cast<uint8_t*>(workspace);
+    fgms::ByteRows x{}, y{};
+    if (copies.a_pitch) {
+      x = {reinterpret_cast<const uint8_t*>(codes), to + copies.a_at, a.rows, a.pitch, copies.a_pitch, c_in};
+      q.g.a = x.dst;
+      a_pitch = copies.a_pitch;
+    }
+    if (copies.b_pitch) {
+      y = {reinterpret_cast<const uint8_t*>(kernel), to + copies.b_at, b.rows, b.pitch, copies.b_pitch, c_in};
+      q.g.b = y.dst;
+      b_pitch = copies.b_pitch;
+    }
+    const long long blocks = (x.rows + y.rows + 7) / 8, most = 8ll * di.sms;
+    if (fgms::launch_pdl(fgms::copy_byte_rows_kernel, dim3((unsigned)(blocks < most ? blocks : most)), fgms::BR_THREADS, 0, st, x, y, q.g.alone) != cudaSuccess)
+      return fail(FGMS_ERR_CUDA, "copy_byte_rows_kernel: %s", cudaGetErrorString(cudaGetLastError()));
+    if (int rc = check_launch("copy_byte_rows_kernel")) return rc;
+  }
+  const int rc = fgms::launch_grouped_i8(q, c_in, a_pitch, b_pitch, st, di.sms, di.max_smem_optin);
+  if (rc != 0) {
+    const cudaError_t e = cudaGetLastError();
+    return fail(FGMS_ERR_CUDA, "grouped_i8_kernel: %s (%d)", cudaGetErrorString(e), rc);
+  }
+  return check_launch("grouped_i8_kernel");
+}
 }  // namespace
 
 extern "C" {
+
+int fgms_b200_grouped_i8_fwd(const int8_t* codes, int64_t codes_pitch, const float* code_scale, const int8_t* kernel, int64_t kernel_pitch,
+                             const float* kernel_scale, void* out, const int32_t* kpos, int n_rows, int c_in, int c_out, int groups, int dtype,
+                             int zero_rest, void* workspace, size_t workspace_bytes, void* stream) {
+  TraceRange trace_range("fgms_b200_grouped_i8_fwd");
+  return run_grouped_i8(codes, codes_pitch, code_scale, kernel, kernel_pitch, kernel_scale, out, kpos, n_rows, c_in, c_out, groups, dtype, zero_rest, workspace,
+                        workspace_bytes, static_cast<cudaStream_t>(stream));
+}
+
+size_t fgms_b200_grouped_i8_workspace_bytes(const int8_t* codes, int64_t codes_pitch, const int8_t* kernel, int64_t kernel_pitch, int n_rows, int c_in, int c_out,
+                                            int groups) {
+  if (n_rows < 1 || c_in < 1 || c_out < 1 || groups < 1) return 0;
+  return i8_copies(RowSpan{codes, n_rows, codes_pitch, c_in, 1}, RowSpan{kernel, (int64_t)groups * c_out, kernel_pitch, c_in, 1}).total;
+}
 
 int fgms_b200_dropout(const fgms_b200_dropout_args* args, void* stream) {
   TraceRange trace_range("fgms_b200_dropout");

@@ -14,6 +14,7 @@
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -1052,6 +1053,57 @@ std::array<Tensor, 3> rms_norm_int8(const Tensor& x_, const Tensor* weight_, con
 }
 
 // ---------------------------------------------------------------------------------------------
+// products in 8 bits
+// ---------------------------------------------------------------------------------------------
+void grouped_i8(const Tensor& codes, const Tensor& scale, const Tensor& kernel, const Tensor& kernel_scale, const Tensor& out, const Tensor* kpos, bool zero_rest) {
+  const int dtype = layer_dtype(out);
+  TORCH_CHECK_VALUE(kernel.is_cuda() && kernel.scalar_type() == at::kChar && kernel.dim() == 3, "kernel must be an int8 CUDA tensor of 3 dimensions");
+  const int64_t groups = kernel.size(0), c_out = kernel.size(1), c_in = kernel.size(2);
+  TORCH_CHECK_VALUE(codes.device() == kernel.device(), "codes must live on ", kernel.device());
+  TORCH_CHECK_VALUE(codes.scalar_type() == at::kChar && codes.dim() == 2, "codes must be an int8 tensor of 2 dimensions");
+  TORCH_CHECK_VALUE(codes.size(1) == c_in, "codes have ", codes.size(1), " channels, the kernel says ", c_in);
+  TORCH_CHECK_VALUE(codes.numel() == 0 || c_in <= 1 || codes.stride(1) == 1, "codes must have the values of a row side by side");
+  TORCH_CHECK_VALUE(codes.numel() == 0 || codes.size(0) <= 1 || codes.stride(0) >= c_in, "codes have rows that overlap");
+  // the kernel's rows, of all groups alike
+  const int64_t apart = c_out > 1 ? kernel.stride(1) : groups > 1 ? kernel.stride(0) : c_in;
+  TORCH_CHECK_VALUE(kernel.numel() == 0 || ((c_in <= 1 || kernel.stride(2) == 1) && apart >= c_in && (groups <= 1 || c_out <= 1 || kernel.stride(0) == c_out * apart)),
+                    "kernel must have the values of a row side by side, and all rows equally far apart");
+  TORCH_CHECK_VALUE(scale.is_contiguous() && scale.dim() == 1 && scale.numel() == codes.size(0) && scale.scalar_type() == at::kFloat && scale.device() == kernel.device(),
+                    "scale must be ", codes.size(0), " float32 values, one a row, on ", kernel.device());
+  TORCH_CHECK_VALUE(kernel_scale.is_contiguous() && kernel_scale.dim() == 2 && kernel_scale.size(0) == groups && kernel_scale.size(1) == c_out &&
+                        kernel_scale.scalar_type() == at::kFloat && kernel_scale.device() == kernel.device(),
+                    "kernel_scale must be ", groups, " x ", c_out, " float32 values, one a channel, on ", kernel.device());
+  check_feat("out", out, 2);
+  TORCH_CHECK_VALUE(out.device() == kernel.device(), "out must live on ", kernel.device());
+  TORCH_CHECK_VALUE(out.size(0) == codes.size(0) && out.size(1) == c_out, "out must be ", codes.size(0), " x ", c_out);
+  if (kpos) {
+    check_index("kpos", *kpos, kernel, 0);
+    TORCH_CHECK_VALUE(kpos->dim() == 1 && kpos->size(0) == groups + 1, "kpos must have one entry more than there are groups: ", groups + 1, ", got ", kpos->numel());
+  } else {
+    TORCH_CHECK_VALUE(groups == 1, "kpos is needed for more than one group");
+  }
+  for (const int64_t n : {codes.size(0), c_in, c_out, groups}) TORCH_CHECK_VALUE(n <= 0x7fffffff, "more than 2^31 - 1 rows or channels");
+  c10::cuda::CUDAGuard guard(kernel.device());
+  const int8_t *a = static_cast<const int8_t*>(ptr(codes)), *b = static_cast<const int8_t*>(ptr(kernel));
+  const int64_t a_pitch = pitch(codes);
+  const int rows = (int)codes.size(0);
+  const size_t bytes = fgms_b200_grouped_i8_workspace_bytes(a, a_pitch, b, apart, rows, (int)c_in, (int)c_out, (int)groups);
+  const Tensor ws = bytes > 0 ? at::empty({(int64_t)bytes}, kernel.options().dtype(at::kByte).requires_grad(false)) : Tensor();
+  check_status(fgms_b200_grouped_i8_fwd(a, a_pitch, static_cast<const float*>(ptr(scale)), b, apart, static_cast<const float*>(ptr(kernel_scale)), ptr(out),
+                                        kpos ? iptr(*kpos) : nullptr, rows, (int)c_in, (int)c_out, (int)groups, dtype, zero_rest, space(ws), space_bytes(ws),
+                                        stream_of(kernel)));
+  written(out);
+}
+
+Tensor int8_linear(const Tensor& codes, const Tensor& scale, const Tensor& kernel_, const Tensor& kernel_scale_, const Tensor* kpos, at::ScalarType type) {
+  const Tensor kernel = kernel_.dim() == 2 ? kernel_.unsqueeze(0) : kernel_, kernel_scale = kernel_scale_.dim() == 1 ? kernel_scale_.unsqueeze(0) : kernel_scale_;
+  TORCH_CHECK_VALUE(kernel.is_cuda() && kernel.dim() == 3 && codes.dim() == 2, "kernel must be an int8 CUDA tensor of 2 or 3 dimensions, codes one of 2");
+  Tensor out = at::empty({codes.size(0), kernel.size(1)}, kernel.options().dtype(type).requires_grad(false));
+  grouped_i8(codes, scale, kernel, kernel_scale, out, kpos, kpos != nullptr);
+  return out;
+}
+
+// ---------------------------------------------------------------------------------------------
 // AdamW over many tensors
 // ---------------------------------------------------------------------------------------------
 int adamw_dtype(const char* name, const Tensor& t) {
@@ -1423,6 +1475,25 @@ PyObject* py_dropout(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// (codes, scale, kernel, kernel_scale, out, kpos, zero_rest)
+PyObject* py_grouped_i8(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  expect(n, 7);
+  grouped_i8(feat_arg(a[0], "codes"), feat_arg(a[1], "scale"), feat_arg(a[2], "kernel"), feat_arg(a[3], "kernel_scale"), feat_arg(a[4], "out"),
+             optional_arg(a[5], "kpos"), bool_arg(a[6]));
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+// (codes, scale, kernel, kernel_scale, kpos, dtype)
+PyObject* py_int8_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  expect(n, 6);
+  TORCH_CHECK_TYPE(THPDtype_Check(a[5]), "dtype must be a torch.dtype");
+  return THPVariable_Wrap(int8_linear(feat_arg(a[0], "codes"), feat_arg(a[1], "scale"), feat_arg(a[2], "kernel"), feat_arg(a[3], "kernel_scale"),
+                                      optional_arg(a[4], "kpos"), reinterpret_cast<THPDtype*>(a[5])->scalar_type));
+  END_HANDLE_TH_ERRORS
+}
+
 #define FGMS_METHOD(name, fn) {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(fn)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {
     FGMS_METHOD("fusion_fwd", py_fusion_fwd), FGMS_METHOD("seq_fwd", py_seq_fwd),         FGMS_METHOD("bwd", py_bwd),
@@ -1435,6 +1506,7 @@ PyMethodDef methods[] = {
     FGMS_METHOD("rms_norm_into", py_rms_norm_into), FGMS_METHOD("rms_norm_bwd", py_rms_norm_bwd), FGMS_METHOD("rms_norm", py_rms_norm),
     FGMS_METHOD("rms_norm_int8", py_rms_norm_int8), FGMS_METHOD("quantize_rows_into", py_quantize_rows_into),
     FGMS_METHOD("dropout_into", py_dropout_into), FGMS_METHOD("dropout_bwd", py_dropout_bwd), FGMS_METHOD("dropout", py_dropout),
+    FGMS_METHOD("grouped_i8", py_grouped_i8), FGMS_METHOD("int8_linear", py_int8_linear),
     FGMS_METHOD("build_pyramid", py_build_pyramid), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -17,7 +17,7 @@ import torch
 from . import _native, backend
 
 __all__ = ["sparse_conv", "sparse_conv_inference", "SparseConv3d", "SparseUNet", "grouped_linear", "GroupedLinear", "rms_norm", "RMSNorm",
-           "rms_norm_int8", "quantize_rows", "rng_state", "dropout", "Dropout"]
+           "rms_norm_int8", "quantize_rows", "rng_state", "dropout", "Dropout", "int8_linear", "Int8GroupedLinear"]
 
 
 def sparse_conv(feats: torch.Tensor, weight: torch.Tensor, kmap, arch80: bool = True) -> torch.Tensor:
@@ -106,6 +106,32 @@ def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, resi
 def quantize_rows(x: torch.Tensor):
     """``(codes, scale)``: the rows of ``x`` in 8 bits with a float32 scale each.  No autograd."""
     return _native.rms_norm_int8(x, None, 0.0, None)
+
+
+def int8_linear(codes: torch.Tensor, scale: torch.Tensor, kernel: torch.Tensor, kernel_scale: torch.Tensor, kpos: torch.Tensor | None = None,
+                dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """``(codes * scale[:, None]) @ (kernel * kernel_scale[:, None]).T`` in 8-bit integers, exact up to the scales, in ``dtype``: ``codes`` from
+    :func:`rms_norm_int8` or :func:`quantize_rows`, ``kernel`` ``[c_out, c_in]`` with a scale a channel, or ``[groups, c_out, c_in]`` with ``kpos`` as in
+    :func:`grouped_linear` (rows of no group are zero).  No autograd."""
+    return _native.int8_linear(codes, scale, kernel, kernel_scale, kpos, dtype)
+
+
+class Int8GroupedLinear(torch.nn.Module):
+    """:class:`GroupedLinear` for serving: its matrices in 8 bits with a scale for each channel, rows in 8 bits with a scale each.
+    ``forward(feats, kpos)`` takes rows, or the ``(codes, scale)`` of :func:`rms_norm_int8` and :func:`quantize_rows`."""
+
+    def __init__(self, weight: torch.Tensor, dtype: torch.dtype | None = None):
+        super().__init__()
+        groups, c_in, c_out = weight.shape
+        codes, scale = quantize_rows(weight.detach().transpose(1, 2).reshape(groups * c_out, c_in))
+        # a channel's codes, a multiple of 16 bytes from the next one's
+        self.register_buffer("kernel", codes.as_strided((groups, c_out, c_in), (c_out * codes.stride(0), codes.stride(0), 1)))
+        self.register_buffer("kernel_scale", scale.view(groups, c_out))
+        self.dtype = weight.dtype if dtype is None else dtype
+
+    def forward(self, feats, kpos: torch.Tensor | None = None) -> torch.Tensor:
+        codes, scale = feats if isinstance(feats, tuple) else quantize_rows(feats)
+        return int8_linear(codes, scale, self.kernel, self.kernel_scale, kpos, self.dtype)
 
 
 def rng_state(seed: int = 0, device="cuda") -> torch.Tensor:

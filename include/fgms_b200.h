@@ -418,6 +418,23 @@ int fgms_b200_quantize_rows(const void* x, int64_t x_pitch, int8_t* codes, int64
                             void* stream);
 
 /* ---------------------------------------------------------------------------------------------
+ * fgms_b200_grouped_fwd in 8 bits, with a scale for each row and each output channel:
+ *
+ *     out[r, c] = (sum over k of codes[r, k] * kernel[g, c, k]) * code_scale[r] * kernel_scale[g, c]        kpos[g] <= r < kpos[g + 1]
+ *
+ * The sum is an exact 32-bit integer (c_in at most 131071); the rest is fp32 and rounded once to the output's type (dtype: F32, F16, BF16).  codes
+ * [n_rows, c_in] and kernel [groups, c_out, c_in] are rows of int8 that are codes_pitch and kernel_pitch bytes apart (the kernel's of all
+ * groups alike); out is [n_rows, c_out], overwritten; rows of no group are left as they were, or become zeros with zero_rest.  kpos as
+ * above; NULL with a single group: all rows.  Rows that do not start on 16-byte boundaries are copied to rows that do, in a workspace of
+ * fgms_b200_grouped_i8_workspace_bytes() bytes, 256-byte aligned (FGMS_ERR_WORKSPACE without); fgms_b200_rms_norm and fgms_b200_quantize_rows can
+ * write rows that need none. */
+int fgms_b200_grouped_i8_fwd(const int8_t* codes, int64_t codes_pitch, const float* code_scale, const int8_t* kernel,
+                             int64_t kernel_pitch, const float* kernel_scale, void* out, const int32_t* kpos, int n_rows, int c_in,
+                             int c_out, int groups, int dtype, int zero_rest, void* workspace, size_t workspace_bytes, void* stream);
+size_t fgms_b200_grouped_i8_workspace_bytes(const int8_t* codes, int64_t codes_pitch, const int8_t* kernel, int64_t kernel_pitch,
+                                            int n_rows, int c_in, int c_out, int groups);
+
+/* ---------------------------------------------------------------------------------------------
  * Multi-GPU: sum of the ranks' fp32 weight-gradient partial sums over peer memory.  No counterpart in the
  * reference (it has no multi-GPU path); it stands where a data-parallel caller would otherwise issue an
  * all-reduce of the [k_vol, c_in, c_out] fp32 sums that fgms_b200_wgrad leaves in its workspace.

@@ -123,3 +123,30 @@ def test_modules_refuse():
         with pytest.raises(ValueError):
             make()
     assert nn.RMSNorm(8, device="cpu").rng is None and nn.rng_state(5, "cpu").tolist() == [5, 0, 0]
+
+
+def product(codes=P, codes_pitch=64, scale=2 * P, kernel=3 * P, kernel_pitch=64, kernel_scale=4 * P, out=5 * P, kpos=6 * P, rows=4, c_in=64, c_out=32, groups=3,
+            dtype=_lib.DTYPE_BF16, ws=None, ws_bytes=0):
+    return L.fgms_b200_grouped_i8_fwd(codes, codes_pitch, scale, kernel, kernel_pitch, kernel_scale, out, kpos, rows, c_in, c_out, groups, dtype, 0, ws, ws_bytes, None)
+
+
+@pytest.mark.parametrize("change,text", [
+    (dict(rows=-1), "negative"), (dict(c_in=0), "channel counts"), (dict(c_out=-1), "channel counts"), (dict(c_in=131072), "131071"), (dict(groups=0), "groups 0"),
+    (dict(groups=1025), "groups 1025"), (dict(groups=1024, c_out=1 << 21), "int32 range"), (dict(dtype=7), "dtype"), (dict(kpos=None), "kpos"),
+    (dict(rows=2 ** 31 - 1024), "rows or channels"), (dict(rows=2 ** 31 - 1026, c_out=2 ** 20), "tiles"), (dict(codes=None), "codes: null"),
+    (dict(kernel=None), "kernel: null"), (dict(out=None), "out: null"), (dict(scale=None), "code_scale: null"), (dict(kernel_scale=None), "kernel_scale: null"),
+    (dict(out=5 * P + 1), "boundary"), (dict(scale=2 * P + 2), "boundary"), (dict(kpos=6 * P + 1), "boundary"), (dict(codes_pitch=63), "apart"),
+    (dict(out=P + 128), "overlaps"), (dict(out=3 * P), "overlaps"), (dict(out=4 * P + 4), "overlaps"), (dict(out=6 * P), "overlaps"),
+])
+def test_products_in_8_bits_refuse(change, text):
+    assert product(**change) == _lib.ERR_INVALID_ARG and text in _lib.last_error(), _lib.last_error()
+
+
+def test_products_in_8_bits_say_what_they_copy():
+    size = L.fgms_b200_grouped_i8_workspace_bytes
+    assert size(P, 64, 3 * P, 64, 4, 64, 32, 3) == 0 and size(P, 64, 3 * P, 64, 4, 50, 32, 3) == 0
+    assert size(P + 1, 64, 3 * P, 64, 4, 64, 32, 3) == 256 and size(P, 50, 3 * P, 64, 4, 50, 32, 3) == 256
+    assert size(P, 64, 3 * P, 65, 4, 64, 32, 3) == 3 * 32 * 64 and size(P + 1, 65, 3 * P, 65, 4, 64, 32, 3) == 256 + 3 * 32 * 64
+    assert product(codes=P + 1) == _lib.ERR_WORKSPACE and product(codes=P + 1, ws=7 * P, ws_bytes=255) == _lib.ERR_WORKSPACE
+    assert product(codes=P + 1, ws=7 * P + 16, ws_bytes=512) == _lib.ERR_WORKSPACE and product(codes=P + 1, ws=5 * P, ws_bytes=512) == _lib.ERR_WORKSPACE
+    assert product(rows=0, codes=None, out=None, scale=None) == _lib.OK
