@@ -45,6 +45,12 @@ class RmsNormBwdArgs(ctypes.Structure):
                 [("rng_used", c_void_p), ("workspace", c_void_p), ("workspace_bytes", c_size_t), ("p", c_double), ("dtype", c_int), ("weight_dtype", c_int)])
 
 
+class ExpertLayerArgs(ctypes.Structure):
+    _fields_ = ([(n, c_void_p) for n in ("x", "router", "w_in", "w_out", "out", "chosen", "gates")] + [("x_pitch", c_int64), ("out_pitch", c_int64)] +
+                [("workspace", c_void_p), ("workspace_bytes", c_size_t)] +
+                [(n, c_int) for n in ("tokens", "experts", "top_k", "width", "hidden", "out_width", "gated", "activation", "dtype", "router_dtype")])
+
+
 # name -> (restype, argtypes); mirrors include/fgms_b200.h declaration by declaration
 SIGNATURES = {
     "fgms_b200_fusion_fwd": (c_int, [c_void_p] * 7 + [c_int64] + [c_int] * 6 + [c_int64] + [c_int] * 3 + [c_void_p]),
@@ -86,6 +92,8 @@ SIGNATURES = {
     "fgms_b200_quantize_rows": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int, c_void_p]),
     "fgms_b200_grouped_i8_fwd": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int64] + [c_void_p] * 3 + [c_int] * 6 + [c_void_p, c_size_t, c_void_p]),
     "fgms_b200_grouped_i8_workspace_bytes": (c_size_t, [c_void_p, c_int64, c_void_p, c_int64] + [c_int] * 4),
+    "fgms_b200_expert_layer_workspace_bytes": (c_size_t, [c_int] * 5),
+    "fgms_b200_expert_layer": (c_int, [c_void_p, c_void_p]),
     "fgms_b200_peer_exchange_flag_bytes": (c_size_t, [c_int]),
     "fgms_b200_peer_exchange": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int64, ctypes.c_uint32, c_int64, c_int, c_void_p]),
     "fgms_b200_kernel_family": (c_int, [c_int] * 6),

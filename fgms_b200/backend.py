@@ -33,7 +33,7 @@ __all__ = ["fgms_fusion_fwd_cuda", "fgms_fwd_cuda", "fgms_bwd_cuda", "fgms_dgrad
            "wgrad_workspace", "wgrad_finalize", "fgms_wgrad_noalloc_cuda", "kernel_family", "fallback_count",
            "device_status", "launch_count", "build_neighbor_table", "fgms_fwd_os_cuda", "fgms_grouped_fwd_cuda",
            "fgms_grouped_dgrad_cuda", "fgms_grouped_wgrad_cuda", "fgms_adamw_cuda", "fgms_rms_norm_cuda", "fgms_rms_norm_bwd_cuda",
-           "fgms_quantize_rows_cuda", "fgms_dropout_cuda", "fgms_dropout_bwd_cuda", "fgms_grouped_i8_fwd_cuda"]
+           "fgms_quantize_rows_cuda", "fgms_dropout_cuda", "fgms_dropout_bwd_cuda", "fgms_grouped_i8_fwd_cuda", "fgms_expert_layer_cuda"]
 
 _L = _lib.lib
 
@@ -350,6 +350,17 @@ def fgms_grouped_i8_fwd_cuda(codes, scale, kernel, kernel_scale, out, kpos=None,
     as :func:`fgms_quantize_rows_cuda` and :func:`fgms_rms_norm_cuda` leave them; the sums are exact (``c_in`` up to 131071).  ``out`` is float16, bfloat16 or
     float32, overwritten; rows of no group are left as they were, or with ``zero_rest`` become zeros.  Rows that do not start 16 bytes apart cost a copy."""
     _native.grouped_i8(codes, scale, kernel, kernel_scale, out, kpos, zero_rest)
+
+
+def fgms_expert_layer_cuda(x, router, w_in, w_out, out, experts, gates, activation="silu"):
+    """A whole layer of experts for up to 64 tokens in two launches (``fgms_b200_expert_layer``): router, choice of the ``top_k`` experts of each
+    token (as many as ``experts`` has columns; of equal logits the lower index first), softmax over those, ``out[t] = sum of gate * (h @ w_out[e])``
+    with ``h = act(x[t] @ w_in[e])``, or ``act(u[:hidden]) * u[hidden:]`` where ``w_in`` is twice as wide as ``w_out`` is high.
+
+    ``x`` ``[tokens, width]``, ``w_in`` ``[experts, width, hidden or 2 hidden]``, ``w_out`` ``[experts, hidden, out_width]`` are float16 or bfloat16,
+    widths multiples of 8; ``router`` ``[experts, width]`` of that type or float32 (logits are summed in 64 bits).  ``out``, ``experts`` (int32) and ``gates``
+    (float32, both ``[tokens, top_k]``) are overwritten.  :func:`fgms_b200.nn.expert_layer` is the same for any number of tokens, with gradients."""
+    _native.expert_layer(x, router, w_in, w_out, out, experts, gates, activation)
 
 
 def kernel_family(pass_: str, c_in: int, c_out: int, dtype: torch.dtype, arch80: bool = True, k_vol: int = 27) -> str:

@@ -6,6 +6,7 @@
 
 #include "host.cuh"
 #include "dropout.cuh"
+#include "expert_layer.cuh"
 #include "grouped_i8.cuh"
 #include "row_norm.cuh"
 
@@ -382,9 +383,100 @@ int run_grouped_i8(const int8_t* codes, int64_t codes_pitch, const float* code_s
   }
   return check_launch("grouped_i8_kernel");
 }
+int run_expert_layer(const fgms_b200_expert_layer_args& a, cudaStream_t st) {
+  if (a.tokens < 0 || a.tokens > fgms::EL_MAX_TOKENS) return fail(FGMS_ERR_INVALID_ARG, "tokens %d outside [0, %d]", a.tokens, fgms::EL_MAX_TOKENS);
+  if (a.experts < 1 || a.experts > fgms::EL_MAX_EXPERTS) return fail(FGMS_ERR_INVALID_ARG, "experts %d outside [1, %d]", a.experts, fgms::EL_MAX_EXPERTS);
+  if (a.top_k < 1 || a.top_k > fgms::EL_MAX_TOP_K || a.top_k > a.experts)
+    return fail(FGMS_ERR_INVALID_ARG, "top_k %d outside [1, %d], or more than the %d experts", a.top_k, fgms::EL_MAX_TOP_K, a.experts);
+  for (const int c : {a.width, a.hidden, a.out_width})
+    if (c < 8 || c > (1 << 20) || c % 8 != 0) return fail(FGMS_ERR_INVALID_ARG, "widths must be multiples of 8 up to 2^20, got %d", c);
+  if (a.dtype != FGMS_DTYPE_F16 && a.dtype != FGMS_DTYPE_BF16) return fail(FGMS_ERR_UNSUPPORTED, "a layer of experts for a few tokens takes F16 or BF16");
+  if (a.router_dtype != a.dtype && a.router_dtype != FGMS_DTYPE_F32) return fail(FGMS_ERR_UNSUPPORTED, "the router's type must be that of the rows, or fp32");
+  if (a.activation != FGMS_ACTIVATION_RELU && a.activation != FGMS_ACTIVATION_SILU) return fail(FGMS_ERR_INVALID_ARG, "unknown activation %d", a.activation);
+  const int64_t wide = a.gated ? 2ll * a.hidden : a.hidden;
+  const int64_t tiles[2] = {(int64_t)a.experts * ((wide + 127) / 128 + 1) * ((a.width + 63) / 64), (int64_t)a.experts * ((a.out_width + 127) / 128) * ((a.hidden + 63) / 64)};
+  if (tiles[0] > 0x3fffffff || tiles[1] > 0x3fffffff) return fail(FGMS_ERR_INVALID_ARG, "weights too large");
+  const int64_t pairs = (int64_t)a.tokens * a.top_k;
+  const RowSpan x{a.x, a.tokens, a.x_pitch, a.width, 2}, out{a.out, a.tokens, a.out_pitch, a.out_width, 2};
+  const RowSpan router{a.router, a.experts, a.width, a.width, layer_elem(a.router_dtype)}, w_in{a.w_in, (int64_t)a.experts * a.width, wide, wide, 2},
+      w_out{a.w_out, (int64_t)a.experts * a.hidden, a.out_width, a.out_width, 2};
+  const RowSpan experts{a.chosen, 1, pairs, pairs, 4}, gates{a.gates, 1, pairs, pairs, 4};
+  if (int rc = check_span("x", x, true)) return rc;
+  if (int rc = check_span("router", router, true)) return rc;
+  if (int rc = check_span("w_in", w_in, true)) return rc;
+  if (int rc = check_span("w_out", w_out, true)) return rc;
+  if (int rc = check_span("out", out, true)) return rc;
+  if (int rc = check_span("chosen", experts, pairs > 0)) return rc;
+  if (int rc = check_span("gates", gates, pairs > 0)) return rc;
+  if (!x.vec(16) || !router.vec(16) || !w_in.vec(16) || !w_out.vec(16)) return fail(FGMS_ERR_INVALID_ARG, "rows and weights must start on 16-byte boundaries");
+  if (a.tokens == 0) return FGMS_OK;
+  const RowSpan outputs[] = {out, experts, gates}, inputs[] = {x, router, w_in, w_out};
+  for (int i = 0; i < 3; ++i) {
+    for (int j = 0; j < 4; ++j)
+      if (outputs[i].collides(inputs[j]) || (outputs[i].same(inputs[j]) && (i > 0 || j > 0))) return fail(FGMS_ERR_INVALID_ARG, "an output overlaps an input");
+    for (int j = 0; j < i; ++j)
+      if (outputs[i].collides(outputs[j]) || outputs[i].same(outputs[j])) return fail(FGMS_ERR_INVALID_ARG, "two outputs overlap");
+  }
+  DeviceInfo di;
+  if (int rc = device_info(&di)) return rc;
+  const fgms::ExpertSpace space = fgms::expert_space(a.tokens, a.experts, a.top_k, a.hidden, a.out_width, di.all);
+  if (!a.workspace || a.workspace_bytes < space.total || (reinterpret_cast<uintptr_t>(a.workspace) & 255))
+    return fail(FGMS_ERR_WORKSPACE, "a workspace of %zu bytes on a 256-byte boundary is needed", space.total);
+  for (const RowSpan* s : {&x, &router, &w_in, &w_out, &out, &experts, &gates})
+    if (Range{a.workspace, space.total}.overlaps(Range{s->p, s->bytes()})) return fail(FGMS_ERR_WORKSPACE, "the workspace overlaps a tensor");
+  uint8_t* at = static_cast<uint8_t*>(a.workspace);
+  fgms::ExpertParams p{};
+  p.x = a.x;
+  p.router = a.router;
+  p.out = a.out;
+  p.experts = a.chosen;
+  p.gates = a.gates;
+  p.tokens = a.tokens;
+  p.n_experts = a.experts;
+  p.top_k = a.top_k;
+  p.width = a.width;
+  p.hidden = a.hidden;
+  p.out_width = a.out_width;
+  p.gated = a.gated != 0;
+  p.activation = a.activation == FGMS_ACTIVATION_SILU;
+  p.x_pitch = a.tokens > 1 ? a.x_pitch : a.width;
+  p.out_pitch = a.tokens > 1 ? a.out_pitch : a.out_width;
+  p.logits = reinterpret_cast<double*>(at + space.logits);
+  p.flags = reinterpret_cast<uint32_t*>(at + space.flags);
+  p.slots = reinterpret_cast<float*>(at + space.slots);
+  p.h = reinterpret_cast<uint16_t*>(at + space.h);
+  p.part = reinterpret_cast<float*>(at + space.part);
+  p.ctas = di.sms;
+  p.x_vec = true;
+  p.alone = di.reserved > 0;
+  const cudaError_t e = with_types(a.dtype, a.router_dtype, [&](auto t, auto r) { return fgms::launch_expert_logits<decltype(t), decltype(r)>(p, st); });
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return fail(FGMS_ERR_CUDA, "expert_logits_kernel: %s", cudaGetErrorString(e));
+  }
+  if (int rc = check_launch("expert_logits_kernel")) return rc;
+  const int rc = a.dtype == FGMS_DTYPE_BF16 ? fgms::launch_expert_layer<true>(p, a.w_in, a.w_out, st, di.max_smem_optin)
+                                            : fgms::launch_expert_layer<false>(p, a.w_in, a.w_out, st, di.max_smem_optin);
+  if (rc != 0) return fail(FGMS_ERR_CUDA, "expert_layer_kernel: %s (%d)", cudaGetErrorString(cudaGetLastError()), rc);
+  return check_launch("expert_layer_kernel");
+}
 }  // namespace
 
 extern "C" {
+
+size_t fgms_b200_expert_layer_workspace_bytes(int tokens, int experts, int top_k, int hidden, int out_width) {
+  DeviceInfo di;
+  if (tokens < 1 || tokens > fgms::EL_MAX_TOKENS || experts < 1 || experts > fgms::EL_MAX_EXPERTS || top_k < 1 || top_k > fgms::EL_MAX_TOP_K || hidden < 1 || out_width < 1 ||
+      device_info(&di) != FGMS_OK)
+    return 0;
+  return fgms::expert_space(tokens, experts, top_k, hidden, out_width, di.all).total;
+}
+
+int fgms_b200_expert_layer(const fgms_b200_expert_layer_args* args, void* stream) {
+  TraceRange trace_range("fgms_b200_expert_layer");
+  if (!args) return fail(FGMS_ERR_INVALID_ARG, "null pointer");
+  return run_expert_layer(*args, static_cast<cudaStream_t>(stream));
+}
 
 int fgms_b200_grouped_i8_fwd(const int8_t* codes, int64_t codes_pitch, const float* code_scale, const int8_t* kernel, int64_t kernel_pitch,
                              const float* kernel_scale, void* out, const int32_t* kpos, int n_rows, int c_in, int c_out, int groups, int dtype,

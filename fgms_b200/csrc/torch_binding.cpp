@@ -1104,6 +1104,63 @@ Tensor int8_linear(const Tensor& codes, const Tensor& scale, const Tensor& kerne
 }
 
 // ---------------------------------------------------------------------------------------------
+// a layer of experts for a few tokens
+// ---------------------------------------------------------------------------------------------
+int activation_of(const std::string& name) {
+  if (name == "silu") return FGMS_ACTIVATION_SILU;
+  TORCH_CHECK_VALUE(name == "relu", "activation must be 'silu' or 'relu', got '", name, "'");
+  return FGMS_ACTIVATION_RELU;
+}
+
+void expert_layer(const Tensor& x, const Tensor& router, const Tensor& w_in, const Tensor& w_out, const Tensor& out, const Tensor& experts, const Tensor& gates,
+                  const std::string& activation) {
+  fgms_b200_expert_layer_args a = {};
+  a.activation = activation_of(activation);
+  TORCH_CHECK_VALUE(x.is_cuda() && x.dim() == 2, "x must be a CUDA tensor of 2 dimensions");
+  check_row_values("x", x, x.scalar_type(), x);
+  a.dtype = layer_dtype(x);
+  check_feat("w_in", w_in, 3, x);
+  check_feat("w_out", w_out, 3, x);
+  check_feat("router", router, 2);
+  a.router_dtype = layer_dtype(router);
+  for (const auto& [name, t] : {std::pair<const char*, const Tensor&>{"w_in", w_in}, {"w_out", w_out}, {"router", router}, {"out", out}, {"experts", experts}, {"gates", gates}})
+    TORCH_CHECK_VALUE(t.device() == x.device(), name, " must live on ", x.device());
+  const int64_t n = w_in.size(0), tokens = x.size(0), width = x.size(1), hidden = w_out.size(1), out_width = w_out.size(2), top_k = experts.dim() == 2 ? experts.size(1) : 0;
+  TORCH_CHECK_VALUE(w_out.size(0) == n && router.size(0) == n, "w_in, w_out and router differ in experts");
+  TORCH_CHECK_VALUE(w_in.size(1) == width && router.size(1) == width, "x has ", width, " channels, w_in ", w_in.size(1), ", the router ", router.size(1));
+  a.gated = hidden > 0 && w_in.size(2) == 2 * hidden;
+  TORCH_CHECK_VALUE(a.gated || w_in.size(2) == hidden, "w_in must be as wide as w_out is high, or twice that");
+  TORCH_CHECK_VALUE(out.scalar_type() == x.scalar_type() && out.dim() == 2 && out.size(0) == tokens && out.size(1) == out_width &&
+                        (out.numel() == 0 || out.stride(1) == 1) && (out.numel() == 0 || tokens <= 1 || out.stride(0) >= out_width),
+                    "out must be ", tokens, " x ", out_width, " values of the rows' type, a row's side by side");
+  TORCH_CHECK_VALUE(experts.scalar_type() == at::kInt && experts.dim() == 2 && experts.size(0) == tokens && experts.is_contiguous(),
+                    "experts must be an int32 tensor of ", tokens, " x top_k");
+  TORCH_CHECK_VALUE(gates.scalar_type() == at::kFloat && gates.sizes() == experts.sizes() && gates.is_contiguous(), "gates must be a float32 tensor of the shape of experts");
+  for (const int64_t v : {n, tokens, width, hidden, out_width}) TORCH_CHECK_VALUE(v <= 0x7fffffff, "more than 2^31 - 1 rows or channels");
+  a.x = ptr(x);
+  a.router = ptr(router);
+  a.w_in = ptr(w_in);
+  a.w_out = ptr(w_out);
+  a.out = ptr(out);
+  a.chosen = static_cast<int32_t*>(ptr(experts));
+  a.gates = static_cast<float*>(ptr(gates));
+  a.x_pitch = pitch(x);
+  a.out_pitch = pitch(out);
+  a.tokens = (int)tokens;
+  a.experts = (int)n;
+  a.top_k = (int)top_k;
+  a.width = (int)width;
+  a.hidden = (int)hidden;
+  a.out_width = (int)out_width;
+  c10::cuda::CUDAGuard guard(x.device());
+  a.workspace_bytes = fgms_b200_expert_layer_workspace_bytes(a.tokens, a.experts, a.top_k, a.hidden, a.out_width);
+  const Tensor ws = a.workspace_bytes > 0 ? at::empty({(int64_t)a.workspace_bytes}, x.options().dtype(at::kByte).requires_grad(false)) : Tensor();
+  a.workspace = space(ws);
+  check_status(fgms_b200_expert_layer(&a, stream_of(x)));
+  for (const Tensor* t : {&out, &experts, &gates}) written(*t);
+}
+
+// ---------------------------------------------------------------------------------------------
 // AdamW over many tensors
 // ---------------------------------------------------------------------------------------------
 int adamw_dtype(const char* name, const Tensor& t) {
@@ -1494,6 +1551,19 @@ PyObject* py_int8_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// (x, router, w_in, w_out, out, experts, gates, activation)
+PyObject* py_expert_layer(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  expect(n, 8);
+  TORCH_CHECK_TYPE(PyUnicode_Check(a[7]), "activation must be a string");
+  const char* activation = PyUnicode_AsUTF8(a[7]);
+  if (!activation) throw python_error();
+  expert_layer(feat_arg(a[0], "x"), feat_arg(a[1], "router"), feat_arg(a[2], "w_in"), feat_arg(a[3], "w_out"), feat_arg(a[4], "out"), feat_arg(a[5], "experts"),
+               feat_arg(a[6], "gates"), activation);
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
 #define FGMS_METHOD(name, fn) {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(fn)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {
     FGMS_METHOD("fusion_fwd", py_fusion_fwd), FGMS_METHOD("seq_fwd", py_seq_fwd),         FGMS_METHOD("bwd", py_bwd),
@@ -1507,6 +1577,7 @@ PyMethodDef methods[] = {
     FGMS_METHOD("rms_norm_int8", py_rms_norm_int8), FGMS_METHOD("quantize_rows_into", py_quantize_rows_into),
     FGMS_METHOD("dropout_into", py_dropout_into), FGMS_METHOD("dropout_bwd", py_dropout_bwd), FGMS_METHOD("dropout", py_dropout),
     FGMS_METHOD("grouped_i8", py_grouped_i8), FGMS_METHOD("int8_linear", py_int8_linear),
+    FGMS_METHOD("expert_layer", py_expert_layer),
     FGMS_METHOD("build_pyramid", py_build_pyramid), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -17,7 +17,7 @@ import torch
 from . import _native, backend
 
 __all__ = ["sparse_conv", "sparse_conv_inference", "SparseConv3d", "SparseUNet", "grouped_linear", "GroupedLinear", "rms_norm", "RMSNorm",
-           "rms_norm_int8", "quantize_rows", "rng_state", "dropout", "Dropout", "int8_linear", "Int8GroupedLinear"]
+           "rms_norm_int8", "quantize_rows", "rng_state", "dropout", "Dropout", "int8_linear", "Int8GroupedLinear", "expert_layer", "ExpertLayer"]
 
 
 def sparse_conv(feats: torch.Tensor, weight: torch.Tensor, kmap, arch80: bool = True) -> torch.Tensor:
@@ -179,6 +179,71 @@ class Dropout(torch.nn.Module):
         if self.training and self.p > 0:
             return dropout(x, self.p, self.rng, residual)
         return x if residual is None else residual + x
+
+
+_FEW_TOKENS, _MOST_EXPERTS, _MOST_CHOSEN = 64, 512, 16  # what backend.fgms_expert_layer_cuda takes
+
+
+def _few_tokens(x, router, w_in, w_out, top_k) -> bool:
+    needs_grad = torch.is_grad_enabled() and any(t.requires_grad for t in (x, router, w_in, w_out))
+    return (not needs_grad and 0 < x.size(0) <= _FEW_TOKENS and router.size(0) <= _MOST_EXPERTS and top_k <= _MOST_CHOSEN
+            and x.dtype in (torch.float16, torch.bfloat16) and x.size(1) % 8 == 0 and w_out.size(1) % 8 == 0 and w_out.size(2) % 8 == 0
+            and all(t.is_contiguous() and t.data_ptr() % 16 == 0 for t in (x, router, w_in, w_out)))
+
+
+def expert_layer(x: torch.Tensor, router: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, top_k: int, activation: str = "silu") -> torch.Tensor:
+    """Each row of ``x`` through the ``top_k`` of its experts that the ``router`` (``[experts, width]``) gives the largest logits, their outputs added up with
+    the softmax over those as weights.  An expert is ``h @ w_out[e]`` with ``h = act(x @ w_in[e])``, or ``act(u[:, :hidden]) * u[:, hidden:]`` where
+    ``w_in`` is twice as wide as ``w_out`` is high; ``activation`` is ``"silu"`` or ``"relu"``.
+
+    Up to 64 rows of float16 or bfloat16 that need no gradient take two launches (:func:`fgms_b200.backend.fgms_expert_layer_cuda`; it chooses by logits in
+    64 bits, the other way by logits in 32).  Otherwise rows are put in the order of their experts and go through :func:`grouped_linear`:
+    differentiable in ``x``, ``router`` (through the weights of the sum), ``w_in`` and ``w_out``."""
+    if activation not in ("silu", "relu"):
+        raise ValueError(f"activation must be 'silu' or 'relu', got {activation!r}")
+    experts, hidden = w_in.size(0), w_out.size(1)
+    if router.dim() != 2 or router.size(0) != experts or w_out.size(0) != experts or not 1 <= top_k <= experts:
+        raise ValueError(f"router, w_in and w_out must have the same experts, and at least top_k = {top_k} of them")
+    if w_in.size(2) not in (hidden, 2 * hidden):
+        raise ValueError("w_in must be as wide as w_out is high, or twice that")
+    rows = x.reshape(-1, x.size(-1))
+    if _few_tokens(rows, router, w_in, w_out, top_k):
+        out = torch.empty((rows.size(0), w_out.size(2)), dtype=x.dtype, device=x.device)
+        chosen = torch.empty((rows.size(0), top_k), dtype=torch.int32, device=x.device)
+        with torch.no_grad():
+            backend.fgms_expert_layer_cuda(rows, router, w_in, w_out, out, chosen, torch.empty(chosen.shape, device=x.device), activation)
+        return out.view(*x.shape[:-1], w_out.size(2))
+    logits = rows.float() @ router.float().T
+    value, chosen = (t[:, :top_k] for t in torch.sort(logits, dim=1, descending=True, stable=True))
+    gate = torch.softmax(value, 1)
+    ids = chosen.reshape(-1)
+    order = ids.argsort(stable=True)
+    kpos = torch.searchsorted(ids[order], torch.arange(experts + 1, device=x.device), out_int32=True)
+    u = grouped_linear(rows[order // top_k], w_in, kpos)
+    act = torch.nn.functional.silu if activation == "silu" else torch.relu
+    h = act(u[:, :hidden]) * u[:, hidden:] if u.size(1) == 2 * hidden and hidden else act(u)
+    y = grouped_linear(h, w_out, kpos)
+    back = torch.empty_like(order).scatter_(0, order, torch.arange(order.numel(), device=x.device))
+    out = (y[back].float().view(rows.size(0), top_k, -1) * gate[:, :, None]).sum(1)
+    return out.to(x.dtype).view(*x.shape[:-1], w_out.size(2))
+
+
+class ExpertLayer(torch.nn.Module):
+    """A layer of ``experts`` experts of ``hidden`` channels, of which every row takes ``top_k``: :func:`expert_layer` with its weights, initialised
+    like ``torch.nn.Linear``.  ``gated``: ``w_in`` is twice as wide, ``act(first half) * second half``."""
+
+    def __init__(self, width: int, hidden: int, experts: int, top_k: int, gated: bool = True, activation: str = "silu", dtype=torch.bfloat16, device="cuda"):
+        super().__init__()
+        if not 1 <= top_k <= experts:
+            raise ValueError(f"top_k must be in [1, {experts}], got {top_k}")
+        self.top_k, self.activation = top_k, activation
+        made = lambda fan_in, *shape: torch.nn.Parameter(((torch.rand(shape, device=device) * 2 - 1) / math.sqrt(fan_in)).to(dtype))
+        self.router = made(width, experts, width)
+        self.w_in = made(width, experts, width, (2 if gated else 1) * hidden)
+        self.w_out = made(hidden, experts, hidden, width)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return expert_layer(x, self.router, self.w_in, self.w_out, self.top_k, self.activation)
 
 
 _LAYER_FORWARD = SparseConv3d.forward

@@ -435,6 +435,39 @@ size_t fgms_b200_grouped_i8_workspace_bytes(const int8_t* codes, int64_t codes_p
                                             int n_rows, int c_in, int c_out, int groups);
 
 /* ---------------------------------------------------------------------------------------------
+ * A whole layer of experts for up to 64 tokens (serving), in two launches:
+ *
+ *     logit[t, e] = x[t] . router[e]        chosen[t, 0 .. top_k - 1]: the largest, descending; of equal ones the lower index first
+ *     gates[t, j] = softmax over the chosen logits
+ *     u = x[t] * w_in[e]      h = activation(u), or gated: activation(u[: hidden]) * u[hidden :]
+ *     out[t] = sum over j of gates[t, j] * (h * w_out[chosen[t, j]])
+ *
+ * x [tokens, width], router [experts, width], w_in [experts, width, hidden] (gated: 2 hidden), w_out [experts, hidden, out_width]; F16 or BF16, the
+ * router of that type or F32.  Logits are summed in 64 bits, products in fp32, each token's sum over its experts in fp32 in their order; h is
+ * rounded to the type once (its magnitude has to be one that the type holds).  The same bits on every run.  Widths are multiples of 8, rows and weights start
+ * on 16-byte boundaries; experts at most 512, top_k at most 16.  A logit that is NaN counts as the lowest; a token with none that is more gets gates of NaN.
+ * out may be x itself.  The second launch is cooperative, a CTA an SM that is not kept free; its waits are bounded (fgms_b200_device_status).
+ * workspace: fgms_b200_expert_layer_workspace_bytes on the current device, 256-byte aligned, whose contents do not matter. */
+#define FGMS_ACTIVATION_RELU 0
+#define FGMS_ACTIVATION_SILU 1
+typedef struct {
+  const void* x;
+  const void* router;
+  const void* w_in;
+  const void* w_out;
+  void* out;
+  int32_t* chosen; /* [tokens, top_k] */
+  float* gates;    /* [tokens, top_k] */
+  int64_t x_pitch, out_pitch;
+  void* workspace;
+  size_t workspace_bytes;
+  int tokens, experts, top_k, width, hidden, out_width, gated, activation, dtype, router_dtype;
+} fgms_b200_expert_layer_args;
+
+size_t fgms_b200_expert_layer_workspace_bytes(int tokens, int experts, int top_k, int hidden, int out_width);
+int fgms_b200_expert_layer(const fgms_b200_expert_layer_args* args, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
  * Multi-GPU: sum of the ranks' fp32 weight-gradient partial sums over peer memory.  No counterpart in the
  * reference (it has no multi-GPU path); it stands where a data-parallel caller would otherwise issue an
  * all-reduce of the [k_vol, c_in, c_out] fp32 sums that fgms_b200_wgrad leaves in its workspace.

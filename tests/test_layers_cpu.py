@@ -150,3 +150,35 @@ def test_products_in_8_bits_say_what_they_copy():
     assert product(codes=P + 1) == _lib.ERR_WORKSPACE and product(codes=P + 1, ws=7 * P, ws_bytes=255) == _lib.ERR_WORKSPACE
     assert product(codes=P + 1, ws=7 * P + 16, ws_bytes=512) == _lib.ERR_WORKSPACE and product(codes=P + 1, ws=5 * P, ws_bytes=512) == _lib.ERR_WORKSPACE
     assert product(rows=0, codes=None, out=None, scale=None) == _lib.OK
+
+
+def experts(**change):
+    a = _lib.ExpertLayerArgs(x=P, router=2 * P, w_in=3 * P, w_out=4 * P, out=5 * P, chosen=6 * P, gates=7 * P, x_pitch=64, out_pitch=64, tokens=4, experts=8, top_k=2,
+                             width=64, hidden=32, out_width=64, gated=1, activation=1, dtype=_lib.DTYPE_BF16, router_dtype=_lib.DTYPE_BF16)
+    for k, v in change.items():
+        setattr(a, k, v)
+    return L.fgms_b200_expert_layer(ctypes.byref(a), None)
+
+
+@pytest.mark.parametrize("change,text", [
+    (dict(tokens=-1), "tokens -1"), (dict(tokens=65), "tokens 65"), (dict(experts=0), "experts 0"), (dict(experts=513), "experts 513"), (dict(top_k=0), "top_k 0"),
+    (dict(top_k=9), "top_k 9"), (dict(top_k=17, experts=64), "top_k 17"), (dict(width=60), "multiples of 8"), (dict(hidden=0), "multiples of 8"),
+    (dict(out_width=2 ** 20 + 8), "multiples of 8"), (dict(width=2 ** 20, hidden=2 ** 20, experts=512, x_pitch=2 ** 20), "too large"), (dict(activation=2), "activation"),
+    (dict(x=None), "x: null"), (dict(router=None), "router: null"), (dict(w_in=None), "w_in: null"), (dict(w_out=None), "w_out: null"), (dict(out=None), "out: null"),
+    (dict(chosen=None), "chosen: null"), (dict(gates=None), "gates: null"), (dict(x=P + 2), "16-byte"), (dict(x_pitch=68), "16-byte"), (dict(w_in=3 * P + 8), "16-byte"),
+    (dict(out=5 * P + 1), "boundary"), (dict(chosen=6 * P + 2), "boundary"), (dict(x_pitch=56), "apart"), (dict(out=P + 64), "overlaps"), (dict(out=2 * P), "overlaps"),
+    (dict(out=4 * P + 2), "overlaps"), (dict(chosen=P), "overlaps"), (dict(gates=6 * P + 16), "two outputs"), (dict(chosen=5 * P + 4), "two outputs"),
+])
+def test_a_layer_of_experts_refuses(change, text):
+    assert experts(**change) == _lib.ERR_INVALID_ARG and text in _lib.last_error(), _lib.last_error()
+
+
+def test_a_layer_of_experts_refuses_what_it_is_not_built_for():
+    assert experts(dtype=_lib.DTYPE_F32, router_dtype=_lib.DTYPE_F32) == _lib.ERR_UNSUPPORTED
+    assert experts(router_dtype=_lib.DTYPE_F16) == _lib.ERR_UNSUPPORTED and "router" in _lib.last_error()
+    assert L.fgms_b200_expert_layer(None, None) == _lib.ERR_INVALID_ARG
+    assert experts(tokens=0, x=None, out=None, chosen=None, gates=None) == _lib.OK
+    size = L.fgms_b200_expert_layer_workspace_bytes
+    assert size(0, 8, 2, 32, 64) == 0 and size(65, 8, 2, 32, 64) == 0 and size(4, 513, 2, 32, 64) == 0 and size(4, 8, 17, 32, 64) == 0
+    with pytest.raises(ValueError, match="top_k"):
+        nn.ExpertLayer(8, 8, 4, 5, device="cpu")
