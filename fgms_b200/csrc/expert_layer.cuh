@@ -8,16 +8,19 @@
 // expert_logits_kernel has a block for an expert and eight tokens.  A choice hangs on the difference of two logits, so they are summed in 64 bits; every
 // expert's in the same order, so that equal rows of the router are equal.
 //
-// expert_layer_kernel is cooperative, a CTA an SM.  What bounds it is the weights of the experts that some token goes to, each read once: a tile of a weight
-// is 64 of the contraction by 128 columns (a TMA copy for each 64 of them, a ring of tiles ahead), and the tiles of all experts, column blocks and
-// contractions are one list, cut into as many equal shares as there are CTAs.  A share may start and end inside a column block: whoever has the
-// block's first tile adds what the others hand over, in their order, so that the sums are the same bits on every run.  The products are
-// mma.sync.m16n8k16 with the columns of the weight as M and an expert's tokens as N, eight a step (rows that are no token are computed and thrown
-// away): beside 16 KB from memory, 0.35 us of an SM's share, eight steps for each of up to eight such groups are nothing.
+// expert_layer_kernel is cooperative, a CTA an SM.  What bounds it is the weights of the experts that some token goes to, each read once.  An item
+// is 64 columns of one expert's weight (gated: 32 of either half of u) with the whole contraction, in tiles of 128 rows that come by TMA, a
+// ring of them ahead; items go around the CTAs, first those of W_in, then those of W_out, so that neighbours read neighbouring columns at about the same time.  No sum
+// crosses CTAs, and the same bits come out on every run: contractions that were shared by CTAs cost 5 us a product in handing sums over, and a barrier of all
+// CTAs between the products as much again.  Instead an item of W_out waits for the items of its expert alone, and whoever finishes a
+// column block of the output last adds up what the token's experts left there.  The products are mma.sync.m16n8k16 with the columns of the weight as M and an
+// expert's tokens as N, eight a step (rows that are no token are computed and thrown away).
 //
-//   warps 0-7   tokens' rows (cp.async, three tiles ahead), products, activation          warp 8   TMA producer
+//   warps 0-7   products: 16 rows of every tile each; their sums meet in shared memory at the end of an item
+//   warp 8      TMA producer of weights          warp 9   producer of the tokens' rows: a bulk copy a row and tile
+//   warps 10-11 report finished items and add the output up: a report waits until all that was stored is there, a microsecond that the products go on in
 //
-// The producer goes on to W_out while the others wait for the last h: what a grid barrier costs, the ring has bridged.  All waits are bounded.
+// All waits are bounded.
 #pragma once
 #include "grouped_umma.cuh"
 #include "row_values.cuh"
@@ -26,14 +29,14 @@ namespace fgms {
 
 constexpr int EL_MAX_TOKENS = 64, EL_MAX_TOP_K = 16, EL_MAX_EXPERTS = 512;
 constexpr int EL_MAX_PAIRS = EL_MAX_TOKENS * EL_MAX_TOP_K;
-constexpr int EL_K = 64;                           // contraction of a tile
-constexpr int EL_TILE_BYTES = EL_K * 128 * 2;      // two blocks of 64 columns
+constexpr int EL_K = 128, EL_COLUMNS = 64;         // a tile
+constexpr int EL_TILE_BYTES = EL_K * EL_COLUMNS * 2;
 constexpr int EL_MAX_STAGES = 12;
-constexpr int EL_X_STAGES = 4;                     // tokens' rows: 64 values each
-constexpr int EL_X_BYTES = EL_MAX_TOKENS * EL_K * 2;
-constexpr int EL_CONSUMERS = 256, EL_THREADS = EL_CONSUMERS + 32;
-constexpr int EL_SLOT = EL_CONSUMERS * 32;         // fp32 sums that a CTA may hand over
-constexpr int EL_ROUTER_THREADS = 128, EL_ROUTER_TOKENS = 8;
+constexpr int EL_X_PITCH = EL_K * 2 + 16;          // tokens' rows, 16 bytes more apart than they are long so that eight of them lie in all banks
+constexpr int EL_X_BYTES = 3 * EL_MAX_TOKENS * EL_X_PITCH;  // three tiles of 64 rows, or as many more as fewer rows allow: a copy's way is as long as three tiles
+constexpr int EL_CONSUMERS = 256, EL_REPORTERS = 64, EL_THREADS = EL_CONSUMERS + 64 + EL_REPORTERS, EL_WARPS = EL_THREADS / 32;
+constexpr int EL_SUMS = 16;                        // of a thread for eight tokens: 64 columns by eight a warp
+constexpr int EL_ROUTER_THREADS = 256, EL_ROUTER_TOKENS = 8;
 
 struct ExpertParams {
   const void *x, *router;
@@ -44,12 +47,10 @@ struct ExpertParams {
   long long x_pitch, out_pitch;
   // workspace
   double* logits;    // [tokens][n_experts]
-  uint32_t* flags;   // [2][ctas], a share's sums are there; then [3], CTAs that have arrived at a barrier
-  float* slots;      // [ctas][EL_SLOT]
+  uint32_t* flags;   // [experts]: items of W_in that are done, by used expert; [blocks of the output]: items of W_out; then CTAs at the barrier
   uint16_t* h;       // [tokens top_k][hidden], in the order of the experts
   float* part;       // [tokens top_k][out_width]
-  int ctas, stages, bf16;
-  bool x_vec;
+  int ctas, stages, n_flags;
   int alone;
 };
 
@@ -59,7 +60,7 @@ __global__ void __launch_bounds__(EL_ROUTER_THREADS) expert_logits_kernel(const 
   umma::griddep_wait();
   if (!p.alone) umma::griddep_launch_dependents();
   if (blockIdx.x == 0 && blockIdx.y == 0)
-    for (int i = threadIdx.x; i < 2 * p.ctas + 3; i += EL_ROUTER_THREADS) p.flags[i] = 0u;
+    for (int i = threadIdx.x; i < p.n_flags; i += EL_ROUTER_THREADS) p.flags[i] = 0u;
   const int e = (int)blockIdx.x, t0 = (int)blockIdx.y * EL_ROUTER_TOKENS, n = min(EL_ROUTER_TOKENS, p.tokens - t0);
   double sum[EL_ROUTER_TOKENS];
 #pragma unroll
@@ -67,15 +68,17 @@ __global__ void __launch_bounds__(EL_ROUTER_THREADS) expert_logits_kernel(const 
   const R* row = static_cast<const R*>(p.router) + (size_t)e * p.width;
   for (int col = (int)threadIdx.x * ROW_CHUNK; col < p.width; col += EL_ROUTER_THREADS * ROW_CHUNK) {  // the width is a multiple of a chunk
     const RowRaw<R> w = row_load(row + col, ROW_CHUNK, true);
+    RowRaw<T> x[EL_ROUTER_TOKENS];  // all on their way together; rows behind the last token's are that one's again
+#pragma unroll
+    for (int t = 0; t < EL_ROUTER_TOKENS; ++t) x[t] = row_load(static_cast<const T*>(p.x) + (t0 + min(t, n - 1)) * p.x_pitch + col, ROW_CHUNK, true);
     double wd[ROW_CHUNK];
 #pragma unroll
     for (int i = 0; i < ROW_CHUNK; ++i) wd[i] = (double)row_value(w, i);
 #pragma unroll
     for (int t = 0; t < EL_ROUTER_TOKENS; ++t) {
       if (t >= n) break;
-      const RowRaw<T> x = row_load(static_cast<const T*>(p.x) + (t0 + t) * p.x_pitch + col, ROW_CHUNK, p.x_vec);
 #pragma unroll
-      for (int i = 0; i < ROW_CHUNK; ++i) sum[t] += (double)row_value(x, i) * wd[i];
+      for (int i = 0; i < ROW_CHUNK; ++i) sum[t] += (double)row_value(x[t], i) * wd[i];
     }
   }
 #pragma unroll
@@ -95,43 +98,42 @@ __global__ void __launch_bounds__(EL_ROUTER_THREADS) expert_logits_kernel(const 
 }
 
 struct ElShared {
-  uint64_t full[EL_MAX_STAGES], empty[EL_MAX_STAGES];
-  int abort_flag, used;
+  uint64_t full[EL_MAX_STAGES], empty[EL_MAX_STAGES], x_full[EL_MAX_STAGES], x_empty[EL_MAX_STAGES], finished[2], reported[2];
+  unsigned long long tokens[EL_MAX_EXPERTS];  // of an expert: a bit for each of its tokens
+  int abort_flag, used, most, last;  // most: tokens of an expert
+  int group_pairs[EL_MAX_EXPERTS / 32], group_used[EL_MAX_EXPERTS / 32];
   float gates[EL_MAX_PAIRS];
-  uint16_t chosen[EL_MAX_PAIRS], list[EL_MAX_PAIRS];        // pairs: token * top_k + j; list: in the order of their experts
-  uint16_t count[EL_MAX_EXPERTS], place[EL_MAX_EXPERTS];    // of an expert: pairs, and the next one's place in the list
+  uint16_t chosen[EL_MAX_PAIRS], list[EL_MAX_PAIRS];           // pairs: token * top_k + j; list: in the order of their experts
+  uint16_t place[EL_MAX_EXPERTS];                              // of an expert: its first pair's place in the list
   uint16_t expert[EL_MAX_EXPERTS], first[EL_MAX_EXPERTS + 1];  // of those that are used: which, and the first pair's place
 };
 
-// A share of the list of tiles: tile `at` is contraction step kb of column block m of the used expert u.
-struct ElWalk {
-  int at, end, u, m, kb, steps, blocks;
-  __device__ __forceinline__ ElWalk(int from, int to, int blocks_, int steps_) : at(from), end(to), steps(steps_), blocks(blocks_) {
-    const int block = from / steps;
-    kb = from - block * steps;
-    u = block / blocks;
-    m = block - u * blocks;
+// This CTA's items of a product: item i is column block i % blocks of the used expert i / blocks, and the i + skip-th of all go around the CTAs.
+struct ElItems {
+  int at, total, ctas, blocks;
+  __device__ __forceinline__ ElItems(int total_, int skip, int cta, int ctas_, int blocks_) : total(total_), ctas(ctas_), blocks(blocks_) {
+    at = cta - skip % ctas;
+    if (at < 0) at += ctas;
   }
-  __device__ __forceinline__ bool left() const { return at < end; }
-  __device__ __forceinline__ void next() {
-    ++at;
-    if (++kb == steps) {
-      kb = 0;
-      if (++m == blocks) {
-        m = 0;
-        ++u;
-      }
-    }
-  }
+  __device__ __forceinline__ bool left() const { return at < total; }
+  __device__ __forceinline__ void next() { at += ctas; }
+  __device__ __forceinline__ int expert() const { return at / blocks; }
+  __device__ __forceinline__ int block() const { return at % blocks; }
 };
-__device__ __forceinline__ int el_share(int total, int cta, int ctas) { return (int)((long long)total * cta / ctas); }
 
+__device__ __forceinline__ void el_sync_reporters() { asm volatile("barrier.cta.sync 2, %0;" ::"n"(EL_REPORTERS) : "memory"); }
 __device__ __forceinline__ void el_sync() { asm volatile("barrier.cta.sync 1, %0;" ::"n"(EL_CONSUMERS) : "memory"); }
 __device__ __forceinline__ uint32_t el_acquire(const uint32_t* at) {
   uint32_t v;
   asm volatile("ld.acquire.gpu.global.b32 %0, [%1];" : "=r"(v) : "l"(at) : "memory");
   return v;
 }
+__device__ __forceinline__ uint32_t el_count(uint32_t* at) {
+  uint32_t before;
+  asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(before) : "l"(at) : "memory");
+  return before;
+}
+__device__ __forceinline__ void el_arrive(uint32_t* at) { asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(at) : "memory"); }
 // until *at is `want` at least
 __device__ __forceinline__ bool el_await(const uint32_t* at, uint32_t want, volatile int* abort_flag) {
   const long long start = clock64();
@@ -148,10 +150,8 @@ __device__ __forceinline__ bool el_await(const uint32_t* at, uint32_t want, vola
 __device__ __forceinline__ void el_grid_sync(uint32_t* counter, int ctas, volatile int* abort_flag) {
   el_sync();
   if (threadIdx.x == 0) {
-    __threadfence();
-    atomicAdd(counter, 1u);
+    el_arrive(counter);
     el_await(counter, (uint32_t)ctas, abort_flag);
-    __threadfence();
   }
   el_sync();
 }
@@ -179,64 +179,64 @@ __device__ __forceinline__ uint16_t el_round(float v) {
 
 // The top_k largest logits of a token, by a warp: (*expert, *gate) of lane j are the j-th one's.  A logit that is not a number counts as minus infinity (and
 // makes the gates such).
+template <int EACH>
 __device__ __forceinline__ void el_choose(const ExpertParams& p, int t, int* expert, float* gate) {
   const int lane = threadIdx.x & 31;
-  constexpr int EACH = EL_MAX_EXPERTS / 32;
-  const double lowest = __longlong_as_double((long long)0xfff0000000000000ull);
-  double v[EACH];
+  // as numbers without a sign that are ordered alike; 0 is what has been taken
+  unsigned long long v[EACH];
 #pragma unroll
   for (int i = 0; i < EACH; ++i) {
-    v[i] = lowest;
+    v[i] = 0;
     if (lane + 32 * i < p.n_experts) {
-      v[i] = __ldcg(p.logits + (size_t)t * p.n_experts + lane + 32 * i);
-      if (!(v[i] >= lowest)) v[i] = lowest;
+      const double x = __ldcg(p.logits + (size_t)t * p.n_experts + lane + 32 * i) + 0.0;  // no minus zero
+      const unsigned long long bits = (unsigned long long)__double_as_longlong(x);
+      v[i] = x != x ? 0x000fffffffffffffull : bits >> 63 ? ~bits : bits | 0x8000000000000000ull;  // minus infinity is 0x000f...f
     }
   }
-  uint32_t taken = 0;
   double top = 0.0;
   float mine = 0.f, total = 0.f;
   for (int j = 0; j < p.top_k; ++j) {
-    double best = lowest;
-    int at = 0x7fffffff;
+    unsigned long long best = v[0];
 #pragma unroll
-    for (int i = 0; i < EACH; ++i) {
+    for (int i = 1; i < EACH; ++i) {
       if (32 * i >= p.n_experts) break;
-      const int e = lane + 32 * i;
-      if (e < p.n_experts && !(taken >> i & 1u) && (v[i] > best || (v[i] == best && e < at))) {
-        best = v[i];
-        at = e;
-      }
+      best = max(best, v[i]);
     }
+    // the largest of the warp's, half by half
+    const uint32_t high = __reduce_max_sync(0xffffffffu, (uint32_t)(best >> 32));
+    const uint32_t low = __reduce_max_sync(0xffffffffu, (uint32_t)(best >> 32) == high ? (uint32_t)best : 0u);
+    best = (unsigned long long)high << 32 | low;
+    uint32_t at = 0xffffffffu;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const double other = __shfl_xor_sync(0xffffffffu, best, o);
-      const int where = __shfl_xor_sync(0xffffffffu, at, o);
-      if (other > best || (other == best && where < at)) {
-        best = other;
-        at = where;
-      }
-    }
-    if ((at & 31) == lane) taken |= 1u << (at >> 5);
-    if (j == 0) top = best;
-    const float share = expf((float)(best - top));
+    for (int i = EACH - 1; i >= 0; --i)
+      if (32 * i < p.n_experts && v[i] == best && lane + 32 * i < p.n_experts) at = (uint32_t)(lane + 32 * i);
+    at = __reduce_min_sync(0xffffffffu, at);
+#pragma unroll
+    for (int i = 0; i < EACH; ++i)
+      if (at == (uint32_t)(lane + 32 * i)) v[i] = 0;
+    const double value = __longlong_as_double((long long)(best >> 63 ? best & 0x7fffffffffffffffull : ~best));
+    if (j == 0) top = value;
+    const float share = expf((float)(value - top));
     total += share;
     if (lane == j) {
       mine = share;
-      *expert = at;
+      *expert = (int)at;
     }
   }
   *gate = mine / total;
 }
+// (few values a lane where there are few experts: code that is not there need not be fetched)
 // Of all tokens, in every CTA.  Up to EL_CHOOSE_ALONE tokens each CTA does it for itself, two rounds of its warps at most; more are dealt out, a token
 // a CTA, and met at a grid barrier, which costs as much as two or three rounds.
-constexpr int EL_CHOOSE_ALONE = 2 * EL_THREADS / 32;
+constexpr int EL_CHOOSE_ALONE = 2 * EL_WARPS;
 __device__ __forceinline__ void el_choose_all(const ExpertParams& p, ElShared* sh) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, cta = (int)blockIdx.x;
   const bool alone = p.tokens <= EL_CHOOSE_ALONE;
-  for (int t = alone ? warp : cta; t < p.tokens && (alone || warp == 0); t += alone ? EL_THREADS / 32 : p.ctas) {
+  for (int t = alone ? warp : cta; t < p.tokens && (alone || warp == 0); t += alone ? EL_WARPS : p.ctas) {
     int expert = 0;
     float gate = 0.f;
-    el_choose(p, t, &expert, &gate);
+    if (p.n_experts <= 64) el_choose<2>(p, t, &expert, &gate);
+    else el_choose<EL_MAX_EXPERTS / 32>(p, t, &expert, &gate);
     if (lane >= p.top_k) continue;
     const int pair = t * p.top_k + lane;
     sh->chosen[pair] = (uint16_t)expert;
@@ -248,7 +248,7 @@ __device__ __forceinline__ void el_choose_all(const ExpertParams& p, ElShared* s
   }
   if (!alone) {
     if (warp < EL_CONSUMERS / 32) {
-      el_grid_sync(p.flags + 2 * p.ctas + 2, p.ctas, &sh->abort_flag);
+      el_grid_sync(p.flags + p.n_flags - 1, p.ctas, &sh->abort_flag);
       for (int i = threadIdx.x; i < p.tokens * p.top_k; i += EL_CONSUMERS) {
         // (a value that no CTA has written, after a wait that ran out, is no expert)
         sh->chosen[i] = (uint16_t)min(max(__ldcg(p.experts + i), 0), p.n_experts - 1);
@@ -259,53 +259,227 @@ __device__ __forceinline__ void el_choose_all(const ExpertParams& p, ElShared* s
   __syncthreads();
 }
 
-// The pairs in the order of their experts (of an expert: of the tokens), by one warp.
+// The pairs in the order of their experts, of an expert in the order of its tokens: a token goes to an expert once at most, so that an expert's
+// pairs are a set of tokens, 64 bits.
 __device__ __forceinline__ void el_sort(const ExpertParams& p, ElShared* sh) {
-  const int lane = threadIdx.x & 31, pairs = p.tokens * p.top_k;
-  for (int e = lane; e < p.n_experts; e += 32) sh->count[e] = 0;
-  __syncwarp();
-  for (int i0 = 0; i0 < pairs; i0 += 32) {
-    const int e = i0 + lane < pairs ? (int)sh->chosen[i0 + lane] : 0x10000 + lane;  // no pair: equal to none
-    const uint32_t peers = __match_any_sync(0xffffffffu, e);
-    if (i0 + lane < pairs && (peers >> lane) == 1u) sh->count[e] += (uint16_t)__popc(peers);  // the last of its expert
-    __syncwarp();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, pairs = p.tokens * p.top_k, groups = (p.n_experts + 31) / 32;
+  if (pairs <= 32) {  // a lane a pair, each counts the ones before it
+    if (warp == 0) {
+      const int e = lane < pairs ? (int)sh->chosen[lane] : 0x10000;
+      const uint32_t peers = __match_any_sync(0xffffffffu, e);  // all lanes take part
+      const bool head = lane < pairs && (peers & ((1u << lane) - 1u)) == 0u;
+      const int key = e << 1 | (head ? 1 : 0);
+      int place = 0, used = 0;
+#pragma unroll 8
+      for (int i = 0; i < 32; ++i) {
+        const int other = __shfl_sync(0xffffffffu, key, i);
+        place += (other >> 1) < e || ((other >> 1) == e && i < lane);
+        used += (other >> 1) < e && (other & 1);
+      }
+      if (lane < pairs) sh->list[place] = (uint16_t)lane;
+      if (head) {
+        sh->expert[used] = (uint16_t)e;
+        sh->first[used] = (uint16_t)place;
+      }
+      const int all = __popc(__ballot_sync(0xffffffffu, head)), most = (int)__reduce_max_sync(0xffffffffu, lane < pairs ? (uint32_t)__popc(peers) : 0u);
+      if (lane == 0) {
+        sh->most = most;
+        sh->used = all;
+        sh->first[all] = (uint16_t)pairs;
+      }
+    }
+    __syncthreads();
+    return;
   }
-  int used = 0, first = 0;
-  for (int e0 = 0; e0 < p.n_experts; e0 += 32) {
-    const int n = e0 + lane < p.n_experts ? (int)sh->count[e0 + lane] : 0;
-    const uint32_t some = __ballot_sync(0xffffffffu, n > 0);
-    int before = n;
+  for (int e = threadIdx.x; e < p.n_experts; e += EL_THREADS) sh->tokens[e] = 0ull;
+  if (threadIdx.x == 0) sh->most = 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i < pairs; i += EL_THREADS) atomicOr(&sh->tokens[sh->chosen[i]], 1ull << (i / p.top_k));
+  __syncthreads();
+  constexpr int ROUNDS = (EL_MAX_EXPERTS / 32 + EL_WARPS - 1) / EL_WARPS;
+  int n[ROUNDS], before[ROUNDS];
+  uint32_t some[ROUNDS];
+#pragma unroll
+  for (int r = 0; r < ROUNDS; ++r) {
+    const int group = warp + r * EL_WARPS, e = group * 32 + lane;
+    if (group >= groups) break;
+    n[r] = e < p.n_experts ? __popcll(sh->tokens[e]) : 0;
+    some[r] = __ballot_sync(0xffffffffu, n[r] > 0);
+    before[r] = n[r];
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, before, o);
-      if (lane >= o) before += v;
+      const int v = __shfl_up_sync(0xffffffffu, before[r], o);
+      if (lane >= o) before[r] += v;
     }
-    const int place = first + before - n;
-    if (n > 0) {
-      const int u = used + __popc(some & ((1u << lane) - 1u));
-      sh->expert[u] = (uint16_t)(e0 + lane);
-      sh->first[u] = (uint16_t)place;
-      sh->place[e0 + lane] = (uint16_t)place;
+    const uint32_t most = __reduce_max_sync(0xffffffffu, (uint32_t)n[r]);
+    if (lane == 31) {
+      atomicMax(&sh->most, (int)most);
+      sh->group_pairs[group] = before[r];
+      sh->group_used[group] = __popc(some[r]);
     }
-    used += __popc(some);
-    first += __shfl_sync(0xffffffffu, before, 31);
   }
-  if (lane == 0) {
-    sh->used = used;
-    sh->first[used] = (uint16_t)pairs;
-  }
-  __syncwarp();
-  for (int i0 = 0; i0 < pairs; i0 += 32) {
-    const int e = i0 + lane < pairs ? (int)sh->chosen[i0 + lane] : 0x10000 + lane;
-    const uint32_t peers = __match_any_sync(0xffffffffu, e);
-    int place = 0;
-    if (i0 + lane < pairs) {
-      place = (int)sh->place[e] + __popc(peers & ((1u << lane) - 1u));
-      sh->list[place] = (uint16_t)(i0 + lane);
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < ROUNDS; ++r) {
+    const int group = warp + r * EL_WARPS, e = group * 32 + lane;
+    if (group >= groups) break;
+    int first = before[r] - n[r], used = __popc(some[r] & ((1u << lane) - 1u));
+    for (int i = 0; i < group; ++i) {
+      first += sh->group_pairs[i];
+      used += sh->group_used[i];
     }
-    __syncwarp();
-    if (i0 + lane < pairs && (peers >> lane) == 1u) sh->place[e] = (uint16_t)(place + 1);
-    __syncwarp();
+    if (n[r] > 0) {
+      sh->expert[used] = (uint16_t)e;
+      sh->first[used] = (uint16_t)first;
+      sh->place[e] = (uint16_t)first;
+    }
+    if (group == groups - 1 && lane == 31) {
+      used += some[r] >> 31;
+      sh->used = used;
+      sh->first[used] = (uint16_t)pairs;
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < pairs; i += EL_THREADS) {
+    const int e = sh->chosen[i], t = i / p.top_k;
+    sh->list[sh->place[e] + __popcll(sh->tokens[e] & ((1ull << t) - 1ull))] = (uint16_t)i;
+  }
+  __syncthreads();
+}
+
+// `bytes` of global memory to shared memory, both from 16-byte boundaries and a multiple of 16; reported to `bar`
+__device__ __forceinline__ void el_bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+
+// What every role goes by: the items, and the ring of the tokens' rows.
+struct ElPlan {
+  int used, ctas, blocks_in, blocks_out, x_bytes, x_stages;
+  __device__ __forceinline__ ElPlan(const ExpertParams& p, const ElShared* sh) {
+    const int h_columns = p.gated ? EL_COLUMNS / 2 : EL_COLUMNS;  // that an item of W_in stands for
+    used = sh->used;
+    ctas = p.ctas;
+    blocks_in = (p.hidden + h_columns - 1) / h_columns;
+    blocks_out = (p.out_width + EL_COLUMNS - 1) / EL_COLUMNS;
+    x_bytes = sh->most * EL_X_PITCH;
+    x_stages = min(EL_MAX_STAGES, EL_X_BYTES / x_bytes);
+  }
+  __device__ __forceinline__ ElItems items(int product) const {
+    return product == 0 ? ElItems(used * blocks_in, 0, (int)blockIdx.x, ctas, blocks_in) : ElItems(used * blocks_out, used * blocks_in, (int)blockIdx.x, ctas, blocks_out);
+  }
+};
+
+// ---------------------------------------------------------------------------------------------
+// The products, by warps 0-7.  NT: groups of eight tokens that an expert may have.
+// ---------------------------------------------------------------------------------------------
+template <bool BF16, int NT>
+__device__ __forceinline__ void el_products(const ExpertParams& p, ElShared* sh, uint32_t tiles0, uint32_t x0, float* sums) {
+  using namespace umma;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  volatile int* abort_flag = &sh->abort_flag;
+  const ElPlan plan(p, sh);
+  bool ok = true;
+  const int g = lane >> 2, c = lane & 3;  // of a fragment: column of the weight; pair of tokens
+  const int matrix = lane >> 3, row = lane & 7;
+  // this lane's row of the tokens' four 8 x 8 matrices: eight tokens by two of eight of the contraction, and eight tokens more
+  const uint32_t rows = x0 + (uint32_t)(((matrix >> 1) * 8 + row) * EL_X_PITCH + warp * 32 + (matrix & 1) * 16);
+  int s = 0, x_at = 0;
+  uint32_t ph = 0, x_ph = 0, count = 0;
+  float acc[NT][4][4];
+#pragma unroll
+  for (int j = 0; j < NT; ++j)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[j][i >> 2][i & 3] = 0.f;
+  for (int product = 0; product < 2; ++product) {
+    const bool gated = product == 0 && p.gated;
+    const int length = product == 0 ? p.width : p.hidden, columns = product == 0 ? p.hidden : p.out_width;
+    // And of the weight's: two groups of eight columns (side by side, or one of each half of u) by two of eight of the contraction.  Gated, a half has rows of
+    // 64 bytes, whose 16-byte chunks are permuted by row / 2 % 4; otherwise rows are 128 bytes and permuted by row % 8.
+    const int r = warp * 16 + (matrix >> 1) * 8 + row;
+    const uint32_t weights = tiles0 + (uint32_t)(gated ? (matrix & 1) * (EL_TILE_BYTES / 2) + r * 64 : r * 128);
+    uint32_t chunk[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) chunk[q] = (uint32_t)((gated ? q ^ (row >> 1) : (2 * q + (matrix & 1)) ^ row) * 16);
+    for (ElItems w = plan.items(product); w.left(); w.next()) {
+      const int u = w.expert(), m = w.block(), first = sh->first[u], n = sh->first[u + 1] - first;
+      for (int k = 0; k < length; k += EL_K) {
+        if (ok) ok = mbar_parked_wait(smem_u32(&sh->x_full[x_at]), x_ph, abort_flag) && mbar_parked_wait(smem_u32(&sh->full[s]), ph, abort_flag);
+        __syncwarp();
+        const int there = (length - k - warp * 16) / 8;  // of this warp's rows: groups of eight that there are
+        if (there > 0) {
+          const uint32_t tile = weights + (uint32_t)(s * EL_TILE_BYTES), x = rows + (uint32_t)(x_at * plan.x_bytes);
+          uint32_t a[4][4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) el_ldmatrix_trans(a[q], tile + chunk[q]);
+#pragma unroll
+          for (int j = 0; j < NT; j += 2) {
+            if (j * 8 < n) {
+              uint32_t b[4];
+              el_ldmatrix(b, x + (uint32_t)(j * 8 * EL_X_PITCH));
+              if (there < 2) b[1] = b[3] = 0u;  // the weights are zeros there, and what lies in the rows' place may be anything
+#pragma unroll
+              for (int q = 0; q < 4; ++q) el_mma<BF16>(acc[j][q], a[q], b[0], b[1]);
+              if (j * 8 + 8 < n) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) el_mma<BF16>(acc[j + 1][q], a[q], b[2], b[3]);
+              }
+            }
+          }
+        }
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(smem_u32(&sh->empty[s]));
+          mbar_arrive(smem_u32(&sh->x_empty[x_at]));
+        }
+        if (++s == p.stages) { s = 0; ph ^= 1u; }
+        if (++x_at == plan.x_stages) { x_at = 0; x_ph ^= 1u; }
+      }
+      // ---------------------------------------------------------------- the item's sums
+      // Eight tokens after eight, always from acc[0], the others moving up: the code is there once.  Thread (warp, lane) finishes what lane's fragments hold for
+      // 16 columns and one token of a pair.
+#pragma unroll 1
+      for (int j = 0; j * 8 < n; ++j) {
+#pragma unroll
+        for (int i = 0; i < EL_SUMS; ++i) sums[(warp * EL_SUMS + i) * 32 + lane] = acc[0][i >> 2][i & 3];
+        el_sync();
+        const int q = warp >> 1, i = warp & 1, token = j * 8 + c * 2 + i;
+        float v0 = 0.f, v1 = 0.f;
+#pragma unroll
+        for (int o = 0; o < EL_CONSUMERS / 32; ++o) {
+          v0 += sums[(o * EL_SUMS + q * 4 + i) * 32 + lane];
+          v1 += sums[(o * EL_SUMS + q * 4 + 2 + i) * 32 + lane];
+        }
+        if (token < n) {
+          const int col = m * (gated ? EL_COLUMNS / 2 : EL_COLUMNS) + q * (gated ? 8 : 16) + g;
+          if (product == 0) {
+            uint16_t* h_row = p.h + (size_t)(first + token) * p.hidden;
+            v0 = el_activated(p.activation, v0);
+            if (gated) {
+              if (col < columns) h_row[col] = el_round<BF16>(v0 * v1);
+            } else {
+              if (col < columns) h_row[col] = el_round<BF16>(v0);
+              if (col + 8 < columns) h_row[col + 8] = el_round<BF16>(el_activated(p.activation, v1));
+            }
+          } else {
+            const int pair = sh->list[first + token];
+            const float gate = sh->gates[pair];
+            float* part_row = p.part + (size_t)pair * p.out_width;
+            if (col < columns) __stcg(part_row + col, gate * v0);
+            if (col + 8 < columns) __stcg(part_row + col + 8, gate * v1);
+          }
+        }
+        el_sync();  // the sums have been read
+#pragma unroll
+        for (int o = 0; o < NT; ++o)
+#pragma unroll
+          for (int t = 0; t < 16; ++t) acc[o][t >> 2][t & 3] = o + 1 < NT ? acc[o + 1 < NT ? o + 1 : o][t >> 2][t & 3] : 0.f;
+      }
+      // (all that was stored is behind the barriers above)
+      if (ok) ok = mbar_parked_wait(smem_u32(&sh->reported[count & 1]), (count >> 1 & 1) ^ 1u, abort_flag);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&sh->finished[count & 1]));
+      ++count;
+    }
   }
 }
 
@@ -315,219 +489,150 @@ __global__ void __launch_bounds__(EL_THREADS, 1)
   using namespace umma;
   extern __shared__ uint8_t el_smem[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(el_smem) + 1023) & ~static_cast<uintptr_t>(1023));
-  ElShared* sh = reinterpret_cast<ElShared*>(smem + (size_t)p.stages * EL_TILE_BYTES + EL_X_STAGES * EL_X_BYTES);
+  float* sums = reinterpret_cast<float*>(smem + (size_t)p.stages * EL_TILE_BYTES + EL_X_BYTES);  // [warps][EL_SUMS][32]
+  ElShared* sh = reinterpret_cast<ElShared*>(sums + EL_CONSUMERS * EL_SUMS);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, cta = (int)blockIdx.x;
   volatile int* abort_flag = &sh->abort_flag;
   if (threadIdx.x == 0) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_in) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_out) : "memory");
     for (int s = 0; s < p.stages; ++s) {
       mbar_init(smem_u32(&sh->full[s]), 1);
       mbar_init(smem_u32(&sh->empty[s]), EL_CONSUMERS / 32);
+    }
+    for (int s = 0; s < EL_MAX_STAGES; ++s) {
+      mbar_init(smem_u32(&sh->x_full[s]), 1);
+      mbar_init(smem_u32(&sh->x_empty[s]), EL_CONSUMERS / 32);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&sh->finished[i]), EL_CONSUMERS / 32);
+      mbar_init(smem_u32(&sh->reported[i]), EL_REPORTERS / 32);
     }
     sh->abort_flag = 0;
     mbar_fence_init();
   }
   __syncthreads();
   el_choose_all(p, sh);
-  if (warp == 0) el_sort(p, sh);
-  __syncthreads();
-  const int used = sh->used;
+  el_sort(p, sh);
+  const ElPlan plan(p, sh);
   const uint32_t tiles0 = smem_u32(smem), x0 = tiles0 + (uint32_t)(p.stages * EL_TILE_BYTES);
-  // of the two products: steps of the contraction, blocks of columns, tiles
-  const int columns = p.gated ? 64 : 128;  // of h that a block stands for
-  int steps[2] = {(p.width + EL_K - 1) / EL_K, (p.hidden + EL_K - 1) / EL_K};
-  int blocks[2] = {(p.hidden + columns - 1) / columns, (p.out_width + 127) / 128};
+  uint32_t *done_in = p.flags, *done_out = p.flags + p.n_experts;
   bool ok = true;
 
   if (warp == EL_CONSUMERS / 32) {
-    // ------------------------------------------------------------------ producer
+    // ------------------------------------------------------------------ weights
     if (elect_one()) {
       int s = 0;
       uint32_t ph = 1;
       for (int product = 0; product < 2 && ok; ++product) {
-        const int total = used * blocks[product] * steps[product];
         const CUtensorMap* map = product == 0 ? &map_in : &map_out;
-        const int second = product == 0 && p.gated ? p.hidden : 64, width = product == 0 ? columns : 128;
-        for (ElWalk w(el_share(total, cta, p.ctas), el_share(total, cta + 1, p.ctas), blocks[product], steps[product]); w.left(); w.next()) {
-          ok = mbar_parked_wait(smem_u32(&sh->empty[s]), ph, abort_flag);
-          if (!ok) break;
-          const uint32_t to = tiles0 + (uint32_t)(s * EL_TILE_BYTES), bar = smem_u32(&sh->full[s]);
-          const int e = sh->expert[w.u];
-          mbar_expect_tx(bar, EL_TILE_BYTES);
-          pair_load_3d<1>(to, map, bar, w.m * width, w.kb * EL_K, e);
-          pair_load_3d<1>(to + EL_TILE_BYTES / 2, map, bar, w.m * width + second, w.kb * EL_K, e);
-          if (++s == p.stages) { s = 0; ph ^= 1u; }
+        const bool gated = product == 0 && p.gated;
+        const int length = product == 0 ? p.width : p.hidden;
+        for (ElItems w = plan.items(product); w.left() && ok; w.next()) {
+          const int e = sh->expert[w.expert()], col = w.block() * (gated ? EL_COLUMNS / 2 : EL_COLUMNS);
+          for (int k = 0; k < length; k += EL_K) {
+            ok = mbar_parked_wait(smem_u32(&sh->empty[s]), ph, abort_flag);
+            if (!ok) break;
+            const uint32_t to = tiles0 + (uint32_t)(s * EL_TILE_BYTES), bar = smem_u32(&sh->full[s]);
+            mbar_expect_tx(bar, EL_TILE_BYTES);
+            pair_load_3d<1>(to, map, bar, col, k, e);
+            if (gated) pair_load_3d<1>(to + EL_TILE_BYTES / 2, map, bar, p.hidden + col, k, e);
+            if (++s == p.stages) { s = 0; ph ^= 1u; }
+          }
         }
       }
     }
     __syncwarp();
-  } else {
-    // ------------------------------------------------------------------ consumers
-    const int g = lane >> 2, c = lane & 3;  // of a fragment: column of the weight; pair of tokens
+  } else if (warp == EL_CONSUMERS / 32 + 1) {
+    // ------------------------------------------------------------------ tokens' rows
     int s = 0;
-    uint32_t ph = 0;
+    uint32_t ph = 1;
+    for (int product = 0; product < 2 && ok; ++product) {
+      const int length = product == 0 ? p.width : p.hidden;
+      for (ElItems w = plan.items(product); w.left() && ok; w.next()) {
+        const int u = w.expert(), first = sh->first[u], n = sh->first[u + 1] - first;
+        if (product == 1) {  // all of the expert's h is there
+          ok = __all_sync(0xffffffffu, el_await(done_in + u, (uint32_t)plan.blocks_in, abort_flag));
+          if (!ok) break;
+          fence_proxy_async_global();
+        }
+        // the rows of two tokens a lane
+        const uint16_t* src[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int row = min(lane + 32 * i, n - 1);
+          src[i] = product == 0 ? static_cast<const uint16_t*>(p.x) + (size_t)(sh->list[first + row] / (uint32_t)p.top_k) * p.x_pitch
+                                : p.h + (size_t)(first + row) * p.hidden;
+        }
+        for (int k = 0; k < length; k += EL_K) {
+          ok = __all_sync(0xffffffffu, mbar_parked_wait(smem_u32(&sh->x_empty[s]), ph, abort_flag));
+          if (!ok) break;
+          const uint32_t bytes = (uint32_t)min(EL_K, length - k) * 2u, bar = smem_u32(&sh->x_full[s]), to = x0 + (uint32_t)(s * plan.x_bytes);
+          if (lane == 0) mbar_expect_tx(bar, bytes * (uint32_t)n);
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            if (lane + 32 * i < n) el_bulk_load(to + (uint32_t)((lane + 32 * i) * EL_X_PITCH), src[i] + k, bytes, bar);
+          if (++s == plan.x_stages) { s = 0; ph ^= 1u; }
+        }
+      }
+    }
+  } else if (warp >= EL_WARPS - EL_REPORTERS / 32) {
+    // ------------------------------------------------------------------ reports, and the sum over a token's experts
+    const int thread = (int)threadIdx.x - (EL_THREADS - EL_REPORTERS);
+    uint32_t count = 0;  // items, of which two may be finished and not reported
     for (int product = 0; product < 2; ++product) {
-      if (product == 1) el_grid_sync(p.flags + 2 * p.ctas, p.ctas, abort_flag);
-      const int total = used * blocks[product] * steps[product], from = el_share(total, cta, p.ctas), to = el_share(total, cta + 1, p.ctas);
-      const bool gated = product == 0 && p.gated;
-      uint32_t* flags = p.flags + product * p.ctas;
-      // a warp's 16 columns: two groups of eight, side by side, or one of each half
-      const int block_a = gated ? 0 : warp >> 2, chunk_a = gated ? warp : (warp & 3) * 2, block_b = gated ? 1 : block_a, chunk_b = gated ? warp : chunk_a + 1;
-      ElWalk ahead(from, to, blocks[product], steps[product]);
-      int x_slot = 0;
-      const auto fetch = [&] {  // the rows of the expert's tokens that the next tile is multiplied with
-        if (ahead.left()) {
-          const int first = sh->first[ahead.u], n = sh->first[ahead.u + 1] - first, k0 = ahead.kb * EL_K;
-          const int width = product == 0 ? p.width : p.hidden;
-          for (int i = threadIdx.x; i < n * 8; i += EL_CONSUMERS) {
-            const int row = i >> 3, chunk = i & 7, k = k0 + chunk * 8;
-            const uint16_t* src;
-            if (product == 0) src = static_cast<const uint16_t*>(p.x) + (size_t)(sh->list[first + row] / (uint32_t)p.top_k) * p.x_pitch;
-            else src = p.h + (size_t)(first + row) * p.hidden;
-            cp_async16(x0 + (uint32_t)(x_slot * EL_X_BYTES + row * 128 + (chunk ^ (row & 7)) * 16), k < width ? src + k : src, k < width);
-          }
-          ahead.next();
-        }
-        cp_async_commit();
-        x_slot = (x_slot + 1) % EL_X_STAGES;
-      };
-#pragma unroll
-      for (int i = 0; i < EL_X_STAGES - 1; ++i) fetch();
-      float acc[8][4];
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[j][i] = 0.f;
-      int head = from;  // where the segment in `acc` began
-      int x_at = 0;
-      for (ElWalk w(from, to, blocks[product], steps[product]); w.left(); w.next()) {
-        cp_async_wait<EL_X_STAGES - 2>();
-        el_sync();  // all have the tile's rows, and are done with the last one's
-        fetch();
-        const int first = sh->first[w.u], n = sh->first[w.u + 1] - first;
-        if (ok) ok = mbar_parked_wait(smem_u32(&sh->full[s]), ph, abort_flag);
-        const uint32_t tile = tiles0 + (uint32_t)(s * EL_TILE_BYTES), x = x0 + (uint32_t)(x_at * EL_X_BYTES);
-        {
-          const int matrix = lane >> 3, row = lane & 7;
-          const uint32_t block = (matrix & 1 ? block_b : block_a) * (EL_TILE_BYTES / 2), chunk = (matrix & 1 ? chunk_b : chunk_a) ^ row;
-          const uint32_t weights = tile + block + (uint32_t)((matrix >> 1) * 8 + row) * 128u + chunk * 16u;
-          uint32_t a[4][4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) el_ldmatrix_trans(a[k], weights + (uint32_t)k * 2048u);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            if (j * 8 >= n) break;
-            uint32_t b[4];
-            const uint32_t tokens = x + (uint32_t)((j * 8 + row) * 128);
-            el_ldmatrix(b, tokens + (uint32_t)((matrix ^ row) * 16));
-            el_mma<BF16>(acc[j], a[0], b[0], b[1]);
-            el_mma<BF16>(acc[j], a[1], b[2], b[3]);
-            el_ldmatrix(b, tokens + (uint32_t)(((matrix + 4) ^ row) * 16));
-            el_mma<BF16>(acc[j], a[2], b[0], b[1]);
-            el_mma<BF16>(acc[j], a[3], b[2], b[3]);
-          }
-        }
+      for (ElItems w = plan.items(product); w.left(); w.next(), ++count) {
+        if (ok) ok = mbar_parked_wait(smem_u32(&sh->finished[count & 1]), count >> 1 & 1, abort_flag);
         __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&sh->empty[s]));
-        if (++s == p.stages) { s = 0; ph ^= 1u; }
-        x_at = (x_at + 1) % EL_X_STAGES;
-        const bool last = w.kb + 1 == steps[product];
-        if (!last && w.at + 1 < to) continue;
-        // ---------------------------------------------------------------- the end of a segment
-        const int block_first = w.at - w.kb, block_end = block_first + steps[product];
-        if (head != block_first) {  // the first segment of this share: its sums go to whoever has the block's first tile
-          float* slot = p.slots + (size_t)cta * EL_SLOT + threadIdx.x;
+        if (product == 0) {
+          if (thread == 0) el_arrive(done_in + w.expert());
+          if (lane == 0) mbar_arrive(smem_u32(&sh->reported[count & 1]));
+          continue;
+        }
+        const int m = w.block(), col = m * EL_COLUMNS + (thread & 15) * 4;  // (the width is a multiple of eight)
+        if (thread == 0) sh->last = el_count(done_out + m) + 1u == (uint32_t)plan.used;
+        el_sync_reporters();
+        if (sh->last && col < p.out_width) {  // the last item of the column block: all of its columns' parts are there
+          for (int t0 = thread >> 4; t0 < p.tokens; t0 += 4 * (EL_REPORTERS / 16)) {
+            float4 sum[4];  // of four tokens, whose parts are on their way together
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            if (j * 8 >= n) break;
+            for (int i = 0; i < 4; ++i) sum[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
+            for (int j = 0; j < p.top_k; ++j) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) __stcg(slot + (j * 4 + i) * EL_CONSUMERS, acc[j][i]);
-          }
-          el_sync();
-          if (threadIdx.x == 0) {
-            __threadfence();
-            asm volatile("st.release.gpu.global.b32 [%0], %1;" ::"l"(flags + cta), "r"(1u) : "memory");
-          }
-        } else {
-          if (!last) {
-            int others = 0;  // shares behind this one that begin inside the block
-            while (cta + 1 + others < p.ctas && el_share(total, cta + 1 + others, p.ctas) < block_end) ++others;
-            for (int i = threadIdx.x; i < others; i += EL_CONSUMERS) {
-              const int o = cta + 1 + i;
-              if (el_share(total, o, p.ctas) < el_share(total, o + 1, p.ctas)) el_await(flags + o, 1u, abort_flag);
-            }
-            __threadfence();
-            el_sync();
-            for (int i = 0; i < others; ++i) {
-              const int o = cta + 1 + i;
-              if (el_share(total, o, p.ctas) == el_share(total, o + 1, p.ctas)) continue;
-              const float* slot = p.slots + (size_t)o * EL_SLOT + threadIdx.x;
-#pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                if (j * 8 >= n) break;
-#pragma unroll
-                for (int q = 0; q < 4; ++q) acc[j][q] += __ldcg(slot + (j * 4 + q) * EL_CONSUMERS);
+              for (int i = 0; i < 4; ++i) {
+                const int t = min(t0 + i * (EL_REPORTERS / 16), p.tokens - 1);
+                const float4 v = __ldcg(reinterpret_cast<const float4*>(p.part + (size_t)(t * p.top_k + j) * p.out_width + col));
+                sum[i].x += v.x;
+                sum[i].y += v.y;
+                sum[i].z += v.z;
+                sum[i].w += v.w;
               }
             }
-          }
-          // the block's sums are whole
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            if (j * 8 >= n) break;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const int token = j * 8 + c * 2 + i;
-              if (token >= n) continue;
-              if (product == 0) {
-                uint16_t* row = p.h + (size_t)(first + token) * p.hidden;
-                if (gated) {
-                  const int col = w.m * 64 + warp * 8 + g;
-                  if (col < p.hidden) row[col] = el_round<BF16>(el_activated(p.activation, acc[j][i]) * acc[j][2 + i]);
-                } else {
-                  const int col = w.m * 128 + warp * 16 + g;
-                  if (col < p.hidden) row[col] = el_round<BF16>(el_activated(p.activation, acc[j][i]));
-                  if (col + 8 < p.hidden) row[col + 8] = el_round<BF16>(el_activated(p.activation, acc[j][2 + i]));
-                }
+            for (int i = 0; i < 4; ++i) {
+              const int t = t0 + i * (EL_REPORTERS / 16);
+              if (t >= p.tokens) continue;
+              uint16_t* to = static_cast<uint16_t*>(p.out) + (size_t)t * p.out_pitch + col;
+              const uint16_t b[4] = {el_round<BF16>(sum[i].x), el_round<BF16>(sum[i].y), el_round<BF16>(sum[i].z), el_round<BF16>(sum[i].w)};
+              if ((reinterpret_cast<uintptr_t>(to) & 7) == 0) {
+                *reinterpret_cast<uint2*>(to) = make_uint2((uint32_t)b[0] | (uint32_t)b[1] << 16, (uint32_t)b[2] | (uint32_t)b[3] << 16);
               } else {
-                const int pair = sh->list[first + token], col = w.m * 128 + warp * 16 + g;
-                const float gate = sh->gates[pair];
-                float* row = p.part + (size_t)pair * p.out_width;
-                if (col < p.out_width) __stcg(row + col, gate * acc[j][i]);
-                if (col + 8 < p.out_width) __stcg(row + col + 8, gate * acc[j][2 + i]);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) to[q] = b[q];
               }
             }
           }
         }
-        head = w.at + 1;
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc[j][i] = 0.f;
-      }
-      cp_async_wait_all();
-    }
-    // ------------------------------------------------------------------ the sum over a token's experts
-    el_grid_sync(p.flags + 2 * p.ctas + 1, p.ctas, abort_flag);
-    const int per_row = p.out_width / 4;  // the width is a multiple of eight
-    for (int i = cta * EL_CONSUMERS + (int)threadIdx.x; i < p.tokens * per_row; i += p.ctas * EL_CONSUMERS) {
-      const int t = i / per_row, col = (i - t * per_row) * 4;
-      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-      for (int j = 0; j < p.top_k; ++j) {
-        const float4 v = __ldcg(reinterpret_cast<const float4*>(p.part + (size_t)(t * p.top_k + j) * p.out_width + col));
-        sum.x += v.x;
-        sum.y += v.y;
-        sum.z += v.z;
-        sum.w += v.w;
-      }
-      uint16_t* to = static_cast<uint16_t*>(p.out) + (size_t)t * p.out_pitch + col;
-      const uint16_t r[4] = {el_round<BF16>(sum.x), el_round<BF16>(sum.y), el_round<BF16>(sum.z), el_round<BF16>(sum.w)};
-      if ((reinterpret_cast<uintptr_t>(to) & 7) == 0) {
-        *reinterpret_cast<uint2*>(to) = make_uint2((uint32_t)r[0] | (uint32_t)r[1] << 16, (uint32_t)r[2] | (uint32_t)r[3] << 16);
-      } else {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) to[q] = r[q];
+        el_sync_reporters();  // `last` has been read
+        if (lane == 0) mbar_arrive(smem_u32(&sh->reported[count & 1]));
       }
     }
+  } else {
+    if (sh->most <= 16) el_products<BF16, 2>(p, sh, tiles0, x0, sums);
+    else if (sh->most <= 32) el_products<BF16, 4>(p, sh, tiles0, x0, sums);
+    else el_products<BF16, 8>(p, sh, tiles0, x0, sums);
   }
   if (*abort_flag && lane == 0) report_problem();
   if (*abort_flag) {  // copies may still be on their way into this CTA's memory
@@ -538,9 +643,10 @@ __global__ void __launch_bounds__(EL_THREADS, 1)
 
 // Bytes of workspace, and where its parts begin.
 struct ExpertSpace {
-  size_t logits, flags, slots, h, part, total;
+  size_t logits, flags, h, part, total;
+  int n_flags;
 };
-inline ExpertSpace expert_space(int tokens, int experts, int top_k, int hidden, int out_width, int ctas) {
+inline ExpertSpace expert_space(int tokens, int experts, int top_k, int hidden, int out_width) {
   ExpertSpace s;
   size_t at = 0;
   const auto take = [&](size_t bytes) {
@@ -548,13 +654,34 @@ inline ExpertSpace expert_space(int tokens, int experts, int top_k, int hidden, 
     at += (bytes + 255) / 256 * 256;
     return here;
   };
+  s.n_flags = experts + (out_width + EL_COLUMNS - 1) / EL_COLUMNS + 1;
   s.logits = take((size_t)tokens * experts * sizeof(double));
-  s.flags = take((size_t)(2 * ctas + 3) * sizeof(uint32_t));
-  s.slots = take((size_t)ctas * EL_SLOT * sizeof(float));
+  s.flags = take((size_t)s.n_flags * sizeof(uint32_t));
   s.h = take((size_t)tokens * top_k * hidden * 2);
   s.part = take((size_t)tokens * top_k * out_width * sizeof(float));
   s.total = at;
   return s;
+}
+
+// A tensor map of `mats` matrices [rows][cols] of 16-bit values, boxes of 128 rows by `box` columns: 64, or 32 (rows of 64 bytes).
+inline int expert_tensor_map(CUtensorMap* map, const void* data, int cols, int rows, int mats, int box, bool bf16) {
+  using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                              const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  const Encode encode = reinterpret_cast<Encode>(tensor_map_encoder());
+  if (encode == nullptr) return -1000 - (int)CUDA_ERROR_NOT_FOUND;
+  const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)mats}, pitch[2] = {(cuuint64_t)cols * 2, (cuuint64_t)cols * 2 * (cuuint64_t)rows};
+  const cuuint32_t boxes[3] = {(cuuint32_t)box, EL_K, 1}, steps[3] = {1, 1, 1};
+  const auto made = [&] {
+    return encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(data), dims, pitch, boxes, steps,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, box == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult rc = made();
+  if (rc == CUDA_ERROR_INVALID_CONTEXT) {  // a host thread that has launched nothing yet: see weight_tensor_map
+    int dev = 0;
+    if (cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess) rc = made();
+  }
+  return rc == CUDA_SUCCESS ? 0 : -1000 - (int)rc;
 }
 
 template <typename T, typename R>
@@ -564,15 +691,15 @@ cudaError_t launch_expert_logits(const ExpertParams& p, cudaStream_t st) {
 
 template <bool BF16>
 int launch_expert_layer(ExpertParams p, const void* w_in, const void* w_out, cudaStream_t st, int max_smem) {
-  const int rest = 1024 + EL_X_STAGES * EL_X_BYTES + (int)sizeof(ElShared);
+  const int rest = 1024 + EL_X_BYTES + EL_CONSUMERS * EL_SUMS * (int)sizeof(float) + (int)sizeof(ElShared);
   p.stages = (max_smem - rest) / EL_TILE_BYTES;
   if (p.stages > EL_MAX_STAGES) p.stages = EL_MAX_STAGES;
   if (p.stages < 2) return -1;
   const int smem = rest + p.stages * EL_TILE_BYTES;
   CUtensorMap in, out;
   const int wide = p.gated ? 2 * p.hidden : p.hidden;
-  int rc = grouped_tensor_map(&in, w_in, wide, wide, p.width, p.n_experts, EL_K, BF16);
-  if (rc == 0) rc = grouped_tensor_map(&out, w_out, p.out_width, p.out_width, p.hidden, p.n_experts, EL_K, BF16);
+  int rc = expert_tensor_map(&in, w_in, wide, p.width, p.n_experts, p.gated ? 32 : 64, BF16);
+  if (rc == 0) rc = expert_tensor_map(&out, w_out, p.out_width, p.hidden, p.n_experts, 64, BF16);
   if (rc != 0) return rc;
   static std::atomic<int> granted[64];
   if (ensure_smem(expert_layer_kernel<BF16>, max_smem, granted) != 0) return -1;

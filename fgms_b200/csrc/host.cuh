@@ -40,7 +40,6 @@ inline int check_launch(const char* what) {
 struct DeviceInfo {
   int sms = 0;       // to launch on
   int reserved = 0;  // to leave free
-  int all = 0;       // that the device has
   int max_smem_optin = 0;
 };
 
@@ -54,7 +53,7 @@ inline int device_info(DeviceInfo* out) {
     cudaDeviceProp prop;
     e = cudaGetDeviceProperties(&prop, dev);
     if (e != cudaSuccess) return fail(FGMS_ERR_CUDA, "cudaGetDeviceProperties: %s", cudaGetErrorString(e));
-    cached.sms = cached.all = prop.multiProcessorCount;
+    cached.sms = prop.multiProcessorCount;
     cached.max_smem_optin = (int)prop.sharedMemPerBlockOptin;
     cached_dev = dev;
   }

@@ -2,6 +2,7 @@
 // (see include/fgms_b200.h for the contract of each).  They have no counterpart in the reference.
 #include "../../include/fgms_b200.h"
 
+#include <algorithm>
 #include <cmath>
 
 #include "host.cuh"
@@ -394,8 +395,8 @@ int run_expert_layer(const fgms_b200_expert_layer_args& a, cudaStream_t st) {
   if (a.router_dtype != a.dtype && a.router_dtype != FGMS_DTYPE_F32) return fail(FGMS_ERR_UNSUPPORTED, "the router's type must be that of the rows, or fp32");
   if (a.activation != FGMS_ACTIVATION_RELU && a.activation != FGMS_ACTIVATION_SILU) return fail(FGMS_ERR_INVALID_ARG, "unknown activation %d", a.activation);
   const int64_t wide = a.gated ? 2ll * a.hidden : a.hidden;
-  const int64_t tiles[2] = {(int64_t)a.experts * ((wide + 127) / 128 + 1) * ((a.width + 63) / 64), (int64_t)a.experts * ((a.out_width + 127) / 128) * ((a.hidden + 63) / 64)};
-  if (tiles[0] > 0x3fffffff || tiles[1] > 0x3fffffff) return fail(FGMS_ERR_INVALID_ARG, "weights too large");
+  // (a tensor map's matrices are less than 2^40 bytes apart; items are then far from leaving an int)
+  if ((int64_t)a.width * wide * 2 >= (1ll << 40) || (int64_t)a.hidden * a.out_width * 2 >= (1ll << 40)) return fail(FGMS_ERR_INVALID_ARG, "weights too large");
   const int64_t pairs = (int64_t)a.tokens * a.top_k;
   const RowSpan x{a.x, a.tokens, a.x_pitch, a.width, 2}, out{a.out, a.tokens, a.out_pitch, a.out_width, 2};
   const RowSpan router{a.router, a.experts, a.width, a.width, layer_elem(a.router_dtype)}, w_in{a.w_in, (int64_t)a.experts * a.width, wide, wide, 2},
@@ -419,7 +420,7 @@ int run_expert_layer(const fgms_b200_expert_layer_args& a, cudaStream_t st) {
   }
   DeviceInfo di;
   if (int rc = device_info(&di)) return rc;
-  const fgms::ExpertSpace space = fgms::expert_space(a.tokens, a.experts, a.top_k, a.hidden, a.out_width, di.all);
+  const fgms::ExpertSpace space = fgms::expert_space(a.tokens, a.experts, a.top_k, a.hidden, a.out_width);
   if (!a.workspace || a.workspace_bytes < space.total || (reinterpret_cast<uintptr_t>(a.workspace) & 255))
     return fail(FGMS_ERR_WORKSPACE, "a workspace of %zu bytes on a 256-byte boundary is needed", space.total);
   for (const RowSpan* s : {&x, &router, &w_in, &w_out, &out, &experts, &gates})
@@ -443,11 +444,10 @@ int run_expert_layer(const fgms_b200_expert_layer_args& a, cudaStream_t st) {
   p.out_pitch = a.tokens > 1 ? a.out_pitch : a.out_width;
   p.logits = reinterpret_cast<double*>(at + space.logits);
   p.flags = reinterpret_cast<uint32_t*>(at + space.flags);
-  p.slots = reinterpret_cast<float*>(at + space.slots);
   p.h = reinterpret_cast<uint16_t*>(at + space.h);
   p.part = reinterpret_cast<float*>(at + space.part);
   p.ctas = di.sms;
-  p.x_vec = true;
+  p.n_flags = space.n_flags;
   p.alone = di.reserved > 0;
   const cudaError_t e = with_types(a.dtype, a.router_dtype, [&](auto t, auto r) { return fgms::launch_expert_logits<decltype(t), decltype(r)>(p, st); });
   if (e != cudaSuccess) {
@@ -465,11 +465,9 @@ int run_expert_layer(const fgms_b200_expert_layer_args& a, cudaStream_t st) {
 extern "C" {
 
 size_t fgms_b200_expert_layer_workspace_bytes(int tokens, int experts, int top_k, int hidden, int out_width) {
-  DeviceInfo di;
-  if (tokens < 1 || tokens > fgms::EL_MAX_TOKENS || experts < 1 || experts > fgms::EL_MAX_EXPERTS || top_k < 1 || top_k > fgms::EL_MAX_TOP_K || hidden < 1 || out_width < 1 ||
-      device_info(&di) != FGMS_OK)
+  if (tokens < 1 || tokens > fgms::EL_MAX_TOKENS || experts < 1 || experts > fgms::EL_MAX_EXPERTS || top_k < 1 || top_k > fgms::EL_MAX_TOP_K || hidden < 1 || out_width < 1)
     return 0;
-  return fgms::expert_space(tokens, experts, top_k, hidden, out_width, di.all).total;
+  return fgms::expert_space(tokens, experts, top_k, hidden, out_width).total;
 }
 
 int fgms_b200_expert_layer(const fgms_b200_expert_layer_args* args, void* stream) {
