@@ -40,8 +40,8 @@ class RmsNormArgs(ctypes.Structure):
 
 
 class RmsNormBwdArgs(ctypes.Structure):
-    _fields_ = ([(n, c_void_p) for n in ("out_grad", "sum", "sum_grad", "weight", "rstd", "x_grad", "residual_grad", "weight_grad")] +
-                [(n, c_int64) for n in ("out_grad_pitch", "sum_pitch", "sum_grad_pitch", "x_grad_pitch", "residual_grad_pitch", "rows", "width")] +
+    _fields_ = ([(n, c_void_p) for n in ("out_grad", "sum", "x", "residual", "sum_grad", "weight", "rstd", "x_grad", "residual_grad", "weight_grad")] +
+                [(n, c_int64) for n in ("out_grad_pitch", "sum_pitch", "x_pitch", "residual_pitch", "sum_grad_pitch", "x_grad_pitch", "residual_grad_pitch", "rows", "width")] +
                 [("rng_used", c_void_p), ("workspace", c_void_p), ("workspace_bytes", c_size_t), ("p", c_double), ("dtype", c_int), ("weight_dtype", c_int)])
 
 

@@ -314,11 +314,13 @@ def fgms_rms_norm_cuda(x, weight, out, eps=1e-6, residual=None, residual_out=Non
     _native.rms_norm_into(x, weight, out, eps, residual, residual_out, scale, rstd, dropout, rng, rng_used)
 
 
-def fgms_rms_norm_bwd_cuda(out_grad, h, weight, rstd, x_grad=None, weight_grad=None, h_grad=None, residual_grad=None, dropout=0.0, rng_used=None):
+def fgms_rms_norm_bwd_cuda(out_grad, h, weight, rstd, x_grad=None, weight_grad=None, h_grad=None, residual_grad=None, dropout=0.0, rng_used=None,
+                           x=None, residual=None):
     """Gradient of :func:`fgms_rms_norm_cuda` from ``h`` (``residual_out``, or ``x`` where there was neither residual nor dropout) and ``rstd``:
     ``residual_grad = dh``, ``x_grad`` the same where x was kept, ``weight_grad`` (the weight's type, summed in float32 in a fixed order).
-    ``h_grad`` is what else flows back into ``h``.  Outputs that are None are left out."""
-    _native.rms_norm_bwd(out_grad, h, weight, rstd, x_grad, weight_grad, h_grad, residual_grad, dropout, rng_used)
+    ``h_grad`` is what else flows back into ``h``.  Outputs that are None are left out.  Rows in 16 bits with a float32 weight: given ``x`` and
+    ``residual`` instead of ``h`` (None), h is computed once more and ``weight_grad`` does not see how it was rounded."""
+    _native.rms_norm_bwd(out_grad, h, weight, rstd, x_grad, weight_grad, h_grad, residual_grad, dropout, rng_used, x, residual)
 
 
 def fgms_quantize_rows_cuda(x, codes, scale):

@@ -5,8 +5,8 @@
 
 namespace fgms {
 
-constexpr int DROP_THREADS = 256;
-constexpr int DROP_AT_ONCE = 4;  // chunks whose loads are on their way together
+constexpr int DROP_THREADS = 256, DROP_BLOCKS = 4;  // of an SM
+constexpr int DROP_AT_ONCE = 2;  // chunks whose loads are on their way together, while their lots are drawn
 
 struct DropoutParams {
   const void *x, *residual;  // residual: or null
@@ -20,7 +20,7 @@ struct DropoutParams {
 
 // A chunk is a thread's; threads go on by the whole grid, whose width in rows and columns is divided once.
 template <typename T, bool BACKWARD>
-__global__ void __launch_bounds__(DROP_THREADS) dropout_kernel(const __grid_constant__ DropoutParams p) {
+__global__ void __launch_bounds__(DROP_THREADS, DROP_BLOCKS) dropout_kernel(const __grid_constant__ DropoutParams p) {
   umma::griddep_wait();
   if (!p.alone) umma::griddep_launch_dependents();
   const DropKey key = drop_key(BACKWARD ? p.drop.used : p.drop.state);
@@ -30,43 +30,36 @@ __global__ void __launch_bounds__(DROP_THREADS) dropout_kernel(const __grid_cons
   const unsigned step_chunk = (unsigned)(step - (unsigned long long)step_row * per_row);
   long long row = (long long)(at / per_row);
   unsigned chunk = (unsigned)(at - (unsigned long long)row * per_row);
-  const auto next = [&] {
-    row += step_row;
-    chunk += step_chunk;
-    if (chunk >= per_row) {
-      chunk -= per_row;
-      ++row;
-    }
-  };
-  while (row < p.rows) {
+  while (__any_sync(0xffffffffu, row < p.rows)) {
     long long rows[DROP_AT_ONCE];
-    unsigned chunks[DROP_AT_ONCE];
+    int cols[DROP_AT_ONCE], there[DROP_AT_ONCE];
     RowRaw<T> x[DROP_AT_ONCE], add[DROP_AT_ONCE];
-    int n = 0;
 #pragma unroll
     for (int i = 0; i < DROP_AT_ONCE; ++i) {
-      rows[i] = row;
-      chunks[i] = chunk;
-      if (row < p.rows) {
-        const int col = (int)(chunk * ROW_CHUNK), there = p.width - col;
-        x[i] = row_load(static_cast<const T*>(p.x) + row * p.x_pitch + col, there, p.x_vec);
-        if (!BACKWARD && p.residual) add[i] = row_load(static_cast<const T*>(p.residual) + row * p.residual_pitch + col, there, p.residual_vec);
-        n = i + 1;
-        next();
+      cols[i] = (int)(chunk * ROW_CHUNK);
+      there[i] = row < p.rows ? p.width - cols[i] : 0;
+      rows[i] = row < p.rows ? row : 0;
+      x[i] = row_load(static_cast<const T*>(p.x) + rows[i] * p.x_pitch + cols[i], there[i], p.x_vec);
+      if (!BACKWARD && p.residual) add[i] = row_load(static_cast<const T*>(p.residual) + rows[i] * p.residual_pitch + cols[i], there[i], p.residual_vec);
+      row += step_row;
+      chunk += step_chunk;
+      if (chunk >= per_row) {
+        chunk -= per_row;
+        ++row;
       }
     }
+    uint32_t keep[DROP_AT_ONCE];
+#pragma unroll
+    for (int i = 0; i < DROP_AT_ONCE; ++i) keep[i] = drop_keep(key, (uint32_t)cols[i] / ROW_CHUNK, (uint32_t)rows[i], p.drop.threshold);
 #pragma unroll
     for (int i = 0; i < DROP_AT_ONCE; ++i) {
-      if (i >= n) continue;
-      const int col = (int)(chunks[i] * ROW_CHUNK);
-      const uint32_t keep = drop_keep(key, chunks[i], (uint32_t)rows[i], p.drop.threshold);
       float y[ROW_CHUNK];
 #pragma unroll
       for (int e = 0; e < ROW_CHUNK; ++e) {
-        y[e] = keep >> e & 1u ? row_value(x[i], e) * p.drop.factor : 0.f;
+        y[e] = keep[i] >> e & 1u ? row_value(x[i], e) * p.drop.factor : 0.f;
         if (!BACKWARD && p.residual) y[e] += row_value(add[i], e);
       }
-      row_store(static_cast<T*>(p.out) + rows[i] * p.out_pitch + col, y, p.width - col, p.out_vec);
+      row_store(static_cast<T*>(p.out) + rows[i] * p.out_pitch + cols[i], y, there[i], p.out_vec, cols[i] == 0);
     }
   }
   if (!BACKWARD) drop_count(p.drop);

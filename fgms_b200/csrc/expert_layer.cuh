@@ -5,8 +5,8 @@
 //   u = x[t] . W_in[e]      h = act(u), or act(first half of u) * second half where W_in is twice as wide as W_out is high
 //   out[t] = sum over j of gate[t, j] (h . W_out[e(t, j)])
 //
-// expert_logits_kernel has a block for an expert and eight tokens.  A choice hangs on the difference of two logits, so they are summed in 64 bits; every
-// expert's in the same order, so that equal rows of the router are equal.
+// expert_choice_kernel has a cluster of up to eight CTAs for a token, a warp for an expert at a time; the logits meet in the first one's shared memory.  A choice
+// hangs on the difference of two logits, so they are summed in 64 bits; every expert's in the same order, so that equal rows of the router are equal.
 //
 // expert_layer_kernel is cooperative, a CTA an SM.  What bounds it is the weights of the experts that some token goes to, each read once.  An item
 // is 64 columns of one expert's weight (gated: 32 of either half of u) with the whole contraction, in tiles of 128 rows that come by TMA, a
@@ -36,7 +36,7 @@ constexpr int EL_X_PITCH = EL_K * 2 + 16;          // tokens' rows, 16 bytes mor
 constexpr int EL_X_BYTES = 3 * EL_MAX_TOKENS * EL_X_PITCH;  // three tiles of 64 rows, or as many more as fewer rows allow: a copy's way is as long as three tiles
 constexpr int EL_CONSUMERS = 256, EL_REPORTERS = 64, EL_THREADS = EL_CONSUMERS + 64 + EL_REPORTERS, EL_WARPS = EL_THREADS / 32;
 constexpr int EL_SUMS = 16;                        // of a thread for eight tokens: 64 columns by eight a warp
-constexpr int EL_ROUTER_THREADS = 256, EL_ROUTER_TOKENS = 8;
+constexpr int EL_ROUTER_THREADS = 256, EL_ROUTER_AT_ONCE = 4;  // chunks of a row whose loads are on their way together
 
 struct ExpertParams {
   const void *x, *router;
@@ -46,54 +46,109 @@ struct ExpertParams {
   int tokens, n_experts, top_k, width, hidden, out_width, gated, activation;  // activation: 0 relu, 1 silu
   long long x_pitch, out_pitch;
   // workspace
-  double* logits;    // [tokens][n_experts]
-  uint32_t* flags;   // [experts]: items of W_in that are done, by used expert; [blocks of the output]: items of W_out; then CTAs at the barrier
+  uint32_t* flags;   // [experts]: items of W_in that are done, by used expert; [blocks of the output]: items of W_out
   uint16_t* h;       // [tokens top_k][hidden], in the order of the experts
   float* part;       // [tokens top_k][out_width]
   int ctas, stages, n_flags;
   int alone;
 };
 
-template <typename T, typename R>
-__global__ void __launch_bounds__(EL_ROUTER_THREADS) expert_logits_kernel(const __grid_constant__ ExpertParams p) {
-  __shared__ double sums[EL_ROUTER_TOKENS][EL_ROUTER_THREADS / 32];
-  umma::griddep_wait();
-  if (!p.alone) umma::griddep_launch_dependents();
-  if (blockIdx.x == 0 && blockIdx.y == 0)
-    for (int i = threadIdx.x; i < p.n_flags; i += EL_ROUTER_THREADS) p.flags[i] = 0u;
-  const int e = (int)blockIdx.x, t0 = (int)blockIdx.y * EL_ROUTER_TOKENS, n = min(EL_ROUTER_TOKENS, p.tokens - t0);
-  double sum[EL_ROUTER_TOKENS];
+// The top_k largest logits of a token, by a warp: (*expert, *gate) of lane j are the j-th one's.  A logit that is not a number counts as minus infinity (and
+// makes the gates such).
+template <int EACH>
+__device__ __forceinline__ void el_choose(const ExpertParams& p, const double* logits, int* expert, float* gate) {
+  const int lane = threadIdx.x & 31;
+  // as numbers without a sign that are ordered alike; 0 is what has been taken
+  unsigned long long v[EACH];
 #pragma unroll
-  for (int t = 0; t < EL_ROUTER_TOKENS; ++t) sum[t] = 0.0;
-  const R* row = static_cast<const R*>(p.router) + (size_t)e * p.width;
-  for (int col = (int)threadIdx.x * ROW_CHUNK; col < p.width; col += EL_ROUTER_THREADS * ROW_CHUNK) {  // the width is a multiple of a chunk
-    const RowRaw<R> w = row_load(row + col, ROW_CHUNK, true);
-    RowRaw<T> x[EL_ROUTER_TOKENS];  // all on their way together; rows behind the last token's are that one's again
-#pragma unroll
-    for (int t = 0; t < EL_ROUTER_TOKENS; ++t) x[t] = row_load(static_cast<const T*>(p.x) + (t0 + min(t, n - 1)) * p.x_pitch + col, ROW_CHUNK, true);
-    double wd[ROW_CHUNK];
-#pragma unroll
-    for (int i = 0; i < ROW_CHUNK; ++i) wd[i] = (double)row_value(w, i);
-#pragma unroll
-    for (int t = 0; t < EL_ROUTER_TOKENS; ++t) {
-      if (t >= n) break;
-#pragma unroll
-      for (int i = 0; i < ROW_CHUNK; ++i) sum[t] += (double)row_value(x[t], i) * wd[i];
+  for (int i = 0; i < EACH; ++i) {
+    v[i] = 0;
+    if (lane + 32 * i < p.n_experts) {
+      const double x = logits[lane + 32 * i] + 0.0;  // no minus zero
+      const unsigned long long bits = (unsigned long long)__double_as_longlong(x);
+      v[i] = x != x ? 0x000fffffffffffffull : bits >> 63 ? ~bits : bits | 0x8000000000000000ull;  // minus infinity is 0x000f...f
     }
   }
+  double top = 0.0;
+  float mine = 0.f, total = 0.f;
+  for (int j = 0; j < p.top_k; ++j) {
+    unsigned long long best = v[0];
 #pragma unroll
-  for (int t = 0; t < EL_ROUTER_TOKENS; ++t) {
-    if (t >= n) break;
+    for (int i = 1; i < EACH; ++i) {
+      if (32 * i >= p.n_experts) break;
+      best = max(best, v[i]);
+    }
+    // the largest of the warp's, half by half
+    const uint32_t high = __reduce_max_sync(0xffffffffu, (uint32_t)(best >> 32));
+    const uint32_t low = __reduce_max_sync(0xffffffffu, (uint32_t)(best >> 32) == high ? (uint32_t)best : 0u);
+    best = (unsigned long long)high << 32 | low;
+    uint32_t at = 0xffffffffu;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum[t] += __shfl_xor_sync(0xffffffffu, sum[t], o);
-    if ((threadIdx.x & 31) == 0) sums[t][threadIdx.x >> 5] = sum[t];
+    for (int i = EACH - 1; i >= 0; --i)
+      if (32 * i < p.n_experts && v[i] == best && lane + 32 * i < p.n_experts) at = (uint32_t)(lane + 32 * i);
+    at = __reduce_min_sync(0xffffffffu, at);
+#pragma unroll
+    for (int i = 0; i < EACH; ++i)
+      if (at == (uint32_t)(lane + 32 * i)) v[i] = 0;
+    const double value = __longlong_as_double((long long)(best >> 63 ? best & 0x7fffffffffffffffull : ~best));
+    if (j == 0) top = value;
+    const float share = expf((float)(value - top));
+    total += share;
+    if (lane == j) {
+      mine = share;
+      *expert = (int)at;
+    }
   }
-  __syncthreads();
-  if ((int)threadIdx.x < n) {
-    double v = 0.0;
+  *gate = mine / total;
+}
+template <typename T, typename R>
+__global__ void __launch_bounds__(EL_ROUTER_THREADS) expert_choice_kernel(const __grid_constant__ ExpertParams p) {
+  __shared__ double logits[EL_MAX_EXPERTS];
+  umma::griddep_wait();
+  if (!p.alone) umma::griddep_launch_dependents();
+  uint32_t rank, size;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(size));
+  const int t = (int)(blockIdx.x / size), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (blockIdx.x == 0)
+    for (int i = threadIdx.x; i < p.n_flags; i += EL_ROUTER_THREADS) p.flags[i] = 0u;
+  const T* x_row = static_cast<const T*>(p.x) + t * p.x_pitch;
+  for (int e = (int)rank + (int)size * warp; e < p.n_experts; e += (int)size * (EL_ROUTER_THREADS / 32)) {
+    const R* row = static_cast<const R*>(p.router) + (size_t)e * p.width;
+    double sum[EL_ROUTER_AT_ONCE] = {};
+    for (int col = lane * ROW_CHUNK; col < p.width; col += 32 * ROW_CHUNK * EL_ROUTER_AT_ONCE) {  // the width is a multiple of a chunk
+      RowRaw<R> w[EL_ROUTER_AT_ONCE];
+      RowRaw<T> x[EL_ROUTER_AT_ONCE];
 #pragma unroll
-    for (int i = 0; i < EL_ROUTER_THREADS / 32; ++i) v += sums[threadIdx.x][i];
-    p.logits[(size_t)(t0 + threadIdx.x) * p.n_experts + e] = v;
+      for (int i = 0; i < EL_ROUTER_AT_ONCE; ++i) {
+        const int at = col + i * 32 * ROW_CHUNK;
+        w[i] = row_load(row + at, at < p.width ? ROW_CHUNK : 0, true);
+        x[i] = row_load(x_row + at, at < p.width ? ROW_CHUNK : 0, true);
+      }
+#pragma unroll
+      for (int k = 0; k < ROW_CHUNK; ++k)
+#pragma unroll
+        for (int i = 0; i < EL_ROUTER_AT_ONCE; ++i) sum[i] += (double)row_value(x[i], k) * (double)row_value(w[i], k);
+    }
+    double v = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if (lane == 0) {
+      uint32_t there;
+      asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(there) : "r"(umma::smem_u32(logits + e)));
+      asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(there), "d"(v) : "memory");
+    }
+  }
+  umma::cluster_sync();
+  if (rank != 0 || warp != 0) return;
+  int expert = 0;
+  float gate = 0.f;
+  // few values a lane where there are few experts: code that is not there need not be fetched
+  if (p.n_experts <= 64) el_choose<2>(p, logits, &expert, &gate);
+  else el_choose<EL_MAX_EXPERTS / 32>(p, logits, &expert, &gate);
+  if (lane < p.top_k) {
+    p.experts[t * p.top_k + lane] = expert;
+    p.gates[t * p.top_k + lane] = gate;
   }
 }
 
@@ -146,16 +201,6 @@ __device__ __forceinline__ bool el_await(const uint32_t* at, uint32_t want, vola
   }
   return true;
 }
-// All consumers of all CTAs: what was written before is there behind it.
-__device__ __forceinline__ void el_grid_sync(uint32_t* counter, int ctas, volatile int* abort_flag) {
-  el_sync();
-  if (threadIdx.x == 0) {
-    el_arrive(counter);
-    el_await(counter, (uint32_t)ctas, abort_flag);
-  }
-  el_sync();
-}
-
 __device__ __forceinline__ void el_ldmatrix(uint32_t (&r)[4], uint32_t at) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
 }
@@ -175,88 +220,6 @@ __device__ __forceinline__ float el_activated(int activation, float v) { return 
 template <bool BF16>
 __device__ __forceinline__ uint16_t el_round(float v) {
   return BF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v)) : __half_as_ushort(__float2half_rn(v));
-}
-
-// The top_k largest logits of a token, by a warp: (*expert, *gate) of lane j are the j-th one's.  A logit that is not a number counts as minus infinity (and
-// makes the gates such).
-template <int EACH>
-__device__ __forceinline__ void el_choose(const ExpertParams& p, int t, int* expert, float* gate) {
-  const int lane = threadIdx.x & 31;
-  // as numbers without a sign that are ordered alike; 0 is what has been taken
-  unsigned long long v[EACH];
-#pragma unroll
-  for (int i = 0; i < EACH; ++i) {
-    v[i] = 0;
-    if (lane + 32 * i < p.n_experts) {
-      const double x = __ldcg(p.logits + (size_t)t * p.n_experts + lane + 32 * i) + 0.0;  // no minus zero
-      const unsigned long long bits = (unsigned long long)__double_as_longlong(x);
-      v[i] = x != x ? 0x000fffffffffffffull : bits >> 63 ? ~bits : bits | 0x8000000000000000ull;  // minus infinity is 0x000f...f
-    }
-  }
-  double top = 0.0;
-  float mine = 0.f, total = 0.f;
-  for (int j = 0; j < p.top_k; ++j) {
-    unsigned long long best = v[0];
-#pragma unroll
-    for (int i = 1; i < EACH; ++i) {
-      if (32 * i >= p.n_experts) break;
-      best = max(best, v[i]);
-    }
-    // the largest of the warp's, half by half
-    const uint32_t high = __reduce_max_sync(0xffffffffu, (uint32_t)(best >> 32));
-    const uint32_t low = __reduce_max_sync(0xffffffffu, (uint32_t)(best >> 32) == high ? (uint32_t)best : 0u);
-    best = (unsigned long long)high << 32 | low;
-    uint32_t at = 0xffffffffu;
-#pragma unroll
-    for (int i = EACH - 1; i >= 0; --i)
-      if (32 * i < p.n_experts && v[i] == best && lane + 32 * i < p.n_experts) at = (uint32_t)(lane + 32 * i);
-    at = __reduce_min_sync(0xffffffffu, at);
-#pragma unroll
-    for (int i = 0; i < EACH; ++i)
-      if (at == (uint32_t)(lane + 32 * i)) v[i] = 0;
-    const double value = __longlong_as_double((long long)(best >> 63 ? best & 0x7fffffffffffffffull : ~best));
-    if (j == 0) top = value;
-    const float share = expf((float)(value - top));
-    total += share;
-    if (lane == j) {
-      mine = share;
-      *expert = (int)at;
-    }
-  }
-  *gate = mine / total;
-}
-// (few values a lane where there are few experts: code that is not there need not be fetched)
-// Of all tokens, in every CTA.  Up to EL_CHOOSE_ALONE tokens each CTA does it for itself, two rounds of its warps at most; more are dealt out, a token
-// a CTA, and met at a grid barrier, which costs as much as two or three rounds.
-constexpr int EL_CHOOSE_ALONE = 2 * EL_WARPS;
-__device__ __forceinline__ void el_choose_all(const ExpertParams& p, ElShared* sh) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, cta = (int)blockIdx.x;
-  const bool alone = p.tokens <= EL_CHOOSE_ALONE;
-  for (int t = alone ? warp : cta; t < p.tokens && (alone || warp == 0); t += alone ? EL_WARPS : p.ctas) {
-    int expert = 0;
-    float gate = 0.f;
-    if (p.n_experts <= 64) el_choose<2>(p, t, &expert, &gate);
-    else el_choose<EL_MAX_EXPERTS / 32>(p, t, &expert, &gate);
-    if (lane >= p.top_k) continue;
-    const int pair = t * p.top_k + lane;
-    sh->chosen[pair] = (uint16_t)expert;
-    sh->gates[pair] = gate;
-    if (!alone || cta == 0) {
-      __stcg(p.experts + pair, expert);
-      __stcg(p.gates + pair, gate);
-    }
-  }
-  if (!alone) {
-    if (warp < EL_CONSUMERS / 32) {
-      el_grid_sync(p.flags + p.n_flags - 1, p.ctas, &sh->abort_flag);
-      for (int i = threadIdx.x; i < p.tokens * p.top_k; i += EL_CONSUMERS) {
-        // (a value that no CTA has written, after a wait that ran out, is no expert)
-        sh->chosen[i] = (uint16_t)min(max(__ldcg(p.experts + i), 0), p.n_experts - 1);
-        sh->gates[i] = __ldcg(p.gates + i);
-      }
-    }
-  }
-  __syncthreads();
 }
 
 // The pairs in the order of their experts, of an expert in the order of its tokens: a token goes to an expert once at most, so that an expert's
@@ -511,8 +474,11 @@ __global__ void __launch_bounds__(EL_THREADS, 1)
     sh->abort_flag = 0;
     mbar_fence_init();
   }
+  for (int i = threadIdx.x; i < p.tokens * p.top_k; i += EL_THREADS) {
+    sh->chosen[i] = (uint16_t)__ldcg(p.experts + i);
+    sh->gates[i] = __ldcg(p.gates + i);
+  }
   __syncthreads();
-  el_choose_all(p, sh);
   el_sort(p, sh);
   const ElPlan plan(p, sh);
   const uint32_t tiles0 = smem_u32(smem), x0 = tiles0 + (uint32_t)(p.stages * EL_TILE_BYTES);
@@ -643,7 +609,7 @@ __global__ void __launch_bounds__(EL_THREADS, 1)
 
 // Bytes of workspace, and where its parts begin.
 struct ExpertSpace {
-  size_t logits, flags, h, part, total;
+  size_t flags, h, part, total;
   int n_flags;
 };
 inline ExpertSpace expert_space(int tokens, int experts, int top_k, int hidden, int out_width) {
@@ -654,8 +620,7 @@ inline ExpertSpace expert_space(int tokens, int experts, int top_k, int hidden, 
     at += (bytes + 255) / 256 * 256;
     return here;
   };
-  s.n_flags = experts + (out_width + EL_COLUMNS - 1) / EL_COLUMNS + 1;
-  s.logits = take((size_t)tokens * experts * sizeof(double));
+  s.n_flags = experts + (out_width + EL_COLUMNS - 1) / EL_COLUMNS;
   s.flags = take((size_t)s.n_flags * sizeof(uint32_t));
   s.h = take((size_t)tokens * top_k * hidden * 2);
   s.part = take((size_t)tokens * top_k * out_width * sizeof(float));
@@ -685,8 +650,21 @@ inline int expert_tensor_map(CUtensorMap* map, const void* data, int cols, int r
 }
 
 template <typename T, typename R>
-cudaError_t launch_expert_logits(const ExpertParams& p, cudaStream_t st) {
-  return launch_pdl(expert_logits_kernel<T, R>, dim3((unsigned)p.n_experts, (unsigned)((p.tokens + EL_ROUTER_TOKENS - 1) / EL_ROUTER_TOKENS)), EL_ROUTER_THREADS, 0, st, p);
+cudaError_t launch_expert_choice(const ExpertParams& p, cudaStream_t st) {
+  const int size = p.n_experts <= 8 ? 1 : p.n_experts <= 16 ? 2 : p.n_experts <= 32 ? 4 : 8;  // a warp an expert, where eight CTAs have as many
+  cudaLaunchConfig_t lc = {};
+  lc.gridDim = dim3((unsigned)(p.tokens * size));
+  lc.blockDim = dim3(EL_ROUTER_THREADS);
+  lc.stream = st;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = (unsigned)size;
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+  lc.attrs = at;
+  lc.numAttrs = 2;
+  return cudaLaunchKernelEx(&lc, expert_choice_kernel<T, R>, p);
 }
 
 template <bool BF16>

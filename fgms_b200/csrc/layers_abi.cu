@@ -112,7 +112,7 @@ int run_dropout(const fgms_b200_dropout_args& a, bool backward, cudaStream_t st)
   p.drop.used = reinterpret_cast<long long*>(a.rng_used);
   p.alone = di.reserved > 0;
   const long long chunks = a.rows * ((a.width + fgms::ROW_CHUNK - 1) / fgms::ROW_CHUNK);
-  const long long blocks = (chunks + fgms::DROP_THREADS - 1) / fgms::DROP_THREADS, most = 8ll * di.sms;
+  const long long blocks = (chunks + fgms::DROP_THREADS - 1) / fgms::DROP_THREADS, most = (long long)fgms::DROP_BLOCKS * di.sms;
   const dim3 grid((unsigned)(blocks < most ? blocks : most));
   const auto launch = [&](auto type) {
     using T = decltype(type);
@@ -217,12 +217,16 @@ int run_rms_norm_bwd(const fgms_b200_rms_norm_bwd_args& a, cudaStream_t st) {
   const bool drop = p.drop.threshold > 0;
   const size_t es = layer_elem(a.dtype);
   const auto span = [&](const void* at, int64_t pitch) { return RowSpan{at, a.rows, pitch, a.width, es}; };
-  const RowSpan dy = span(a.out_grad, a.out_grad_pitch), h = span(a.sum, a.sum_pitch), dsum = span(a.sum_grad, a.sum_grad_pitch), dx = span(a.x_grad, a.x_grad_pitch),
+  if (a.x && (a.dtype == FGMS_DTYPE_F32 || a.weight_dtype != FGMS_DTYPE_F32))
+    return fail(FGMS_ERR_UNSUPPORTED, "x is read for rows in 16 bits with a weight in fp32; otherwise sum is");
+  const RowSpan dy = span(a.out_grad, a.out_grad_pitch), h = a.x ? span(a.x, a.x_pitch) : span(a.sum, a.sum_pitch),
+                residual = span(a.x ? a.residual : nullptr, a.residual_pitch), dsum = span(a.sum_grad, a.sum_grad_pitch), dx = span(a.x_grad, a.x_grad_pitch),
                 dresidual = span(a.residual_grad, a.residual_grad_pitch);
   const RowSpan weight{a.weight, 1, a.width, a.width, layer_elem(a.weight_dtype)}, dw{a.weight_grad, 1, a.width, a.width, layer_elem(a.weight_dtype)},
       rstd{a.rstd, 1, a.rows, a.rows, 4};
   if (int rc = check_span("out_grad", dy, true)) return rc;
-  if (int rc = check_span("sum", h, true)) return rc;
+  if (int rc = check_span(a.x ? "x" : "sum", h, true)) return rc;
+  if (int rc = check_span("residual", residual, false)) return rc;
   if (int rc = check_span("sum_grad", dsum, false)) return rc;
   if (int rc = check_span("x_grad", dx, false)) return rc;
   if (int rc = check_span("residual_grad", dresidual, false)) return rc;
@@ -237,10 +241,10 @@ int run_rms_norm_bwd(const fgms_b200_rms_norm_bwd_args& a, cudaStream_t st) {
   if (needed > 0 && (!a.workspace || a.workspace_bytes < needed || (reinterpret_cast<uintptr_t>(a.workspace) & 15)))
     return fail(FGMS_ERR_WORKSPACE, "a workspace of %zu bytes on a 16-byte boundary is needed", needed);
   const RowSpan space{needed ? a.workspace : nullptr, 1, (int64_t)needed, (int64_t)needed, 1}, used{drop ? a.rng_used : nullptr, 1, 2, 2, 8};
-  const RowSpan outputs[] = {dx, dresidual, dw, space}, inputs[] = {dy, h, dsum, weight, rstd, used};
+  const RowSpan outputs[] = {dx, dresidual, dw, space}, inputs[] = {dy, h, dsum, residual, weight, rstd, used};
   for (int i = 0; i < 4; ++i) {
-    for (int j = 0; j < 6; ++j)
-      if (outputs[i].collides(inputs[j]) || (outputs[i].same(inputs[j]) && (i >= 2 || j >= 3))) return fail(FGMS_ERR_INVALID_ARG, "an output overlaps an input");
+    for (int j = 0; j < 7; ++j)
+      if (outputs[i].collides(inputs[j]) || (outputs[i].same(inputs[j]) && (i >= 2 || j >= 4))) return fail(FGMS_ERR_INVALID_ARG, "an output overlaps an input");
     for (int j = 0; j < i; ++j)
       if (outputs[i].collides(outputs[j]) || outputs[i].same(outputs[j])) return fail(FGMS_ERR_INVALID_ARG, "two outputs overlap");
   }
@@ -251,6 +255,8 @@ int run_rms_norm_bwd(const fgms_b200_rms_norm_bwd_args& a, cudaStream_t st) {
   }
   p.dy = a.out_grad;
   p.sum = a.sum;
+  p.x = a.x;
+  p.residual = residual.p;
   p.dsum = a.sum_grad;
   p.weight = a.weight;
   p.rstd = a.rstd;
@@ -259,7 +265,9 @@ int run_rms_norm_bwd(const fgms_b200_rms_norm_bwd_args& a, cudaStream_t st) {
   p.parts = a.weight_grad ? static_cast<float*>(a.workspace) : nullptr;
   p.rows = a.rows;
   p.dy_pitch = a.out_grad_pitch;
-  p.sum_pitch = a.sum_pitch;
+  p.sum_pitch = a.x ? a.x_pitch : a.sum_pitch;
+  p.residual_pitch = a.residual_pitch;
+  p.residual_vec = residual.vec(16);
   p.dsum_pitch = a.sum_grad_pitch;
   p.dx_pitch = a.x_grad_pitch;
   p.dresidual_pitch = a.residual_grad_pitch;
@@ -442,19 +450,18 @@ int run_expert_layer(const fgms_b200_expert_layer_args& a, cudaStream_t st) {
   p.activation = a.activation == FGMS_ACTIVATION_SILU;
   p.x_pitch = a.tokens > 1 ? a.x_pitch : a.width;
   p.out_pitch = a.tokens > 1 ? a.out_pitch : a.out_width;
-  p.logits = reinterpret_cast<double*>(at + space.logits);
   p.flags = reinterpret_cast<uint32_t*>(at + space.flags);
   p.h = reinterpret_cast<uint16_t*>(at + space.h);
   p.part = reinterpret_cast<float*>(at + space.part);
   p.ctas = di.sms;
   p.n_flags = space.n_flags;
   p.alone = di.reserved > 0;
-  const cudaError_t e = with_types(a.dtype, a.router_dtype, [&](auto t, auto r) { return fgms::launch_expert_logits<decltype(t), decltype(r)>(p, st); });
+  const cudaError_t e = with_types(a.dtype, a.router_dtype, [&](auto t, auto r) { return fgms::launch_expert_choice<decltype(t), decltype(r)>(p, st); });
   if (e != cudaSuccess) {
     cudaGetLastError();
-    return fail(FGMS_ERR_CUDA, "expert_logits_kernel: %s", cudaGetErrorString(e));
+    return fail(FGMS_ERR_CUDA, "expert_choice_kernel: %s", cudaGetErrorString(e));
   }
-  if (int rc = check_launch("expert_logits_kernel")) return rc;
+  if (int rc = check_launch("expert_choice_kernel")) return rc;
   const int rc = a.dtype == FGMS_DTYPE_BF16 ? fgms::launch_expert_layer<true>(p, a.w_in, a.w_out, st, di.max_smem_optin)
                                             : fgms::launch_expert_layer<false>(p, a.w_in, a.w_out, st, di.max_smem_optin);
   if (rc != 0) return fail(FGMS_ERR_CUDA, "expert_layer_kernel: %s (%d)", cudaGetErrorString(cudaGetLastError()), rc);

@@ -17,7 +17,7 @@
 namespace fgms {
 
 constexpr int NORM_MAX_THREADS = 1024;
-constexpr int NORM_WARP_ROWS = 4;  // rows (warps) of a block where a row is a warp's
+constexpr int NORM_WARP_ROWS = 4, NORM_GRAD_WARP_ROWS = 8;  // rows (warps) of a block where a row is a warp's
 
 struct NormParams {
   const void *x, *residual, *weight;  // residual: or null; weight: null without a norm (norm = 0)
@@ -61,7 +61,7 @@ __device__ __forceinline__ uint32_t row_max(uint32_t v, uint32_t* part) {
 
 // T: rows; W: the weight; CH: chunks a thread; WARP: a row is a warp's; EIGHT: the output is codes of 8 bits
 template <typename T, typename W, int CH, bool WARP, bool EIGHT, bool DROP>
-__global__ void __launch_bounds__(WARP ? 32 * NORM_WARP_ROWS : NORM_MAX_THREADS) rms_norm_kernel(const __grid_constant__ NormParams p) {
+__global__ void __launch_bounds__(WARP ? 32 * NORM_WARP_ROWS : NORM_MAX_THREADS, 1) rms_norm_kernel(const __grid_constant__ NormParams p) {
   __shared__ float parts[4][32];
   umma::griddep_wait();
   if (!p.alone) umma::griddep_launch_dependents();
@@ -90,7 +90,7 @@ __global__ void __launch_bounds__(WARP ? 32 * NORM_WARP_ROWS : NORM_MAX_THREADS)
         if (p.residual) h[c][e] += row_value(add[c], e);
         sum += h[c][e] * h[c][e];
       }
-      if (p.sum) row_store(static_cast<T*>(p.sum) + row * p.sum_pitch + col, h[c], p.width - col, p.sum_vec);
+      if (p.sum) row_store(static_cast<T*>(p.sum) + row * p.sum_pitch + col, h[c], p.width - col, p.sum_vec, chunk == 0);
     }
     float r = 1.f;
     if (p.norm) {
@@ -101,14 +101,7 @@ __global__ void __launch_bounds__(WARP ? 32 * NORM_WARP_ROWS : NORM_MAX_THREADS)
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       const int col = (c * per_row + thread) * ROW_CHUNK, there = p.width - col;
-      if (there <= 0) {
-        if (EIGHT) {
-#pragma unroll
-          for (int e = 0; e < ROW_CHUNK; ++e) h[c][e] = 0.f;
-        }
-        continue;
-      }
-      if (p.norm) {
+      if (p.norm && there > 0) {
         float w[ROW_CHUNK];
         const W* from = static_cast<const W*>(p.weight) + col;
         if (p.weight_vec && there >= ROW_CHUNK) {  // every row reads it again: from L1
@@ -128,7 +121,7 @@ __global__ void __launch_bounds__(WARP ? 32 * NORM_WARP_ROWS : NORM_MAX_THREADS)
 #pragma unroll
         for (int e = 0; e < ROW_CHUNK; ++e) largest = max(largest, e < there ? magnitude(h[c][e]) : 0u);
       } else {
-        row_store(static_cast<T*>(p.out) + row * p.out_pitch + col, h[c], there, p.out_vec);
+        row_store(static_cast<T*>(p.out) + row * p.out_pitch + col, h[c], there, p.out_vec, col == 0);
       }
     }
     if (EIGHT) {
@@ -158,63 +151,90 @@ __global__ void __launch_bounds__(WARP ? 32 * NORM_WARP_ROWS : NORM_MAX_THREADS)
 }
 
 struct NormGradParams {
-  const void *dy, *sum, *dsum, *weight;  // dsum: or null
+  const void *dy, *sum, *x, *residual, *dsum, *weight;  // h: read from sum, or with x computed again; residual, dsum: or null
   const float* rstd;
   void *dx, *dresidual;  // either may be null
   float* parts;          // [blocks][width]: what each block's rows add to the weight's gradient, or null
-  long long rows, dy_pitch, sum_pitch, dsum_pitch, dx_pitch, dresidual_pitch;
+  long long rows, dy_pitch, sum_pitch, residual_pitch, dsum_pitch, dx_pitch, dresidual_pitch;  // sum_pitch: x's
   int width;
-  bool dy_vec, sum_vec, dsum_vec, dx_vec, dresidual_vec, weight_vec;
+  bool dy_vec, sum_vec, residual_vec, dsum_vec, dx_vec, dresidual_vec, weight_vec;
   float inverse_width;
   DropParams drop;
   int alone;
 };
 
-// The block's rows one after the other, their share of the weight's gradient in registers until the last one.
-template <typename T, typename W, int CH, bool WARP, bool DROP, int THREADS>
-__global__ void __launch_bounds__(THREADS) rms_norm_grad_kernel(const __grid_constant__ NormGradParams p) {
+// The block's rows one after the other, the next one's values on their way meanwhile; their share of the weight's gradient in registers until the last
+// one.  FROM_X: h = residual + drop(x) once more, unrounded, for a weight whose gradient holds more than the h that was stored: rows in bf16 with a weight in fp32
+// have its gradient off by 2^-9.3 with that, by 2^-22 so, for a read more.
+template <typename T, typename W, int CH, bool WARP, bool DROP, bool FROM_X, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1) rms_norm_grad_kernel(const __grid_constant__ NormGradParams p) {
+  constexpr bool AHEAD = CH * sizeof(T) <= 4;  // where the registers are there
   __shared__ float parts[2][32];
-  __shared__ float share[WARP ? NORM_WARP_ROWS : 1][WARP ? 32 * CH * ROW_CHUNK : 1];
+  __shared__ float share[WARP ? NORM_GRAD_WARP_ROWS : 1][WARP ? 32 * CH * ROW_CHUNK : 1];
   umma::griddep_wait();
   if (!p.alone) umma::griddep_launch_dependents();
   DropKey key;
   if (DROP) key = drop_key(p.drop.used);
   const int per_row = WARP ? 32 : (int)blockDim.x, thread = WARP ? (int)threadIdx.x & 31 : (int)threadIdx.x;
-  const long long rows_at_once = WARP ? (long long)gridDim.x * NORM_WARP_ROWS : (long long)gridDim.x;
+  const long long rows_at_once = WARP ? (long long)gridDim.x * NORM_GRAD_WARP_ROWS : (long long)gridDim.x;
   float dw[CH][ROW_CHUNK];
 #pragma unroll
   for (int c = 0; c < CH; ++c)
 #pragma unroll
     for (int e = 0; e < ROW_CHUNK; ++e) dw[c][e] = 0.f;
-  int turn = 0;
-  for (long long row = WARP ? (long long)blockIdx.x * NORM_WARP_ROWS + (threadIdx.x >> 5) : (long long)blockIdx.x; row < p.rows; row += rows_at_once) {
-    RowRaw<T> dy[CH], h[CH], extra[CH];
-    RowRaw<W> w[CH];
+  RowRaw<T> dy[CH], h[CH], add[CH], extra[CH], next_dy[AHEAD ? CH : 1], next_h[AHEAD ? CH : 1], next_add[AHEAD ? CH : 1], next_extra[AHEAD ? CH : 1];
+  float r = 0.f, next_r = 0.f;
+  const auto load = [&](long long row, auto& dy, auto& h, auto& add, auto& extra, float& r) {
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       const int col = (c * per_row + thread) * ROW_CHUNK, there = p.width - col;
       dy[c] = row_load(static_cast<const T*>(p.dy) + row * p.dy_pitch + col, there, p.dy_vec);
-      h[c] = row_load(static_cast<const T*>(p.sum) + row * p.sum_pitch + col, there, p.sum_vec);
+      h[c] = row_load(static_cast<const T*>(FROM_X ? p.x : p.sum) + row * p.sum_pitch + col, there, p.sum_vec);
+      if (FROM_X && p.residual) add[c] = row_load(static_cast<const T*>(p.residual) + row * p.residual_pitch + col, there, p.residual_vec);
       if (p.dsum) extra[c] = row_load(static_cast<const T*>(p.dsum) + row * p.dsum_pitch + col, there, p.dsum_vec);
     }
-    const float r = __ldg(p.rstd + row);
+    r = __ldg(p.rstd + row);
+  };
+  int turn = 0;
+  long long row = WARP ? (long long)blockIdx.x * NORM_GRAD_WARP_ROWS + (threadIdx.x >> 5) : (long long)blockIdx.x;
+  if (AHEAD && row < p.rows) load(row, dy, h, add, extra, r);
+  for (; row < p.rows; row += rows_at_once) {
+    if constexpr (AHEAD) {
+      if (row + rows_at_once < p.rows) load(row + rows_at_once, next_dy, next_h, next_add, next_extra, next_r);
+    } else {
+      load(row, dy, h, add, extra, r);
+    }
+    uint32_t keep[CH];
+    RowRaw<W> w[CH];
     const auto weights = [&](int c) {
       const int col = (c * per_row + thread) * ROW_CHUNK, there = p.width - col;
       const W* from = static_cast<const W*>(p.weight) + col;
-      if (p.weight_vec && there >= ROW_CHUNK) {
+      if (p.weight_vec && there >= ROW_CHUNK) {  // every row reads it again: from L1
 #pragma unroll
-        for (int q = 0; q < (int)sizeof(W) / 2; ++q) *reinterpret_cast<uint4*>(w[c].w + 4 * q) = __ldg(reinterpret_cast<const uint4*>(from) + q);
+        for (int q = 0; q < (int)sizeof(W) / 2; ++q) {
+          const uint4 v = __ldg(reinterpret_cast<const uint4*>(from) + q);
+          w[c].w[4 * q] = v.x; w[c].w[4 * q + 1] = v.y; w[c].w[4 * q + 2] = v.z; w[c].w[4 * q + 3] = v.w;
+        }
       } else {
         w[c] = row_load(from, there, false);
       }
     };
+    const auto sum_of = [&](int c, int e) {
+      float v = row_value(h[c], e);
+      if (FROM_X) {
+        if (DROP) v = keep[c] >> e & 1u ? v * p.drop.factor : 0.f;
+        if (p.residual) v += row_value(add[c], e);
+      }
+      return v;
+    };
     float dot = 0.f;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
+      if (DROP) keep[c] = drop_keep(key, (uint32_t)(c * per_row + thread), (uint32_t)row, p.drop.threshold);
       weights(c);
 #pragma unroll
       for (int e = 0; e < ROW_CHUNK; ++e) {
-        const float n = row_value(h[c], e) * r, d = row_value(dy[c], e);
+        const float n = sum_of(c, e) * r, d = row_value(dy[c], e);
         dot += d * row_value(w[c], e) * n;
         dw[c][e] += d * n;
       }
@@ -224,23 +244,31 @@ __global__ void __launch_bounds__(THREADS) rms_norm_grad_kernel(const __grid_con
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       const int chunk = c * per_row + thread, col = chunk * ROW_CHUNK, there = p.width - col;
-      if (there <= 0) continue;
       if (CH > 1) weights(c);  // again from L1, instead of registers meanwhile
       float dh[ROW_CHUNK];
 #pragma unroll
       for (int e = 0; e < ROW_CHUNK; ++e) {
-        dh[e] = r * (row_value(dy[c], e) * row_value(w[c], e) - row_value(h[c], e) * r * mean);
+        dh[e] = r * (row_value(dy[c], e) * row_value(w[c], e) - sum_of(c, e) * r * mean);
         if (p.dsum) dh[e] += row_value(extra[c], e);
       }
-      if (p.dresidual) row_store(static_cast<T*>(p.dresidual) + row * p.dresidual_pitch + col, dh, there, p.dresidual_vec);
+      if (p.dresidual) row_store(static_cast<T*>(p.dresidual) + row * p.dresidual_pitch + col, dh, there, p.dresidual_vec, chunk == 0);
       if (p.dx) {
         if (DROP) {
-          const uint32_t keep = drop_keep(key, (uint32_t)chunk, (uint32_t)row, p.drop.threshold);
 #pragma unroll
-          for (int e = 0; e < ROW_CHUNK; ++e) dh[e] = keep >> e & 1u ? dh[e] * p.drop.factor : 0.f;
+          for (int e = 0; e < ROW_CHUNK; ++e) dh[e] = keep[c] >> e & 1u ? dh[e] * p.drop.factor : 0.f;
         }
-        row_store(static_cast<T*>(p.dx) + row * p.dx_pitch + col, dh, there, p.dx_vec);
+        row_store(static_cast<T*>(p.dx) + row * p.dx_pitch + col, dh, there, p.dx_vec, chunk == 0);
       }
+    }
+    if constexpr (AHEAD) {
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        dy[c] = next_dy[c];
+        h[c] = next_h[c];
+        add[c] = next_add[c];
+        extra[c] = next_extra[c];
+      }
+      r = next_r;
     }
   }
   if (!p.parts) return;
@@ -252,25 +280,31 @@ __global__ void __launch_bounds__(THREADS) rms_norm_grad_kernel(const __grid_con
 #pragma unroll
       for (int e = 0; e < ROW_CHUNK; ++e) share[warp][(c * 32 + thread) * ROW_CHUNK + e] = dw[c][e];
     __syncthreads();
-    for (int col = (int)threadIdx.x; col < p.width; col += 32 * NORM_WARP_ROWS) {
+    for (int col = (int)threadIdx.x; col < p.width; col += 32 * NORM_GRAD_WARP_ROWS) {
       float sum = 0.f;
 #pragma unroll
-      for (int i = 0; i < NORM_WARP_ROWS; ++i) sum += share[i][col];
+      for (int i = 0; i < NORM_GRAD_WARP_ROWS; ++i) sum += share[i][col];
       to[col] = sum;
     }
   } else {
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       const int col = (c * per_row + thread) * ROW_CHUNK;
+      if ((p.width & 3) == 0) {
 #pragma unroll
-      for (int e = 0; e < ROW_CHUNK; ++e)
-        if (col + e < p.width) to[col + e] = dw[c][e];
+        for (int q = 0; q < 2; ++q)
+          if (col + 4 * q < p.width) *reinterpret_cast<float4*>(to + col + 4 * q) = make_float4(dw[c][4 * q], dw[c][4 * q + 1], dw[c][4 * q + 2], dw[c][4 * q + 3]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < ROW_CHUNK; ++e)
+          if (col + e < p.width) to[col + e] = dw[c][e];
+      }
     }
   }
 }
 
-// The blocks' shares in their order, 32 columns a block: eight rows of threads take every eighth share each and are added up in their order.
-constexpr int NORM_SHARES_Y = 8;
+// The blocks' shares in their order, 32 columns a block: 32 rows of threads take every 32nd share each and are added up in their order.
+constexpr int NORM_SHARES_Y = 32;
 template <typename W>
 __global__ void __launch_bounds__(32 * NORM_SHARES_Y) rms_norm_weight_grad_kernel(const float* __restrict__ parts, int n, int width, W* dw, int alone) {
   __shared__ float sums[NORM_SHARES_Y][32];
@@ -328,20 +362,27 @@ inline NormGradCut norm_grad_cut(long long rows, int width, int sms) {
   NormGradCut c;
   c.warp = width <= 512;
   c.ch = width <= 256 ? 1 : width <= 512 ? 2 : width <= 4096 ? 1 : width <= 8192 ? 2 : 4;
-  c.threads = c.warp ? 32 * NORM_WARP_ROWS : norm_threads(width, c.ch);
-  const long long blocks = c.warp ? (rows + NORM_WARP_ROWS - 1) / NORM_WARP_ROWS : rows, at_once = (long long)sms * (c.threads <= 1024 ? 1024 / c.threads : 1);
+  c.threads = c.warp ? 32 * NORM_GRAD_WARP_ROWS : norm_threads(width, c.ch);
+  const long long blocks = c.warp ? (rows + NORM_GRAD_WARP_ROWS - 1) / NORM_GRAD_WARP_ROWS : rows, at_once = (long long)sms * (c.threads <= 768 ? 768 / c.threads : 1);
   c.blocks = (int)(blocks < at_once ? blocks : at_once);
   return c;
 }
 template <typename T, typename W, int CH, bool WARP, int THREADS>
 cudaError_t launch_rms_norm_grad_as(const NormGradParams& p, const NormGradCut& cut, cudaStream_t st) {
   const dim3 grid((unsigned)cut.blocks);
-  if (p.drop.threshold > 0) return launch_pdl(rms_norm_grad_kernel<T, W, CH, WARP, true, THREADS>, grid, cut.threads, 0, st, p);
-  return launch_pdl(rms_norm_grad_kernel<T, W, CH, WARP, false, THREADS>, grid, cut.threads, 0, st, p);
+  const bool drop = p.drop.threshold > 0;
+  if constexpr (!std::is_same<T, W>::value) {
+    if (p.x)
+      return drop ? launch_pdl(rms_norm_grad_kernel<T, W, CH, WARP, true, true, THREADS>, grid, cut.threads, 0, st, p)
+                  : launch_pdl(rms_norm_grad_kernel<T, W, CH, WARP, false, true, THREADS>, grid, cut.threads, 0, st, p);
+  }
+  return drop ? launch_pdl(rms_norm_grad_kernel<T, W, CH, WARP, true, false, THREADS>, grid, cut.threads, 0, st, p)
+              : launch_pdl(rms_norm_grad_kernel<T, W, CH, WARP, false, false, THREADS>, grid, cut.threads, 0, st, p);
 }
 template <typename T, typename W>
 cudaError_t launch_rms_norm_grad(const NormGradParams& p, const NormGradCut& cut, cudaStream_t st) {
-  if (cut.warp) return cut.ch == 1 ? launch_rms_norm_grad_as<T, W, 1, true, 32 * NORM_WARP_ROWS>(p, cut, st) : launch_rms_norm_grad_as<T, W, 2, true, 32 * NORM_WARP_ROWS>(p, cut, st);
+  if (cut.warp)
+    return cut.ch == 1 ? launch_rms_norm_grad_as<T, W, 1, true, 32 * NORM_GRAD_WARP_ROWS>(p, cut, st) : launch_rms_norm_grad_as<T, W, 2, true, 32 * NORM_GRAD_WARP_ROWS>(p, cut, st);
   if (cut.ch == 1) return launch_rms_norm_grad_as<T, W, 1, false, 512>(p, cut, st);
   return cut.ch == 2 ? launch_rms_norm_grad_as<T, W, 2, false, 512>(p, cut, st) : launch_rms_norm_grad_as<T, W, 4, false, 1024>(p, cut, st);
 }

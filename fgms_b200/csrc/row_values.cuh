@@ -13,9 +13,28 @@ template <typename T>
 struct RowRaw {
   uint32_t w[2 * sizeof(T)];
 };
-// `there` of the eight values from `p` on (at most eight; none: zeros); vec: rows start on 16-byte boundaries.  Values that are read once pass L1 by.
+// The bytes from `off` on (0 .. 15, a multiple of the values' size, the same in all lanes) of N words and the four behind them.
+template <int N>
+__device__ __forceinline__ void row_shift_down(uint32_t (&w)[N + 4], uint32_t off) {
+  if (off & 8u) {
+#pragma unroll
+    for (int i = 0; i < N + 2; ++i) w[i] = w[i + 2];
+  }
+  if (off & 4u) {
+#pragma unroll
+    for (int i = 0; i < N + 1; ++i) w[i] = w[i + 1];
+  }
+  if (off & 2u) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], 16);
+  }
+}
+// `there` of the eight values from `p` on (at most eight; none: zeros); vec: rows start on 16-byte boundaries.  Values that are read once pass L1 by.  Off such a
+// boundary the 16-byte blocks that the values lie in are read, whose other bytes are a neighbour's (or behind the last row's end, in a block that row is
+// in as well), and shifted: 16384 rows of 1001 fp16 values take XXX us so, and YYY a value at a time.
 template <typename T>
-__device__ __forceinline__ RowRaw<T> row_load(const T* __restrict__ p, int there, bool vec) {
+__device__ __forceinline__ RowRaw<T> row_load(const T* p, int there, bool vec) {
+  constexpr int N = 2 * sizeof(T);
   RowRaw<T> r;
   if (vec && there >= ROW_CHUNK) {
     const uint4 a = __ldcs(reinterpret_cast<const uint4*>(p));
@@ -26,13 +45,25 @@ __device__ __forceinline__ RowRaw<T> row_load(const T* __restrict__ p, int there
     }
     return r;
   }
+  const uint32_t off = (uint32_t)reinterpret_cast<uintptr_t>(p) & 15u;
+  const uint4* blocks = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(p) & ~(uintptr_t)15);
+  const int bytes = min(there, ROW_CHUNK) * (int)sizeof(T) + (int)off;  // that are needed, from the first block on
+  uint32_t w[N + 4];
 #pragma unroll
-  for (int i = 0; i < (int)(2 * sizeof(T)); ++i) r.w[i] = 0u;
+  for (int i = 0; i < N / 4 + 1; ++i) {
+    const uint4 v = there > 0 && bytes > 16 * i ? __ldca(blocks + i) : make_uint4(0, 0, 0, 0);
+    w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+  }
+  row_shift_down<N>(w, off);
 #pragma unroll
-  for (int e = 0; e < ROW_CHUNK; ++e) {
-    if (e >= there) continue;
-    if constexpr (sizeof(T) == 4) r.w[e] = reinterpret_cast<const uint32_t*>(p)[e];
-    else r.w[e / 2] |= (uint32_t)reinterpret_cast<const uint16_t*>(p)[e] << (16 * (e % 2));
+  for (int i = 0; i < N; ++i) {
+    r.w[i] = w[i];
+    if (sizeof(T) == 4) {
+      if (i >= there) r.w[i] = 0u;
+    } else {
+      if (2 * i >= there) r.w[i] = 0u;
+      else if (2 * i + 1 >= there) r.w[i] &= 0xffffu;
+    }
   }
   return r;
 }
@@ -46,20 +77,46 @@ __device__ __forceinline__ float row_value(const RowRaw<T>& r, int e) {
     else return __uint_as_float((uint32_t)h << 16);
   }
 }
-// rounded once to their type
+// Rounded once to their type.  All lanes of a warp call it (with none there, if it must be); lanes that follow one another hold chunks that do, of the
+// same row as long as there are any.  Off 16-byte boundaries (`vec` false) a lane takes the next one's first values and stores the 16-byte blocks that its own
+// values end in; what the warp's first and last chunk, or a row's, have beyond such blocks goes value by value.
 template <typename T>
-__device__ __forceinline__ void row_store(T* p, const float (&x)[ROW_CHUNK], int there, bool vec) {
+__device__ __forceinline__ void row_store(T* p, const float (&x)[ROW_CHUNK], int there, bool vec, bool first_of_row) {
+  constexpr int N = 2 * sizeof(T), EACH = 4 / sizeof(T);  // words; values of a word
   __align__(16) T h[ROW_CHUNK];
 #pragma unroll
   for (int e = 0; e < ROW_CHUNK; ++e) h[e] = from_f32<T>(x[e]);
-  if (vec && there >= ROW_CHUNK) {
+  if (vec) {
+    if (there >= ROW_CHUNK) {
 #pragma unroll
-    for (int q = 0; q < (int)sizeof(T) / 2; ++q) reinterpret_cast<uint4*>(p)[q] = reinterpret_cast<const uint4*>(h)[q];
-  } else {
+      for (int q = 0; q < (int)sizeof(T) / 2; ++q) reinterpret_cast<uint4*>(p)[q] = reinterpret_cast<const uint4*>(h)[q];
+    } else {
 #pragma unroll
-    for (int e = 0; e < ROW_CHUNK; ++e)
-      if (e < there) p[e] = h[e];
+      for (int e = 0; e < ROW_CHUNK; ++e)
+        if (e < there) p[e] = h[e];
+    }
+    return;
   }
+  const int lane = threadIdx.x & 31;
+  const uint32_t off = (uint32_t)reinterpret_cast<uintptr_t>(p) & 15u;
+  const int head = (int)((16u - off) & 15u) / (int)sizeof(T);  // values in front of the first block that begins inside this chunk
+  uint32_t w[N + 4];
+#pragma unroll
+  for (int i = 0; i < N; ++i) w[i] = reinterpret_cast<const uint32_t*>(h)[i];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[N + i] = __shfl_down_sync(0xffffffffu, w[i], 1);
+  const bool joined = lane < 31 && there - ROW_CHUNK >= head;       // the next chunk has the values that this one's last block lacks
+  const bool covered = lane > 0 && !first_of_row && there >= head;  // and the one before has stored this one's head
+  const int whole = joined ? N / 4 : there >= ROW_CHUNK ? (ROW_CHUNK - head) * (int)sizeof(T) / 16 : 0;  // blocks that are stored
+  row_shift_down<N>(w, (16u - off) & 15u);
+  uint4* blocks = reinterpret_cast<uint4*>(p + head);
+#pragma unroll
+  for (int i = 0; i < N / 4; ++i)
+    if (i < whole) blocks[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+  const int stored_to = whole > 0 ? head + whole * 4 * EACH : head;  // from `head` on
+#pragma unroll
+  for (int e = 0; e < ROW_CHUNK; ++e)
+    if (e < there && (e < head ? !covered : e >= stored_to)) p[e] = h[e];
 }
 
 // ---------------------------------------------------------------------------------------------

@@ -845,15 +845,18 @@ void rms_norm(const NormCall& c) {
 }
 
 struct NormGradCall {
-  const Tensor &out_grad, &sum, &weight, &rstd;
-  const Tensor *sum_grad, *x_grad, *residual_grad, *weight_grad, *used;
+  const Tensor &out_grad, &weight, &rstd;
+  const Tensor *sum, *x, *residual, *sum_grad, *x_grad, *residual_grad, *weight_grad, *used;  // sum, or x with residual or none
   double p;
 };
 void rms_norm_bwd(const NormGradCall& c) {
-  const Tensor& h = c.sum;
+  TORCH_CHECK_VALUE((c.sum != nullptr) != (c.x != nullptr), "either h or x is needed");
+  TORCH_CHECK_VALUE(c.x || !c.residual, "residual goes with x");
+  const Tensor& h = c.x ? *c.x : *c.sum;
   fgms_b200_rms_norm_bwd_args a = {};
   a.dtype = layer_dtype(h);
-  check_row_values("h", h, h.scalar_type(), h);
+  check_row_values(c.x ? "x" : "h", h, h.scalar_type(), h);
+  if (c.residual) check_row_values("residual", *c.residual, h.scalar_type(), h);
   check_row_values("out_grad", c.out_grad, h.scalar_type(), h);
   if (c.sum_grad) check_row_values("h_grad", *c.sum_grad, h.scalar_type(), h);
   if (c.x_grad) check_row_values("x_grad", *c.x_grad, h.scalar_type(), h);
@@ -868,8 +871,9 @@ void rms_norm_bwd(const NormGradCall& c) {
   if (h.size(1) == 0) return;
   a.out_grad = ptr(c.out_grad);
   a.out_grad_pitch = pitch(c.out_grad);
-  a.sum = ptr(h);
-  a.sum_pitch = pitch(h);
+  (c.x ? a.x : a.sum) = ptr(h);
+  (c.x ? a.x_pitch : a.sum_pitch) = pitch(h);
+  if (c.residual) a.residual = ptr(*c.residual), a.residual_pitch = pitch(*c.residual);
   if (c.sum_grad) a.sum_grad = ptr(*c.sum_grad), a.sum_grad_pitch = pitch(*c.sum_grad);
   if (c.x_grad) a.x_grad = ptr(*c.x_grad), a.x_grad_pitch = pitch(*c.x_grad);
   if (c.residual_grad) a.residual_grad = ptr(*c.residual_grad), a.residual_grad_pitch = pitch(*c.residual_grad);
@@ -939,6 +943,9 @@ void check_norm_shapes(const Tensor& x, const Tensor& weight, const Tensor* resi
   TORCH_CHECK_VALUE(!residual || residual->sizes() == x.sizes(), "residual must have the shape of x");
 }
 
+// Where the weight's gradient holds more than the stored sum does.
+bool exact_sum_needed(const Tensor& x, const Tensor& weight) { return weight.scalar_type() == at::kFloat && x.scalar_type() != at::kFloat; }
+
 // The norm of one call: out, and with a residual or dropout the sum that it is the norm of.
 struct Normed {
   Tensor out, sum, rstd, used;  // 2-D, but out and sum
@@ -951,7 +958,7 @@ Normed norm_forward(const Tensor& x_, const Tensor& weight_, const Tensor* resid
   const bool drop = drops(p);
   const Tensor out = as_rows(n.out);
   Tensor sum;
-  if (residual_ || (drop && for_backward)) {
+  if (residual_ || (drop && for_backward && !exact_sum_needed(x_, weight_))) {
     n.sum = at::empty_like(n.out);
     sum = as_rows(n.sum);
   }
@@ -969,7 +976,9 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
     Normed n = norm_forward(x, weight, residual ? &*residual : nullptr, eps, p, rng ? &*rng : nullptr, true);
     ctx->saved_data["p"] = p;
     ctx->saved_data["residual"] = residual.has_value();
-    ctx->save_for_backward({n.sum.defined() ? n.sum : x, weight, n.rstd, n.used});
+    const bool from_x = (residual || drops(p)) && weight.requires_grad() && exact_sum_needed(x, weight);
+    ctx->saved_data["from_x"] = from_x;
+    ctx->save_for_backward({from_x || !n.sum.defined() ? x : n.sum, weight, n.rstd, n.used, from_x && residual ? *residual : Tensor()});
     ctx->set_materialize_grads(false);
     if (residual) return {n.out, n.sum};
     return {n.out};
@@ -986,8 +995,10 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
     if (want_x) x_grad = new_like(h);
     if (want_residual && (drop || !want_x)) residual_grad = new_like(h);
     if (ctx->needs_input_grad(1)) weight_grad = new_like(weight);
-    rms_norm_bwd({dy, h, weight, saved[2], maybe_tensor(dsum), maybe_tensor(x_grad), maybe_tensor(residual_grad), maybe_tensor(weight_grad),
-                  maybe_tensor(saved[3]), p});
+    const bool from_x = ctx->saved_data["from_x"].toBool();
+    const Tensor added = saved[4].defined() ? as_rows(saved[4]) : Tensor();
+    rms_norm_bwd({dy, weight, saved[2], from_x ? nullptr : &h, from_x ? &h : nullptr, maybe_tensor(added), maybe_tensor(dsum), maybe_tensor(x_grad),
+                  maybe_tensor(residual_grad), maybe_tensor(weight_grad), maybe_tensor(saved[3]), p});
     if (x_grad.defined()) x_grad = x_grad.view(saved[0].sizes());
     if (residual_grad.defined()) residual_grad = residual_grad.view(saved[0].sizes());
     if (want_residual && !residual_grad.defined()) residual_grad = x_grad;  // the same values
@@ -1459,12 +1470,12 @@ PyObject* py_rms_norm_into(PyObject*, PyObject* const* a, Py_ssize_t n) {
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
 }
-// (out_grad, h, weight, rstd, x_grad, weight_grad, h_grad, residual_grad, p, rng_used)
+// (out_grad, h, weight, rstd, x_grad, weight_grad, h_grad, residual_grad, p, rng_used, x, residual)
 PyObject* py_rms_norm_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  expect(n, 10);
-  rms_norm_bwd({feat_arg(a[0], "out_grad"), feat_arg(a[1], "h"), feat_arg(a[2], "weight"), feat_arg(a[3], "rstd"), maybe_arg(a[6], "h_grad"),
-                maybe_arg(a[4], "x_grad"), maybe_arg(a[7], "residual_grad"), maybe_arg(a[5], "weight_grad"), maybe_arg(a[9], "rng_used"), double_arg(a[8])});
+  expect(n, 12);
+  rms_norm_bwd({feat_arg(a[0], "out_grad"), feat_arg(a[2], "weight"), feat_arg(a[3], "rstd"), maybe_arg(a[1], "h"), maybe_arg(a[10], "x"),
+                maybe_arg(a[11], "residual"), maybe_arg(a[6], "h_grad"), maybe_arg(a[4], "x_grad"), maybe_arg(a[7], "residual_grad"), maybe_arg(a[5], "weight_grad"), maybe_arg(a[9], "rng_used"), double_arg(a[8])});
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
 }

@@ -387,7 +387,8 @@ typedef struct {
 
 int fgms_b200_rms_norm(const fgms_b200_rms_norm_args* args, void* stream);
 
-/* Its gradient, from `sum` (x itself where there was neither residual nor dropout) and `rstd`:
+/* Its gradient, from `sum` (x itself where there was neither residual nor dropout) and `rstd`; or, rows in 16 bits with an F32 weight, from `x` and
+ * `residual`, with which h is computed once more, so that the weight's gradient does not see the rounding of `sum` (which may be NULL then):
  *   residual_grad = dh = rstd (g - n mean(g n)) + sum_grad     with g = out_grad weight, n = sum rstd
  *   x_grad = dh where x was kept, times the factor             weight_grad = sum over the rows of out_grad n, added up in fp32 in a fixed order
  * sum_grad (what else flows back into `sum`), x_grad, residual_grad and weight_grad (weight_dtype) may each be NULL; weight_grad needs a
@@ -395,13 +396,15 @@ int fgms_b200_rms_norm(const fgms_b200_rms_norm_args* args, void* stream);
 typedef struct {
   const void* out_grad;
   const void* sum;
+  const void* x;        /* or NULL */
+  const void* residual; /* with x; or NULL */
   const void* sum_grad; /* or NULL */
   const void* weight;
   const float* rstd;
   void* x_grad;        /* or NULL */
   void* residual_grad; /* or NULL */
   void* weight_grad;   /* or NULL */
-  int64_t out_grad_pitch, sum_pitch, sum_grad_pitch, x_grad_pitch, residual_grad_pitch;
+  int64_t out_grad_pitch, sum_pitch, x_pitch, residual_pitch, sum_grad_pitch, x_grad_pitch, residual_grad_pitch;
   int64_t rows, width;
   const int64_t* rng_used; /* p > 0 */
   void* workspace;

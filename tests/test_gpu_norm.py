@@ -180,7 +180,7 @@ def test_strides_alignment_and_shapes(dtype):
     c = Case(dtype, 70, 264)
     want, total = nn.rms_norm(c.x, c.w, residual=c.res)
     wide = made(9, 70, 900, dtype=t)
-    for at in (0, 1, 8, 271):  # on and off 16-byte boundaries
+    for at in (0, 1, 2, 3, 5, 7, 8, 271):  # on and off 16-byte boundaries
         x, out = wide[:, at:at + 264], wide[:, at + 300:at + 564]
         x.copy_(c.x)
         keep = wide.clone()
@@ -203,6 +203,39 @@ def test_strides_alignment_and_shapes(dtype):
     assert torch.equal(codes, again) and torch.equal(scale, scales)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("width", [1, 7, 9, 31, 255, 257, 1003, 2046, 5001, 9999, 20001])
+def test_rows_off_every_boundary(dtype, width):
+    """Rows at every distance from a 16-byte boundary, on both sides of what stays as it was: the same bits as aligned rows, nothing else written."""
+    from fgms_b200 import backend, nn
+    c = Case(dtype, 21, width, seed=width)
+    rng, rstd, used = nn.rng_state(SEED), torch.empty(21, device="cuda"), torch.empty(2, dtype=torch.int64, device="cuda")
+    room = (width + 39) // 8 * 8
+    plain = lambda t: torch.zeros((21, room), dtype=t.dtype, device="cuda")[:, :width].copy_(t)  # rows on boundaries
+    x, res, dy = plain(c.x), plain(c.res), plain(c.dy)
+    out, total, dx, dropped = plain(c.x), plain(c.x), plain(c.x), plain(c.x)
+    dw = torch.empty_like(c.w)
+
+    def run(x, res, dy, out, total, dx, dropped):
+        backend.fgms_rms_norm_cuda(x, c.w, out, residual=res, residual_out=total, rstd=rstd, dropout=0.25, rng=rng, rng_used=used)
+        backend.fgms_rms_norm_bwd_cuda(dy, total, c.w, rstd, x_grad=dx, weight_grad=dw, h_grad=res, dropout=0.25, rng_used=used)
+        backend.fgms_dropout_cuda(x, dropped, 0.25, rng, residual=dy)
+        return dw.clone()
+
+    want = run(x, res, dy, out, total, dx, dropped)
+    for shift in (1, 2, 3, 4, 5, 6, 7):
+        rng.copy_(nn.rng_state(SEED))
+        flat = [torch.full((21 * (width + 3) + 16,), 5.0, dtype=c.x.dtype, device="cuda") for _ in range(7)]
+        views = [f[shift:shift + 21 * (width + 3)].view(21, width + 3)[:, :width] for f in flat]  # every row at another distance
+        for v, t in zip(views, (x, res, dy)):
+            v.copy_(t)
+        assert torch.equal(run(*views), want)
+        assert all(torch.equal(a, b) for a, b in zip(views, (x, res, dy, out, total, dx, dropped)))
+        for f, v in zip(flat, views):
+            v.fill_(5.0)
+            assert (f == 5.0).all()
+
+
 def test_gradients_in_pieces():
     """What is asked for alone is what it is together; gradients that are expanded; a sum whose gradient alone is given."""
     from fgms_b200 import backend, nn
@@ -223,8 +256,18 @@ def test_gradients_in_pieces():
     backend.fgms_rms_norm_cuda(c.x, c.w, out, residual=c.res, residual_out=total, rstd=rstd, dropout=0.5, rng=nn.rng_state(SEED), rng_used=used)
     assert torch.equal(out, y) and torch.equal(total, h) and used.tolist() == [SEED, 0]
     dx, dres, dw = c.dy.clone(), torch.empty_like(c.x), torch.empty_like(c.w)
-    backend.fgms_rms_norm_bwd_cuda(dx, total, c.w, rstd, x_grad=dx, weight_grad=dw, h_grad=c.dsum, residual_grad=dres, dropout=0.5, rng_used=used)  # dx over dy
+    backend.fgms_rms_norm_bwd_cuda(dx, None, c.w, rstd, x_grad=dx, weight_grad=dw, h_grad=c.dsum, residual_grad=dres, dropout=0.5, rng_used=used, x=c.x,
+                                   residual=c.res)  # dx over dy
     assert torch.equal(dx, both[0]) and torch.equal(dw, both[1]) and torch.equal(dres, both[2])
+    ref = Norm(c.x, c.w, 1e-6, c.res, mask_of(c, 0.5))
+    ref.stored = ref.unit  # from the sum as it was stored
+    grads = torch.empty_like(c.x), torch.empty_like(c.x), torch.empty_like(c.w)
+    backend.fgms_rms_norm_bwd_cuda(c.dy, total, c.w, rstd, x_grad=grads[0], residual_grad=grads[1], weight_grad=grads[2], h_grad=c.dsum, dropout=0.5, rng_used=used)
+    for got, want in zip(grads, ref.backward(c.dy, c.dsum, torch.float32)):
+        near(got, *want)
+    for args in (dict(h=None), dict(h=total, x=c.x), dict(h=total, residual=c.res)):
+        with pytest.raises(ValueError, match="either h or x|goes with x"):
+            backend.fgms_rms_norm_bwd_cuda(c.dy, weight=c.w, rstd=rstd, x_grad=grads[0], **args)
     with pytest.raises(RuntimeError, match="not differentiable twice"):
         y, h = nn.rms_norm(leaves[0], leaves[1], residual=leaves[2])
         grads = torch.autograd.grad((y * y).sum(), leaves, create_graph=True)

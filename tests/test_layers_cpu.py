@@ -79,6 +79,8 @@ def test_the_gradient_refuses():
                          (dict(dtype=9), "dtype"), (dict(x_grad_pitch=3), "apart"), (dict(residual_grad=6 * P + 1), "boundary")):
         assert bwd(**change) == _lib.ERR_INVALID_ARG and text in _lib.last_error(), _lib.last_error()
     assert bwd(weight_dtype=_lib.DTYPE_BF16) == _lib.ERR_UNSUPPORTED
+    assert bwd(x=8 * P, weight_dtype=_lib.DTYPE_F16) == _lib.ERR_UNSUPPORTED and "x is read" in _lib.last_error()
+    assert bwd(x=8 * P + 1, x_pitch=64) == _lib.ERR_INVALID_ARG and "x is not" in _lib.last_error()
     assert L.fgms_b200_rms_norm_bwd(None, None) == _lib.ERR_INVALID_ARG
     assert L.fgms_b200_rms_norm_bwd_workspace_bytes(0, 64) == 0 and L.fgms_b200_rms_norm_bwd_workspace_bytes(4, 40000) == 0
 
