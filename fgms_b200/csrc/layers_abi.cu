@@ -116,8 +116,12 @@ int run_dropout(const fgms_b200_dropout_args& a, bool backward, cudaStream_t st)
   const dim3 grid((unsigned)(blocks < most ? blocks : most));
   const auto launch = [&](auto type) {
     using T = decltype(type);
-    return backward ? fgms::launch_pdl(fgms::dropout_kernel<T, true>, grid, fgms::DROP_THREADS, 0, st, p)
-                    : fgms::launch_pdl(fgms::dropout_kernel<T, false>, grid, fgms::DROP_THREADS, 0, st, p);
+    const bool some = p.drop.threshold > 0;
+    if (backward)
+      return some ? fgms::launch_pdl(fgms::dropout_kernel<T, true, true>, grid, fgms::DROP_THREADS, 0, st, p)
+                  : fgms::launch_pdl(fgms::dropout_kernel<T, true, false>, grid, fgms::DROP_THREADS, 0, st, p);
+    return some ? fgms::launch_pdl(fgms::dropout_kernel<T, false, true>, grid, fgms::DROP_THREADS, 0, st, p)
+                : fgms::launch_pdl(fgms::dropout_kernel<T, false, false>, grid, fgms::DROP_THREADS, 0, st, p);
   };
   const cudaError_t e = a.dtype == FGMS_DTYPE_F32 ? launch(float()) : a.dtype == FGMS_DTYPE_F16 ? launch(__half()) : launch(__nv_bfloat16());
   if (e != cudaSuccess) {

@@ -9,15 +9,17 @@
 // below 2^-100 is zeros with a scale of zero; a row that holds a value which is not finite has a scale of NaN and codes of zero, so that a product with
 // it is NaN.
 //
-// One pass: a row's values stay in registers from their load to their store, CH chunks of eight a thread, `threads_per_row` threads a row.  Rows of up
-// to 256 CH values are a warp's each, wider ones a block's, with one exchange through shared memory for each reduction.
+// One pass: a row's values stay in registers from their load to their store, CH chunks of eight a thread.  Rows of up to 256 values are a warp's each, wider
+// ones a block's (of the gradient, up to 512, two warps' of eight such pairs in a block, so that the blocks' shares of the weight's gradient
+// stay few), with one exchange through shared memory for each reduction.
 #pragma once
 #include "row_values.cuh"
 
 namespace fgms {
 
 constexpr int NORM_MAX_THREADS = 1024;
-constexpr int NORM_WARP_ROWS = 4, NORM_GRAD_WARP_ROWS = 8;  // rows (warps) of a block where a row is a warp's
+constexpr int NORM_WARP_ROWS = 4;   // rows (warps) of a block where a row is a warp's
+constexpr int NORM_GRAD_ROWS = 8;   // rows that a block of the gradient has at a time where a row is a warp's or two
 
 struct NormParams {
   const void *x, *residual, *weight;  // residual: or null; weight: null without a norm (norm = 0)
@@ -59,14 +61,26 @@ __device__ __forceinline__ uint32_t row_max(uint32_t v, uint32_t* part) {
   return __reduce_max_sync(0xffffffffu, lane < warps ? part[lane] : 0u);
 }
 
+// Of the gradient: `GROUP` warps a row, 0 the whole block.
+template <int GROUP>
+__device__ __forceinline__ float group_sum(float v, float* part) {
+  if (GROUP <= 1) return row_sum<GROUP == 1>(v, part);
+  v = warp_sum(v);
+  const int warp = (int)threadIdx.x >> 5;
+  if ((threadIdx.x & 31) == 0) part[warp] = v;
+  asm volatile("barrier.cta.sync %0, %1;" ::"r"(1 + warp / GROUP), "n"(32 * (GROUP ? GROUP : 1)) : "memory");
+  return part[warp / 2 * 2] + part[warp / 2 * 2 + 1];  // (of two)
+}
+
 // T: rows; W: the weight; CH: chunks a thread; WARP: a row is a warp's; EIGHT: the output is codes of 8 bits
-template <typename T, typename W, int CH, bool WARP, bool EIGHT, bool DROP>
-__global__ void __launch_bounds__(WARP ? 32 * NORM_WARP_ROWS : NORM_MAX_THREADS, 1) rms_norm_kernel(const __grid_constant__ NormParams p) {
+template <typename T, typename W, int CH, bool WARP, bool EIGHT, bool DROP, int THREADS>
+__global__ void __launch_bounds__(THREADS, THREADS == 512 ? (CH == 1 ? 3 : 2) : 1) rms_norm_kernel(const __grid_constant__ NormParams p) {
   __shared__ float parts[4][32];
   umma::griddep_wait();
   if (!p.alone) umma::griddep_launch_dependents();
   DropKey key;
   if (DROP) key = drop_key(p.drop.state);
+  const uint32_t below = drop_below(p.drop.threshold);
   const int per_row = WARP ? 32 : (int)blockDim.x, thread = WARP ? (int)threadIdx.x & 31 : (int)threadIdx.x;
   const long long rows_at_once = WARP ? (long long)gridDim.x * NORM_WARP_ROWS : (long long)gridDim.x;
   int turn = 0;  // a row's reductions use other words than the last one's, which a slower warp may still read
@@ -82,14 +96,21 @@ __global__ void __launch_bounds__(WARP ? 32 * NORM_WARP_ROWS : NORM_MAX_THREADS,
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       const int chunk = c * per_row + thread, col = chunk * ROW_CHUNK;
-      const uint32_t keep = DROP ? drop_keep(key, (uint32_t)chunk, (uint32_t)row, p.drop.threshold) : 0u;
+      DropLots lots;
+      if (DROP) lots = drop_lots(key, (uint32_t)chunk, (uint32_t)row);
+      row_values(raw[c], h[c]);
+      if (DROP) {
 #pragma unroll
-      for (int e = 0; e < ROW_CHUNK; ++e) {
-        h[c][e] = row_value(raw[c], e);
-        if (DROP) h[c][e] = keep >> e & 1u ? h[c][e] * p.drop.factor : 0.f;
-        if (p.residual) h[c][e] += row_value(add[c], e);
-        sum += h[c][e] * h[c][e];
+        for (int e = 0; e < ROW_CHUNK; ++e) h[c][e] = lots.kept(e, below) ? h[c][e] * p.drop.factor : 0.f;
       }
+      if (p.residual) {
+        float r[ROW_CHUNK];
+        row_values(add[c], r);
+#pragma unroll
+        for (int e = 0; e < ROW_CHUNK; ++e) h[c][e] += r[e];
+      }
+#pragma unroll
+      for (int e = 0; e < ROW_CHUNK; ++e) sum += h[c][e] * h[c][e];
       if (p.sum) row_store(static_cast<T*>(p.sum) + row * p.sum_pitch + col, h[c], p.width - col, p.sum_vec, chunk == 0);
     }
     float r = 1.f;
@@ -108,8 +129,7 @@ __global__ void __launch_bounds__(WARP ? 32 * NORM_WARP_ROWS : NORM_MAX_THREADS,
           RowRaw<W> v;
 #pragma unroll
           for (int q = 0; q < (int)sizeof(W) / 2; ++q) *reinterpret_cast<uint4*>(v.w + 4 * q) = __ldg(reinterpret_cast<const uint4*>(from) + q);
-#pragma unroll
-          for (int e = 0; e < ROW_CHUNK; ++e) w[e] = row_value(v, e);
+          row_values(v, w);
         } else {
 #pragma unroll
           for (int e = 0; e < ROW_CHUNK; ++e) w[e] = e < there ? to_f32(from[e]) : 0.f;
@@ -163,28 +183,29 @@ struct NormGradParams {
   int alone;
 };
 
-// The block's rows one after the other, the next one's values on their way meanwhile; their share of the weight's gradient in registers until the last
-// one.  FROM_X: h = residual + drop(x) once more, unrounded, for a weight whose gradient holds more than the h that was stored: rows in bf16 with a weight in fp32
+// The block's rows one after the other, their share of the weight's gradient in registers until the last one: 1024 threads an SM with 64 registers each, where the
+// next row's values on their way meanwhile and half as many threads took 58 us instead of XX (8192 x 2048, bf16).  FROM_X: h = residual + drop(x) once more, unrounded, for a weight whose gradient holds more than the h that was stored: rows in bf16 with a weight in fp32
 // have its gradient off by 2^-9.3 with that, by 2^-22 so, for a read more.
-template <typename T, typename W, int CH, bool WARP, bool DROP, bool FROM_X, int THREADS>
-__global__ void __launch_bounds__(THREADS, 1) rms_norm_grad_kernel(const __grid_constant__ NormGradParams p) {
-  constexpr bool AHEAD = CH * sizeof(T) <= 4;  // where the registers are there
+template <typename T, typename W, int CH, int GROUP, bool DROP, bool FROM_X, int THREADS>
+__global__ void __launch_bounds__(THREADS, CH == 1 ? 1024 / THREADS : 1) rms_norm_grad_kernel(const __grid_constant__ NormGradParams p) {
   __shared__ float parts[2][32];
-  __shared__ float share[WARP ? NORM_GRAD_WARP_ROWS : 1][WARP ? 32 * CH * ROW_CHUNK : 1];
+  __shared__ float share[GROUP ? NORM_GRAD_ROWS : 1][GROUP ? 32 * GROUP * CH * ROW_CHUNK : 1];
   umma::griddep_wait();
   if (!p.alone) umma::griddep_launch_dependents();
   DropKey key;
   if (DROP) key = drop_key(p.drop.used);
-  const int per_row = WARP ? 32 : (int)blockDim.x, thread = WARP ? (int)threadIdx.x & 31 : (int)threadIdx.x;
-  const long long rows_at_once = WARP ? (long long)gridDim.x * NORM_GRAD_WARP_ROWS : (long long)gridDim.x;
+  const uint32_t below = drop_below(p.drop.threshold);
+  constexpr int EACH = GROUP ? 32 * GROUP : 1;  // threads of a row
+  const int per_row = GROUP ? EACH : (int)blockDim.x, thread = GROUP ? (int)threadIdx.x % EACH : (int)threadIdx.x, group = GROUP ? (int)threadIdx.x / EACH : 0;
+  const long long rows_at_once = GROUP ? (long long)gridDim.x * NORM_GRAD_ROWS : (long long)gridDim.x;
   float dw[CH][ROW_CHUNK];
 #pragma unroll
   for (int c = 0; c < CH; ++c)
 #pragma unroll
     for (int e = 0; e < ROW_CHUNK; ++e) dw[c][e] = 0.f;
-  RowRaw<T> dy[CH], h[CH], add[CH], extra[CH], next_dy[AHEAD ? CH : 1], next_h[AHEAD ? CH : 1], next_add[AHEAD ? CH : 1], next_extra[AHEAD ? CH : 1];
-  float r = 0.f, next_r = 0.f;
-  const auto load = [&](long long row, auto& dy, auto& h, auto& add, auto& extra, float& r) {
+  RowRaw<T> dy[CH], h[CH], add[CH], extra[CH];
+  int turn = 0;
+  for (long long row = GROUP ? (long long)blockIdx.x * NORM_GRAD_ROWS + group : (long long)blockIdx.x; row < p.rows; row += rows_at_once) {
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       const int col = (c * per_row + thread) * ROW_CHUNK, there = p.width - col;
@@ -193,97 +214,84 @@ __global__ void __launch_bounds__(THREADS, 1) rms_norm_grad_kernel(const __grid_
       if (FROM_X && p.residual) add[c] = row_load(static_cast<const T*>(p.residual) + row * p.residual_pitch + col, there, p.residual_vec);
       if (p.dsum) extra[c] = row_load(static_cast<const T*>(p.dsum) + row * p.dsum_pitch + col, there, p.dsum_vec);
     }
-    r = __ldg(p.rstd + row);
-  };
-  int turn = 0;
-  long long row = WARP ? (long long)blockIdx.x * NORM_GRAD_WARP_ROWS + (threadIdx.x >> 5) : (long long)blockIdx.x;
-  if (AHEAD && row < p.rows) load(row, dy, h, add, extra, r);
-  for (; row < p.rows; row += rows_at_once) {
-    if constexpr (AHEAD) {
-      if (row + rows_at_once < p.rows) load(row + rows_at_once, next_dy, next_h, next_add, next_extra, next_r);
-    } else {
-      load(row, dy, h, add, extra, r);
-    }
-    uint32_t keep[CH];
-    RowRaw<W> w[CH];
-    const auto weights = [&](int c) {
-      const int col = (c * per_row + thread) * ROW_CHUNK, there = p.width - col;
+    const float r = __ldg(p.rstd + row);
+    DropLots lots[CH];
+    float n[CH][ROW_CHUNK], g[CH][ROW_CHUNK], dot = 0.f;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int chunk = c * per_row + thread, col = chunk * ROW_CHUNK, there = p.width - col;
+      if (DROP) lots[c] = drop_lots(key, (uint32_t)chunk, (uint32_t)row);
+      row_values(h[c], n[c]);
+      if (FROM_X) {
+        if (DROP) {
+#pragma unroll
+          for (int e = 0; e < ROW_CHUNK; ++e) n[c][e] = lots[c].kept(e, below) ? n[c][e] * p.drop.factor : 0.f;
+        }
+        if (p.residual) {
+          float v[ROW_CHUNK];
+          row_values(add[c], v);
+#pragma unroll
+          for (int e = 0; e < ROW_CHUNK; ++e) n[c][e] += v[e];
+        }
+      }
+      RowRaw<W> raw;
       const W* from = static_cast<const W*>(p.weight) + col;
       if (p.weight_vec && there >= ROW_CHUNK) {  // every row reads it again: from L1
 #pragma unroll
         for (int q = 0; q < (int)sizeof(W) / 2; ++q) {
           const uint4 v = __ldg(reinterpret_cast<const uint4*>(from) + q);
-          w[c].w[4 * q] = v.x; w[c].w[4 * q + 1] = v.y; w[c].w[4 * q + 2] = v.z; w[c].w[4 * q + 3] = v.w;
+          raw.w[4 * q] = v.x; raw.w[4 * q + 1] = v.y; raw.w[4 * q + 2] = v.z; raw.w[4 * q + 3] = v.w;
         }
       } else {
-        w[c] = row_load(from, there, false);
+        raw = row_load(from, there, false);
       }
-    };
-    const auto sum_of = [&](int c, int e) {
-      float v = row_value(h[c], e);
-      if (FROM_X) {
-        if (DROP) v = keep[c] >> e & 1u ? v * p.drop.factor : 0.f;
-        if (p.residual) v += row_value(add[c], e);
-      }
-      return v;
-    };
-    float dot = 0.f;
-#pragma unroll
-    for (int c = 0; c < CH; ++c) {
-      if (DROP) keep[c] = drop_keep(key, (uint32_t)(c * per_row + thread), (uint32_t)row, p.drop.threshold);
-      weights(c);
+      float w[ROW_CHUNK];
+      row_values(raw, w);
+      row_values(dy[c], g[c]);
 #pragma unroll
       for (int e = 0; e < ROW_CHUNK; ++e) {
-        const float n = sum_of(c, e) * r, d = row_value(dy[c], e);
-        dot += d * row_value(w[c], e) * n;
-        dw[c][e] += d * n;
+        n[c][e] *= r;
+        dw[c][e] += g[c][e] * n[c][e];
+        g[c][e] *= w[e];
+        dot += g[c][e] * n[c][e];
       }
     }
-    const float mean = row_sum<WARP>(dot, parts[turn]) * p.inverse_width;
-    if (!WARP) turn ^= 1;
+    const float mean = group_sum<GROUP>(dot, parts[turn]) * p.inverse_width;
+    if (GROUP != 1) turn ^= 1;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       const int chunk = c * per_row + thread, col = chunk * ROW_CHUNK, there = p.width - col;
-      if (CH > 1) weights(c);  // again from L1, instead of registers meanwhile
       float dh[ROW_CHUNK];
 #pragma unroll
-      for (int e = 0; e < ROW_CHUNK; ++e) {
-        dh[e] = r * (row_value(dy[c], e) * row_value(w[c], e) - sum_of(c, e) * r * mean);
-        if (p.dsum) dh[e] += row_value(extra[c], e);
+      for (int e = 0; e < ROW_CHUNK; ++e) dh[e] = r * (g[c][e] - n[c][e] * mean);
+      if (p.dsum) {
+        float v[ROW_CHUNK];
+        row_values(extra[c], v);
+#pragma unroll
+        for (int e = 0; e < ROW_CHUNK; ++e) dh[e] += v[e];
       }
       if (p.dresidual) row_store(static_cast<T*>(p.dresidual) + row * p.dresidual_pitch + col, dh, there, p.dresidual_vec, chunk == 0);
       if (p.dx) {
         if (DROP) {
 #pragma unroll
-          for (int e = 0; e < ROW_CHUNK; ++e) dh[e] = keep[c] >> e & 1u ? dh[e] * p.drop.factor : 0.f;
+          for (int e = 0; e < ROW_CHUNK; ++e) dh[e] = lots[c].kept(e, below) ? dh[e] * p.drop.factor : 0.f;
         }
         row_store(static_cast<T*>(p.dx) + row * p.dx_pitch + col, dh, there, p.dx_vec, chunk == 0);
       }
     }
-    if constexpr (AHEAD) {
-#pragma unroll
-      for (int c = 0; c < CH; ++c) {
-        dy[c] = next_dy[c];
-        h[c] = next_h[c];
-        add[c] = next_add[c];
-        extra[c] = next_extra[c];
-      }
-      r = next_r;
-    }
   }
   if (!p.parts) return;
   float* to = p.parts + (size_t)blockIdx.x * p.width;
-  if (WARP) {  // the block's warps in their order
-    const int warp = (int)threadIdx.x >> 5;
+  if (GROUP) {  // the block's groups in their order
 #pragma unroll
     for (int c = 0; c < CH; ++c)
 #pragma unroll
-      for (int e = 0; e < ROW_CHUNK; ++e) share[warp][(c * 32 + thread) * ROW_CHUNK + e] = dw[c][e];
+      for (int e = 0; e < ROW_CHUNK; ++e) share[group][(c * per_row + thread) * ROW_CHUNK + e] = dw[c][e];
     __syncthreads();
-    for (int col = (int)threadIdx.x; col < p.width; col += 32 * NORM_GRAD_WARP_ROWS) {
+    for (int col = (int)threadIdx.x; col < p.width; col += EACH * NORM_GRAD_ROWS) {
       float sum = 0.f;
 #pragma unroll
-      for (int i = 0; i < NORM_GRAD_WARP_ROWS; ++i) sum += share[i][col];
+      for (int i = 0; i < NORM_GRAD_ROWS; ++i) sum += share[i][col];
       to[col] = sum;
     }
   } else {
@@ -332,59 +340,57 @@ inline int norm_threads(int width, int ch) {
   return ((chunks + ch - 1) / ch + 31) / 32 * 32;
 }
 
-template <typename T, typename W, int CH, bool WARP, bool EIGHT>
+template <typename T, typename W, int CH, bool WARP, bool EIGHT, int THREADS>
 cudaError_t launch_rms_norm_as(const NormParams& p, cudaStream_t st, int sms) {
   const int threads = WARP ? 32 * NORM_WARP_ROWS : norm_threads(p.width, CH);
   const long long blocks = WARP ? (p.rows + NORM_WARP_ROWS - 1) / NORM_WARP_ROWS : p.rows;
-  const long long at_once = (long long)sms * (2048 / threads);
+  const long long at_once = (long long)sms * ((THREADS == 512 ? (CH == 1 ? 1536 : 1024) : 2048) / threads);
   const dim3 grid((unsigned)(blocks < at_once ? blocks : at_once));
-  if (!EIGHT && p.drop.threshold > 0) return launch_pdl(rms_norm_kernel<T, W, CH, WARP, false, true>, grid, threads, 0, st, p);
-  return launch_pdl(rms_norm_kernel<T, W, CH, WARP, EIGHT, false>, grid, threads, 0, st, p);
+  if (!EIGHT && p.drop.threshold > 0) return launch_pdl(rms_norm_kernel<T, W, CH, WARP, false, true, THREADS>, grid, threads, 0, st, p);
+  return launch_pdl(rms_norm_kernel<T, W, CH, WARP, EIGHT, false, THREADS>, grid, threads, 0, st, p);
 }
 template <typename T, typename W, bool EIGHT>
 cudaError_t launch_rms_norm(const NormParams& p, cudaStream_t st, int sms) {
-  if (p.width <= 256) return launch_rms_norm_as<T, W, 1, true, EIGHT>(p, st, sms);
-  if (p.width <= 512) return launch_rms_norm_as<T, W, 2, true, EIGHT>(p, st, sms);
-  if (p.rows < sms || p.width <= 2048) {
-    if (p.width <= 8192) return launch_rms_norm_as<T, W, 1, false, EIGHT>(p, st, sms);
-  }
-  if (p.width <= 16384) return launch_rms_norm_as<T, W, 2, false, EIGHT>(p, st, sms);
-  return launch_rms_norm_as<T, W, 4, false, EIGHT>(p, st, sms);
+  constexpr int WARPS = 32 * NORM_WARP_ROWS;
+  if (p.width <= 256) return launch_rms_norm_as<T, W, 1, true, EIGHT, WARPS>(p, st, sms);
+  // few rows: as many threads as there are chunks
+  if (p.width <= (p.rows < sms ? 4096 : 2048)) return launch_rms_norm_as<T, W, 1, false, EIGHT, 512>(p, st, sms);
+  if (p.width <= 8192) return launch_rms_norm_as<T, W, 2, false, EIGHT, 512>(p, st, sms);
+  return launch_rms_norm_as<T, W, 4, false, EIGHT, NORM_MAX_THREADS>(p, st, sms);
 }
 constexpr int NORM_MAX_WIDTH = NORM_MAX_THREADS * 4 * ROW_CHUNK;
 
 // What a gradient is cut into: the blocks each leave a share of the weight's gradient.
 struct NormGradCut {
-  int ch, threads, blocks;
-  bool warp;
+  int ch, group, threads, blocks;  // group: warps a row, 0 a block
 };
 inline NormGradCut norm_grad_cut(long long rows, int width, int sms) {
   NormGradCut c;
-  c.warp = width <= 512;
-  c.ch = width <= 256 ? 1 : width <= 512 ? 2 : width <= 4096 ? 1 : width <= 8192 ? 2 : 4;
-  c.threads = c.warp ? 32 * NORM_GRAD_WARP_ROWS : norm_threads(width, c.ch);
-  const long long blocks = c.warp ? (rows + NORM_GRAD_WARP_ROWS - 1) / NORM_GRAD_WARP_ROWS : rows, at_once = (long long)sms * (c.threads <= 768 ? 768 / c.threads : 1);
+  c.group = width <= 256 ? 1 : width <= 512 ? 2 : 0;
+  c.ch = width <= 4096 ? 1 : width <= 8192 ? 2 : 4;
+  c.threads = c.group ? 32 * c.group * NORM_GRAD_ROWS : norm_threads(width, c.ch);
+  const long long blocks = c.group ? (rows + NORM_GRAD_ROWS - 1) / NORM_GRAD_ROWS : rows, at_once = (long long)sms * (c.threads <= 1024 ? 1024 / c.threads : 1);
   c.blocks = (int)(blocks < at_once ? blocks : at_once);
   return c;
 }
-template <typename T, typename W, int CH, bool WARP, int THREADS>
+template <typename T, typename W, int CH, int GROUP, int THREADS>
 cudaError_t launch_rms_norm_grad_as(const NormGradParams& p, const NormGradCut& cut, cudaStream_t st) {
   const dim3 grid((unsigned)cut.blocks);
   const bool drop = p.drop.threshold > 0;
   if constexpr (!std::is_same<T, W>::value) {
     if (p.x)
-      return drop ? launch_pdl(rms_norm_grad_kernel<T, W, CH, WARP, true, true, THREADS>, grid, cut.threads, 0, st, p)
-                  : launch_pdl(rms_norm_grad_kernel<T, W, CH, WARP, false, true, THREADS>, grid, cut.threads, 0, st, p);
+      return drop ? launch_pdl(rms_norm_grad_kernel<T, W, CH, GROUP, true, true, THREADS>, grid, cut.threads, 0, st, p)
+                  : launch_pdl(rms_norm_grad_kernel<T, W, CH, GROUP, false, true, THREADS>, grid, cut.threads, 0, st, p);
   }
-  return drop ? launch_pdl(rms_norm_grad_kernel<T, W, CH, WARP, true, false, THREADS>, grid, cut.threads, 0, st, p)
-              : launch_pdl(rms_norm_grad_kernel<T, W, CH, WARP, false, false, THREADS>, grid, cut.threads, 0, st, p);
+  return drop ? launch_pdl(rms_norm_grad_kernel<T, W, CH, GROUP, true, false, THREADS>, grid, cut.threads, 0, st, p)
+              : launch_pdl(rms_norm_grad_kernel<T, W, CH, GROUP, false, false, THREADS>, grid, cut.threads, 0, st, p);
 }
 template <typename T, typename W>
 cudaError_t launch_rms_norm_grad(const NormGradParams& p, const NormGradCut& cut, cudaStream_t st) {
-  if (cut.warp)
-    return cut.ch == 1 ? launch_rms_norm_grad_as<T, W, 1, true, 32 * NORM_GRAD_WARP_ROWS>(p, cut, st) : launch_rms_norm_grad_as<T, W, 2, true, 32 * NORM_GRAD_WARP_ROWS>(p, cut, st);
-  if (cut.ch == 1) return launch_rms_norm_grad_as<T, W, 1, false, 512>(p, cut, st);
-  return cut.ch == 2 ? launch_rms_norm_grad_as<T, W, 2, false, 512>(p, cut, st) : launch_rms_norm_grad_as<T, W, 4, false, 1024>(p, cut, st);
+  if (cut.group == 1) return launch_rms_norm_grad_as<T, W, 1, 1, 32 * NORM_GRAD_ROWS>(p, cut, st);
+  if (cut.group == 2) return launch_rms_norm_grad_as<T, W, 1, 2, 64 * NORM_GRAD_ROWS>(p, cut, st);
+  if (cut.ch == 1) return launch_rms_norm_grad_as<T, W, 1, 0, 512>(p, cut, st);
+  return cut.ch == 2 ? launch_rms_norm_grad_as<T, W, 2, 0, 512>(p, cut, st) : launch_rms_norm_grad_as<T, W, 4, 0, 1024>(p, cut, st);
 }
 template <typename W>
 cudaError_t launch_rms_norm_weight_grad(const float* parts, int n, int width, void* dw, int alone, cudaStream_t st) {

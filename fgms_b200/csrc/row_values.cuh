@@ -13,6 +13,84 @@ template <typename T>
 struct RowRaw {
   uint32_t w[2 * sizeof(T)];
 };
+// `there` of the eight values from `p` on (at most eight; none: zeros); vec: rows start on 16-byte boundaries.  Values that are read once pass L1 by.  Off such a
+// boundary they come as words, of which the outer two may hold a neighbour's value as well, and are shifted by a value if need be.
+template <typename T>
+__device__ __forceinline__ RowRaw<T> row_load(const T* p, int there, bool vec) {
+  constexpr int N = 2 * sizeof(T);
+  RowRaw<T> r;
+  if (vec && there >= ROW_CHUNK) {
+    const uint4 a = __ldcs(reinterpret_cast<const uint4*>(p));
+    r.w[0] = a.x; r.w[1] = a.y; r.w[2] = a.z; r.w[3] = a.w;
+    if constexpr (sizeof(T) == 4) {
+      const uint4 b = __ldcs(reinterpret_cast<const uint4*>(p) + 1);
+      r.w[4] = b.x; r.w[5] = b.y; r.w[6] = b.z; r.w[7] = b.w;
+    }
+    return r;
+  }
+  if (there >= ROW_CHUNK) {
+    const uint32_t* words = reinterpret_cast<const uint32_t*>(reinterpret_cast<uintptr_t>(p) & ~(uintptr_t)3);
+#pragma unroll
+    for (int i = 0; i < N; ++i) r.w[i] = __ldca(words + i);
+    if (sizeof(T) == 2 && (reinterpret_cast<uintptr_t>(p) & 2)) {
+      const uint32_t last = __ldca(words + N);
+#pragma unroll
+      for (int i = 0; i < N; ++i) r.w[i] = __funnelshift_r(r.w[i], i + 1 < N ? r.w[i + 1 < N ? i + 1 : i] : last, 16);
+    }
+    return r;
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) r.w[i] = 0u;
+#pragma unroll
+  for (int e = 0; e < ROW_CHUNK; ++e) {
+    if (e >= there) continue;
+    if constexpr (sizeof(T) == 4) r.w[e] = reinterpret_cast<const uint32_t*>(p)[e];
+    else r.w[e / 2] |= (uint32_t)reinterpret_cast<const uint16_t*>(p)[e] << (16 * (e % 2));
+  }
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ float row_value(const RowRaw<T>& r, int e) {
+  if constexpr (sizeof(T) == 4) {
+    return __uint_as_float(r.w[e]);
+  } else {
+    const uint16_t h = (uint16_t)(r.w[e / 2] >> (16 * (e % 2)));
+    if constexpr (std::is_same<T, __half>::value) return __half2float(__ushort_as_half(h));
+    else return __uint_as_float((uint32_t)h << 16);
+  }
+}
+template <typename T>
+__device__ __forceinline__ void row_values(const RowRaw<T>& r, float (&x)[ROW_CHUNK]) {
+#pragma unroll
+  for (int i = 0; i < ROW_CHUNK / 2; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      x[2 * i] = __uint_as_float(r.w[2 * i]);
+      x[2 * i + 1] = __uint_as_float(r.w[2 * i + 1]);
+    } else if constexpr (std::is_same<T, __half>::value) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&r.w[i]));
+      x[2 * i] = f.x;
+      x[2 * i + 1] = f.y;
+    } else {
+      x[2 * i] = __uint_as_float(r.w[i] << 16);
+      x[2 * i + 1] = __uint_as_float(r.w[i] & 0xffff0000u);
+    }
+  }
+}
+template <typename T>
+__device__ __forceinline__ RowRaw<T> row_rounded(const float (&x)[ROW_CHUNK]) {
+  RowRaw<T> r;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < ROW_CHUNK; ++i) r.w[i] = __float_as_uint(x[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < ROW_CHUNK / 2; ++i) {
+      if constexpr (std::is_same<T, __half>::value) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r.w[i]) : "f"(x[2 * i + 1]), "f"(x[2 * i]));
+      else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r.w[i]) : "f"(x[2 * i + 1]), "f"(x[2 * i]));
+    }
+  }
+  return r;
+}
 // The bytes from `off` on (0 .. 15, a multiple of the values' size, the same in all lanes) of N words and the four behind them.
 template <int N>
 __device__ __forceinline__ void row_shift_down(uint32_t (&w)[N + 4], uint32_t off) {
@@ -29,71 +107,25 @@ __device__ __forceinline__ void row_shift_down(uint32_t (&w)[N + 4], uint32_t of
     for (int i = 0; i < N; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], 16);
   }
 }
-// `there` of the eight values from `p` on (at most eight; none: zeros); vec: rows start on 16-byte boundaries.  Values that are read once pass L1 by.  Off such a
-// boundary the 16-byte blocks that the values lie in are read, whose other bytes are a neighbour's (or behind the last row's end, in a block that row is
-// in as well), and shifted: 16384 rows of 1001 fp16 values take XXX us so, and YYY a value at a time.
-template <typename T>
-__device__ __forceinline__ RowRaw<T> row_load(const T* p, int there, bool vec) {
-  constexpr int N = 2 * sizeof(T);
-  RowRaw<T> r;
-  if (vec && there >= ROW_CHUNK) {
-    const uint4 a = __ldcs(reinterpret_cast<const uint4*>(p));
-    r.w[0] = a.x; r.w[1] = a.y; r.w[2] = a.z; r.w[3] = a.w;
-    if constexpr (sizeof(T) == 4) {
-      const uint4 b = __ldcs(reinterpret_cast<const uint4*>(p) + 1);
-      r.w[4] = b.x; r.w[5] = b.y; r.w[6] = b.z; r.w[7] = b.w;
-    }
-    return r;
-  }
-  const uint32_t off = (uint32_t)reinterpret_cast<uintptr_t>(p) & 15u;
-  const uint4* blocks = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(p) & ~(uintptr_t)15);
-  const int bytes = min(there, ROW_CHUNK) * (int)sizeof(T) + (int)off;  // that are needed, from the first block on
-  uint32_t w[N + 4];
-#pragma unroll
-  for (int i = 0; i < N / 4 + 1; ++i) {
-    const uint4 v = there > 0 && bytes > 16 * i ? __ldca(blocks + i) : make_uint4(0, 0, 0, 0);
-    w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
-  }
-  row_shift_down<N>(w, off);
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    r.w[i] = w[i];
-    if (sizeof(T) == 4) {
-      if (i >= there) r.w[i] = 0u;
-    } else {
-      if (2 * i >= there) r.w[i] = 0u;
-      else if (2 * i + 1 >= there) r.w[i] &= 0xffffu;
-    }
-  }
-  return r;
-}
-template <typename T>
-__device__ __forceinline__ float row_value(const RowRaw<T>& r, int e) {
-  if constexpr (sizeof(T) == 4) {
-    return __uint_as_float(r.w[e]);
-  } else {
-    const uint16_t h = (uint16_t)(r.w[e / 2] >> (16 * (e % 2)));
-    if constexpr (std::is_same<T, __half>::value) return __half2float(__ushort_as_half(h));
-    else return __uint_as_float((uint32_t)h << 16);
-  }
-}
 // Rounded once to their type.  All lanes of a warp call it (with none there, if it must be); lanes that follow one another hold chunks that do, of the
 // same row as long as there are any.  Off 16-byte boundaries (`vec` false) a lane takes the next one's first values and stores the 16-byte blocks that its own
 // values end in; what the warp's first and last chunk, or a row's, have beyond such blocks goes value by value.
 template <typename T>
 __device__ __forceinline__ void row_store(T* p, const float (&x)[ROW_CHUNK], int there, bool vec, bool first_of_row) {
   constexpr int N = 2 * sizeof(T), EACH = 4 / sizeof(T);  // words; values of a word
-  __align__(16) T h[ROW_CHUNK];
-#pragma unroll
-  for (int e = 0; e < ROW_CHUNK; ++e) h[e] = from_f32<T>(x[e]);
+  const RowRaw<T> h = row_rounded<T>(x);
+  const auto put = [&](int e) {
+    if constexpr (sizeof(T) == 4) reinterpret_cast<uint32_t*>(p)[e] = h.w[e];
+    else reinterpret_cast<uint16_t*>(p)[e] = (uint16_t)(h.w[e / 2] >> (16 * (e % 2)));
+  };
   if (vec) {
     if (there >= ROW_CHUNK) {
 #pragma unroll
-      for (int q = 0; q < (int)sizeof(T) / 2; ++q) reinterpret_cast<uint4*>(p)[q] = reinterpret_cast<const uint4*>(h)[q];
+      for (int q = 0; q < N / 4; ++q) reinterpret_cast<uint4*>(p)[q] = make_uint4(h.w[4 * q], h.w[4 * q + 1], h.w[4 * q + 2], h.w[4 * q + 3]);
     } else {
 #pragma unroll
       for (int e = 0; e < ROW_CHUNK; ++e)
-        if (e < there) p[e] = h[e];
+        if (e < there) put(e);
     }
     return;
   }
@@ -102,7 +134,7 @@ __device__ __forceinline__ void row_store(T* p, const float (&x)[ROW_CHUNK], int
   const int head = (int)((16u - off) & 15u) / (int)sizeof(T);  // values in front of the first block that begins inside this chunk
   uint32_t w[N + 4];
 #pragma unroll
-  for (int i = 0; i < N; ++i) w[i] = reinterpret_cast<const uint32_t*>(h)[i];
+  for (int i = 0; i < N; ++i) w[i] = h.w[i];
 #pragma unroll
   for (int i = 0; i < 4; ++i) w[N + i] = __shfl_down_sync(0xffffffffu, w[i], 1);
   const bool joined = lane < 31 && there - ROW_CHUNK >= head;       // the next chunk has the values that this one's last block lacks
@@ -116,7 +148,7 @@ __device__ __forceinline__ void row_store(T* p, const float (&x)[ROW_CHUNK], int
   const int stored_to = whole > 0 ? head + whole * 4 * EACH : head;  // from `head` on
 #pragma unroll
   for (int e = 0; e < ROW_CHUNK; ++e)
-    if (e < there && (e < head ? !covered : e >= stored_to)) p[e] = h[e];
+    if (e < there && (e < head ? !covered : e >= stored_to)) put(e);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -132,7 +164,7 @@ __device__ __forceinline__ void row_store(T* p, const float (&x)[ROW_CHUNK], int
 struct DropParams {
   long long* state;       // forward: [3]
   long long* used;        // forward: null, or [2], where seed and number of the call are left; backward: those
-  uint32_t threshold;     // 0: nothing is dropped, 65536: everything
+  uint32_t threshold;     // 1 .. 65536 (everything); 0: nothing is dropped, and no lots are drawn
   float factor;           // of what is kept
 };
 struct DropKey {
@@ -140,10 +172,18 @@ struct DropKey {
 };
 __device__ __forceinline__ DropKey drop_key(const long long* at) {
   const long long seed = __ldcg(at), call = __ldcg(at + 1);
-  return {(uint32_t)seed, (uint32_t)((unsigned long long)seed >> 32), (uint32_t)call, (uint32_t)((unsigned long long)call >> 32)};
+  // the same in all lanes, and known to be: what is added to the key round after round is then no lane's work
+  const auto one = [](uint32_t v) { return __reduce_or_sync(0xffffffffu, v); };
+  return {one((uint32_t)seed), one((uint32_t)((unsigned long long)seed >> 32)), one((uint32_t)call), one((uint32_t)((unsigned long long)call >> 32))};
 }
-// bit e: the chunk's value e is kept
-__device__ __forceinline__ uint32_t drop_keep(const DropKey& k, uint32_t chunk, uint32_t row, uint32_t threshold) {
+// The lots of a chunk, and whether its value e is kept: lots are compared in the upper halves of words with (threshold << 16) - 1, which they are above where they are
+// not below the threshold (which is 1 at least; of 65536 no word is above).
+struct DropLots {
+  uint32_t w[4];
+  __device__ __forceinline__ bool kept(int e, uint32_t below) const { return (e & 1 ? w[e / 2] : w[e / 2] << 16) > below; }
+};
+__device__ __forceinline__ uint32_t drop_below(uint32_t threshold) { return (threshold << 16) - 1u; }
+__device__ __forceinline__ DropLots drop_lots(const DropKey& k, uint32_t chunk, uint32_t row) {
   uint32_t c0 = chunk, c1 = row, c2 = k.call0, c3 = k.call1, k0 = k.key0, k1 = k.key1;
 #pragma unroll
   for (int i = 0; i < 10; ++i) {
@@ -155,11 +195,7 @@ __device__ __forceinline__ uint32_t drop_keep(const DropKey& k, uint32_t chunk, 
     k0 += 0x9E3779B9u;
     k1 += 0xBB67AE85u;
   }
-  const uint32_t w[4] = {c0, c1, c2, c3};
-  uint32_t keep = 0;
-#pragma unroll
-  for (int e = 0; e < ROW_CHUNK; ++e) keep |= ((e & 1 ? w[e / 2] >> 16 : w[e / 2] & 0xffffu) >= threshold ? 1u : 0u) << e;
-  return keep;
+  return {{c0, c1, c2, c3}};
 }
 // Every thread of the grid has read the state before: the last block counts the call.
 __device__ __forceinline__ void drop_count(const DropParams& d) {
