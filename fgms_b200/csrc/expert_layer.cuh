@@ -17,7 +17,8 @@
 // expert's tokens as N, eight a step (rows that are no token are computed and thrown away).
 //
 //   warps 0-7   products: 16 rows of every tile each; their sums meet in shared memory at the end of an item
-//   warp 8      TMA producer of weights          warp 9   producer of the tokens' rows: a bulk copy a row and tile
+//   warp 8      TMA producer of weights          warp 9   producer of the tokens' rows (cp.async: as a bulk copy a row and tile, 56 ns each, 64 tokens a tile took
+//               ten times as long as its weights)
 //   warps 10-11 report finished items and add the output up: a report waits until all that was stored is there, a microsecond that the products go on in
 //
 // All waits are bounded.
@@ -159,6 +160,7 @@ struct ElShared {
   int group_pairs[EL_MAX_EXPERTS / 32], group_used[EL_MAX_EXPERTS / 32];
   float gates[EL_MAX_PAIRS];
   uint16_t chosen[EL_MAX_PAIRS], list[EL_MAX_PAIRS];           // pairs: token * top_k + j; list: in the order of their experts
+  uint8_t token[EL_MAX_PAIRS];                                 // of the pairs of the list
   uint16_t place[EL_MAX_EXPERTS];                              // of an expert: its first pair's place in the list
   uint16_t expert[EL_MAX_EXPERTS], first[EL_MAX_EXPERTS + 1];  // of those that are used: which, and the first pair's place
 };
@@ -239,7 +241,10 @@ __device__ __forceinline__ void el_sort(const ExpertParams& p, ElShared* sh) {
         place += (other >> 1) < e || ((other >> 1) == e && i < lane);
         used += (other >> 1) < e && (other & 1);
       }
-      if (lane < pairs) sh->list[place] = (uint16_t)lane;
+      if (lane < pairs) {
+        sh->list[place] = (uint16_t)lane;
+        sh->token[place] = (uint8_t)(lane / p.top_k);
+      }
       if (head) {
         sh->expert[used] = (uint16_t)e;
         sh->first[used] = (uint16_t)place;
@@ -305,14 +310,11 @@ __device__ __forceinline__ void el_sort(const ExpertParams& p, ElShared* sh) {
   __syncthreads();
   for (int i = threadIdx.x; i < pairs; i += EL_THREADS) {
     const int e = sh->chosen[i], t = i / p.top_k;
-    sh->list[sh->place[e] + __popcll(sh->tokens[e] & ((1ull << t) - 1ull))] = (uint16_t)i;
+    const int place = sh->place[e] + __popcll(sh->tokens[e] & ((1ull << t) - 1ull));
+    sh->list[place] = (uint16_t)i;
+    sh->token[place] = (uint8_t)t;
   }
   __syncthreads();
-}
-
-// `bytes` of global memory to shared memory, both from 16-byte boundaries and a multiple of 16; reported to `bar`
-__device__ __forceinline__ void el_bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-  asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
 
 // What every role goes by: the items, and the ring of the tokens' rows.
@@ -464,7 +466,7 @@ __global__ void __launch_bounds__(EL_THREADS, 1)
       mbar_init(smem_u32(&sh->empty[s]), EL_CONSUMERS / 32);
     }
     for (int s = 0; s < EL_MAX_STAGES; ++s) {
-      mbar_init(smem_u32(&sh->x_full[s]), 1);
+      mbar_init(smem_u32(&sh->x_full[s]), 32);
       mbar_init(smem_u32(&sh->x_empty[s]), EL_CONSUMERS / 32);
     }
     for (int i = 0; i < 2; ++i) {
@@ -520,25 +522,19 @@ __global__ void __launch_bounds__(EL_THREADS, 1)
         if (product == 1) {  // all of the expert's h is there
           ok = __all_sync(0xffffffffu, el_await(done_in + u, (uint32_t)plan.blocks_in, abort_flag));
           if (!ok) break;
-          fence_proxy_async_global();
-        }
-        // the rows of two tokens a lane
-        const uint16_t* src[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int row = min(lane + 32 * i, n - 1);
-          src[i] = product == 0 ? static_cast<const uint16_t*>(p.x) + (size_t)(sh->list[first + row] / (uint32_t)p.top_k) * p.x_pitch
-                                : p.h + (size_t)(first + row) * p.hidden;
         }
         for (int k = 0; k < length; k += EL_K) {
           ok = __all_sync(0xffffffffu, mbar_parked_wait(smem_u32(&sh->x_empty[s]), ph, abort_flag));
           if (!ok) break;
-          const uint32_t bytes = (uint32_t)min(EL_K, length - k) * 2u, bar = smem_u32(&sh->x_full[s]), to = x0 + (uint32_t)(s * plan.x_bytes);
-          if (lane == 0) mbar_expect_tx(bar, bytes * (uint32_t)n);
-          __syncwarp();
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-            if (lane + 32 * i < n) el_bulk_load(to + (uint32_t)((lane + 32 * i) * EL_X_PITCH), src[i] + k, bytes, bar);
+          // half a warp a row; zeros behind the contraction's end
+          const int at = k + (lane & 15) * 8;
+          const uint32_t to = x0 + (uint32_t)(s * plan.x_bytes + (lane & 15) * 16);
+#pragma unroll 4
+          for (int row = lane >> 4; row < n; row += 2) {
+            const uint16_t* src = product == 0 ? static_cast<const uint16_t*>(p.x) + sh->token[first + row] * p.x_pitch : p.h + (size_t)(first + row) * p.hidden;
+            cp_async16(to + (uint32_t)(row * EL_X_PITCH), at < length ? src + at : src, at < length);
+          }
+          cp_async_arrive_noinc(smem_u32(&sh->x_full[s]));
           if (++s == plan.x_stages) { s = 0; ph ^= 1u; }
         }
       }

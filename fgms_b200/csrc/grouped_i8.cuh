@@ -10,8 +10,8 @@
 // is told half as many channels.  An MMA takes 32 values where that one takes 16, in the same time.
 //
 //   warp 0      producer          warp 1      MMA issuer (of the pair's even CTA)
-//   warps 4-11  epilogue: scales, a transposition through shared memory and 16-byte stores; outputs in fp32 or off 16-byte boundaries go straight to
-//               memory, 32 channels a store
+//   warps 4-11  epilogue: scales, a transposition through shared memory and 16-byte stores; outputs off 16-byte boundaries go straight to
+//               memory, 32 channels a store (9444 rows 1232 -> 952 in fp32 32 us so, XX through the patch)
 #pragma once
 #include "grouped_umma.cuh"
 #include "row_values.cuh"
@@ -24,7 +24,7 @@ struct GroupedI8Params {
   GroupedParams g;  // as the walk takes it: c_in the output's channels, c_out the contraction in units of two values; a: rows, b: weights; kpos: or null
   const float *row_scale, *channel_scale;
   int dtype;   // of the output: 0 fp32, 1 fp16, 2 bf16
-  int direct;  // the output is stored without the patch
+  int store;   // 0: 16-bit rows through the patch, 1: fp32 rows through it, 2: straight to memory
 };
 
 namespace umma {
@@ -185,14 +185,37 @@ __global__ void __launch_bounds__(GU_THREADS, 1)
       float channel[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int c = m0 + quarter * 32 + (q.direct ? lane : i * 8 + (lane >> 2));
+        const int c = m0 + quarter * 32 + (q.store > 0 ? lane : i * 8 + (lane >> 2));
         channel[i] = c < channels ? __ldg(scales + c) : 0.f;
       }
       ok = four_agree(half, pair_wait<false>(smem_u32(&sh->tmem_full[buf]), ph, abort_flag, tile_wait_limit(tile.blocks)));
       if (!ok) break;
       tc_fence_after();
       const uint32_t from = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * cfg.tile_n);
-      if (q.direct) {
+      if (q.store == 1) {
+        const int c = m0 + lane * 4;
+        float* to = static_cast<float*>(p.d) + (size_t)tile.n0 * p.d_pitch + c;
+        for (int j0 = half * 16; j0 < tile.n_mma; j0 += 32) {  // 16 rows of the warp's 32 channels, then four rows of all 128
+          uint32_t v[16];
+          tmem_ld16(from + (uint32_t)j0, v);
+          const float scale = lane < 16 && j0 + lane < tile.n ? __ldg(q.row_scale + tile.n0 + j0 + lane) : 0.f;
+          tmem_ld_wait();
+          four_sync(half);  // the patch has been read
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            asm volatile("st.shared.f32 [%0], %1;" ::"r"(patch + (uint32_t)(j * 512 + (quarter * 32 + lane) * 4)),
+                         "f"(i8_scaled(v[j], __shfl_sync(0xffffffffu, scale, j), channel[0]))
+                         : "memory");
+          four_sync(half);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int row = quarter * 4 + i;
+            float4 o;
+            asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(o.x), "=f"(o.y), "=f"(o.z), "=f"(o.w) : "r"(patch + (uint32_t)(row * 512 + lane * 16)) : "memory");
+            if (j0 + row < tile.n && c < channels) *reinterpret_cast<float4*>(to + (size_t)(j0 + row) * p.d_pitch) = o;
+          }
+        }
+      } else if (q.store == 2) {
         const int c = m0 + quarter * 32 + lane;
         for (int j0 = half * 32; j0 < tile.n_mma; j0 += 64) {
 #pragma unroll
@@ -200,12 +223,14 @@ __global__ void __launch_bounds__(GU_THREADS, 1)
             if (j0 + part >= tile.n_mma) break;
             uint32_t v[16];
             tmem_ld16(from + (uint32_t)(j0 + part), v);
+            const int r0 = j0 + part;
+            const float scale = lane < 16 && r0 + lane < tile.n ? __ldg(q.row_scale + tile.n0 + r0 + lane) : 0.f;
             tmem_ld_wait();
+            size_t at = (size_t)(tile.n0 + r0) * p.d_pitch + c;
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              const int r = j0 + part + j;
-              if (r < tile.n && c < channels)
-                i8_store(q, (size_t)(tile.n0 + r) * p.d_pitch + c, i8_scaled(v[j], __ldg(q.row_scale + tile.n0 + r), channel[0]));
+            for (int j = 0; j < 16; ++j, at += p.d_pitch) {
+              const float row = __shfl_sync(0xffffffffu, scale, j);
+              if (r0 + j < tile.n && c < channels) i8_store(q, at, i8_scaled(v[j], row, channel[0]));
             }
           }
         }

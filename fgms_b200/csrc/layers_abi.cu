@@ -369,7 +369,8 @@ int run_grouped_i8(const int8_t* codes, int64_t codes_pitch, const float* code_s
   q.row_scale = code_scale;
   q.channel_scale = kernel_scale;
   q.dtype = dtype == FGMS_DTYPE_F32 ? 0 : dtype == FGMS_DTYPE_F16 ? 1 : 2;
-  q.direct = dtype == FGMS_DTYPE_F32 || !d.vec(16) || c_out % 8 != 0;
+  q.store = !d.vec(16) ? 2 : dtype == FGMS_DTYPE_F32 ? 1 : 0;  // (contiguous rows: all of them on 16-byte boundaries, or a single one)
+  if (c_out % (dtype == FGMS_DTYPE_F32 ? 4 : 8) != 0) q.store = 2;
   long long a_pitch = a.rows > 1 ? a.pitch : (c_in + 15) / 16 * 16, b_pitch = b.rows > 1 ? b.pitch : (c_in + 15) / 16 * 16;
   if (copies.total > 0) {
     uint8_t* to = static_cast<uint8_t*>(workspace);
