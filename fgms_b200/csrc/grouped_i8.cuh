@@ -11,7 +11,7 @@
 //
 //   warp 0      producer          warp 1      MMA issuer (of the pair's even CTA)
 //   warps 4-11  epilogue: scales, a transposition through shared memory and 16-byte stores; outputs off 16-byte boundaries go straight to
-//               memory, 32 channels a store (9444 rows 1232 -> 952 in fp32 32 us so, XX through the patch)
+//               memory, 32 channels a store (9444 rows 1232 -> 952 in fp32 32 us so, 26 through the patch)
 #pragma once
 #include "grouped_umma.cuh"
 #include "row_values.cuh"

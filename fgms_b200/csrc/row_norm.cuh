@@ -184,7 +184,7 @@ struct NormGradParams {
 };
 
 // The block's rows one after the other, their share of the weight's gradient in registers until the last one: 1024 threads an SM with 64 registers each, where the
-// next row's values on their way meanwhile and half as many threads took 58 us instead of XX (8192 x 2048, bf16).  FROM_X: h = residual + drop(x) once more, unrounded, for a weight whose gradient holds more than the h that was stored: rows in bf16 with a weight in fp32
+// next row's values on their way meanwhile and half as many threads took 58 us instead of 43 (8192 x 2048, bf16, with dropout).  FROM_X: h = residual + drop(x) once more, unrounded, for a weight whose gradient holds more than the h that was stored: rows in bf16 with a weight in fp32
 // have its gradient off by 2^-9.3 with that, by 2^-22 so, for a read more.
 template <typename T, typename W, int CH, int GROUP, bool DROP, bool FROM_X, int THREADS>
 __global__ void __launch_bounds__(THREADS, CH == 1 ? 1024 / THREADS : 1) rms_norm_grad_kernel(const __grid_constant__ NormGradParams p) {
@@ -355,8 +355,10 @@ cudaError_t launch_rms_norm(const NormParams& p, cudaStream_t st, int sms) {
   if (p.width <= 256) return launch_rms_norm_as<T, W, 1, true, EIGHT, WARPS>(p, st, sms);
   // A warp with two chunks a lane, if nothing is dropped (23491 x 288 in fp16 12.4 us, two warps with one 18.9; with the lots of two chunks it has 103 registers).
   if (p.width <= 512 && p.drop.threshold == 0) return launch_rms_norm_as<T, W, 2, true, EIGHT, WARPS>(p, st, sms);
-  // few rows: as many threads as there are chunks
-  if (p.width <= (p.rows < sms ? 4096 : 2048)) return launch_rms_norm_as<T, W, 1, false, EIGHT, 512>(p, st, sms);
+  // Few rows, or lots to draw: as many threads as there are chunks.
+  const bool drop = p.drop.threshold > 0;
+  if (p.width <= (p.rows < sms || drop ? 4096 : 2048)) return launch_rms_norm_as<T, W, 1, false, EIGHT, 512>(p, st, sms);
+  if (p.width <= 8192 && p.rows < sms) return launch_rms_norm_as<T, W, 1, false, EIGHT, NORM_MAX_THREADS>(p, st, sms);
   if (p.width <= 8192) return launch_rms_norm_as<T, W, 2, false, EIGHT, 512>(p, st, sms);
   return launch_rms_norm_as<T, W, 4, false, EIGHT, NORM_MAX_THREADS>(p, st, sms);
 }
@@ -369,7 +371,8 @@ struct NormGradCut {
 inline NormGradCut norm_grad_cut(long long rows, int width, int sms) {
   NormGradCut c;
   c.group = width <= 256 ? 1 : width <= 512 ? 2 : 0;
-  c.ch = width <= 4096 ? 1 : width <= 8192 ? 2 : 4;
+  // as many threads as there are chunks, 64 registers each: 920 x 4448 in fp16 with its forward 37.6 us with two chunks a thread, 35.7 so
+  c.ch = width <= 8192 ? 1 : width <= 16384 ? 2 : 4;
   c.threads = c.group ? 32 * c.group * NORM_GRAD_ROWS : norm_threads(width, c.ch);
   const long long blocks = c.group ? (rows + NORM_GRAD_ROWS - 1) / NORM_GRAD_ROWS : rows, at_once = (long long)sms * (c.threads <= 1024 ? 1024 / c.threads : 1);
   c.blocks = (int)(blocks < at_once ? blocks : at_once);
@@ -391,8 +394,8 @@ template <typename T, typename W>
 cudaError_t launch_rms_norm_grad(const NormGradParams& p, const NormGradCut& cut, cudaStream_t st) {
   if (cut.group == 1) return launch_rms_norm_grad_as<T, W, 1, 1, 32 * NORM_GRAD_ROWS>(p, cut, st);
   if (cut.group == 2) return launch_rms_norm_grad_as<T, W, 1, 2, 64 * NORM_GRAD_ROWS>(p, cut, st);
-  if (cut.ch == 1) return launch_rms_norm_grad_as<T, W, 1, 0, 512>(p, cut, st);
-  return cut.ch == 2 ? launch_rms_norm_grad_as<T, W, 2, 0, 512>(p, cut, st) : launch_rms_norm_grad_as<T, W, 4, 0, 1024>(p, cut, st);
+  if (cut.ch == 1) return cut.threads <= 512 ? launch_rms_norm_grad_as<T, W, 1, 0, 512>(p, cut, st) : launch_rms_norm_grad_as<T, W, 1, 0, 1024>(p, cut, st);
+  return cut.ch == 2 ? launch_rms_norm_grad_as<T, W, 2, 0, 1024>(p, cut, st) : launch_rms_norm_grad_as<T, W, 4, 0, 1024>(p, cut, st);
 }
 template <typename W>
 cudaError_t launch_rms_norm_weight_grad(const float* parts, int n, int width, void* dw, int alone, cudaStream_t st) {
