@@ -14,7 +14,9 @@
 // crosses CTAs, and the same bits come out on every run: contractions that were shared by CTAs cost 5 us a product in handing sums over, and a barrier of all
 // CTAs between the products as much again.  Instead an item of W_out waits for the items of its expert alone, and whoever finishes a
 // column block of the output last adds up what the token's experts left there.  The products are mma.sync.m16n8k16 with the columns of the weight as M and an
-// expert's tokens as N, eight a step (rows that are no token are computed and thrown away).
+// expert's tokens as N, eight a step (rows that are no token are computed and thrown away).  h is held as the sum of two values of the type, its rounding
+// and what that left, and multiplied twice: rounded once, the output was off by 2^-8.6 in bf16 where its own rounding is 2^-9.2, and the tensor cores have
+// nothing else to do.
 //
 //   warps 0-7   products: 16 rows of every tile each; their sums meet in shared memory at the end of an item
 //   warp 8      TMA producer of weights          warp 9   producer of the tokens' rows (cp.async: as a bulk copy a row and tile, 56 ns each, 64 tokens a tile took
@@ -34,7 +36,6 @@ constexpr int EL_K = 128, EL_COLUMNS = 64;         // a tile
 constexpr int EL_TILE_BYTES = EL_K * EL_COLUMNS * 2;
 constexpr int EL_MAX_STAGES = 12;
 constexpr int EL_X_PITCH = EL_K * 2 + 16;          // tokens' rows, 16 bytes more apart than they are long so that eight of them lie in all banks
-constexpr int EL_X_BYTES = 3 * EL_MAX_TOKENS * EL_X_PITCH;  // three tiles of 64 rows, or as many more as fewer rows allow: a copy's way is as long as three tiles
 constexpr int EL_CONSUMERS = 256, EL_REPORTERS = 64, EL_THREADS = EL_CONSUMERS + 64 + EL_REPORTERS, EL_WARPS = EL_THREADS / 32;
 constexpr int EL_SUMS = 16;                        // of a thread for eight tokens: 64 columns by eight a warp
 constexpr int EL_ROUTER_THREADS = 256, EL_ROUTER_AT_ONCE = 4;  // chunks of a row whose loads are on their way together
@@ -48,9 +49,9 @@ struct ExpertParams {
   long long x_pitch, out_pitch;
   // workspace
   uint32_t* flags;   // [experts]: items of W_in that are done, by used expert; [blocks of the output]: items of W_out
-  uint16_t* h;       // [tokens top_k][hidden], in the order of the experts
+  uint16_t* h;       // [tokens top_k][2][hidden], in the order of the experts: rounded, and the remainders
   float* part;       // [tokens top_k][out_width]
-  int ctas, stages, n_flags;
+  int ctas, n_flags, ring_bytes;  // ring_bytes: of shared memory, for weights and tokens' rows
   int alone;
 };
 
@@ -220,9 +221,15 @@ __device__ __forceinline__ void el_mma(float (&d)[4], const uint32_t (&a)[4], ui
 }
 __device__ __forceinline__ float el_activated(int activation, float v) { return activation == 0 ? (v != v ? v : fmaxf(v, 0.f)) : v / (1.f + __expf(-v)); }
 template <bool BF16>
+__device__ __forceinline__ float el_widen(uint16_t h) {
+  return BF16 ? __uint_as_float((uint32_t)h << 16) : __half2float(__ushort_as_half(h));
+}
+template <bool BF16>
 __device__ __forceinline__ uint16_t el_round(float v) {
   return BF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v)) : __half_as_ushort(__float2half_rn(v));
 }
+
+constexpr int EL_FIXED_BYTES = (EL_CONSUMERS * EL_SUMS * (int)sizeof(float) + (int)sizeof(ElShared) + 1023) / 1024 * 1024;
 
 // The pairs in the order of their experts, of an expert in the order of its tokens: a token goes to an expert once at most, so that an expert's
 // pairs are a set of tokens, 64 bits.
@@ -317,17 +324,19 @@ __device__ __forceinline__ void el_sort(const ExpertParams& p, ElShared* sh) {
   __syncthreads();
 }
 
-// What every role goes by: the items, and the ring of the tokens' rows.
+// What every role goes by: the items, and the rings.  The tokens' rows (of the expert that has the most, with their remainders) get up to twelve tiles but leave six of
+// weights at least, two in any case; the weights get the rest.
 struct ElPlan {
-  int used, ctas, blocks_in, blocks_out, x_bytes, x_stages;
+  int used, ctas, blocks_in, blocks_out, x_bytes, x_stages, stages;
   __device__ __forceinline__ ElPlan(const ExpertParams& p, const ElShared* sh) {
     const int h_columns = p.gated ? EL_COLUMNS / 2 : EL_COLUMNS;  // that an item of W_in stands for
     used = sh->used;
     ctas = p.ctas;
     blocks_in = (p.hidden + h_columns - 1) / h_columns;
     blocks_out = (p.out_width + EL_COLUMNS - 1) / EL_COLUMNS;
-    x_bytes = sh->most * EL_X_PITCH;
-    x_stages = min(EL_MAX_STAGES, EL_X_BYTES / x_bytes);
+    x_bytes = 2 * sh->most * EL_X_PITCH;  // (W_in's have no remainders and leave half of it)
+    x_stages = min(EL_MAX_STAGES, max(2, (p.ring_bytes - 6 * EL_TILE_BYTES) / x_bytes));
+    stages = min(EL_MAX_STAGES, (p.ring_bytes - x_stages * x_bytes) / EL_TILE_BYTES);
   }
   __device__ __forceinline__ ElItems items(int product) const {
     return product == 0 ? ElItems(used * blocks_in, 0, (int)blockIdx.x, ctas, blocks_in) : ElItems(used * blocks_out, used * blocks_in, (int)blockIdx.x, ctas, blocks_out);
@@ -370,8 +379,7 @@ __device__ __forceinline__ void el_products(const ExpertParams& p, ElShared* sh,
       for (int k = 0; k < length; k += EL_K) {
         if (ok) ok = mbar_parked_wait(smem_u32(&sh->x_full[x_at]), x_ph, abort_flag) && mbar_parked_wait(smem_u32(&sh->full[s]), ph, abort_flag);
         __syncwarp();
-        const int there = (length - k - warp * 16) / 8;  // of this warp's rows: groups of eight that there are
-        if (there > 0) {
+        if (k + warp * 16 < length) {  // (behind the contraction's end both operands are zeros)
           const uint32_t tile = weights + (uint32_t)(s * EL_TILE_BYTES), x = rows + (uint32_t)(x_at * plan.x_bytes);
           uint32_t a[4][4];
 #pragma unroll
@@ -379,14 +387,22 @@ __device__ __forceinline__ void el_products(const ExpertParams& p, ElShared* sh,
 #pragma unroll
           for (int j = 0; j < NT; j += 2) {
             if (j * 8 < n) {
-              uint32_t b[4];
+              uint32_t b[4], rest[4];
               el_ldmatrix(b, x + (uint32_t)(j * 8 * EL_X_PITCH));
-              if (there < 2) b[1] = b[3] = 0u;  // the weights are zeros there, and what lies in the rows' place may be anything
+              if (product == 1) el_ldmatrix(rest, x + (uint32_t)(plan.x_bytes / 2 + j * 8 * EL_X_PITCH));  // what h's rounding left
 #pragma unroll
               for (int q = 0; q < 4; ++q) el_mma<BF16>(acc[j][q], a[q], b[0], b[1]);
               if (j * 8 + 8 < n) {
 #pragma unroll
                 for (int q = 0; q < 4; ++q) el_mma<BF16>(acc[j + 1][q], a[q], b[2], b[3]);
+              }
+              if (product == 1) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) el_mma<BF16>(acc[j][q], a[q], rest[0], rest[1]);
+                if (j * 8 + 8 < n) {
+#pragma unroll
+                  for (int q = 0; q < 4; ++q) el_mma<BF16>(acc[j + 1][q], a[q], rest[2], rest[3]);
+                }
               }
             }
           }
@@ -396,7 +412,7 @@ __device__ __forceinline__ void el_products(const ExpertParams& p, ElShared* sh,
           mbar_arrive(smem_u32(&sh->empty[s]));
           mbar_arrive(smem_u32(&sh->x_empty[x_at]));
         }
-        if (++s == p.stages) { s = 0; ph ^= 1u; }
+        if (++s == plan.stages) { s = 0; ph ^= 1u; }
         if (++x_at == plan.x_stages) { x_at = 0; x_ph ^= 1u; }
       }
       // ---------------------------------------------------------------- the item's sums
@@ -417,13 +433,19 @@ __device__ __forceinline__ void el_products(const ExpertParams& p, ElShared* sh,
         if (token < n) {
           const int col = m * (gated ? EL_COLUMNS / 2 : EL_COLUMNS) + q * (gated ? 8 : 16) + g;
           if (product == 0) {
-            uint16_t* h_row = p.h + (size_t)(first + token) * p.hidden;
+            uint16_t* h_row = p.h + (size_t)(first + token) * 2 * p.hidden;
+            const auto put = [&](int at, float v) {  // (an h that the type does not hold has no remainder)
+              const uint16_t rounded = el_round<BF16>(v);
+              const float left = v - el_widen<BF16>(rounded);
+              h_row[at] = rounded;
+              h_row[p.hidden + at] = el_round<BF16>(fabsf(left) <= fabsf(v) ? left : 0.f);
+            };
             v0 = el_activated(p.activation, v0);
             if (gated) {
-              if (col < columns) h_row[col] = el_round<BF16>(v0 * v1);
+              if (col < columns) put(col, v0 * v1);
             } else {
-              if (col < columns) h_row[col] = el_round<BF16>(v0);
-              if (col + 8 < columns) h_row[col + 8] = el_round<BF16>(el_activated(p.activation, v1));
+              if (col < columns) put(col, v0);
+              if (col + 8 < columns) put(col + 8, el_activated(p.activation, v1));
             }
           } else {
             const int pair = sh->list[first + token];
@@ -454,14 +476,15 @@ __global__ void __launch_bounds__(EL_THREADS, 1)
   using namespace umma;
   extern __shared__ uint8_t el_smem[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(el_smem) + 1023) & ~static_cast<uintptr_t>(1023));
-  float* sums = reinterpret_cast<float*>(smem + (size_t)p.stages * EL_TILE_BYTES + EL_X_BYTES);  // [warps][EL_SUMS][32]
+  float* sums = reinterpret_cast<float*>(smem);  // [warps][EL_SUMS][32]
   ElShared* sh = reinterpret_cast<ElShared*>(sums + EL_CONSUMERS * EL_SUMS);
+  const uint32_t ring = smem_u32(smem) + EL_FIXED_BYTES;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, cta = (int)blockIdx.x;
   volatile int* abort_flag = &sh->abort_flag;
   if (threadIdx.x == 0) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(&map_in) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&map_out) : "memory");
-    for (int s = 0; s < p.stages; ++s) {
+    for (int s = 0; s < EL_MAX_STAGES; ++s) {
       mbar_init(smem_u32(&sh->full[s]), 1);
       mbar_init(smem_u32(&sh->empty[s]), EL_CONSUMERS / 32);
     }
@@ -483,7 +506,7 @@ __global__ void __launch_bounds__(EL_THREADS, 1)
   __syncthreads();
   el_sort(p, sh);
   const ElPlan plan(p, sh);
-  const uint32_t tiles0 = smem_u32(smem), x0 = tiles0 + (uint32_t)(p.stages * EL_TILE_BYTES);
+  const uint32_t tiles0 = ring, x0 = tiles0 + (uint32_t)(plan.stages * EL_TILE_BYTES);
   uint32_t *done_in = p.flags, *done_out = p.flags + p.n_experts;
   bool ok = true;
 
@@ -505,7 +528,7 @@ __global__ void __launch_bounds__(EL_THREADS, 1)
             mbar_expect_tx(bar, EL_TILE_BYTES);
             pair_load_3d<1>(to, map, bar, col, k, e);
             if (gated) pair_load_3d<1>(to + EL_TILE_BYTES / 2, map, bar, p.hidden + col, k, e);
-            if (++s == p.stages) { s = 0; ph ^= 1u; }
+            if (++s == plan.stages) { s = 0; ph ^= 1u; }
           }
         }
       }
@@ -531,8 +554,9 @@ __global__ void __launch_bounds__(EL_THREADS, 1)
           const uint32_t to = x0 + (uint32_t)(s * plan.x_bytes + (lane & 15) * 16);
 #pragma unroll 4
           for (int row = lane >> 4; row < n; row += 2) {
-            const uint16_t* src = product == 0 ? static_cast<const uint16_t*>(p.x) + sh->token[first + row] * p.x_pitch : p.h + (size_t)(first + row) * p.hidden;
+            const uint16_t* src = product == 0 ? static_cast<const uint16_t*>(p.x) + sh->token[first + row] * p.x_pitch : p.h + (size_t)(first + row) * 2 * p.hidden;
             cp_async16(to + (uint32_t)(row * EL_X_PITCH), at < length ? src + at : src, at < length);
+            if (product == 1) cp_async16(to + (uint32_t)((sh->most + row) * EL_X_PITCH), at < length ? src + p.hidden + at : src, at < length);
           }
           cp_async_arrive_noinc(smem_u32(&sh->x_full[s]));
           if (++s == plan.x_stages) { s = 0; ph ^= 1u; }
@@ -618,7 +642,7 @@ inline ExpertSpace expert_space(int tokens, int experts, int top_k, int hidden, 
   };
   s.n_flags = experts + (out_width + EL_COLUMNS - 1) / EL_COLUMNS;
   s.flags = take((size_t)s.n_flags * sizeof(uint32_t));
-  s.h = take((size_t)tokens * top_k * hidden * 2);
+  s.h = take((size_t)tokens * top_k * 2 * hidden * 2);
   s.part = take((size_t)tokens * top_k * out_width * sizeof(float));
   s.total = at;
   return s;
@@ -665,11 +689,9 @@ cudaError_t launch_expert_choice(const ExpertParams& p, cudaStream_t st) {
 
 template <bool BF16>
 int launch_expert_layer(ExpertParams p, const void* w_in, const void* w_out, cudaStream_t st, int max_smem) {
-  const int rest = 1024 + EL_X_BYTES + EL_CONSUMERS * EL_SUMS * (int)sizeof(float) + (int)sizeof(ElShared);
-  p.stages = (max_smem - rest) / EL_TILE_BYTES;
-  if (p.stages > EL_MAX_STAGES) p.stages = EL_MAX_STAGES;
-  if (p.stages < 2) return -1;
-  const int smem = rest + p.stages * EL_TILE_BYTES;
+  p.ring_bytes = max_smem - 1024 - EL_FIXED_BYTES;
+  if (p.ring_bytes < 6 * EL_TILE_BYTES + 4 * EL_MAX_TOKENS * EL_X_PITCH) return -1;
+  const int smem = max_smem;
   CUtensorMap in, out;
   const int wide = p.gated ? 2 * p.hidden : p.hidden;
   int rc = expert_tensor_map(&in, w_in, wide, p.width, p.n_experts, p.gated ? 32 : 64, BF16);

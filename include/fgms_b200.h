@@ -447,7 +447,7 @@ size_t fgms_b200_grouped_i8_workspace_bytes(const int8_t* codes, int64_t codes_p
  *
  * x [tokens, width], router [experts, width], w_in [experts, width, hidden] (gated: 2 hidden), w_out [experts, hidden, out_width]; F16 or BF16, the
  * router of that type or F32.  Logits are summed in 64 bits, products in fp32, each token's sum over its experts in fp32 in their order; h is
- * rounded to the type once (its magnitude has to be one that the type holds).  The same bits on every run.  Widths are multiples of 8, rows and weights start
+ * held as the sum of two values of the type (its magnitude has to be one that the type holds).  The same bits on every run.  Widths are multiples of 8, rows and weights start
  * on 16-byte boundaries; experts at most 512, top_k at most 16.  A logit that is NaN counts as the lowest; a token with none that is more gets gates of NaN.
  * out may be x itself.  The second launch is cooperative, a CTA an SM that is not kept free; its waits are bounded (fgms_b200_device_status).
  * workspace: fgms_b200_expert_layer_workspace_bytes on the current device, 256-byte aligned, whose contents do not matter. */
