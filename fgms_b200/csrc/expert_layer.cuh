@@ -324,8 +324,24 @@ __device__ __forceinline__ void el_sort(const ExpertParams& p, ElShared* sh) {
   __syncthreads();
 }
 
-// What every role goes by: the items, and the rings.  The tokens' rows (of the expert that has the most, with their remainders) get up to twelve tiles but leave six of
-// weights at least, two in any case; the weights get the rest.
+// The two rings in `bytes` of shared memory, weights first.  The tokens' rows (`most` of them, with their remainders) get up to twelve tiles but leave six of weights
+// at least, two in any case; the weights get the rest.  Fragments are read 16 rows at a time, of which the last ones may be none of the tile's: behind the
+// last tile there is room for them (what they hold does not matter).
+struct ElRings {
+  int x_bytes, x_stages, stages;  // a tile of rows; tiles
+};
+constexpr int EL_X_ROOM = 16 * EL_X_PITCH;
+__host__ __device__ __forceinline__ ElRings el_rings(int bytes, int most) {
+  ElRings r;
+  r.x_bytes = 2 * most * EL_X_PITCH;  // (W_in's have no remainders and leave half of it)
+  const int free = bytes - EL_X_ROOM, x = (free - 6 * EL_TILE_BYTES) / r.x_bytes;
+  r.x_stages = x < 2 ? 2 : x < EL_MAX_STAGES ? x : EL_MAX_STAGES;
+  const int w = (free - r.x_stages * r.x_bytes) / EL_TILE_BYTES;
+  r.stages = w < EL_MAX_STAGES ? w : EL_MAX_STAGES;
+  return r;
+}
+
+// What every role goes by: the items, and the rings.
 struct ElPlan {
   int used, ctas, blocks_in, blocks_out, x_bytes, x_stages, stages;
   __device__ __forceinline__ ElPlan(const ExpertParams& p, const ElShared* sh) {
@@ -334,9 +350,10 @@ struct ElPlan {
     ctas = p.ctas;
     blocks_in = (p.hidden + h_columns - 1) / h_columns;
     blocks_out = (p.out_width + EL_COLUMNS - 1) / EL_COLUMNS;
-    x_bytes = 2 * sh->most * EL_X_PITCH;  // (W_in's have no remainders and leave half of it)
-    x_stages = min(EL_MAX_STAGES, max(2, (p.ring_bytes - 6 * EL_TILE_BYTES) / x_bytes));
-    stages = min(EL_MAX_STAGES, (p.ring_bytes - x_stages * x_bytes) / EL_TILE_BYTES);
+    const ElRings r = el_rings(p.ring_bytes, sh->most);
+    x_bytes = r.x_bytes;
+    x_stages = r.x_stages;
+    stages = r.stages;
   }
   __device__ __forceinline__ ElItems items(int product) const {
     return product == 0 ? ElItems(used * blocks_in, 0, (int)blockIdx.x, ctas, blocks_in) : ElItems(used * blocks_out, used * blocks_in, (int)blockIdx.x, ctas, blocks_out);
@@ -690,7 +707,7 @@ cudaError_t launch_expert_choice(const ExpertParams& p, cudaStream_t st) {
 template <bool BF16>
 int launch_expert_layer(ExpertParams p, const void* w_in, const void* w_out, cudaStream_t st, int max_smem) {
   p.ring_bytes = max_smem - 1024 - EL_FIXED_BYTES;
-  if (p.ring_bytes < 6 * EL_TILE_BYTES + 4 * EL_MAX_TOKENS * EL_X_PITCH) return -1;
+  if (p.ring_bytes < 6 * EL_TILE_BYTES + 4 * EL_MAX_TOKENS * EL_X_PITCH + EL_X_ROOM) return -1;
   const int smem = max_smem;
   CUtensorMap in, out;
   const int wide = p.gated ? 2 * p.hidden : p.hidden;

@@ -950,7 +950,8 @@ bool exact_sum_needed(const Tensor& x, const Tensor& weight) { return weight.sca
 struct Normed {
   Tensor out, sum, rstd, used;  // 2-D, but out and sum
 };
-Normed norm_forward(const Tensor& x_, const Tensor& weight_, const Tensor* residual_, double eps, double p, const Tensor* rng, bool for_backward) {
+// `for_backward`: what a gradient needs is left as well; `from_x`: it will go by x and the residual instead of the sum
+Normed norm_forward(const Tensor& x_, const Tensor& weight_, const Tensor* residual_, double eps, double p, const Tensor* rng, bool for_backward, bool from_x) {
   const Tensor x = as_rows(x_), weight = weight_.contiguous(), residual = residual_ ? as_rows(*residual_) : Tensor();
   Normed n;
   n.out = new_like(x_.is_contiguous() ? x_ : x);
@@ -958,7 +959,7 @@ Normed norm_forward(const Tensor& x_, const Tensor& weight_, const Tensor* resid
   const bool drop = drops(p);
   const Tensor out = as_rows(n.out);
   Tensor sum;
-  if (residual_ || (drop && for_backward && !exact_sum_needed(x_, weight_))) {
+  if (residual_ || (drop && for_backward && !from_x)) {
     n.sum = at::empty_like(n.out);
     sum = as_rows(n.sum);
   }
@@ -973,10 +974,10 @@ Normed norm_forward(const Tensor& x_, const Tensor& weight_, const Tensor* resid
 struct RmsNorm : torch::autograd::Function<RmsNorm> {
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& weight,
                                                 const std::optional<Tensor>& residual, const std::optional<Tensor>& rng, double eps, double p) {
-    Normed n = norm_forward(x, weight, residual ? &*residual : nullptr, eps, p, rng ? &*rng : nullptr, true);
+    const bool from_x = (residual || drops(p)) && weight.requires_grad() && exact_sum_needed(x, weight);
+    Normed n = norm_forward(x, weight, residual ? &*residual : nullptr, eps, p, rng ? &*rng : nullptr, true, from_x);
     ctx->saved_data["p"] = p;
     ctx->saved_data["residual"] = residual.has_value();
-    const bool from_x = (residual || drops(p)) && weight.requires_grad() && exact_sum_needed(x, weight);
     ctx->saved_data["from_x"] = from_x;
     ctx->save_for_backward({from_x || !n.sum.defined() ? x : n.sum, weight, n.rstd, n.used, from_x && residual ? *residual : Tensor()});
     ctx->set_materialize_grads(false);
@@ -1517,7 +1518,7 @@ PyObject* py_rms_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     out = r[0];
     if (residual) sum = r[1];
   } else {
-    const Normed r = norm_forward(x, weight, residual, eps, p, rng, false);
+    const Normed r = norm_forward(x, weight, residual, eps, p, rng, false, false);
     out = r.out;
     sum = r.sum;
   }

@@ -187,7 +187,8 @@ _FEW_TOKENS, _MOST_EXPERTS, _MOST_CHOSEN = 64, 512, 16  # what backend.fgms_expe
 def _few_tokens(x, router, w_in, w_out, top_k) -> bool:
     needs_grad = torch.is_grad_enabled() and any(t.requires_grad for t in (x, router, w_in, w_out))
     return (not needs_grad and 0 < x.size(0) <= _FEW_TOKENS and router.size(0) <= _MOST_EXPERTS and top_k <= _MOST_CHOSEN
-            and x.dtype in (torch.float16, torch.bfloat16) and x.size(1) % 8 == 0 and w_out.size(1) % 8 == 0 and w_out.size(2) % 8 == 0
+            and x.dtype in (torch.float16, torch.bfloat16) and w_in.dtype == w_out.dtype == x.dtype and router.dtype in (x.dtype, torch.float32)
+            and x.size(1) % 8 == 0 and w_out.size(1) % 8 == 0 and w_out.size(2) % 8 == 0
             and all(t.is_contiguous() and t.data_ptr() % 16 == 0 for t in (x, router, w_in, w_out)))
 
 
@@ -224,7 +225,7 @@ def expert_layer(x: torch.Tensor, router: torch.Tensor, w_in: torch.Tensor, w_ou
     h = act(u[:, :hidden]) * u[:, hidden:] if u.size(1) == 2 * hidden and hidden else act(u)
     y = grouped_linear(h, w_out, kpos)
     back = torch.empty_like(order).scatter_(0, order, torch.arange(order.numel(), device=x.device))
-    out = (y[back].float().view(rows.size(0), top_k, -1) * gate[:, :, None]).sum(1)
+    out = (y[back].float().view(rows.size(0), top_k, w_out.size(2)) * gate[:, :, None]).sum(1)
     return out.to(x.dtype).view(*x.shape[:-1], w_out.size(2))
 
 

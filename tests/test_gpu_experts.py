@@ -90,6 +90,14 @@ def test_against_the_definition(case, dtype):
     assert all(torch.equal(a, b) for a, b in zip(first, layer.run()))
 
 
+@pytest.mark.parametrize("tokens", range(1, 65))
+def test_every_number_of_tokens_that_an_expert_may_have(tokens):
+    """The rings in shared memory are cut by it (``test_expert_rings_cpu.py`` has their sizes): all tokens to the first of two experts."""
+    layer = Layer("bf16", tokens, 2, 1, 264, 200, seed=tokens)
+    layer.router[1] = layer.router[0]
+    layer.check(layer.run())
+
+
 def test_equal_logits_go_to_the_lower_index():
     layer = Layer("bf16", 30, 40, 6, 64, 64, seed=2)
     layer.router[7:33] = layer.router[5]
@@ -244,6 +252,10 @@ def test_both_ways_give_the_same_layer():
     near(routed.detach(), out, allowed + 4.5 * 2.0 ** -8 * size)
     with torch.no_grad():
         assert torch.equal(module(layer.x.repeat(2, 1))[:40], module(layer.x.repeat(2, 1))[40:])
+        assert module(layer.x[:0]).shape == (0, 128) and module(layer.x[0]).shape == (128,)
+        assert torch.equal(module(layer.x[0]), few.view(40, 128)[0])
+        fp16 = nn.expert_layer(layer.x, module.router.half(), module.w_in, module.w_out, 2)  # a router of another 16-bit type: not through the kernel
+        assert (fp16.float() - few.view(40, 128).float()).abs().max() < 1.0
 
 
 def test_a_block_in_training_and_in_serving():

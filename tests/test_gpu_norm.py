@@ -277,6 +277,21 @@ def test_gradients_in_pieces():
         g.sum().backward()
 
 
+@pytest.mark.parametrize("weight", ["same", "fp32"])
+@pytest.mark.parametrize("residual", [False, True])
+def test_a_weight_that_is_frozen(weight, residual):
+    from fgms_b200 import nn
+    c = Case("bf16", 50, 130, weight, seed=3)
+    x, res = c.x.clone().requires_grad_(), c.res.clone().requires_grad_() if residual else None
+    got = nn.rms_norm(x, c.w, 1e-5, residual=res, dropout=0.5, rng=nn.rng_state(SEED))
+    ref = Norm(c.x, c.w, 1e-5, c.res if residual else None, mask_of(c, 0.5))
+    ref.stored = ref.unit
+    leaves = (x, res) if residual else (x,)
+    grads = torch.autograd.grad(got[0] if residual else got, leaves, c.dy)
+    for g, want in zip(grads, ref.backward(c.dy, None, torch.float32)):
+        near(g, *want)
+
+
 def test_no_rows():
     from fgms_b200 import nn
     x, w, rng = torch.zeros((0, 64), device="cuda", requires_grad=True), torch.ones(64, device="cuda", requires_grad=True), nn.rng_state(1)
