@@ -20,7 +20,7 @@ struct DropoutParams {
 
 // A chunk is a thread's; threads go on by the whole grid, whose width in rows and columns is divided once, and so are the ways through the tensors.  What
 // bounds it are instructions as much as memory: 228 a chunk of eight at first (masks of bits, products for addresses, conversions one by one), 168 now, of
-// which the lots are some 70.  SOME: something is dropped.
+// which the lots are some 70: 32768 x 2048 in bf16 with a residual 72 us, its gradient 64, 85 and 64 % of the measured copy rate.  SOME: something is dropped.
 template <typename T, bool BACKWARD, bool SOME>
 __global__ void __launch_bounds__(DROP_THREADS, DROP_BLOCKS) dropout_kernel(const __grid_constant__ DropoutParams p) {
   umma::griddep_wait();

@@ -7,7 +7,8 @@
 //
 // Both operands have the contraction side by side in memory (weights are [groups, c_out, c_in]: a channel's row is what has a scale), 128 values a
 // stage: the bytes of a stage, the walk over the tiles and the cut of a call are those of the input gradient in 16 bits (grouped_umma.cuh), which
-// is told half as many channels.  An MMA takes 32 values where that one takes 16, in the same time.
+// is told half as many channels.  An MMA takes 32 values where that one takes 16, in the same time: 16384 rows 2048 -> 4096 to bf16 90 us, 3.06 POP/s, kept
+// busy 110 (the power limit), the tensor pipe active 78 % of it; one row 8.6 us, latency.
 //
 //   warp 0      producer          warp 1      MMA issuer (of the pair's even CTA)
 //   warps 4-11  epilogue: scales, a transposition through shared memory and 16-byte stores; outputs off 16-byte boundaries go straight to
