@@ -15,14 +15,14 @@ def philox(counter, key):
     return np.stack(c, -1).astype(np.uint32)
 
 
-def kept(rows, width, p, seed, call):
-    """What each value is multiplied by: 0, or the factor of those that are kept (a float64 array [rows, width])."""
+def kept(rows, width, p, seed, call, first=0):
+    """What each value is multiplied by: 0, or the factor of those that are kept (a float64 array of the rows from `first` on)."""
     threshold = int(np.rint(p * 65536.0))
     if threshold == 65536:
         return np.zeros((rows, width))
     blocks = (width + 7) // 8
     counter = np.empty((rows, blocks, 4), dtype=np.uint64)
-    counter[..., 0], counter[..., 1] = np.arange(blocks)[None, :], np.arange(rows)[:, None]
+    counter[..., 0], counter[..., 1] = np.arange(blocks)[None, :], first + np.arange(rows)[:, None]
     counter[..., 2], counter[..., 3] = call & 0xFFFFFFFF, (call >> 32) & 0xFFFFFFFF
     words = philox(counter, (seed & 0xFFFFFFFF, (seed >> 32) & 0xFFFFFFFF))
     lots = np.stack([words & 0xFFFF, words >> 16], -1).reshape(rows, blocks * 8)[:, :width]

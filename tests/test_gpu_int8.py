@@ -171,6 +171,16 @@ def test_with_sms_kept_free():
     assert torch.equal(got, want)
 
 
+def test_outputs_beyond_32_bits():
+    from fgms_b200 import nn
+    rows, c_out, tail = 560000, 4000, 100
+    layer = Layer([rows], 48, c_out, seed=12, scale=0.001)
+    for dtype in (torch.bfloat16, torch.float32):
+        out = nn.int8_linear(layer.codes, layer.scale, layer.kernel, layer.kernel_scale, layer.kpos, dtype)
+        assert torch.equal(out[-tail:], nn.int8_linear(layer.codes[-tail:], layer.scale[-tail:].clone(), layer.kernel, layer.kernel_scale, dtype=dtype))
+        del out
+
+
 def test_a_block_for_serving():
     """Norm into 8 bits, a layer of groups in 8 bits, norm, a plain matrix: within the steps of the codes of the same in 64 bits.
 

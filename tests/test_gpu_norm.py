@@ -354,6 +354,33 @@ def test_replays_drop_other_values_and_streams_do_not_disturb():
     assert rng.tolist() == [SEED, 8, 0]
 
 
+def test_values_beyond_32_bits():
+    """2.2e9 values: the last rows are what they are by themselves, and so are their gradients and what is dropped of them."""
+    from fgms_b200 import backend, nn
+    rows, width, tail = 67000, 32760, 8
+    x = torch.empty((rows, width), dtype=torch.float16, device="cuda")
+    x.fill_(0.5)
+    x[-tail:] = made(1, tail, width, dtype=torch.float16)
+    w = (1 + 0.3 * made(2, width)).half()
+    y = nn.rms_norm(x, w)
+    assert torch.equal(y[-tail:], nn.rms_norm(x[-tail:].clone(), w))
+    out, rng, used = y, nn.rng_state(SEED), torch.empty(2, dtype=torch.int64, device="cuda")
+    backend.fgms_dropout_cuda(x, out, 0.25, rng, rng_used=used)
+    m = torch.from_numpy(kept(tail, width, 0.25, SEED, 0, first=rows - tail)).cuda()
+    want = x[-tail:].double() * m
+    near(out[-tail:], want, want.abs() * (2.0 ** -11 + 2.0 ** -23) + tiny(torch.float16))
+    backend.fgms_dropout_bwd_cuda(out, out, 0.25, used)  # twice the same lots: dropped where it was dropped
+    assert torch.equal(out[-tail:] == 0, (m == 0) | (x[-tail:] == 0))
+    rstd = torch.ones(rows, device="cuda")
+    dx = torch.empty((tail, width), dtype=torch.float16, device="cuda")
+    backend.fgms_rms_norm_bwd_cuda(out[-tail:].clone(), x[-tail:].clone(), w, rstd[-tail:].clone(), x_grad=dx)
+    backend.fgms_rms_norm_bwd_cuda(out, x, w, rstd, x_grad=out)  # over what flows in
+    assert torch.equal(out[-tail:], dx)
+    codes, scale = nn.quantize_rows(x)
+    few = nn.quantize_rows(x[-tail:].clone())
+    assert torch.equal(codes[-tail:], few[0]) and torch.equal(scale[-tail:], few[1])
+
+
 def test_modules():
     from fgms_b200 import nn
     c = Case("bf16", 40, 128)
