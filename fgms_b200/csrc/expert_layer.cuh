@@ -23,7 +23,7 @@
 //               a tile ten times as long as its weights)
 //   warps 10-11 report finished items and add the output up: a report waits until all that was stored is there, a microsecond that the products go on in
 //
-// All waits are bounded.  bf16: one token, 2 of 8 experts 512 x 1024, 16.4 us, which is latency; 16 tokens, 4 of 64 experts 2048 x 1024 each, 517 MB of weights, 104 us (79
+// All waits are bounded.  bf16: one token, 2 of 8 experts 512 x 1024, 17.7 us, which is latency; 16 tokens, 4 of 64 experts 2048 x 1024 each, 517 MB of weights, 104 us (79
 // at the measured copy rate), 5.6 TB/s between the first tile and the last; 64 tokens, 2 of 32 experts 1024 x 2048 without a gate, 264 MB, 71 us (40).  With 33 tokens an expert and
 // more the products take longer than the weights' way: 64 tokens, all of 4 experts 2048 x 1024, 86 us.
 #pragma once
@@ -108,7 +108,9 @@ __device__ __forceinline__ void el_choose(const ExpertParams& p, const double* l
 template <typename T, typename R>
 __global__ void __launch_bounds__(EL_ROUTER_THREADS) expert_choice_kernel(const __grid_constant__ ExpertParams p) {
   __shared__ double logits[EL_MAX_EXPERTS];
+  umma::cluster_arrive();  // another CTA's shared memory is written only once that CTA is known to run; the kernel before this one is waited for meanwhile
   umma::griddep_wait();
+  umma::cluster_wait();
   if (!p.alone) umma::griddep_launch_dependents();
   uint32_t rank, size;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
@@ -142,6 +144,7 @@ __global__ void __launch_bounds__(EL_ROUTER_THREADS) expert_choice_kernel(const 
       asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(there) : "r"(umma::smem_u32(logits + e)));
       asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(there), "d"(v) : "memory");
     }
+    __syncwarp();
   }
   umma::cluster_sync();
   if (rank != 0 || warp != 0) return;

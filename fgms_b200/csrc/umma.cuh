@@ -123,6 +123,9 @@ __device__ __forceinline__ void fence_proxy_async_global() { asm volatile("fence
 
 // all threads of all CTAs of the cluster
 __device__ __forceinline__ void cluster_sync() { asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory"); }
+// the two halves of cluster_sync, for work that can be done between them; every thread runs each of them once
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
 
 // ------------------------------------------------------------------ cp.async (16-byte, zero fill)
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
