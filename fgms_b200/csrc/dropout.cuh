@@ -18,6 +18,17 @@ struct DropoutParams {
   int alone;  // see GmsParams
 };
 
+// Where a thread goes from (row, chunk of the row): by `step_row` rows and `step_chunk` chunks of `per_row` a row.  Whether that wrapped into a row further; a row beyond the last one is
+// n_rows, and stays it.
+__host__ __device__ __forceinline__ bool drop_next(int& row, unsigned& chunk, int n_rows, int step_row, unsigned step_chunk, unsigned per_row) {
+  row = row < n_rows - step_row ? row + step_row : n_rows;  // (rows and steps together may leave an int)
+  chunk += step_chunk;
+  if (chunk < per_row) return false;
+  chunk -= per_row;
+  if (row < n_rows) ++row;
+  return true;
+}
+
 // A chunk is a thread's; threads go on by the whole grid, whose width in rows and columns is divided once, and so are the ways through the tensors.  What
 // bounds it are instructions as much as memory: 228 a chunk of eight at first (masks of bits, products for addresses, conversions one by one), 168 now, of
 // which the lots are some 70: 32768 x 2048 in bf16 with a residual 72 us, its gradient 64, 85 and 64 % of the measured copy rate.  SOME: something is dropped.
@@ -55,14 +66,10 @@ __global__ void __launch_bounds__(DROP_THREADS, DROP_BLOCKS) dropout_kernel(cons
       out[i] = static_cast<T*>(p.out) + out_way.at;
       x[i] = row_load(static_cast<const T*>(p.x) + x_way.at, there[i], p.x_vec);
       if (!BACKWARD && p.residual) add[i] = row_load(static_cast<const T*>(p.residual) + add_way.at, there[i], p.residual_vec);
-      row = row < n_rows - step_row ? row + step_row : n_rows;  // (rows and steps together may leave an int)
-      chunk += step_chunk;
       x_way.at += x_way.step;
       out_way.at += out_way.step;
       if (!BACKWARD) add_way.at += add_way.step;
-      if (chunk >= per_row) {
-        chunk -= per_row;
-        row = min(row + 1, n_rows);
+      if (drop_next(row, chunk, n_rows, step_row, step_chunk, per_row)) {
         x_way.at += x_way.wrap;
         out_way.at += out_way.wrap;
         if (!BACKWARD) add_way.at += add_way.wrap;
