@@ -148,17 +148,27 @@ def dropout(x: torch.Tensor, p: float, rng: torch.Tensor, residual: torch.Tensor
     return _native.dropout(x, p, rng, residual)
 
 
+def _module_state(seed: int | None, device) -> torch.Tensor:
+    """The state of a module's generator.  Lots hang on (seed, call, row, column) alone: modules of one seed drop the same values in every step.  Without a seed it is
+    drawn from PyTorch's generator of the host (``torch.manual_seed`` repeats it), moved apart by the rank where there are several."""
+    if seed is None:
+        seed = int(torch.randint(2 ** 63 - 1, (), dtype=torch.int64, device="cpu"))
+        if torch.distributed.is_available() and torch.distributed.is_initialized():
+            seed = (seed + torch.distributed.get_rank() * 0x9E3779B97F4A7C15) % 2 ** 63  # an odd number: no two ranks alike
+    return rng_state(seed, device)
+
+
 class RMSNorm(torch.nn.Module):
     """:func:`rms_norm` with its weight; ``forward(x)`` is the normed rows, ``forward(x, residual)`` those and the sum.  ``dropout`` is applied to ``x`` in
-    training, with a state of its own (``seed``)."""
+    training, with a state of its own, the buffer ``rng``; ``seed``: see :class:`Dropout`."""
 
-    def __init__(self, width: int, eps: float = 1e-6, dropout: float = 0.0, dtype=torch.float32, device="cuda", seed: int = 0):
+    def __init__(self, width: int, eps: float = 1e-6, dropout: float = 0.0, dtype=torch.float32, device="cuda", seed: int | None = None):
         super().__init__()
         if not 0.0 <= dropout <= 1.0:
             raise ValueError(f"dropout must be in [0, 1], got {dropout}")
         self.width, self.eps, self.dropout = width, eps, dropout
         self.weight = torch.nn.Parameter(torch.ones(width, dtype=dtype, device=device))
-        self.register_buffer("rng", rng_state(seed, device) if dropout > 0 else None)
+        self.register_buffer("rng", _module_state(seed, device) if dropout > 0 else None)
 
     def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None):
         p = self.dropout if self.training else 0.0
@@ -166,14 +176,18 @@ class RMSNorm(torch.nn.Module):
 
 
 class Dropout(torch.nn.Module):
-    """:func:`dropout` with a state of its own; outside training ``x``, or ``residual + x``."""
+    """:func:`dropout` with a state of its own, the buffer ``rng``; outside training ``x``, or ``residual + x``.
 
-    def __init__(self, p: float = 0.5, device="cuda", seed: int = 0):
+    ``seed``: None draws another one for every module, from PyTorch's generator of the host, and every rank of an initialised process group has its own.
+    Modules of one seed, copies of a module and ranks whose buffers are one rank's (a checkpoint, ``broadcast_buffers`` of
+    ``DistributedDataParallel``) drop the same values: ``module.rng.copy_(rng_state(another))`` moves them apart."""
+
+    def __init__(self, p: float = 0.5, device="cuda", seed: int | None = None):
         super().__init__()
         if not 0.0 <= p <= 1.0:
             raise ValueError(f"p must be in [0, 1], got {p}")
         self.p = p
-        self.register_buffer("rng", rng_state(seed, device))
+        self.register_buffer("rng", _module_state(seed, device))
 
     def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:
         if self.training and self.p > 0:
