@@ -17,7 +17,7 @@ import torch
 from . import _native, backend
 
 __all__ = ["sparse_conv", "sparse_conv_inference", "SparseConv3d", "SparseUNet", "grouped_linear", "GroupedLinear", "rms_norm", "RMSNorm",
-           "rms_norm_int8", "quantize_rows", "rng_state", "dropout", "Dropout", "int8_linear", "Int8GroupedLinear", "expert_layer", "ExpertLayer"]
+           "rms_norm_int8", "quantize_rows", "rng_state", "recomputed", "dropout", "Dropout", "int8_linear", "Int8GroupedLinear", "expert_layer", "ExpertLayer"]
 
 
 def sparse_conv(feats: torch.Tensor, weight: torch.Tensor, kmap, arch80: bool = True) -> torch.Tensor:
@@ -93,7 +93,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual:
              rng: torch.Tensor | None = None):
     """``h * weight / sqrt(mean(h ** 2) + eps)`` over the last dimension of ``h = residual + dropout(x)``; differentiable in ``x``, ``weight`` and
     ``residual``.  With a ``residual`` the result is ``(out, h)``, ``h`` being what the next layer adds to; without one it is ``out``.  One pass over
-    the rows for all of it.  ``weight`` is of the type of ``x`` or float32.  ``rng``: see :func:`dropout`."""
+    the rows for all of it.  ``weight`` is of the type of ``x`` or float32.  ``rng``: see :func:`dropout`; a call that drops nothing (``dropout = 0``) leaves it alone."""
     return _native.rms_norm(x, weight, eps, residual, dropout, rng)
 
 
@@ -141,10 +141,50 @@ def rng_state(seed: int = 0, device="cuda") -> torch.Tensor:
     return torch.tensor([seed, 0, 0], dtype=torch.int64, device=device)
 
 
+class _From:
+    """While it is open, the states go on from where ``first`` says they were; without ``again`` it notes that."""
+
+    def __init__(self, states, first, again):
+        self.states, self.first, self.again, self.later = states, first, again, None
+
+    def __enter__(self):
+        was = [s.clone() for s in self.states]
+        if not self.again:
+            self.first[:] = was
+            return
+        self.later = was
+        for s, f in zip(self.states, self.first):
+            s.copy_(f)
+
+    def __exit__(self, *_):
+        if self.again:
+            for s, now in zip(self.states, self.later):
+                s.copy_(now)
+
+
+def recomputed(*of):
+    """What ``torch.utils.checkpoint`` needs for a segment that drops values, as its ``context_fn``::
+
+        checkpoint(block, x, use_reentrant=False, context_fn=lambda: nn.recomputed(block))
+
+    A segment that is computed again for its backward would count its calls again and drop other values than the ones that made the loss, so that its gradients would belong
+    to another mask.  With this it goes by the calls of the first time, and the states are left as they were.  ``of``: states (:func:`rng_state`), and modules whose
+    :class:`Dropout` and :class:`RMSNorm` layers are meant.  Copies on the device alone: it can be captured into a graph (with ``preserve_rng_state=False``)."""
+    states = []
+    for o in of:
+        found = [m.rng for m in o.modules() if isinstance(m, (Dropout, RMSNorm)) and m.rng is not None] if isinstance(o, torch.nn.Module) else [o]
+        states += [s for s in found if not any(s is t for t in states)]
+    if not all(isinstance(s, torch.Tensor) and s.dtype == torch.int64 and s.shape == (3,) for s in states):
+        raise ValueError("states of rng_state, or modules, are needed")
+    first = []
+    return _From(states, first, False), _From(states, first, True)
+
+
 def dropout(x: torch.Tensor, p: float, rng: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:
     """``residual + x * kept / (1 - p)``, with a mask that is never stored: the backward draws the same lots again.  ``rng`` comes from
     :func:`rng_state` and counts the calls, on the device: a replayed graph drops other values every time.  Differentiable in ``x`` and
-    ``residual``.  The lots of a value hang on its row and column, the last dimension being the columns."""
+    ``residual``.  The lots of a value hang on its row and column, the last dimension being the columns.  A call with ``p = 0`` counts too.  Segments that are computed again
+    for their backward (``torch.utils.checkpoint``) need :func:`recomputed`."""
     return _native.dropout(x, p, rng, residual)
 
 

@@ -43,3 +43,24 @@ def test_every_rank_has_its_own(monkeypatch):
         torch.manual_seed(4)
         assert seeds(seed=5) == [5] * 4
     assert len(set(found)) == 64 and all(0 <= s < 2 ** 63 for s in found)
+
+
+def test_states_of_a_segment_that_is_computed_again():
+    a, b = nn.rng_state(1, "cpu"), nn.Dropout(0.5, device="cpu", seed=2)
+    layers = torch.nn.Sequential(b, nn.RMSNorm(8, device="cpu"))  # of which one has no state
+    forward, again = nn.recomputed(a, layers, b.rng)
+    a[1], b.rng[1] = 4, 5
+    with forward:
+        a[1] += 2
+        b.rng[1] += 1
+    a[1] += 10
+    for _ in range(2):
+        with pytest.raises(RuntimeError, match="stopped"):
+            with again:
+                assert a.tolist() == [1, 4, 0] and b.rng.tolist() == [2, 5, 0]
+                a[1] += 1
+                raise RuntimeError("stopped")
+        assert a.tolist() == [1, 16, 0] and b.rng.tolist() == [2, 6, 0]
+    for bad in (3, None, torch.zeros(3), torch.zeros(2, dtype=torch.int64)):
+        with pytest.raises(ValueError, match="states of rng_state"):
+            nn.recomputed(bad)
