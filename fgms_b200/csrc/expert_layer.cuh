@@ -57,8 +57,8 @@ struct ExpertParams {
   int alone;
 };
 
-// The top_k largest logits of a token, by a warp: (*expert, *gate) of lane j are the j-th one's.  A logit that is not a number counts as minus infinity (and
-// makes the gates such).
+// The top_k largest logits of a token, by a warp: (*expert, *gate) of lane j are the j-th one's.  A logit that is not a number counts as minus infinity (where
+// the largest is that, the gates are not numbers).
 template <int EACH>
 __device__ __forceinline__ void el_choose(const ExpertParams& p, const double* logits, int* expert, float* gate) {
   const int lane = threadIdx.x & 31;

@@ -252,7 +252,7 @@ def expert_layer(x: torch.Tensor, router: torch.Tensor, w_in: torch.Tensor, w_ou
     ``w_in`` is twice as wide as ``w_out`` is high; ``activation`` is ``"silu"`` or ``"relu"``.
 
     Up to 64 rows of float16 or bfloat16 that need no gradient take two launches (:func:`fgms_b200.backend.fgms_expert_layer_cuda`; it chooses by logits in
-    64 bits, the other way by logits in 32).  Otherwise rows are put in the order of their experts and go through :func:`grouped_linear`:
+    64 bits, the other way by logits in 32; a logit that is not a number is the lowest in both).  Otherwise rows are put in the order of their experts and go through :func:`grouped_linear`:
     differentiable in ``x``, ``router`` (through the weights of the sum), ``w_in`` and ``w_out``."""
     if activation not in ("silu", "relu"):
         raise ValueError(f"activation must be 'silu' or 'relu', got {activation!r}")
@@ -269,6 +269,7 @@ def expert_layer(x: torch.Tensor, router: torch.Tensor, w_in: torch.Tensor, w_ou
             backend.fgms_expert_layer_cuda(rows, router, w_in, w_out, out, chosen, torch.empty(chosen.shape, device=x.device), activation)
         return out.view(*x.shape[:-1], w_out.size(2))
     logits = rows.float() @ router.float().T
+    logits = torch.where(logits != logits, float("-inf"), logits)  # a sort would put what is not a number first
     value, chosen = (t[:, :top_k] for t in torch.sort(logits, dim=1, descending=True, stable=True))
     gate = torch.softmax(value, 1)
     ids = chosen.reshape(-1)
