@@ -246,13 +246,31 @@ def _few_tokens(x, router, w_in, w_out, top_k) -> bool:
             and all(t.is_contiguous() and t.data_ptr() % 16 == 0 for t in (x, router, w_in, w_out)))
 
 
+def _library_has_32_bits() -> bool:
+    """Whether a library product of float32 matrices is one: a process may allow TF32, which keeps 10 bits of the operands, or be inside autocast, which keeps fewer."""
+    try:
+        return not torch.backends.cuda.matmul.allow_tf32 and not torch.is_autocast_enabled("cuda")
+    except RuntimeError:  # it was allowed under another name
+        return False
+
+
+def _logits(rows, router):
+    """``rows @ router.T`` in 32 bits: a choice hangs on the difference of two.  By the library where it has them (16384 rows of 4096 to 64 experts 353 us, 840 with
+    gradients), otherwise by the grouped products, as one group (443 and 1170)."""
+    n = rows.size(0)
+    if n == 0 or _library_has_32_bits():
+        return rows.float() @ router.float().T
+    return grouped_linear(rows.float(), router.float().T[None], torch.arange(0, n + 1, n, dtype=torch.int32, device=rows.device))
+
+
 def expert_layer(x: torch.Tensor, router: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, top_k: int, activation: str = "silu") -> torch.Tensor:
     """Each row of ``x`` through the ``top_k`` of its experts that the ``router`` (``[experts, width]``) gives the largest logits, their outputs added up with
     the softmax over those as weights.  An expert is ``h @ w_out[e]`` with ``h = act(x @ w_in[e])``, or ``act(u[:, :hidden]) * u[:, hidden:]`` where
     ``w_in`` is twice as wide as ``w_out`` is high; ``activation`` is ``"silu"`` or ``"relu"``.
 
     Up to 64 rows of float16 or bfloat16 that need no gradient take two launches (:func:`fgms_b200.backend.fgms_expert_layer_cuda`; it chooses by logits in
-    64 bits, the other way by logits in 32; a logit that is not a number is the lowest in both).  Otherwise rows are put in the order of their experts and go through :func:`grouped_linear`:
+    64 bits, the other way by logits in 32, whatever the process allows library products; a logit that is not a number is the lowest in
+    both).  Otherwise rows are put in the order of their experts and go through :func:`grouped_linear`:
     differentiable in ``x``, ``router`` (through the weights of the sum), ``w_in`` and ``w_out``."""
     if activation not in ("silu", "relu"):
         raise ValueError(f"activation must be 'silu' or 'relu', got {activation!r}")
@@ -268,7 +286,7 @@ def expert_layer(x: torch.Tensor, router: torch.Tensor, w_in: torch.Tensor, w_ou
         with torch.no_grad():
             backend.fgms_expert_layer_cuda(rows, router, w_in, w_out, out, chosen, torch.empty(chosen.shape, device=x.device), activation)
         return out.view(*x.shape[:-1], w_out.size(2))
-    logits = rows.float() @ router.float().T
+    logits = _logits(rows, router)
     logits = torch.where(logits != logits, float("-inf"), logits)  # a sort would put what is not a number first
     value, chosen = (t[:, :top_k] for t in torch.sort(logits, dim=1, descending=True, stable=True))
     gate = torch.softmax(value, 1)

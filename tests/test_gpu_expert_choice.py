@@ -47,3 +47,42 @@ def test_a_router_row_that_is_not_a_number_is_the_last_choice():
         for got in ways(layer, top_k):
             assert torch.isnan(got[11]).all()
             near(got[fine], want[fine], allowed[fine])
+
+
+@pytest.fixture(params=["as it is", "tf32 allowed", "tf32 by name", "autocast"])
+def process(request):
+    """What a process allows products of float32 matrices."""
+    matmul = torch.backends.cuda.matmul
+    if request.param == "tf32 allowed":
+        was, matmul.allow_tf32 = matmul.allow_tf32, True
+        yield
+        matmul.allow_tf32 = was
+    elif request.param == "tf32 by name":
+        was, matmul.fp32_precision = matmul.fp32_precision, "tf32"
+        yield
+        matmul.fp32_precision = was
+    elif request.param == "autocast":
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            yield
+    else:
+        yield
+
+
+def test_a_choice_that_32_bits_tell_and_fewer_do_not(process):
+    """Experts 1 and 6 have rows of the router in the ratio 1 : 1 + 2^-14, which TF32 and bf16 round to the same; all logits are positive multiples of what 32 bits add up without
+    an error of that size (256 values of one sign: 257 2^-24 = 2^-16 at most)."""
+    layer = Layer("bf16", 20, 8, 1, 256, 64, seed=22, router_type=torch.float32)
+    layer.x.abs_()
+    layer.router.abs_()
+    layer.router[1] = layer.router[1].bfloat16().float() * 4
+    layer.router[6] = layer.router[1] * (1 + 2.0 ** -14)
+    with torch.autocast("cuda", enabled=False):
+        want, allowed = definition(layer)
+        assert (layer.exact()[2] == 6).all()
+    for got in ways(layer):
+        near(got, want, allowed)
+    x, router = layer.x.repeat(4, 1).requires_grad_(), layer.router.clone().requires_grad_()
+    from fgms_b200 import nn
+    grads = torch.autograd.grad(nn.expert_layer(x, router, layer.w_in, layer.w_out, 3).float().square().sum(), (x, router))
+    assert all(torch.isfinite(g).all() for g in grads) and grads[1].abs().amax(1)[[1, 6]].min() > 0
+    assert nn.expert_layer(x[:0], router, layer.w_in, layer.w_out, 3).shape == (0, 256)
