@@ -118,7 +118,9 @@ def int8_linear(codes: torch.Tensor, scale: torch.Tensor, kernel: torch.Tensor, 
 
 class Int8GroupedLinear(torch.nn.Module):
     """:class:`GroupedLinear` for serving: its matrices in 8 bits with a scale for each channel, rows in 8 bits with a scale each.
-    ``forward(feats, kpos)`` takes rows, or the ``(codes, scale)`` of :func:`rms_norm_int8` and :func:`quantize_rows`."""
+    ``forward(feats, kpos)`` takes rows, or the ``(codes, scale)`` of :func:`rms_norm_int8` and :func:`quantize_rows`; the output is of ``dtype``, or
+    the type that ``weight`` had.  A cast of the module (``.bfloat16()``) changes neither that nor the scales, which stay float32.  At most 32768
+    channels in, as many as :func:`quantize_rows` takes."""
 
     def __init__(self, weight: torch.Tensor, dtype: torch.dtype | None = None):
         super().__init__()
@@ -128,6 +130,13 @@ class Int8GroupedLinear(torch.nn.Module):
         self.register_buffer("kernel", codes.as_strided((groups, c_out, c_in), (c_out * codes.stride(0), codes.stride(0), 1)))
         self.register_buffer("kernel_scale", scale.view(groups, c_out))
         self.dtype = weight.dtype if dtype is None else dtype
+
+    def _apply(self, fn, recurse=True):
+        scale = self.kernel_scale
+        super()._apply(fn, recurse)
+        if self.kernel_scale.dtype != torch.float32:  # whatever a model's rows and weights are cast to
+            self.kernel_scale = scale.to(self.kernel_scale.device)
+        return self
 
     def forward(self, feats, kpos: torch.Tensor | None = None) -> torch.Tensor:
         codes, scale = feats if isinstance(feats, tuple) else quantize_rows(feats)
