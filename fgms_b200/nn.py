@@ -116,6 +116,17 @@ def int8_linear(codes: torch.Tensor, scale: torch.Tensor, kernel: torch.Tensor, 
     return _native.int8_linear(codes, scale, kernel, kernel_scale, kpos, dtype)
 
 
+def _spaced(kernel: torch.Tensor) -> torch.Tensor:
+    """The codes ``[groups, c_out, c_in]`` with a channel's a multiple of 16 bytes from the next one's, as the products read them: a copy that made them dense (a move to another
+    device) would have every call copy all of them first."""
+    groups, c_out, c_in = kernel.shape
+    room = (c_in + 15) // 16 * 16
+    if kernel.stride() == (c_out * room, room, 1) and (kernel.is_meta or kernel.data_ptr() % 16 == 0):
+        return kernel
+    spaced = torch.zeros((groups, c_out, room), dtype=kernel.dtype, device=kernel.device)[:, :, :c_in]
+    return spaced.copy_(kernel)
+
+
 class Int8GroupedLinear(torch.nn.Module):
     """:class:`GroupedLinear` for serving: its matrices in 8 bits with a scale for each channel, rows in 8 bits with a scale each.
     ``forward(feats, kpos)`` takes rows, or the ``(codes, scale)`` of :func:`rms_norm_int8` and :func:`quantize_rows`; the output is of ``dtype``, or
@@ -126,8 +137,7 @@ class Int8GroupedLinear(torch.nn.Module):
         super().__init__()
         groups, c_in, c_out = weight.shape
         codes, scale = quantize_rows(weight.detach().transpose(1, 2).reshape(groups * c_out, c_in))
-        # a channel's codes, a multiple of 16 bytes from the next one's
-        self.register_buffer("kernel", codes.as_strided((groups, c_out, c_in), (c_out * codes.stride(0), codes.stride(0), 1)))
+        self.register_buffer("kernel", _spaced(codes.as_strided((groups, c_out, c_in), (c_out * codes.stride(0), codes.stride(0), 1))))
         self.register_buffer("kernel_scale", scale.view(groups, c_out))
         self.dtype = weight.dtype if dtype is None else dtype
 
@@ -136,7 +146,16 @@ class Int8GroupedLinear(torch.nn.Module):
         super()._apply(fn, recurse)
         if self.kernel_scale.dtype != torch.float32:  # whatever a model's rows and weights are cast to
             self.kernel_scale = scale.to(self.kernel_scale.device)
+        self.kernel = _spaced(self.kernel)
         return self
+
+    def _load_from_state_dict(self, *args):
+        super()._load_from_state_dict(*args)
+        self.kernel = _spaced(self.kernel)
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self.kernel = _spaced(self.kernel)
 
     def forward(self, feats, kpos: torch.Tensor | None = None) -> torch.Tensor:
         codes, scale = feats if isinstance(feats, tuple) else quantize_rows(feats)

@@ -29,3 +29,33 @@ def test_scales_stay_in_32_bits(layer, cast):
     assert model[0].weight.dtype != torch.float32 and layer.kernel_scale.dtype == torch.float32 and layer.dtype == torch.bfloat16
     assert torch.equal(layer.kernel_scale, scale) and torch.equal(layer.kernel, kernel)
     assert set(layer.state_dict()) == {"kernel", "kernel_scale"}
+
+
+def stays(layer, kernel):
+    assert torch.equal(layer.kernel, kernel) and layer.kernel.shape == (3, 20, 50) and layer.kernel.stride() == (20 * 64, 64, 1) and layer.kernel.data_ptr() % 16 == 0
+
+
+def test_codes_stay_16_bytes_apart(layer):
+    """Through everything that copies a module's buffers, or puts others in their place."""
+    kernel = layer.kernel.clone()
+    stays(layer, kernel)
+    stays(copy.deepcopy(layer), kernel)
+    layer._apply(lambda t: t.clone())  # what a move to another device does
+    stays(layer, kernel)
+    for assign in (False, True):
+        other = copy.deepcopy(layer)
+        other.kernel.zero_()
+        other.load_state_dict({k: v.clone(memory_format=torch.contiguous_format) for k, v in layer.state_dict().items()}, assign=assign)
+        stays(other, kernel)
+    empty = copy.deepcopy(layer).to("meta").to_empty(device="cpu")
+    empty.load_state_dict(layer.state_dict())
+    stays(empty, kernel)
+
+
+def test_a_saved_module(layer, tmp_path):
+    kernel = layer.kernel.clone()
+    torch.save(layer, tmp_path / "layer.pt")
+    stays(torch.load(tmp_path / "layer.pt", weights_only=False), kernel)
+    layer._buffers["kernel"] = kernel  # as an earlier release may have saved it
+    torch.save(layer, tmp_path / "layer.pt")
+    stays(torch.load(tmp_path / "layer.pt", weights_only=False), kernel)
