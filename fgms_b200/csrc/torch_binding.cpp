@@ -936,6 +936,12 @@ void end_graph(std::initializer_list<Tensor*> grads, const char* what) {
 }
 const Tensor* maybe_tensor(const Tensor& t) { return t.defined() ? &t : nullptr; }
 
+// Forward-mode differentiation is not built: a tangent would be dropped without a word where nothing needs a gradient.
+void check_no_tangent(const char* what, std::initializer_list<const Tensor*> tensors) {
+  for (const Tensor* t : tensors)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t || !t->defined() || !t->_fw_grad(0).defined(), what, " has no forward-mode gradient");
+}
+
 void check_norm_shapes(const Tensor& x, const Tensor& weight, const Tensor* residual) {
   TORCH_CHECK_VALUE(x.is_cuda(), "x must be a CUDA tensor");
   TORCH_CHECK_VALUE(x.dim() >= 1, "x must have at least one dimension");
@@ -1036,6 +1042,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
 Tensor nn_dropout(const Tensor& x, double p, const Tensor& rng, const Tensor* residual) {
   TORCH_CHECK_VALUE(x.is_cuda(), "x must be a CUDA tensor");
   TORCH_CHECK_VALUE(!residual || residual->sizes() == x.sizes(), "residual must have the shape of x");
+  check_no_tangent("dropout", {&x, residual});
   if (at::GradMode::is_enabled() && (x.requires_grad() || (residual && residual->requires_grad())))
     return Dropout::apply(x, p, rng, residual ? std::optional<Tensor>(*residual) : std::nullopt);
   const Tensor rows = as_rows(x), other = residual ? as_rows(*residual) : Tensor(), out = new_like(rows);
@@ -1053,6 +1060,7 @@ Tensor new_codes(int64_t rows, int64_t width, const Tensor& like) {
 // (codes, scale, sum): without a weight there is no norm; the sum is undefined without a residual
 std::array<Tensor, 3> rms_norm_int8(const Tensor& x_, const Tensor* weight_, const Tensor* residual_, double eps) {
   if (weight_) check_norm_shapes(x_, *weight_, residual_);
+  check_no_tangent("an output in 8 bits", {&x_, weight_, residual_});
   TORCH_CHECK_VALUE(x_.dim() == 2, "x must have 2 dimensions, got ", x_.dim());
   TORCH_CHECK_VALUE(!(at::GradMode::is_enabled() && (x_.requires_grad() || (weight_ && weight_->requires_grad()) || (residual_ && residual_->requires_grad()))),
                     "codes of 8 bits have no gradient: call it under torch.no_grad()");
@@ -1110,6 +1118,7 @@ void grouped_i8(const Tensor& codes, const Tensor& scale, const Tensor& kernel, 
 Tensor int8_linear(const Tensor& codes, const Tensor& scale, const Tensor& kernel_, const Tensor& kernel_scale_, const Tensor* kpos, at::ScalarType type) {
   const Tensor kernel = kernel_.dim() == 2 ? kernel_.unsqueeze(0) : kernel_, kernel_scale = kernel_scale_.dim() == 1 ? kernel_scale_.unsqueeze(0) : kernel_scale_;
   TORCH_CHECK_VALUE(kernel.is_cuda() && kernel.dim() == 3 && codes.dim() == 2, "kernel must be an int8 CUDA tensor of 2 or 3 dimensions, codes one of 2");
+  check_no_tangent("int8_linear", {&scale, &kernel_scale_});
   Tensor out = at::empty({codes.size(0), kernel.size(1)}, kernel.options().dtype(type).requires_grad(false));
   grouped_i8(codes, scale, kernel, kernel_scale, out, kpos, kpos != nullptr);
   return out;
@@ -1126,6 +1135,7 @@ int activation_of(const std::string& name) {
 
 void expert_layer(const Tensor& x, const Tensor& router, const Tensor& w_in, const Tensor& w_out, const Tensor& out, const Tensor& experts, const Tensor& gates,
                   const std::string& activation) {
+  check_no_tangent("expert_layer", {&x, &router, &w_in, &w_out});
   fgms_b200_expert_layer_args a = {};
   a.activation = activation_of(activation);
   TORCH_CHECK_VALUE(x.is_cuda() && x.dim() == 2, "x must be a CUDA tensor of 2 dimensions");
@@ -1512,6 +1522,7 @@ PyObject* py_rms_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const Tensor &x = feat_arg(a[0], "x"), &weight = feat_arg(a[1], "weight"), *residual = maybe_arg(a[3], "residual"), *rng = maybe_arg(a[5], "rng");
   const double eps = double_arg(a[2]), p = double_arg(a[4]);
   check_norm_shapes(x, weight, residual);
+  check_no_tangent("rms_norm", {&x, &weight, residual});
   Tensor out, sum;
   if (at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad() || (residual && residual->requires_grad()))) {
     auto r = RmsNorm::apply(x, weight, residual ? std::optional<Tensor>(*residual) : std::nullopt, rng ? std::optional<Tensor>(*rng) : std::nullopt, eps, p);
