@@ -18,16 +18,10 @@ struct DropoutParams {
   int alone;  // see GmsParams
 };
 
-// Where a thread goes from (row, chunk of the row): by `step_row` rows and `step_chunk` chunks of `per_row` a row.  Whether that wrapped into a row further; a row beyond the last one is
-// n_rows, and stays it.
-__host__ __device__ __forceinline__ bool drop_next(int& row, unsigned& chunk, int n_rows, int step_row, unsigned step_chunk, unsigned per_row) {
-  row = row < n_rows - step_row ? row + step_row : n_rows;  // (rows and steps together may leave an int)
-  chunk += step_chunk;
-  if (chunk < per_row) return false;
-  chunk -= per_row;
-  if (row < n_rows) ++row;
-  return true;
-}
+// The row `step` rows further, and the next one: n_rows where there is none, and from n_rows on.  (Rows and steps together may leave an int; 2^31 - 1 rows and one more do, but
+// for a number without a sign.)
+__host__ __device__ __forceinline__ int drop_row_after(int row, int step, int n_rows) { return row < n_rows - step ? row + step : n_rows; }
+__host__ __device__ __forceinline__ int drop_next_row(int row, int n_rows) { return (int)min((unsigned)row + 1u, (unsigned)n_rows); }
 
 // A chunk is a thread's; threads go on by the whole grid, whose width in rows and columns is divided once, and so are the ways through the tensors.  What
 // bounds it are instructions as much as memory: 228 a chunk of eight at first (masks of bits, products for addresses, conversions one by one), 168 now, of
@@ -66,10 +60,14 @@ __global__ void __launch_bounds__(DROP_THREADS, DROP_BLOCKS) dropout_kernel(cons
       out[i] = static_cast<T*>(p.out) + out_way.at;
       x[i] = row_load(static_cast<const T*>(p.x) + x_way.at, there[i], p.x_vec);
       if (!BACKWARD && p.residual) add[i] = row_load(static_cast<const T*>(p.residual) + add_way.at, there[i], p.residual_vec);
+      row = drop_row_after(row, step_row, n_rows);
+      chunk += step_chunk;
       x_way.at += x_way.step;
       out_way.at += out_way.step;
       if (!BACKWARD) add_way.at += add_way.step;
-      if (drop_next(row, chunk, n_rows, step_row, step_chunk, per_row)) {
+      if (chunk >= per_row) {
+        chunk -= per_row;
+        row = drop_next_row(row, n_rows);
         x_way.at += x_way.wrap;
         out_way.at += out_way.wrap;
         if (!BACKWARD) add_way.at += add_way.wrap;

@@ -24,7 +24,12 @@ int main() {
               return 1;
             }
             behind += !there;
-            drop_next(row, chunk, (int)rows, step_row, step_chunk, per_row);
+            row = drop_row_after(row, step_row, (int)rows);
+            chunk += step_chunk;
+            if (chunk >= per_row) {
+              chunk -= per_row;
+              row = drop_next_row(row, (int)rows);
+            }
           }
         }
       }
