@@ -1064,7 +1064,8 @@ std::array<Tensor, 3> rms_norm_int8(const Tensor& x_, const Tensor* weight_, con
   TORCH_CHECK_VALUE(x_.dim() == 2, "x must have 2 dimensions, got ", x_.dim());
   TORCH_CHECK_VALUE(!(at::GradMode::is_enabled() && (x_.requires_grad() || (weight_ && weight_->requires_grad()) || (residual_ && residual_->requires_grad()))),
                     "codes of 8 bits have no gradient: call it under torch.no_grad()");
-  const Tensor x = x_.stride(1) == 1 || x_.size(1) <= 1 ? x_ : x_.contiguous(), weight = weight_ ? weight_->contiguous() : Tensor();
+  const bool as_it_lies = (x_.stride(1) == 1 || x_.size(1) <= 1) && (x_.stride(0) >= x_.size(1) || x_.size(0) <= 1);
+  const Tensor x = as_it_lies ? x_ : x_.contiguous(), weight = weight_ ? weight_->contiguous() : Tensor();
   const Tensor residual = residual_ ? as_rows(*residual_) : Tensor();
   std::array<Tensor, 3> r = {new_codes(x.size(0), x.size(1), x), at::empty({x.size(0)}, x.options().dtype(at::kFloat).requires_grad(false)),
                              residual_ ? at::empty({x.size(0), x.size(1)}, x.options().requires_grad(false)) : Tensor()};
