@@ -318,7 +318,7 @@ def fgms_rms_norm_bwd_cuda(out_grad, h, weight, rstd, x_grad=None, weight_grad=N
                            x=None, residual=None):
     """Gradient of :func:`fgms_rms_norm_cuda` from ``h`` (``residual_out``, or ``x`` where there was neither residual nor dropout) and ``rstd``:
     ``residual_grad = dh``, ``x_grad`` the same where x was kept, ``weight_grad`` (the weight's type, summed in float32 in a fixed order).
-    ``h_grad`` is what else flows back into ``h``.  Outputs that are None are left out.  Rows in 16 bits with a float32 weight: given ``x`` and
+    ``h_grad`` is what else flows back into ``h``.  Outputs that are None are left out.  Rows in 16 bits: given ``x`` and
     ``residual`` instead of ``h`` (None), h is computed once more and ``weight_grad`` does not see how it was rounded."""
     _native.rms_norm_bwd(out_grad, h, weight, rstd, x_grad, weight_grad, h_grad, residual_grad, dropout, rng_used, x, residual)
 

@@ -221,8 +221,8 @@ int run_rms_norm_bwd(const fgms_b200_rms_norm_bwd_args& a, cudaStream_t st) {
   const bool drop = p.drop.threshold > 0;
   const size_t es = layer_elem(a.dtype);
   const auto span = [&](const void* at, int64_t pitch) { return RowSpan{at, a.rows, pitch, a.width, es}; };
-  if (a.x && (a.dtype == FGMS_DTYPE_F32 || a.weight_dtype != FGMS_DTYPE_F32))
-    return fail(FGMS_ERR_UNSUPPORTED, "x is read for rows in 16 bits with a weight in fp32; otherwise sum is");
+  if (a.x && (a.dtype == FGMS_DTYPE_F32 || (a.weight_dtype != FGMS_DTYPE_F32 && a.sum)))
+    return fail(FGMS_ERR_UNSUPPORTED, "x is read for rows in 16 bits, with a weight of their type where there is no sum; otherwise sum is");
   const RowSpan dy = span(a.out_grad, a.out_grad_pitch), h = a.x ? span(a.x, a.x_pitch) : span(a.sum, a.sum_pitch),
                 residual = span(a.x ? a.residual : nullptr, a.residual_pitch), dsum = span(a.sum_grad, a.sum_grad_pitch), dx = span(a.x_grad, a.x_grad_pitch),
                 dresidual = span(a.residual_grad, a.residual_grad_pitch);

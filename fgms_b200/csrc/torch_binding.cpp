@@ -949,8 +949,8 @@ void check_norm_shapes(const Tensor& x, const Tensor& weight, const Tensor* resi
   TORCH_CHECK_VALUE(!residual || residual->sizes() == x.sizes(), "residual must have the shape of x");
 }
 
-// Where the weight's gradient holds more than the stored sum does.
-bool exact_sum_needed(const Tensor& x, const Tensor& weight) { return weight.scalar_type() == at::kFloat && x.scalar_type() != at::kFloat; }
+// Where the weight's gradient would see how the stored sum was rounded.
+bool exact_sum_needed(const Tensor& x) { return x.scalar_type() != at::kFloat; }
 
 // The norm of one call: out, and with a residual or dropout the sum that it is the norm of.
 struct Normed {
@@ -980,7 +980,7 @@ Normed norm_forward(const Tensor& x_, const Tensor& weight_, const Tensor* resid
 struct RmsNorm : torch::autograd::Function<RmsNorm> {
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& weight,
                                                 const std::optional<Tensor>& residual, const std::optional<Tensor>& rng, double eps, double p) {
-    const bool from_x = (residual || drops(p)) && weight.requires_grad() && exact_sum_needed(x, weight);
+    const bool from_x = (residual || drops(p)) && weight.requires_grad() && exact_sum_needed(x);
     Normed n = norm_forward(x, weight, residual ? &*residual : nullptr, eps, p, rng ? &*rng : nullptr, true, from_x);
     ctx->saved_data["p"] = p;
     ctx->saved_data["residual"] = residual.has_value();

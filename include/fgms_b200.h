@@ -387,8 +387,9 @@ typedef struct {
 
 int fgms_b200_rms_norm(const fgms_b200_rms_norm_args* args, void* stream);
 
-/* Its gradient, from `sum` (x itself where there was neither residual nor dropout) and `rstd`; or, rows in 16 bits with an F32 weight, from `x` and
- * `residual`, with which h is computed once more, so that the weight's gradient does not see the rounding of `sum` (which may be NULL then):
+/* Its gradient, from `sum` (x itself where there was neither residual nor dropout) and `rstd`; or, rows in 16 bits, from `x` and `residual`, with
+ * which h is computed once more, so that the weight's gradient does not see the rounding of `sum` (which may be NULL then, and has to be for a weight of
+ * the rows' type: FGMS_ERR_UNSUPPORTED):
  *   residual_grad = dh = rstd (g - n mean(g n)) + sum_grad     with g = out_grad weight, n = sum rstd
  *   x_grad = dh where x was kept, times the factor             weight_grad = sum over the rows of out_grad n, added up in fp32 in a fixed order
  * sum_grad (what else flows back into `sum`), x_grad, residual_grad and weight_grad (weight_dtype) may each be NULL; weight_grad needs a
