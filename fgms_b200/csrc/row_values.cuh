@@ -155,7 +155,7 @@ __device__ __forceinline__ void row_store(T* p, const float (&x)[ROW_CHUNK], int
 // Dropout.  Philox 4x32 with ten rounds (Salmon, Moraes, Dror, Shaw: "Parallel random numbers: as easy as 1, 2, 3", SC 2011): the
 // key is the seed, the counter (column / 8, row, call), whose 128 bits are eight lots of 16 bits for the eight columns of a chunk.  A value is dropped
 // where its lot is below the threshold, round(p 65536); the others are multiplied by 65536 / (65536 - threshold), so that the mean is kept exactly
-// at the probability as it is rounded.  16 bits a lot: 32 would be two evaluations a chunk, 80 wide multiplications instead of 40.
+// at the probability as it is rounded.  16 bits a lot: 32 would be two evaluations a chunk, 40 wide multiplications instead of 20.
 // Nothing is stored: the backward evaluates the same lots again.
 //
 // State in device memory, [seed, calls made, blocks of this call that have finished]: a call takes the number of calls made as its own number

@@ -99,12 +99,12 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual:
 
 def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: torch.Tensor | None = None):
     """:func:`rms_norm` with the output in 8 bits, for the products behind it: ``(codes, scale)`` or ``(codes, scale, h)``, where
-    ``codes * scale[:, None]`` is the normed row.  Codes are int8 rows that start 16 bytes apart.  No autograd."""
+    ``codes * scale[:, None]`` is the normed row.  ``x`` has two dimensions.  Codes are int8 rows that start 16 bytes apart.  No autograd."""
     return _native.rms_norm_int8(x, weight, eps, residual)
 
 
 def quantize_rows(x: torch.Tensor):
-    """``(codes, scale)``: the rows of ``x`` in 8 bits with a float32 scale each.  No autograd."""
+    """``(codes, scale)``: the rows of ``x``, which has two dimensions and up to 32768 columns, in 8 bits with a float32 scale each.  No autograd."""
     return _native.rms_norm_int8(x, None, 0.0, None)
 
 

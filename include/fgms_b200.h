@@ -344,7 +344,8 @@ int fgms_b200_adamw(const fgms_b200_adamw_tensor* tensors, int n, const fgms_b20
  * 4x32-10: key the seed, counter (column / 8, row, number of the call), eight lots a counter, the lower half of a word before the upper one.  No mask is
  * stored: the backward evaluates the same lots from rng_used.
  *   rng       device, three int64: the seed, the number of calls made, and 0.  A call counts itself there, so that a replayed graph drops other
- *             values every time; two calls on the same state must not run at the same time.  A call without rows is not counted.
+ *             values every time; two calls on the same state must not run at the same time.  A call without rows is not counted,
+ *             one that drops nothing (p = 0) is by fgms_b200_dropout and not by the norm, which needs no rng then.
  *   rng_used  device, two int64: where the call leaves seed and number for its backward (NULL: nowhere); read by the backward.
  * fgms_b200_dropout: out = residual + dropped x (residual may be NULL).  fgms_b200_dropout_bwd: out = dropped x with the lots of rng_used, where x
  * is the gradient of the output; the residual's gradient is that itself. */
