@@ -23,7 +23,7 @@
 //               a tile ten times as long as its weights)
 //   warps 10-11 report finished items and add the output up: a report waits until all that was stored is there, a microsecond that the products go on in
 //
-// All waits are bounded.  bf16: one token, 2 of 8 experts 512 x 1024, 16.4 to 18.2 us, which is latency; 16 tokens, 4 of 64 experts 2048 x 1024 each, 517 MB of weights, 96 to 99 us (79
+// All waits are bounded.  bf16: one token, 2 of 8 experts 512 x 1024, 16.4 to 18.2 us, which is latency; 16 tokens, 4 of 64 experts 2048 x 1024 each, 517 MB of weights, 96 to 101 us (79
 // at the measured copy rate), 5.6 TB/s between the first tile and the last; 64 tokens, 2 of 32 experts 1024 x 2048 without a gate, 264 MB, 72 us (40).  With 33 tokens an expert and
 // more the products take longer than the weights' way: 64 tokens, all of 4 experts 2048 x 1024, 86 us.
 #pragma once
